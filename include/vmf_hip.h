@@ -43,7 +43,12 @@ enum vmf_status {
   VMF_ERR_UNSUPPORTED = -4  /* valid request this build has no kernel for (e.g. m > 2048) */
 };
 
-enum vmf_dtype { VMF_F32 = 0, VMF_F64 = 1 };
+enum vmf_dtype {
+  VMF_F32 = 0,
+  VMF_F64 = 1,
+  VMF_F16 = 2, /* VMF_F16 and VMF_BF16: taken by the layer norm and the 8-bit block calls only */
+  VMF_BF16 = 3
+};
 
 enum vmf_kl_variant {
   VMF_KL_SPHERICAL_PIECEWISE = 0, /* model/spherical_vae.py:141-184 (clamp, <1e-3 -> 0, >20 asymptote) */
@@ -281,6 +286,27 @@ int vmf_latent_loss_fwd(const void* z, const void* labels, void* per_row_out, vo
 int vmf_latent_loss_bwd(const void* z, const void* labels, const void* grad_mean, void* dz, int64_t n, int zdim,
                         int64_t n_labels, int label_cols, int variant, double R, double r, int dtype,
                         vmf_stream_t stream);
+
+/* ---- wide hidden layers: layer norm ------------------------------------------------------------------------
+ * The reference's hidden layers are Linear + softplus (model/spherical_vae.py:51-66) without a norm; these calls
+ * have no counterpart there.  Rows of `width` values (1 <= width <= VMF_LAYER_NORM_MAX_WIDTH) of dtype VMF_F32,
+ * VMF_F64, VMF_F16 or VMF_BF16 with a row stride in elements (any stride, 0 included; no alignment beyond the
+ * element's); weight and bias (each may be null: 1 and 0) are of weight_dtype, the rows' dtype or VMF_F32 with 16-bit rows.
+ *   xhat = (x - mean) rstd, rstd = 1 / sqrt(mean((x - mean)^2) + eps), y = xhat weight + bias
+ * y and gx are dense.  mean_out / rstd_out (both or neither; n values, float, or double for VMF_F64) are what bwd takes.
+ * Sums and statistics are held in 32 bits, in 64 for VMF_F64.
+ * bwd: h = gy weight, gx = rstd (h - mean(h) - xhat mean(h xhat)), gweight = sum over rows of gy xhat, gbias = sum of
+ * gy, both of weight_dtype, added in a fixed order (the same bits on every run); each output may be null.  n == 0 gives
+ * gweight = gbias = 0.  workspace: needed with gweight or gbias, vmf_layer_norm_bwd_workspace bytes, 16-byte aligned. */
+#define VMF_LAYER_NORM_MAX_WIDTH ((int64_t)1 << 24)
+int vmf_layer_norm_fwd(const void* x, int64_t x_stride, const void* weight, const void* bias, void* y, void* mean_out,
+                       void* rstd_out, int64_t n, int64_t width, double eps, int dtype, int weight_dtype,
+                       vmf_stream_t stream);
+int vmf_layer_norm_bwd_workspace(int64_t n, int64_t width, int dtype, int64_t* bytes_out);
+int vmf_layer_norm_bwd(const void* x, int64_t x_stride, const void* gy, int64_t gy_stride, const void* weight,
+                       const void* mean, const void* rstd, void* gx, void* gweight, void* gbias, int64_t n,
+                       int64_t width, void* workspace, int64_t workspace_bytes, int dtype, int weight_dtype,
+                       vmf_stream_t stream);
 
 /* ---- multi-GPU ---------------------------------------------------------------------------------------
  * The path shards by row and exchanges nothing but loss scalars: the `.mean()` / `.sum()` of

@@ -12,7 +12,8 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _DEFAULT = os.path.join(_HERE, "libvmf_hip.so")
 
-VMF_F32, VMF_F64 = 0, 1
+VMF_F32, VMF_F64, VMF_F16, VMF_BF16 = range(4)
+FLOAT_CODES = {torch.float32: VMF_F32, torch.float64: VMF_F64, torch.float16: VMF_F16, torch.bfloat16: VMF_BF16}
 FLAG_NORMALIZE_MU = 1
 FLAG_SOFTPLUS_KAPPA = 2
 KIND_GENERAL, KIND_ROWS, KIND_OUTER = 0, 1, 2
@@ -64,6 +65,9 @@ _PROTOS = {
     "vmf_build_torus_bwd": [_P, _P, _P, _P, _P, _I64, _I, _D, _D, _I, _P],
     "vmf_latent_loss_fwd": [_P, _P, _P, _P, _P, _I64, _I, _I64, _I, _I, _D, _D, _I, _P],
     "vmf_latent_loss_bwd": [_P, _P, _P, _P, _I64, _I, _I64, _I, _I, _D, _D, _I, _P],
+    "vmf_layer_norm_fwd": [_P, _I64, _P, _P, _P, _P, _P, _I64, _I64, _D, _I, _I, _P],
+    "vmf_layer_norm_bwd_workspace": [_I64, _I64, _I, _I64P],
+    "vmf_layer_norm_bwd": [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _I64, _I, _I, _P],
 }
 EXPORTS = sorted(list(_PROTOS) + ["vmf_version", "vmf_last_error_string"])
 
@@ -110,6 +114,31 @@ def dtype_code(t):
     if t.dtype == torch.float64:
         return VMF_F64
     raise TypeError(f"libvmf_hip supports float32 and float64 tensors, got {t.dtype}")
+
+
+def float_code(t, what, accepted):
+    """the library's code of a tensor's type, for the calls that take more than dtype_code's two"""
+    if t.dtype not in accepted:
+        names = ", ".join(str(d).replace("torch.", "") for d in accepted)
+        raise TypeError(f"{what} takes {names} tensors, got {t.dtype}")
+    return FLOAT_CODES[t.dtype]
+
+
+def as_rows(t):
+    """(n, width) view of a tensor with its row stride; a copy only where the last dimension is not dense or the
+    leading ones have no common stride"""
+    width = t.shape[-1]
+    n = t.numel() // width if width else 0
+    if t.dim() == 2 and (t.stride(1) == 1 or width == 1):
+        r = t
+    else:
+        try:
+            r = t.view(n, width)
+        except RuntimeError:
+            r = t.contiguous().view(n, width)
+        if r.stride(1) != 1 and width != 1:
+            r = r.contiguous()
+    return r, (r.stride(0) if n > 1 else width)
 
 
 def require_hip(*tensors):

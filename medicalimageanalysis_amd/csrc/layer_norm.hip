@@ -1,0 +1,478 @@
+// layer_norm.hip -- layer norm over the last dimension, forward and backward.
+//
+//   xhat = (x - mean) rstd,  rstd = 1 / sqrt(mean((x - mean)^2) + eps),  y = xhat w + b
+//   h = gy w,  gx = rstd (h - mean(h) - xhat mean(h xhat)),  gw = sum_rows gy xhat,  gb = sum_rows gy
+//
+// Both directions are streams of HBM: the forward pass reads x and writes y, the backward pass reads x and gy and
+// writes gx, about 8 and 20 operations per element against 8 and 12 bytes (fp32).  A row is held in the registers of
+// TPR lanes, so it is read once and the variance is summed from centred values (no difference of large squares).
+// Statistics, sums and the partial gradients are 32-bit (64-bit for double rows).
+#include "lowp.h"
+
+namespace {
+
+constexpr int THREADS = 256;
+
+template <typename T> struct LnVec { static constexpr int value = 16 / (int)sizeof(T); };
+
+// sum over the TPR threads that share a row; `red` holds one value per wave and a second set alternates with it, so
+// that one barrier per sum is enough (a wave can only be one sum ahead of the others)
+template <int TPR, typename A>
+__device__ __forceinline__ A row_sum(A v, A* red, int& flip) {
+  if constexpr (TPR <= 64) {
+    return lane_sum<TPR>(v);
+  } else {
+    constexpr int WAVES = TPR / 64;
+    v = lane_sum<64>(v);
+    A* r = red + flip * WAVES;
+    flip ^= 1;
+    if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
+    __syncthreads();
+    A s = 0;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) s += r[i];
+    return s;
+  }
+}
+
+template <typename T, typename W, int TPR, int NCH>
+__global__ __launch_bounds__(TPR > THREADS ? TPR : THREADS) void ln_fwd_kernel(
+    const T* __restrict__ x, int64_t x_stride, const W* __restrict__ w, const W* __restrict__ b, T* __restrict__ y,
+    typename AccOf<T>::type* __restrict__ mean_out, typename AccOf<T>::type* __restrict__ rstd_out, int64_t n,
+    int width, double eps) {
+  using A = typename AccOf<T>::type;
+  constexpr int V = LnVec<T>::value;
+  constexpr int NT = TPR > THREADS ? TPR : THREADS;
+  constexpr int ROWS = NT / TPR;
+  __shared__ A red[2 * (TPR > 64 ? TPR / 64 : 1)];
+  int flip = 0;
+  const int lane = threadIdx.x % TPR;
+  const A inv = (A)1 / (A)width;
+  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR; row < n; row += (int64_t)gridDim.x * ROWS) {
+    const T* xr = x + row * x_stride;
+    A v[NCH][V];
+    A s = 0;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int col = (c * TPR + lane) * V;
+      load_some<V>(xr + col, (int64_t)width - col, (A)0, v[c]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) s += v[c][i];
+    }
+    const A mean = row_sum<TPR>(s, red, flip) * inv;
+    s = 0;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int left = width - (c * TPR + lane) * V;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        v[c][i] -= mean;
+        s += i < left ? v[c][i] * v[c][i] : (A)0;
+      }
+    }
+    const A rstd = (A)1 / M<A>::sqrt(row_sum<TPR>(s, red, flip) * inv + (A)eps);
+    if (lane == 0 && mean_out) {
+      mean_out[row] = mean;
+      rstd_out[row] = rstd;
+    }
+    T* yr = y + row * (int64_t)width;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int col = (c * TPR + lane) * V;
+      A wv[V], bv[V];
+      if (w) load_some<V>(w + col, (int64_t)width - col, (A)0, wv);
+      if (b) load_some<V>(b + col, (int64_t)width - col, (A)0, bv);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[c][i] = v[c][i] * rstd * (w ? wv[i] : (A)1) + (b ? bv[i] : (A)0);
+      store_some<V>(yr + col, (int64_t)width - col, v[c]);
+    }
+  }
+}
+
+// Rows that do not fit the registers: the same sums over three reads of the row (the second and third out of the L2).
+template <typename T, typename W>
+__global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__ x, int64_t x_stride,
+                                                           const W* __restrict__ w, const W* __restrict__ b,
+                                                           T* __restrict__ y,
+                                                           typename AccOf<T>::type* __restrict__ mean_out,
+                                                           typename AccOf<T>::type* __restrict__ rstd_out, int64_t n,
+                                                           int64_t width, double eps) {
+  using A = typename AccOf<T>::type;
+  constexpr int V = LnVec<T>::value;
+  __shared__ A red[32];
+  int flip = 0;
+  for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
+    const T* xr = x + row * x_stride;
+    A v[V], s = 0;
+    for (int64_t col = (int64_t)threadIdx.x * V; col < width; col += 1024 * V) {
+      load_some<V>(xr + col, width - col, (A)0, v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) s += v[i];
+    }
+    const A mean = row_sum<1024>(s, red, flip) / (A)width;
+    s = 0;
+    for (int64_t col = (int64_t)threadIdx.x * V; col < width; col += 1024 * V) {
+      load_some<V>(xr + col, width - col, mean, v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) s += (v[i] - mean) * (v[i] - mean);
+    }
+    const A rstd = (A)1 / M<A>::sqrt(row_sum<1024>(s, red, flip) / (A)width + (A)eps);
+    if (threadIdx.x == 0 && mean_out) {
+      mean_out[row] = mean;
+      rstd_out[row] = rstd;
+    }
+    for (int64_t col = (int64_t)threadIdx.x * V; col < width; col += 1024 * V) {
+      A wv[V], bv[V];
+      load_some<V>(xr + col, width - col, (A)0, v);
+      if (w) load_some<V>(w + col, width - col, (A)0, wv);
+      if (b) load_some<V>(b + col, width - col, (A)0, bv);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = (v[i] - mean) * rstd * (w ? wv[i] : (A)1) + (b ? bv[i] : (A)0);
+      store_some<V>(y + row * width + col, width - col, v);
+    }
+  }
+}
+
+// Backward.  A lane keeps the same columns for every row it sees, so gw and gb grow in its registers; a workgroup
+// leaves one partial row of each (after adding its rows side by side in LDS), and ln_reduce_kernel adds the
+// workgroups' partials in a fixed order: the same bits on every run.
+template <typename T, typename W, int TPR, int NCH>
+__global__ __launch_bounds__(TPR > THREADS ? TPR : THREADS) void ln_bwd_kernel(
+    const T* __restrict__ x, int64_t x_stride, const T* __restrict__ gy, int64_t gy_stride, const W* __restrict__ w,
+    const typename AccOf<T>::type* __restrict__ mean_in, const typename AccOf<T>::type* __restrict__ rstd_in,
+    T* __restrict__ gx, typename AccOf<T>::type* __restrict__ partial, int64_t n, int width) {
+  using A = typename AccOf<T>::type;
+  constexpr int V = LnVec<T>::value;
+  constexpr int NT = TPR > THREADS ? TPR : THREADS;
+  constexpr int ROWS = NT / TPR;
+  __shared__ A red[2 * (TPR > 64 ? TPR / 64 : 1)];
+  __shared__ A side[ROWS > 1 ? (ROWS - 1) * TPR * V : 1];
+  int flip = 0;
+  const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  const A inv = (A)1 / (A)width;
+  A wv[NCH][V], gw[NCH][V], gb[NCH][V];
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    const int col = (c * TPR + lane) * V;
+    if (w) load_some<V>(w + col, (int64_t)width - col, (A)0, wv[c]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (!w) wv[c][i] = (A)1;
+      gw[c][i] = gb[c][i] = 0;
+    }
+  }
+  for (int64_t row = (int64_t)blockIdx.x * ROWS + sub; row < n; row += (int64_t)gridDim.x * ROWS) {
+    const T* xr = x + row * x_stride;
+    const T* gr = gy + row * gy_stride;
+    const A mean = mean_in[row], rstd = rstd_in[row];
+    A xh[NCH][V], h[NCH][V];
+    A s1 = 0, s2 = 0;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int col = (c * TPR + lane) * V;
+      load_some<V>(xr + col, (int64_t)width - col, mean, xh[c]);
+      load_some<V>(gr + col, (int64_t)width - col, (A)0, h[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < NCH; ++c)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        xh[c][i] = (xh[c][i] - mean) * rstd;
+        gw[c][i] += h[c][i] * xh[c][i];
+        gb[c][i] += h[c][i];
+        h[c][i] *= wv[c][i];
+        s1 += h[c][i];
+        s2 += h[c][i] * xh[c][i];
+      }
+    if (gx) {
+      s1 = row_sum<TPR>(s1, red, flip) * inv;
+      s2 = row_sum<TPR>(s2, red, flip) * inv;
+      T* out = gx + row * (int64_t)width;
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) {
+        const int col = (c * TPR + lane) * V;
+#pragma unroll
+        for (int i = 0; i < V; ++i) h[c][i] = (h[c][i] - s1 - xh[c][i] * s2) * rstd;
+        store_some<V>(out + col, (int64_t)width - col, h[c]);
+      }
+    }
+  }
+  if (!partial) return;
+  A* out = partial + (int64_t)blockIdx.x * 2 * width;
+#pragma unroll
+  for (int which = 0; which < 2; ++which)
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      A(&g)[V] = which ? gb[c] : gw[c];
+      if constexpr (ROWS > 1) {
+        __syncthreads();
+        if (sub > 0)
+#pragma unroll
+          for (int i = 0; i < V; ++i) side[((sub - 1) * TPR + lane) * V + i] = g[i];
+        __syncthreads();
+        if (sub == 0)
+          for (int r = 0; r < ROWS - 1; ++r)
+#pragma unroll
+            for (int i = 0; i < V; ++i) g[i] += side[(r * TPR + lane) * V + i];
+      }
+      const int col = (c * TPR + lane) * V;
+      if (sub == 0) store_some<V>(out + (int64_t)which * width + col, (int64_t)width - col, g);
+    }
+}
+
+// Rows that do not fit: gx alone, a workgroup per row ...
+template <typename T, typename W>
+__global__ __launch_bounds__(1024) void ln_bwd_long_kernel(
+    const T* __restrict__ x, int64_t x_stride, const T* __restrict__ gy, int64_t gy_stride, const W* __restrict__ w,
+    const typename AccOf<T>::type* __restrict__ mean_in, const typename AccOf<T>::type* __restrict__ rstd_in,
+    T* __restrict__ gx, int64_t n, int64_t width) {
+  using A = typename AccOf<T>::type;
+  constexpr int V = LnVec<T>::value;
+  __shared__ A red[32];
+  int flip = 0;
+  for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
+    const T* xr = x + row * x_stride;
+    const T* gr = gy + row * gy_stride;
+    const A mean = mean_in[row], rstd = rstd_in[row];
+    A xv[V], hv[V], wv[V], s1 = 0, s2 = 0;
+    for (int64_t col = (int64_t)threadIdx.x * V; col < width; col += 1024 * V) {
+      load_some<V>(xr + col, width - col, mean, xv);
+      load_some<V>(gr + col, width - col, (A)0, hv);
+      if (w) load_some<V>(w + col, width - col, (A)0, wv);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const A h = w ? hv[i] * wv[i] : hv[i];
+        s1 += h;
+        s2 += h * ((xv[i] - mean) * rstd);
+      }
+    }
+    s1 = row_sum<1024>(s1, red, flip) / (A)width;
+    s2 = row_sum<1024>(s2, red, flip) / (A)width;
+    for (int64_t col = (int64_t)threadIdx.x * V; col < width; col += 1024 * V) {
+      load_some<V>(xr + col, width - col, mean, xv);
+      load_some<V>(gr + col, width - col, (A)0, hv);
+      if (w) load_some<V>(w + col, width - col, (A)0, wv);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const A h = w ? hv[i] * wv[i] : hv[i];
+        hv[i] = (h - s1 - (xv[i] - mean) * rstd * s2) * rstd;
+      }
+      store_some<V>(gx + row * width + col, width - col, hv);
+    }
+  }
+}
+// ... and gw, gb by columns: a workgroup takes 256 columns and one slice of the rows
+template <typename T>
+__global__ __launch_bounds__(256) void ln_cols_kernel(const T* __restrict__ x, int64_t x_stride,
+                                                      const T* __restrict__ gy, int64_t gy_stride,
+                                                      const typename AccOf<T>::type* __restrict__ mean_in,
+                                                      const typename AccOf<T>::type* __restrict__ rstd_in,
+                                                      typename AccOf<T>::type* __restrict__ partial, int64_t n,
+                                                      int64_t width) {
+  using A = typename AccOf<T>::type;
+  const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (col >= width) return;
+  A gw = 0, gb = 0;
+  for (int64_t row = blockIdx.y; row < n; row += gridDim.y) {
+    const A g = (A)gy[row * gy_stride + col];
+    gw += g * (((A)x[row * x_stride + col] - mean_in[row]) * rstd_in[row]);
+    gb += g;
+  }
+  partial[((int64_t)blockIdx.y * 2) * width + col] = gw;
+  partial[((int64_t)blockIdx.y * 2 + 1) * width + col] = gb;
+}
+
+// gw / gb from `parts` partial rows of 2 * width values: a workgroup takes 16 columns, 16 threads share one
+template <typename A, typename W>
+__global__ __launch_bounds__(256) void ln_reduce_kernel(const A* __restrict__ partial, W* __restrict__ gw,
+                                                        W* __restrict__ gb, int parts, int64_t width) {
+  __shared__ A red[256];
+  const int64_t col = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);  // 0 .. 2 width
+  A s = 0;
+  if (col < 2 * width)
+    for (int p = threadIdx.x >> 4; p < parts; p += 16) s += partial[(int64_t)p * 2 * width + col];
+  red[threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.x < 16 && col < 2 * width) {
+#pragma unroll
+    for (int r = 1; r < 16; ++r) s += red[r * 16 + threadIdx.x];
+    if (col < width) {
+      if (gw) gw[col] = (W)s;
+    } else if (gb) {
+      gb[col - width] = (W)s;
+    }
+  }
+}
+
+// How many workgroups of the backward pass leave a partial: enough to fill 256 compute units, and no more than there
+// are rows to share (each partial costs 2 * width values written and read back).
+int bwd_groups(int64_t n, int rows_per_group) {
+  const int64_t g = (n + rows_per_group - 1) / rows_per_group;
+  return (int)(g < 512 ? (g < 1 ? 1 : g) : 512);
+}
+// lanes per row by the width in vectors of 16 bytes: as few as hold the row in at most `chunks` registers' worth each
+int lanes_for(int64_t vectors, int chunks) {
+  for (int tpr = 16; tpr <= 1024; tpr *= tpr == 64 ? 4 : tpr == 256 ? 4 : 2)
+    if (vectors <= (int64_t)tpr * chunks) return tpr;
+  return 0;
+}
+
+template <typename T, typename W, int TPR, int NCH>
+void launch_fwd(const void* x, int64_t xs, const void* w, const void* b, void* y, void* mean, void* rstd, int64_t n,
+                int64_t width, double eps, hipStream_t st) {
+  using A = typename AccOf<T>::type;
+  constexpr int NT = TPR > THREADS ? TPR : THREADS;
+  const int grid = vmf_grid_for(n, NT / TPR, 1 << 16);
+  ln_fwd_kernel<T, W, TPR, NCH><<<grid, NT, 0, st>>>((const T*)x, xs, (const W*)w, (const W*)b, (T*)y, (A*)mean,
+                                                      (A*)rstd, n, (int)width, eps);
+}
+template <typename T, typename W>
+void run_fwd(const void* x, int64_t xs, const void* w, const void* b, void* y, void* mean, void* rstd, int64_t n,
+             int64_t width, double eps, hipStream_t st) {
+  using A = typename AccOf<T>::type;
+  constexpr int V = LnVec<T>::value;
+  constexpr int MAXC = 32 / V;  // 32 values per lane
+  const int64_t vectors = (width + V - 1) / V;
+#define LN_FWD(TPR, NCH) \
+  if (vectors <= (int64_t)(TPR) * (NCH)) return launch_fwd<T, W, TPR, NCH>(x, xs, w, b, y, mean, rstd, n, width, eps, st)
+  LN_FWD(16, 1);
+  LN_FWD(32, 1);
+  LN_FWD(64, 1);
+  LN_FWD(64, 2);
+  LN_FWD(64, MAXC / 2 < 2 ? 2 : MAXC / 2);
+  LN_FWD(64, MAXC);
+  LN_FWD(256, MAXC / 2 < 2 ? 2 : MAXC / 2);
+  LN_FWD(256, MAXC);
+  LN_FWD(1024, MAXC);
+#undef LN_FWD
+  ln_fwd_long_kernel<T, W><<<vmf_grid_for(n, 1, 1 << 16), 1024, 0, st>>>((const T*)x, xs, (const W*)w, (const W*)b,
+                                                                         (T*)y, (A*)mean, (A*)rstd, n, width, eps);
+}
+
+template <typename T> constexpr int bwd_chunks() { return 16 / LnVec<T>::value; }  // 16 values per lane
+
+// partial rows of the backward pass (host arithmetic shared with the workspace query)
+template <typename T>
+int bwd_parts(int64_t n, int64_t width) {
+  constexpr int V = LnVec<T>::value;
+  const int tpr = lanes_for((width + V - 1) / V, bwd_chunks<T>());
+  if (tpr == 0) return bwd_groups(n, 64);
+  return bwd_groups(n, tpr < THREADS ? THREADS / tpr : 1);
+}
+
+template <typename T, typename W>
+int run_bwd(const void* x, int64_t xs, const void* gy, int64_t gs, const void* w, const void* mean, const void* rstd,
+            void* gx, void* gw, void* gb, void* ws, int64_t n, int64_t width, hipStream_t st) {
+  using A = typename AccOf<T>::type;
+  constexpr int V = LnVec<T>::value;
+  constexpr int C = bwd_chunks<T>();
+  const int parts = bwd_parts<T>(n, width);
+  A* partial = gw || gb ? (A*)ws : nullptr;
+  const int64_t vectors = (width + V - 1) / V;
+  const int tpr = lanes_for(vectors, C);
+#define LN_BWD(TPR, NCH)                                                                                        \
+  ln_bwd_kernel<T, W, TPR, NCH><<<parts, TPR > THREADS ? TPR : THREADS, 0, st>>>(                                \
+      (const T*)x, xs, (const T*)gy, gs, (const W*)w, (const A*)mean, (const A*)rstd, (T*)gx, partial, n, (int)width)
+  if (tpr == 16) {
+    if (vectors <= 16) LN_BWD(16, 1);
+    else LN_BWD(16, C);
+  } else if (tpr == 32) {
+    LN_BWD(32, C);
+  } else if (tpr == 64) {
+    LN_BWD(64, C);
+  } else if (tpr == 256) {
+    LN_BWD(256, C);
+  } else if (tpr == 1024) {
+    LN_BWD(1024, C);
+  } else {
+    if (gx)
+      ln_bwd_long_kernel<T, W><<<vmf_grid_for(n, 1, 1 << 16), 1024, 0, st>>>(
+          (const T*)x, xs, (const T*)gy, gs, (const W*)w, (const A*)mean, (const A*)rstd, (T*)gx, n, width);
+    if (partial)
+      ln_cols_kernel<T><<<dim3((unsigned)((width + 255) / 256), (unsigned)parts), 256, 0, st>>>(
+          (const T*)x, xs, (const T*)gy, gs, (const A*)mean, (const A*)rstd, partial, n, width);
+  }
+#undef LN_BWD
+  int rc = vmf_check_launch("vmf_layer_norm_bwd");
+  if (rc != VMF_OK || !partial) return rc;
+  ln_reduce_kernel<A, W><<<(unsigned)((2 * width + 15) / 16), 256, 0, st>>>(partial, (W*)gw, (W*)gb, parts, width);
+  return vmf_check_launch("vmf_layer_norm_bwd sums");
+}
+
+int check_common(const char* what, int64_t n, int64_t width, int64_t stride, int dtype, int wdtype) {
+  VMF_REQUIRE(n >= 0, VMF_ERR_BAD_ARG, "%s: n < 0", what);
+  VMF_REQUIRE(width >= 1, VMF_ERR_BAD_ARG, "%s: width must be at least 1", what);
+  VMF_REQUIRE(width <= VMF_LAYER_NORM_MAX_WIDTH, VMF_ERR_UNSUPPORTED, "%s: width > %lld", what,
+              (long long)VMF_LAYER_NORM_MAX_WIDTH);
+  VMF_REQUIRE(stride >= 0, VMF_ERR_BAD_ARG, "%s: negative row stride", what);
+  VMF_REQUIRE(dtype >= VMF_F32 && dtype <= VMF_BF16, VMF_ERR_DTYPE, "%s: dtype %d", what, dtype);
+  VMF_REQUIRE(wdtype == dtype || (wdtype == VMF_F32 && dtype != VMF_F64), VMF_ERR_DTYPE,
+              "%s: the weight's dtype is the rows' or VMF_F32, got %d", what, wdtype);
+  return VMF_OK;
+}
+
+}  // namespace
+
+// (T, W) pairs: weights in the rows' type, or fp32 ones with 16-bit rows
+#define LN_DISPATCH(dtype, wdtype, CALL)                                   \
+  do {                                                                     \
+    if ((dtype) == VMF_F32) { using T = float; using W = float; CALL; }    \
+    else if ((dtype) == VMF_F64) { using T = double; using W = double; CALL; } \
+    else if ((dtype) == VMF_F16) {                                         \
+      using T = f16_t;                                                     \
+      if ((wdtype) == VMF_F32) { using W = float; CALL; } else { using W = f16_t; CALL; } \
+    } else {                                                               \
+      using T = bf16_t;                                                    \
+      if ((wdtype) == VMF_F32) { using W = float; CALL; } else { using W = bf16_t; CALL; } \
+    }                                                                      \
+  } while (0)
+
+extern "C" int vmf_layer_norm_fwd(const void* x, int64_t x_stride, const void* weight, const void* bias, void* y,
+                                  void* mean_out, void* rstd_out, int64_t n, int64_t width, double eps, int dtype,
+                                  int weight_dtype, vmf_stream_t stream) {
+  VMF_RANGE("vmf_layer_norm_fwd");
+  int rc = check_common("vmf_layer_norm_fwd", n, width, x_stride, dtype, weight_dtype);
+  if (rc != VMF_OK) return rc;
+  if (n == 0) return VMF_OK;
+  VMF_REQUIRE(x && y, VMF_ERR_BAD_ARG, "vmf_layer_norm_fwd: null pointer");
+  VMF_REQUIRE(!mean_out == !rstd_out, VMF_ERR_BAD_ARG, "vmf_layer_norm_fwd: mean_out and rstd_out go together");
+  hipStream_t st = (hipStream_t)stream;
+  LN_DISPATCH(dtype, weight_dtype,
+              (run_fwd<T, W>(x, x_stride, weight, bias, y, mean_out, rstd_out, n, width, eps, st)));
+  return vmf_check_launch("vmf_layer_norm_fwd");
+}
+
+extern "C" int vmf_layer_norm_bwd_workspace(int64_t n, int64_t width, int dtype, int64_t* bytes_out) {
+  int rc = check_common("vmf_layer_norm_bwd_workspace", n, width, 0, dtype, dtype);
+  if (rc != VMF_OK) return rc;
+  VMF_REQUIRE(bytes_out, VMF_ERR_BAD_ARG, "vmf_layer_norm_bwd_workspace: null pointer");
+  int parts;
+  if (dtype == VMF_F32) parts = bwd_parts<float>(n, width);
+  else if (dtype == VMF_F64) parts = bwd_parts<double>(n, width);
+  else parts = bwd_parts<f16_t>(n, width);
+  *bytes_out = (int64_t)parts * 2 * width * (dtype == VMF_F64 ? 8 : 4);
+  return VMF_OK;
+}
+
+extern "C" int vmf_layer_norm_bwd(const void* x, int64_t x_stride, const void* gy, int64_t gy_stride,
+                                  const void* weight, const void* mean, const void* rstd, void* gx, void* gweight,
+                                  void* gbias, int64_t n, int64_t width, void* workspace, int64_t workspace_bytes,
+                                  int dtype, int weight_dtype, vmf_stream_t stream) {
+  VMF_RANGE("vmf_layer_norm_bwd");
+  int rc = check_common("vmf_layer_norm_bwd", n, width, x_stride < gy_stride ? x_stride : gy_stride, dtype,
+                        weight_dtype);
+  if (rc != VMF_OK) return rc;
+  VMF_REQUIRE(n == 0 || (x && gy && mean && rstd), VMF_ERR_BAD_ARG, "vmf_layer_norm_bwd: null pointer");
+  if (gweight || gbias) {
+    int64_t need = 0;
+    vmf_layer_norm_bwd_workspace(n, width, dtype, &need);
+    VMF_REQUIRE(workspace && workspace_bytes >= need, VMF_ERR_BAD_ARG,
+                "vmf_layer_norm_bwd: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  } else if (!gx || n == 0) {
+    return VMF_OK;
+  }
+  hipStream_t st = (hipStream_t)stream;
+  LN_DISPATCH(dtype, weight_dtype, (rc = run_bwd<T, W>(x, x_stride, gy, gy_stride, weight, mean, rstd, gx, gweight,
+                                                       gbias, workspace, n, width, st)));
+  return rc;
+}

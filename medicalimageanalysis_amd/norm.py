@@ -1,0 +1,108 @@
+"""Layer norm over the last dimension, for the hidden layers of wide models:
+
+    y = (x - mean) / sqrt(var + eps) * weight + bias
+
+layer_norm is differentiable once, in x, weight and bias; LayerNorm is the module.  The rows may be float32, float64,
+float16 or bfloat16, the weight and the bias of the same type or, with 16-bit rows, float32; sums and statistics are held
+in 32 bits (64 for float64 rows).  x may be any view whose last dimension is dense and whose rows have one stride; other
+views are copied.  There is no CPU path.
+"""
+import ctypes as C
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+
+def _check(x, weight, bias):
+    if x.dim() < 1:
+        raise ValueError("layer_norm: x needs at least one dimension")
+    width = x.shape[-1]
+    if width < 1:
+        raise ValueError("layer_norm: the last dimension is empty")
+    code = _lib.float_code(x, "layer_norm", (torch.float32, torch.float64, torch.float16, torch.bfloat16))
+    params = [p for p in (weight, bias) if p is not None]
+    for p in params:
+        if tuple(p.shape) != (width,):
+            raise ValueError(f"layer_norm: weight and bias must have shape ({width},), got {tuple(p.shape)}")
+        if p.dtype != params[0].dtype:
+            raise TypeError(f"layer_norm: weight and bias differ in type ({params[0].dtype}, {p.dtype})")
+        if p.dtype != x.dtype and not (p.dtype == torch.float32 and x.dtype in (torch.float16, torch.bfloat16)):
+            raise TypeError(f"layer_norm: weight and bias of {x.dtype} rows are {x.dtype}"
+                            f"{' or float32' if x.dtype in (torch.float16, torch.bfloat16) else ''}, got {p.dtype}")
+    wcode = _lib.FLOAT_CODES[params[0].dtype] if params else code
+    return _lib.require_hip(x, weight, bias), code, wcode
+
+
+def _forward(x, weight, bias, eps, dev, code, wcode, keep):
+    rows, stride = _lib.as_rows(x.detach())
+    n, width = rows.shape
+    w = None if weight is None else weight.detach().contiguous()
+    b = None if bias is None else bias.detach().contiguous()
+    y = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    stats = torch.empty((2, n), device=dev, dtype=torch.float64 if x.dtype == torch.float64 else torch.float32) if keep else None
+    with _lib.on_device(dev):
+        rc = _lib.lib().vmf_layer_norm_fwd(_lib.ptr(rows), stride, _lib.ptr(w), _lib.ptr(b), _lib.ptr(y),
+                                           _lib.ptr(stats[0]) if keep else None, _lib.ptr(stats[1]) if keep else None,
+                                           n, width, eps, code, wcode, _lib.stream_ptr(dev))
+    _lib.check(rc, "vmf_layer_norm_fwd")
+    return y, rows, stride, w, stats
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, dev, code, wcode):
+        y, rows, stride, w, stats = _forward(x, weight, bias, eps, dev, code, wcode, True)
+        ctx.save_for_backward(rows, w, stats)
+        ctx.meta = (x.shape, stride, None if bias is None else bias.dtype, code, wcode)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        rows, w, stats = ctx.saved_tensors
+        shape, x_stride, bias_dtype, code, wcode = ctx.meta
+        dev = rows.device
+        g, g_stride = _lib.as_rows(gy)
+        n, width = rows.shape
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        gx = torch.empty(shape, device=dev, dtype=rows.dtype) if need_x else None
+        gw = torch.empty(width, device=dev, dtype=w.dtype) if need_w else None
+        gb = torch.empty(width, device=dev, dtype=bias_dtype) if need_b else None
+        ws, ws_bytes = None, 0
+        lib = _lib.lib()
+        if need_w or need_b:
+            nb = C.c_int64(0)
+            _lib.check(lib.vmf_layer_norm_bwd_workspace(n, width, code, C.byref(nb)), "vmf_layer_norm_bwd_workspace")
+            ws_bytes = nb.value
+            ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+        with _lib.on_device(dev):
+            rc = lib.vmf_layer_norm_bwd(_lib.ptr(rows), x_stride, _lib.ptr(g), g_stride, _lib.ptr(w),
+                                        _lib.ptr(stats[0]), _lib.ptr(stats[1]), _lib.ptr(gx), _lib.ptr(gw),
+                                        _lib.ptr(gb), n, width, _lib.ptr(ws), ws_bytes, code, wcode,
+                                        _lib.stream_ptr(dev))
+        _lib.check(rc, "vmf_layer_norm_bwd")
+        return gx, gw, gb, None, None, None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x."""
+    dev, code, wcode = _check(x, weight, bias)
+    eps = float(eps)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _LayerNorm.apply(x, weight, bias, eps, dev, code, wcode)
+    return _forward(x, weight, bias, eps, dev, code, wcode, False)[0]
+
+
+class LayerNorm(torch.nn.LayerNorm):
+    """torch.nn.LayerNorm over one dimension with the kernels of this module: the same parameters and state dict."""
+
+    def __init__(self, width, eps=1e-5, elementwise_affine=True, bias=True, device=None, dtype=None):
+        super().__init__(int(width), eps=eps, elementwise_affine=elementwise_affine, bias=bias, device=device,
+                         dtype=dtype)
+
+    def forward(self, x):
+        if x.dim() < 1 or x.shape[-1] != self.normalized_shape[0]:
+            raise ValueError(f"LayerNorm({self.normalized_shape[0]}): got the shape {tuple(x.shape)}")
+        return layer_norm(x, self.weight, self.bias, self.eps)
