@@ -308,6 +308,52 @@ int vmf_layer_norm_bwd(const void* x, int64_t x_stride, const void* gy, int64_t 
                        int64_t width, void* workspace, int64_t workspace_bytes, int dtype, int weight_dtype,
                        vmf_stream_t stream);
 
+/* ---- wide hidden layers: 8-bit blocks -------------------------------------------------------------------------
+ * No counterpart in the reference (its dense layers are fp32 torch, model/spherical_vae.py:30-47).  A hidden layer's
+ * activation is kept as 8-bit blocks: the operand of the next layer's product and, in place of a 16- or 32-bit copy,
+ * what the backward pass reads.  A block is 128 consecutive elements of a row (a weight: a tile of 128 x 128): e4m3
+ * values (OCP: 448 the largest, no infinity) and one exponent e, an element is value * 2^e.  e is the smallest integer
+ * with 448 * 2^e >= the block's largest finite magnitude, inside [-110, 119]; values are rounded to nearest even,
+ * larger ones than 448 * 2^119 to that.  NaN and infinities become NaN.
+ *   values     rows of ceil(width / 128) * 128 bytes, the padding zero; 16-byte aligned
+ *   exponents  bytes e + 127, [ceil(width / 128)][exp_pitch]: by rows exp_pitch >= rows (products: a multiple of 16,
+ *              so that the array's end is a multiple of 16 too), by tiles exp_pitch = ceil(rows / 128)
+ * x, g, out: VMF_F32, VMF_F16 or VMF_BF16, row strides in elements as in the layer norm; out is dense. */
+#define VMF_BLOCKS8_MAX_ROWS ((int64_t)1 << 31)
+#define VMF_BLOCKS8_MAX_WIDTH ((int64_t)1 << 22)
+enum vmf_activation { VMF_ACT_NONE = 0, VMF_ACT_SOFTPLUS = 1 };
+/* blocks of x, or of softplus(x) = log(1 + exp(beta x)) / beta: the bytes of its exact value, whatever x's type */
+int vmf_blocks8_quantize(const void* x, int64_t x_stride, uint8_t* values, uint8_t* exponents, int64_t exp_pitch,
+                         int64_t rows, int64_t width, int activation, double beta, int dtype, vmf_stream_t stream);
+/* tiles of w (rows, width), and the same tiles of its transpose (both or neither of values_t, exponents_t) */
+int vmf_blocks8_quantize_tiles(const void* w, int64_t w_stride, uint8_t* values, uint8_t* exponents, uint8_t* values_t,
+                               uint8_t* exponents_t, int64_t rows, int64_t width, int dtype, vmf_stream_t stream);
+int vmf_blocks8_dequantize(const uint8_t* values, const uint8_t* exponents, int64_t exp_pitch, int tiled, void* out,
+                           int64_t rows, int64_t width, int dtype, vmf_stream_t stream);
+/* out = g * (1 - exp(-beta a)), a the blocks of softplus(h): the gradient through the softplus */
+int vmf_blocks8_softplus_grad(const void* g, int64_t g_stride, const uint8_t* values, const uint8_t* exponents,
+                              int64_t exp_pitch, void* out, int64_t rows, int64_t width, double beta, int dtype,
+                              vmf_stream_t stream);
+
+/* out[m][n] = (sum_k a[m][k] b[n][k] + bias[n]) * slope, a: m rows, b: n rows, both of width k, in blocks by rows or
+ * (tiled = 1) by tiles.  slope (gate not null; blocks by rows, m x n): 1 - exp(-beta gate[m][n]), the softplus gradient.
+ * out: dense, VMF_F32, VMF_F16 or VMF_BF16; bias (may be null): one of these types.  Sums are 32-bit for VMF_F32; for the
+ * 16-bit types the 8-bit matrix instruction's, 1.3e-5 relative.  The same bits on every run.
+ * workspace: vmf_blocks8_matmul_workspace bytes (0 for most sizes), 16-byte aligned. */
+int vmf_blocks8_matmul_workspace(int64_t m, int64_t n, int64_t k, int out_dtype, int64_t* bytes_out);
+int vmf_blocks8_matmul(const uint8_t* a, const uint8_t* a_exponents, int64_t a_exp_pitch, int a_tiled, const uint8_t* b,
+                       const uint8_t* b_exponents, int64_t b_exp_pitch, int b_tiled, const void* bias, int bias_dtype,
+                       const uint8_t* gate, const uint8_t* gate_exponents, int64_t gate_exp_pitch, double beta, void* out,
+                       int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes, int out_dtype,
+                       vmf_stream_t stream);
+/* gweight[n][k] = sum_m gy[m][n] a[m][k], gbias[n] = sum_m gy[m][n] (may be null): gy (m, n) of dtype, a: m rows of width
+ * k in blocks by rows, outputs of out_dtype (VMF_F32 or dtype).  Products are exact, sums 32-bit, in a fixed order.
+ * m == 0 gives zeros. */
+int vmf_blocks8_weight_grad_workspace(int64_t m, int64_t n, int64_t k, int64_t* bytes_out);
+int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const uint8_t* a, const uint8_t* a_exponents,
+                            int64_t a_exp_pitch, void* gweight, void* gbias, int64_t m, int64_t n, int64_t k,
+                            void* workspace, int64_t workspace_bytes, int dtype, int out_dtype, vmf_stream_t stream);
+
 /* ---- multi-GPU ---------------------------------------------------------------------------------------
  * The path shards by row and exchanges nothing but loss scalars: the `.mean()` / `.sum()` of
  * model/spherical_vae.py:134,136 and regular_cnn/s1_vae.py:75,90 taken over all ranks' rows.  buf (device, `count`

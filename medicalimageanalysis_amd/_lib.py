@@ -22,6 +22,7 @@ KL_WORKSPACE_DOUBLES = 1024
 KL_STATIC_MAX_N = 1 << 30
 ELBO_WORKSPACE_DOUBLES = 2048
 LATENT_S1, LATENT_S2, LATENT_T2 = range(3)
+ACT_NONE, ACT_SOFTPLUS = range(2)
 
 # (the module object `C` is re-used by callers for byref / c_int64)
 _P, _I64, _U64, _I, _D = C.c_void_p, C.c_int64, C.c_uint64, C.c_int, C.c_double
@@ -68,6 +69,15 @@ _PROTOS = {
     "vmf_layer_norm_fwd": [_P, _I64, _P, _P, _P, _P, _P, _I64, _I64, _D, _I, _I, _P],
     "vmf_layer_norm_bwd_workspace": [_I64, _I64, _I, _I64P],
     "vmf_layer_norm_bwd": [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _I64, _I, _I, _P],
+    "vmf_blocks8_quantize": [_P, _I64, _P, _P, _I64, _I64, _I64, _I, _D, _I, _P],
+    "vmf_blocks8_quantize_tiles": [_P, _I64, _P, _P, _P, _P, _I64, _I64, _I, _P],
+    "vmf_blocks8_dequantize": [_P, _P, _I64, _I, _P, _I64, _I64, _I, _P],
+    "vmf_blocks8_softplus_grad": [_P, _I64, _P, _P, _I64, _P, _I64, _I64, _D, _I, _P],
+    "vmf_blocks8_matmul_workspace": [_I64, _I64, _I64, _I, _I64P],
+    "vmf_blocks8_matmul": [_P, _P, _I64, _I, _P, _P, _I64, _I, _P, _I, _P, _P, _I64, _D, _P, _I64, _I64, _I64, _P, _I64,
+                           _I, _P],
+    "vmf_blocks8_weight_grad_workspace": [_I64, _I64, _I64, _I64P],
+    "vmf_blocks8_weight_grad": [_P, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I, _I, _P],
 }
 EXPORTS = sorted(list(_PROTOS) + ["vmf_version", "vmf_last_error_string"])
 
@@ -208,6 +218,16 @@ def ptr(t):
 
 def stream_ptr(device):
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def address(t):
+    """a tensor's address as a plain integer (ctypes takes it for a pointer argument without building an object)"""
+    return None if t is None else t.data_ptr()
+
+
+def raw_stream(device):
+    """the current stream's handle as a plain integer"""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def i64_array(seq):

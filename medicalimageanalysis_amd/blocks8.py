@@ -1,0 +1,323 @@
+"""8-bit blocks: activations kept and multiplied in 8 bits, for the hidden layers of wide models.
+
+A block is 128 consecutive elements of a row, for a weight matrix a tile of 128 x 128: e4m3 values and one power-of-two
+scale.  A hidden layer's activation in blocks is one byte per element where float32 keeps four, and it serves twice: as the
+operand of the next layer's product and as the checkpoint that the backward pass reads.
+
+  quantize(x, activation, beta)    blocks of x, or of softplus(x)                       -> Blocks8
+  quantize_weight(w)               tiles of w and of its transpose                      -> Weight8
+  Blocks8.dequantize(dtype)        what the blocks hold
+  matmul(a, b, bias, dtype)        a b^T + bias
+  softplus_grad(g, q, beta)        g * (1 - exp(-beta q)): the gradient through the softplus that q keeps
+  weight_grad(g, q)                g^T q and the sum of g's rows: the gradients of the weight and the bias
+  linear(x, weight, bias, activation, beta)
+                                   blocks(activation(x)) tiles(weight)^T + bias, differentiable once
+
+linear's gradients: gx = (blocks(gy) tiles(weight)) * softplus slope, gw = gy^T blocks(activation(x)), gb = the sum of
+gy's rows; the roundings to 8 bits pass their gradient on as it is.  float32 results come from 32-bit sums, float16 and
+bfloat16 ones from the faster 8-bit matrix instruction (1.3e-5 relative, a hundredth of their own rounding).  NaN and
+infinities are NaN in blocks.  There is no CPU path.
+"""
+import ctypes as C
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+BLOCK = 128
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_ACTIVATIONS = {None: _lib.ACT_NONE, "softplus": _lib.ACT_SOFTPLUS}
+
+
+def _up(n, to):
+    return -(-n // to) * to
+
+
+class Blocks8:
+    """A tensor in 8-bit blocks along its last dimension; `tiled`: one exponent per 128 x 128 tile (a weight).
+
+    values     (rows, ceil(width / 128) * 128) uint8, e4m3 bits, zero behind the width
+    exponents  (ceil(width / 128), pitch) uint8, e + 127; column r belongs to row r, tiled to rows 128 r ... 128 r + 127
+    One allocation holds both."""
+
+    __slots__ = ("storage", "shape", "rows", "width", "tiled", "exp_pitch", "exp_offset", "offset")
+
+    def __init__(self, storage, shape, tiled=False, offset=0):
+        self.storage, self.shape, self.tiled, self.offset = storage, torch.Size(shape), tiled, offset
+        self.width = self.shape[-1]
+        self.rows = self.shape.numel() // self.width
+        self.exp_pitch = max(1, _up(self.rows, BLOCK) // BLOCK) if tiled else max(16, _up(self.rows, 16))
+        self.exp_offset = offset + self.rows * _up(self.width, BLOCK)
+
+    @staticmethod
+    def bytes_for(rows, width, tiled=False):
+        pitch = max(1, _up(rows, BLOCK) // BLOCK) if tiled else max(16, _up(rows, 16))
+        return _up(rows * _up(width, BLOCK) + _up(width, BLOCK) // BLOCK * pitch, 16)
+
+    @property
+    def device(self):
+        return self.storage.device
+
+    @property
+    def values(self):
+        pitch = _up(self.width, BLOCK)
+        return self.storage[self.offset:self.offset + self.rows * pitch].view(self.rows, pitch)
+
+    @property
+    def exponents(self):
+        blocks = _up(self.width, BLOCK) // BLOCK
+        return self.storage[self.exp_offset:self.exp_offset + blocks * self.exp_pitch].view(blocks, self.exp_pitch)
+
+    def _addresses(self):
+        base = self.storage.data_ptr()
+        return base + self.offset, base + self.exp_offset
+
+    def dequantize(self, dtype=torch.float32):
+        """the elements as `dtype` (every one is exact in float32 and bfloat16)"""
+        code = _code(dtype, "dequantize")
+        dev = self.device
+        out = torch.empty(self.shape, device=dev, dtype=dtype)
+        v, e = self._addresses()
+        with _lib.on_device(dev):
+            rc = _lib.lib().vmf_blocks8_dequantize(v, e, self.exp_pitch, self.tiled, out.data_ptr(), self.rows,
+                                                   self.width, code, _lib.raw_stream(dev))
+        _lib.check(rc, "vmf_blocks8_dequantize")
+        return out
+
+    def __repr__(self):
+        return f"Blocks8({tuple(self.shape)}{', tiled' if self.tiled else ''}, device='{self.device}')"
+
+
+class Weight8:
+    """A weight matrix (n, k) laid out for `linear`: its 128 x 128 tiles (`rows`, k wide) and the same tiles transposed
+    (`columns`, n wide; None if left out), which the gradient of the layer's input reads."""
+
+    __slots__ = ("rows", "columns", "dtype")
+
+    def __init__(self, rows, columns, dtype):
+        self.rows, self.columns, self.dtype = rows, columns, dtype
+
+    @property
+    def shape(self):
+        return self.rows.shape
+
+    @property
+    def device(self):
+        return self.rows.device
+
+
+def _code(dtype, what):
+    if dtype not in _FLOATS:
+        raise TypeError(f"{what} takes float32, float16 or bfloat16, got {dtype}")
+    return _lib.FLOAT_CODES[dtype]
+
+
+def _activation(activation, beta, what):
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"{what}: activation must be None or 'softplus', got {activation!r}")
+    beta = float(beta)
+    if activation is not None and not 1e-30 <= beta <= 1e30:
+        raise ValueError(f"{what}: beta must be positive, got {beta}")
+    return _ACTIVATIONS[activation], beta
+
+
+def _width(x, what):
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{what}: the last dimension must hold at least one element, got the shape {tuple(x.shape)}")
+
+
+def _quantize(x, act, beta, code, dev):
+    rows, stride = _lib.as_rows(x.detach())
+    n, width = rows.shape
+    q = Blocks8(torch.empty(Blocks8.bytes_for(n, width), device=dev, dtype=torch.uint8), x.shape)
+    v, e = q._addresses()
+    with _lib.on_device(dev):
+        rc = _lib.lib().vmf_blocks8_quantize(rows.data_ptr(), stride, v, e, q.exp_pitch, n, width, act, beta, code,
+                                             _lib.raw_stream(dev))
+    _lib.check(rc, "vmf_blocks8_quantize")
+    return q
+
+
+def quantize(x, activation=None, beta=1.0):
+    """8-bit blocks of x, or with activation="softplus" of log(1 + exp(beta x)) / beta."""
+    _width(x, "quantize")
+    code = _code(x.dtype, "quantize")
+    act, beta = _activation(activation, beta, "quantize")
+    return _quantize(x, act, beta, code, _lib.require_hip(x))
+
+
+def _quantize_weight(w, transpose, dev):
+    rows, stride = _lib.as_rows(w.detach())
+    n, k = w.shape
+    first = Blocks8.bytes_for(n, k, True)
+    storage = torch.empty(first + (Blocks8.bytes_for(k, n, True) if transpose else 0), device=dev, dtype=torch.uint8)
+    by_rows = Blocks8(storage, (n, k), True)
+    by_columns = Blocks8(storage, (k, n), True, first) if transpose else None
+    v, e = by_rows._addresses()
+    vt, et = by_columns._addresses() if transpose else (None, None)
+    with _lib.on_device(dev):
+        rc = _lib.lib().vmf_blocks8_quantize_tiles(rows.data_ptr(), stride, v, e, vt, et, n, k,
+                                                   _lib.FLOAT_CODES[w.dtype], _lib.raw_stream(dev))
+    _lib.check(rc, "vmf_blocks8_quantize_tiles")
+    return Weight8(by_rows, by_columns, w.dtype)
+
+
+def quantize_weight(w, transpose=True):
+    """The 128 x 128 tiles of a weight matrix (n, k); transpose=False leaves out what only an input gradient reads."""
+    if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1:
+        raise ValueError(f"quantize_weight: a matrix is wanted, got the shape {tuple(w.shape)}")
+    _code(w.dtype, "quantize_weight")
+    return _quantize_weight(w, transpose, _lib.require_hip(w))
+
+
+def _matmul(a, b, bias, gate, beta, dtype, dev):
+    m, n, k = a.rows, b.rows, a.width
+    code = _lib.FLOAT_CODES[dtype]
+    out = torch.empty(a.shape[:-1] + (n,), device=dev, dtype=dtype)
+    lib = _lib.lib()
+    need = C.c_int64(0)
+    _lib.check(lib.vmf_blocks8_matmul_workspace(m, n, k, code, need), "vmf_blocks8_matmul_workspace")
+    ws = torch.empty(need.value, device=dev, dtype=torch.uint8) if need.value else None
+    av, ae = a._addresses()
+    bv, be = b._addresses()
+    gv, ge = gate._addresses() if gate is not None else (None, None)
+    with _lib.on_device(dev):
+        rc = lib.vmf_blocks8_matmul(av, ae, a.exp_pitch, a.tiled, bv, be, b.exp_pitch, b.tiled, _lib.address(bias),
+                                    _lib.FLOAT_CODES[bias.dtype] if bias is not None else 0, gv, ge,
+                                    gate.exp_pitch if gate is not None else 0, beta, out.data_ptr(), m, n, k,
+                                    _lib.address(ws), need.value, code, _lib.raw_stream(dev))
+    _lib.check(rc, "vmf_blocks8_matmul")
+    return out
+
+
+def _check_bias(bias, n, what):
+    if bias is not None:
+        if tuple(bias.shape) != (n,):
+            raise ValueError(f"{what}: the bias must have shape ({n},), got {tuple(bias.shape)}")
+        _code(bias.dtype, what)
+
+
+def matmul(a, b, bias=None, dtype=torch.float32):
+    """a b^T + bias of two Blocks8 of the same width: (..., k), (n, k) -> (..., n)."""
+    if not isinstance(a, Blocks8) or not isinstance(b, Blocks8):
+        raise TypeError("matmul takes Blocks8 (quantize, or the rows / columns of quantize_weight)")
+    if len(b.shape) != 2 or a.width != b.width:
+        raise ValueError(f"matmul: shapes {tuple(a.shape)} and {tuple(b.shape)}")
+    _code(dtype, "matmul")
+    _check_bias(bias, b.rows, "matmul")
+    dev = _lib.require_hip(a.storage, b.storage, bias)
+    return _matmul(a, b, None if bias is None else bias.detach().contiguous(), None, 1.0, dtype, dev)
+
+
+def softplus_grad(g, q, beta=1.0):
+    """g * (1 - exp(-beta q)), q = quantize(h, "softplus", beta): the gradient with respect to h."""
+    code = _code(g.dtype, "softplus_grad")
+    _, beta = _activation("softplus", beta, "softplus_grad")
+    if g.shape != q.shape or q.tiled:
+        raise ValueError(f"softplus_grad: shapes {tuple(g.shape)} and {tuple(q.shape)}")
+    dev = _lib.require_hip(g, q.storage)
+    rows, stride = _lib.as_rows(g.detach())
+    out = torch.empty(g.shape, device=dev, dtype=g.dtype)
+    v, e = q._addresses()
+    with _lib.on_device(dev):
+        rc = _lib.lib().vmf_blocks8_softplus_grad(rows.data_ptr(), stride, v, e, q.exp_pitch, out.data_ptr(), q.rows,
+                                                  q.width, beta, code, _lib.raw_stream(dev))
+    _lib.check(rc, "vmf_blocks8_softplus_grad")
+    return out
+
+
+def _weight_grad(g, q, bias, dtype, dev):
+    rows, stride = _lib.as_rows(g.detach())
+    m, n = rows.shape
+    k = q.width
+    gw = torch.empty((n, k), device=dev, dtype=dtype)
+    gb = torch.empty(n, device=dev, dtype=dtype) if bias else None
+    lib = _lib.lib()
+    need = C.c_int64(0)
+    _lib.check(lib.vmf_blocks8_weight_grad_workspace(m, n, k, need), "vmf_blocks8_weight_grad_workspace")
+    ws = torch.empty(need.value, device=dev, dtype=torch.uint8) if need.value else None
+    v, e = q._addresses()
+    with _lib.on_device(dev):
+        rc = lib.vmf_blocks8_weight_grad(rows.data_ptr(), stride, v, e, q.exp_pitch, gw.data_ptr(), _lib.address(gb), m,
+                                         n, k, _lib.address(ws), need.value, _lib.FLOAT_CODES[g.dtype],
+                                         _lib.FLOAT_CODES[dtype], _lib.raw_stream(dev))
+    _lib.check(rc, "vmf_blocks8_weight_grad")
+    return gw, gb
+
+
+def weight_grad(g, q, bias=True, dtype=torch.float32):
+    """(g^T q, sum of g's rows) over all leading dimensions: the gradients of a layer's weight and bias from the
+    gradient g (..., n) of its result and its kept input q (..., k); bias=False leaves the second out (None)."""
+    _code(g.dtype, "weight_grad")
+    _width(g, "weight_grad")
+    if dtype not in (torch.float32, g.dtype):
+        raise TypeError(f"weight_grad: results are float32 or the gradient's {g.dtype}, got {dtype}")
+    if q.tiled or g.shape[:-1] != q.shape[:-1]:
+        raise ValueError(f"weight_grad: shapes {tuple(g.shape)} and {tuple(q.shape)}")
+    return _weight_grad(g, q, bias, dtype, _lib.require_hip(g, q.storage))
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, laid_out, bias, act, beta, dev):
+        need_x, need_w, _, need_b = ctx.needs_input_grad[:4]
+        q = _quantize(x, act, beta, _lib.FLOAT_CODES[x.dtype], dev)
+        w8 = laid_out if weight is None else _quantize_weight(weight, need_x, dev)
+        y = _matmul(q, w8.rows, None if bias is None else bias.detach().contiguous(), None, 1.0, x.dtype, dev)
+        # kept for the backward pass: x in 8 bits and, for its own gradient, the weight in 8 bits
+        keep_q = need_w or need_b or (need_x and act)
+        if need_x and w8.columns is None:
+            raise ValueError("linear: the laid-out weight has no columns (quantize_weight(..., transpose=True)), which "
+                             "the gradient of x reads")
+        ctx.save_for_backward(q.storage if keep_q else None, w8.columns.storage if need_x else None)
+        ctx.meta = (x.shape, (w8.columns.shape, w8.columns.offset) if need_x else None, act, beta,
+                    w8.dtype if weight is None else weight.dtype, None if bias is None else bias.dtype, dev)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        q_storage, w_storage = ctx.saved_tensors
+        shape, columns, act, beta, w_dtype, bias_dtype, dev = ctx.meta
+        need_x, need_w, _, need_b = ctx.needs_input_grad[:4]
+        q = Blocks8(q_storage, shape) if q_storage is not None else None
+        gx = gw = gb = None
+        if need_x:
+            gq = _quantize(gy, _lib.ACT_NONE, 1.0, _lib.FLOAT_CODES[gy.dtype], dev)
+            w = Blocks8(w_storage, columns[0], True, columns[1])
+            gx = _matmul(gq, w, None, q if act else None, beta, gy.dtype, dev)
+        if need_w or need_b:
+            gw, gb = _weight_grad(gy, q, need_b, w_dtype if w_dtype in (torch.float32, gy.dtype) else torch.float32, dev)
+            if gb is not None and gb.dtype != bias_dtype:
+                gb = gb.to(bias_dtype)
+            if not need_w:
+                gw = None
+        return gx, gw, None, gb, None, None, None
+
+
+def linear(x, weight, bias=None, activation=None, beta=1.0):
+    """blocks(activation(x)) tiles(weight)^T + bias for x (..., k): (..., n) of x's type.
+
+    weight: a matrix (n, k) of x's type or float32, quantised in the call (training), or a Weight8 that was laid out once
+    (serving; no gradient of its own).  Keeps one byte per element of x for the backward pass."""
+    _width(x, "linear")
+    _code(x.dtype, "linear")
+    act, beta = _activation(activation, beta, "linear")
+    laid_out = weight if isinstance(weight, Weight8) else None
+    if laid_out is None:
+        if weight.dim() != 2 or weight.shape[0] < 1:
+            raise ValueError(f"linear: the weight must be a matrix, got the shape {tuple(weight.shape)}")
+        if weight.dtype not in (torch.float32, x.dtype):
+            raise TypeError(f"linear: the weight of {x.dtype} rows is {x.dtype} or float32, got {weight.dtype}")
+    n, k = weight.shape
+    if k != x.shape[-1]:
+        raise ValueError(f"linear: x of shape {tuple(x.shape)} and a weight of shape {tuple(weight.shape)}")
+    _check_bias(bias, n, "linear")
+    dev = _lib.require_hip(x, weight if laid_out is None else laid_out.rows.storage, bias)
+    tensor = weight if laid_out is None else None
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, tensor, bias)):
+        return _Linear.apply(x, tensor, laid_out, bias, act, beta, dev)
+    q = _quantize(x, act, beta, _lib.FLOAT_CODES[x.dtype], dev)
+    w8 = laid_out if tensor is None else _quantize_weight(tensor, False, dev)
+    return _matmul(q, w8.rows, None if bias is None else bias.detach().contiguous(), None, 1.0, x.dtype, dev)

@@ -1,0 +1,719 @@
+// blocks8_mm.hip -- products of 8-bit blocks.
+//
+//   out[m][n] = sum over block columns of 2^(ea + eb) sum_k a[m][k] b[n][k]  (+ bias[n]) (* softplus slope at gate[m][n])
+//   gweight[n][k] = sum_m gy[m][n] a[m][k],  gbias[n] = sum_m gy[m][n]
+//
+// Both are bound by the matrix instructions for large sizes and by the bytes of the operands for few rows.
+//
+// The 8-bit matrix instruction takes a whole block column (K = 128) and both exponent bytes, so the scales cost no vector
+// work.  Its sums are not quite 32-bit: measured on normal values the result is off by 1.3e-5 relative, for K = 128 as for
+// K = 8192 (the products of one instruction are aligned to the largest of them).  That is a hundredth of a step of a
+// 16-bit result, and it is used for those.  A 32-bit result is computed with the bf16 instruction instead: an element of
+// a block is exact in bf16, so are the products, and the sums are 32-bit (4e-8 at K = 1024).
+#include "blocks8_dev.h"
+
+namespace {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef int v8i_at16 __attribute__((ext_vector_type(8), aligned(16)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+
+#define LDS_PTR(T, p) ((__attribute__((address_space(3))) T*)(p))
+#define GLOBAL_PTR(p) ((__attribute__((address_space(1))) const void*)(p))
+
+struct Operand {
+  const uint8_t* values;
+  const uint8_t* exps;
+  int64_t pitch, exp_pitch;  // bytes
+  int64_t rows;
+  int tiled;  // one exponent per 128 rows
+};
+struct MmArgs {
+  Operand a, b, gate;  // gate.values null: none
+  const void* bias;
+  void* out;
+  float* partial;  // split over the block columns: [split][m][n]
+  int64_t m, n;
+  int blocks, blocks_per_split;
+  int mt, nt;  // tiles
+  int bias_code;
+  float beta;
+};
+
+// F exponent bytes of the rows row0 + F * (lane & 15) + 0..F-1, in one word.  Rows behind the last one get some byte of
+// the array (their products are dropped).
+template <int F>
+__device__ __forceinline__ int load_exps(const Operand& o, int64_t kb, int64_t row0, int lane) {
+  const uint8_t* e = o.exps + kb * o.exp_pitch;
+  if (o.tiled) {
+    int64_t r = row0 >> 7;
+    r = r < o.exp_pitch ? r : o.exp_pitch - 1;
+    return (int)e[r] * 0x01010101;
+  }
+  int64_t r = row0 + F * (lane & 15);
+  const int64_t last = o.exp_pitch - F;
+  r = r < last ? r : last;
+  if constexpr (F == 4) return *reinterpret_cast<const int*>(e + r);
+  if constexpr (F == 2) return *reinterpret_cast<const uint16_t*>(e + r);
+  return e[r];
+}
+
+// acc += A B for one block column of a 16 x 16 tile; IA, IB: which byte of the exponent words
+template <int IA, int IB>
+__device__ __forceinline__ v4f mm_step(v8i a, v8i b, v4f acc, int ea, int eb) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 0, 0, IA, ea, IB, eb);
+}
+// the 32 values of a lane as four bf16 operands, scaled (exact: 4 bits times a power of two)
+__device__ __forceinline__ void to_bf16(v8i v, float scale, v8b* out) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const v2b lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * q + h], scale, false);
+      const v2b hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * q + h], scale, true);
+      out[q][4 * h] = lo[0];
+      out[q][4 * h + 1] = lo[1];
+      out[q][4 * h + 2] = hi[0];
+      out[q][4 * h + 3] = hi[1];
+    }
+}
+__device__ __forceinline__ v4f mm_step_bf16(const v8b* a, const v8b* b, v4f acc) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[q], b[q], acc, 0, 0, 0);
+  return acc;
+}
+
+__device__ __forceinline__ float load_bias(const void* bias, int code, int64_t i) {
+  return code == VMF_F32 ? ((const float*)bias)[i]
+                         : code == VMF_F16 ? (float)((const f16_t*)bias)[i] : (float)((const bf16_t*)bias)[i];
+}
+
+// bias, gate and rounding of NC consecutive columns of one row
+template <int NC, typename OUT>
+__device__ __forceinline__ void finish(const MmArgs& p, int64_t row, int64_t col, const float* bias, float* v) {
+#pragma unroll
+  for (int j = 0; j < NC; ++j) v[j] += bias[j];
+  if (p.gate.values) {
+    const uint8_t* q = p.gate.values + row * p.gate.pitch + col;
+    const float scale = b8_scale(p.gate.exps[(col >> 7) * p.gate.exp_pitch + row]);
+    float a[4];
+    if constexpr (NC == 4) {
+      b8_unpack4(*reinterpret_cast<const uint32_t*>(q), scale, a);
+    } else {
+      uint32_t w = 0;
+#pragma unroll
+      for (int j = 0; j < NC; ++j) w |= (uint32_t)q[j] << (8 * j);
+      b8_unpack4(w, scale, a);
+    }
+#pragma unroll
+    for (int j = 0; j < NC; ++j) v[j] *= b8_softplus_slope(a[j], p.beta);
+  }
+  store_some<NC>((OUT*)p.out + row * p.n + col, p.n - col, v);
+}
+
+// Tile of BM x BN over the block columns, waves of WM x WN side by side.
+//   LDS: two stages of the tile's rows of 128 bytes, filled by loads that go from global memory straight into LDS; while
+//   one stage is multiplied the next is on its way, one barrier per block column.
+//   A 16-row operand tile takes the rows F * (lane & 15) + i (i = 0 .. F - 1 the tile's number): the exponents of a
+//   lane's F tiles are then one word, and a lane's results are F consecutive columns of a row.
+//   The 16-byte pieces of a row lie at piece ^ (row / F) & 7, so that the eight lanes that are served together read from
+//   all banks.
+template <int BM, int BN, int WM, int WN, bool WIDE, typename OUT>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p) {
+  constexpr int WAVES_N = BN / WN, WAVES = (BM / WM) * WAVES_N;
+  constexpr int FM = WM / 16 < 4 ? WM / 16 : 4, FN = WN / 16 < 4 ? WN / 16 : 4;  // tiles that share an exponent word
+  constexpr int GM = WM / (16 * FM), GN = WN / (16 * FN);
+  constexpr int STAGE = (BM + BN) * B8;
+  constexpr int LOADS = (BM + BN) / 8 / WAVES;  // one fills eight rows
+  static_assert((BM + BN) % (8 * WAVES) == 0, "every wave loads the same number of rows");
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Workgroup b runs on XCD b % 8: give each XCD a contiguous run of tiles, and walk the run in columns of 8 row tiles, so
+  // that the rows and columns in use at a time fit its L2.
+  const int tiles = p.mt * p.nt;
+  int id = (int)blockIdx.x;
+  {
+    const int q = tiles >> 3, r = tiles & 7, x = id & 7;
+    id = x * q + (x < r ? x : r) + (id >> 3);
+  }
+  const int group = id / (8 * p.nt), first = group * 8, high = p.mt - first < 8 ? p.mt - first : 8;
+  const int in_group = id - group * 8 * p.nt;
+  const int64_t m0 = (int64_t)(first + in_group % high) * BM, n0 = (int64_t)(in_group / high) * BN;
+  const int kb0 = (int)blockIdx.y * p.blocks_per_split;
+  const int kb1 = kb0 + p.blocks_per_split < p.blocks ? kb0 + p.blocks_per_split : p.blocks;
+
+  // where this lane's loads read: row (clamped to the last one) and 16-byte piece
+  const uint8_t* src[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int r8 = wave * LOADS + i;  // eight rows of the stage: first A's, then B's
+    const bool is_b = r8 >= BM / 8;
+    const int r = (is_b ? r8 - BM / 8 : r8) * 8 + (lane >> 3);
+    const int piece = (lane & 7) ^ ((is_b ? r / FN : r / FM) & 7);
+    const Operand& o = is_b ? p.b : p.a;
+    int64_t row = (is_b ? n0 : m0) + r;
+    row = row < o.rows ? row : o.rows - 1;
+    src[i] = o.values + row * o.pitch + piece * 16;
+  }
+  const int wm = (wave / WAVES_N) * WM, wn = (wave % WAVES_N) * WN;
+
+  v4f acc[GM * FM][GN * FN];
+#pragma unroll
+  for (int i = 0; i < GM * FM; ++i)
+#pragma unroll
+    for (int j = 0; j < GN * FN; ++j) acc[i][j] = v4f{0, 0, 0, 0};
+
+  int ea[2][GM], eb[2][GN];
+  auto fetch = [&](int kb, int stage) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+      __builtin_amdgcn_global_load_lds(GLOBAL_PTR(src[i] + (int64_t)kb * B8),
+                                       LDS_PTR(void, lds + stage * STAGE + (wave * LOADS + i) * 1024), 16, 0, 0);
+  };
+  auto fetch_exps = [&](int kb, int slot) {
+#pragma unroll
+    for (int g = 0; g < GM; ++g) ea[slot][g] = load_exps<FM>(p.a, kb, m0 + wm + g * 16 * FM, lane);
+#pragma unroll
+    for (int g = 0; g < GN; ++g) eb[slot][g] = load_exps<FN>(p.b, kb, n0 + wn + g * 16 * FN, lane);
+  };
+  auto operand = [&](const uint8_t* rows, int row, int f) -> v8i {
+    const int s = (row / f) & 7, c = (lane >> 4) * 2;
+    const v4i lo = *reinterpret_cast<const v4i*>(rows + row * B8 + ((c ^ s) << 4));
+    const v4i hi = *reinterpret_cast<const v4i*>(rows + row * B8 + (((c + 1) ^ s) << 4));
+    return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  };
+  auto multiply = [&](int stage, const int* xa, const int* xb) {
+    const uint8_t* A = lds + stage * STAGE;
+    const uint8_t* B = A + BM * B8;
+#pragma unroll
+    for (int g = 0; g < GM; ++g) {
+      if constexpr (!WIDE) {
+        v8i a[FM];
+#pragma unroll
+        for (int i = 0; i < FM; ++i) a[i] = operand(A, wm + g * 16 * FM + FM * (lane & 15) + i, FM);
+#pragma unroll
+        for (int h = 0; h < GN; ++h)
+          static_for<FN>([&](auto J) {
+            constexpr int j = decltype(J)::value;
+            const v8i b = operand(B, wn + h * 16 * FN + FN * (lane & 15) + j, FN);
+            static_for<FM>([&](auto I) {
+              constexpr int i = decltype(I)::value;
+              v4f& c = acc[g * FM + i][h * FN + j];
+              c = mm_step<i, j>(a[i], b, c, xa[g], xb[h]);
+            });
+          });
+      } else {
+        v8b a[FM][4], b[4];
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+          to_bf16(operand(A, wm + g * 16 * FM + FM * (lane & 15) + i, FM), b8_scale((xa[g] >> (8 * i)) & 0xff), a[i]);
+#pragma unroll
+        for (int h = 0; h < GN; ++h)
+#pragma unroll
+          for (int j = 0; j < FN; ++j) {
+            to_bf16(operand(B, wn + h * 16 * FN + FN * (lane & 15) + j, FN), b8_scale((xb[h] >> (8 * j)) & 0xff), b);
+#pragma unroll
+            for (int i = 0; i < FM; ++i) acc[g * FM + i][h * FN + j] = mm_step_bf16(a[i], b, acc[g * FM + i][h * FN + j]);
+          }
+      }
+    }
+  };
+
+  if (kb0 < kb1) {
+    fetch(kb0, 0);
+    fetch_exps(kb0, 0);
+  }
+  for (int kb = kb0; kb < kb1; kb += 2) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (kb + half < kb1) {
+        // this wave's share of the stage has arrived; after the barrier everyone's has, and the other stage is free
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (kb + half + 1 < kb1) {
+          fetch(kb + half + 1, half ^ 1);
+          fetch_exps(kb + half + 1, half ^ 1);
+        }
+        multiply(half, ea[half], eb[half]);
+      }
+    }
+  }
+
+  // lane: rows FM * (4 * (lane / 16) + r) + i, columns FN * (lane % 16) + 0 .. FN - 1 of each group
+#pragma unroll
+  for (int h = 0; h < GN; ++h) {
+    const int64_t col = n0 + wn + h * 16 * FN + FN * (lane & 15);
+    if (col >= p.n) continue;
+    float bias[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) bias[j] = p.bias && !p.partial && col + j < p.n ? load_bias(p.bias, p.bias_code, col + j) : 0.0f;
+#pragma unroll
+    for (int g = 0; g < GM; ++g)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+          const int64_t row = m0 + wm + g * 16 * FM + FM * (4 * (lane >> 4) + r) + i;
+          if (row >= p.m) continue;
+          float v[FN];
+#pragma unroll
+          for (int j = 0; j < FN; ++j) v[j] = acc[g * FM + i][h * FN + j][r];
+          if (p.partial)
+            store_some<FN>(p.partial + ((int64_t)blockIdx.y * p.m + row) * p.n + col, p.n - col, v);
+          else
+            finish<FN, OUT>(p, row, col, bias, v);
+        }
+  }
+}
+
+// Up to 16 rows: the weight's bytes are what there is to move.  A workgroup takes 16 columns, its eight waves share the
+// block columns and read both operands straight into registers; their sums are added through LDS.
+template <bool WIDE, typename OUT>
+__global__ __launch_bounds__(512) void mm_few_kernel(MmArgs p) {
+  __shared__ float sums[8][16][17];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int kb0 = (int)blockIdx.y * p.blocks_per_split;
+  const int kb1 = kb0 + p.blocks_per_split < p.blocks ? kb0 + p.blocks_per_split : p.blocks;
+  const int64_t ra = (lane & 15) < p.m ? (lane & 15) : p.m - 1;
+  const int64_t rb = n0 + (lane & 15) < p.n ? n0 + (lane & 15) : p.n - 1;
+  const uint8_t* A = p.a.values + ra * p.a.pitch + (lane >> 4) * 32;
+  const uint8_t* B = p.b.values + rb * p.b.pitch + (lane >> 4) * 32;
+  const uint8_t* ea = p.a.exps + (p.a.tiled ? ra >> 7 : ra);
+  const uint8_t* eb = p.b.exps + (p.b.tiled ? rb >> 7 : rb);
+  v4f acc = {0, 0, 0, 0};
+  for (int kb = kb0 + wave; kb < kb1; kb += 8) {
+    const v8i a = *reinterpret_cast<const v8i_at16*>(A + (int64_t)kb * B8);
+    const v8i b = *reinterpret_cast<const v8i_at16*>(B + (int64_t)kb * B8);
+    const int xa = ea[(int64_t)kb * p.a.exp_pitch], xb = eb[(int64_t)kb * p.b.exp_pitch];
+    if constexpr (!WIDE) {
+      acc = mm_step<0, 0>(a, b, acc, xa, xb);
+    } else {
+      v8b aw[4], bw[4];
+      to_bf16(a, b8_scale(xa), aw);
+      to_bf16(b, b8_scale(xb), bw);
+      acc = mm_step_bf16(aw, bw, acc);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) sums[wave][4 * (lane >> 4) + r][lane & 15] = acc[r];
+  __syncthreads();
+  if (threadIdx.x >= 256) return;
+  const int64_t row = threadIdx.x >> 4, col = n0 + (threadIdx.x & 15);
+  if (row >= p.m || col >= p.n) return;
+  float v = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) v += sums[w][threadIdx.x >> 4][threadIdx.x & 15];
+  if (p.partial) {
+    p.partial[((int64_t)blockIdx.y * p.m + row) * p.n + col] = v;
+  } else {
+    const float bias = p.bias ? load_bias(p.bias, p.bias_code, col) : 0.0f;
+    finish<1, OUT>(p, row, col, &bias, &v);
+  }
+}
+
+// the splits' sums in their order, then what the tile would have done
+template <typename OUT>
+__global__ __launch_bounds__(256) void mm_join_kernel(MmArgs p, int splits) {
+  const int64_t total = p.m * p.n;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    float v = 0;
+    for (int s = 0; s < splits; ++s) v += p.partial[s * total + i];
+    const int64_t row = i / p.n, col = i - row * p.n;
+    const float bias = p.bias ? load_bias(p.bias, p.bias_code, col) : 0.0f;
+    finish<1, OUT>(p, row, col, &bias, &v);
+  }
+}
+
+enum MmKind { MM_FEW, MM_64, MM_128, MM_256 };
+struct MmPlan {
+  MmKind kind;
+  int splits, per_split, mt, nt;
+};
+// The largest tile that still gives every compute unit (256) a workgroup; where even the smallest does not, the block
+// columns are split, at least four of them to a split.
+MmPlan mm_plan(int64_t m, int64_t n, int64_t blocks, bool wide) {
+  MmPlan p;
+  auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
+  int64_t groups;
+  if (m <= 16) {
+    p.kind = MM_FEW;
+    p.mt = 1;
+    p.nt = (int)((n + 15) / 16);
+    groups = p.nt;
+  } else {
+    const int t = !wide && tiles(256) >= 256 ? 256 : tiles(128) >= 256 ? 128 : 64;
+    p.kind = t == 256 ? MM_256 : t == 128 ? MM_128 : MM_64;
+    p.mt = (int)((m + t - 1) / t);
+    p.nt = (int)((n + t - 1) / t);
+    groups = (int64_t)p.mt * p.nt;
+  }
+  const int64_t least = p.kind == MM_FEW ? 16 : 4;
+  int64_t s = (256 + groups - 1) / groups;
+  if (s > blocks / least) s = blocks / least;
+  if (s < 1) s = 1;
+  p.per_split = (int)((blocks + s - 1) / s);
+  p.splits = (int)((blocks + p.per_split - 1) / p.per_split);
+  return p;
+}
+
+template <bool WIDE, typename OUT>
+void mm_launch(const MmPlan& pl, const MmArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)(pl.mt * pl.nt), (unsigned)pl.splits);
+  if (pl.kind == MM_FEW) mm_few_kernel<WIDE, OUT><<<grid, 512, 0, st>>>(a);
+  else if (pl.kind == MM_64) mm_kernel<64, 64, 32, 32, WIDE, OUT><<<grid, 256, 0, st>>>(a);
+  else if (pl.kind == MM_128) mm_kernel<128, 128, 64, 64, WIDE, OUT><<<grid, 256, 0, st>>>(a);
+  else if constexpr (!WIDE) mm_kernel<256, 256, 128, 64, false, OUT><<<grid, 512, 0, st>>>(a);
+  if (a.partial) mm_join_kernel<OUT><<<vmf_grid_for(a.m * a.n, 256, 1 << 14), 256, 0, st>>>(a, pl.splits);
+}
+
+// ---- weight gradient ---------------------------------------------------------------------------------------------
+
+// A value of gy as bf16 terms whose sum is the value: 8 bits each, so 1 term for bf16, 2 for fp16 (11 bits), 3 for fp32.
+// Cut off, not rounded: no term overflows.  NaN and infinity stay in the first term.
+template <typename T> struct Terms;
+template <> struct Terms<bf16_t> { static constexpr int count = 1; };
+template <> struct Terms<f16_t> { static constexpr int count = 2; };
+template <> struct Terms<float> { static constexpr int count = 3; };
+__device__ __forceinline__ uint32_t cut(float& v) {  // the upper 16 bits; v becomes the rest
+  uint32_t u = __float_as_uint(v) & 0xffff0000u;
+  if (!(fabsf(v) < __builtin_inff())) {
+    if (v != v) u = 0x7fc00000u;
+    v = 0;
+  } else {
+    v -= __uint_as_float(u);
+  }
+  return u >> 16;
+}
+
+struct WgArgs {
+  const void* gy;
+  int64_t gy_stride;
+  Operand a;
+  void* gw;
+  void* gb;
+  float* partial;       // [split][n][k] then [split][n]; null with one split
+  int64_t m, n, k;
+  int64_t rows_per_split;
+  int nt, kt;
+};
+
+// Tile of 128 (n) x 128 (k, one block column), 32 rows of the batch at a time: gy's terms and a's values as bf16 rows in
+// LDS, read back transposed (the rows are the products' inner dimension).  Two stages, one barrier per 32 rows; the next
+// rows are loaded into registers while these are multiplied.
+constexpr int WG_ROWS = 32;
+constexpr int WG_PITCH = 2 * B8 + 32;  // bytes; 32 more than the row, so that the rows of a transposed read start 8 banks apart
+
+template <typename T, typename W>
+__global__ __launch_bounds__(256) void wgrad_kernel(WgArgs p) {
+  constexpr int NT = Terms<T>::count;
+  constexpr int PLANE = WG_ROWS * WG_PITCH;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * (NT + 1) * PLANE];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int nt = (int)blockIdx.x / p.kt, kt = (int)blockIdx.x % p.kt;
+  const int64_t n0 = (int64_t)nt * B8;
+  const int64_t m0 = (int64_t)blockIdx.y * p.rows_per_split;
+  const int64_t m1 = m0 + p.rows_per_split < p.m ? m0 + p.rows_per_split : p.m;
+  const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 16;  // this thread's row of the 32 and its 16 columns
+  const T* gsrc = (const T*)p.gy + n0 + c;
+  const uint8_t* asrc = p.a.values + (int64_t)kt * B8 + c;
+  const uint8_t* esrc = p.a.exps + (int64_t)kt * p.a.exp_pitch;
+  const int64_t left = p.n - n0 - c;
+
+  float g[16];
+  v4i av;
+  uint32_t ae;
+  float gsum[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) gsum[i] = 0;
+  auto fetch = [&](int64_t m) {
+    const int64_t row = m + r;
+    const bool in = row < m1;
+    load_some<8>(gsrc + row * p.gy_stride, in ? left : 0, 0.0f, g);
+    load_some<8>(gsrc + row * p.gy_stride + 8, in ? left - 8 : 0, 0.0f, g + 8);
+    av = v4i{0, 0, 0, 0};
+    ae = 127;
+    if (in) {
+      av = *reinterpret_cast<const v4i*>(asrc + row * p.a.pitch);
+      ae = esrc[row];
+    }
+  };
+  auto put = [&](int stage) {
+    uint8_t* base = lds + stage * (NT + 1) * PLANE + r * WG_PITCH + c * 2;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) gsum[i] += g[i];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t lo = cut(g[2 * i]), hi = cut(g[2 * i + 1]);
+        w[i] = lo | hi << 16;
+      }
+      uint4* d = reinterpret_cast<uint4*>(base + t * PLANE);
+      d[0] = uint4{w[0], w[1], w[2], w[3]};
+      d[1] = uint4{w[4], w[5], w[6], w[7]};
+    }
+    const float scale = b8_scale(ae);
+    v2b* d = reinterpret_cast<v2b*>(base + NT * PLANE);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      d[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(av[i], scale, false);
+      d[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(av[i], scale, true);
+    }
+  };
+  // 32 columns from `col` of the 16 rows from `row` of a plane, as the operand of a 32 x 32 x 16 product: lane l gets
+  // column l % 32, rows 8 * (l / 32) .. + 7
+  auto transposed = [&](const uint8_t* plane, int row, int col) -> v8b {
+    const int q = lane & 15, grp = lane >> 4;
+    const uint8_t* s = plane + (row + (grp >> 1) * 8 + (q >> 2)) * WG_PITCH + (col + (grp & 1) * 16 + (q & 3) * 4) * 2;
+    union {
+      v4s h[2];
+      v8b v;
+    } u;
+    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(v4s, s));
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(v4s, s + 4 * WG_PITCH));
+    return u.v;
+  };
+  const int wn = (wave >> 1) * 64, wk = (wave & 1) * 64;
+  v16f acc[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+
+  int stage = 0;
+  if (m0 < m1) fetch(m0);
+  for (int64_t m = m0; m < m1; m += WG_ROWS) {
+    put(stage);
+    if (m + WG_ROWS < m1) fetch(m + WG_ROWS);
+    // one barrier is enough: the stage written next was read before the previous barrier
+    __syncthreads();
+    const uint8_t* base = lds + stage * (NT + 1) * PLANE;
+#pragma unroll
+    for (int s = 0; s < WG_ROWS; s += 16) {
+      const v8b b0 = transposed(base + NT * PLANE, s, wk), b1 = transposed(base + NT * PLANE, s, wk + 32);
+#pragma unroll
+      for (int t = NT - 1; t >= 0; --t) {
+        const v8b a0 = transposed(base + t * PLANE, s, wn), a1 = transposed(base + t * PLANE, s, wn + 32);
+        acc[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0, b0, acc[0][0], 0, 0, 0);
+        acc[0][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0, b1, acc[0][1], 0, 0, 0);
+        acc[1][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1, b0, acc[1][0], 0, 0, 0);
+        acc[1][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1, b1, acc[1][1], 0, 0, 0);
+      }
+    }
+    stage ^= 1;
+  }
+
+  // D: column (k) lane % 32, rows (n) (e & 3) + 8 (e >> 2) + 4 (lane / 32)
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int64_t k = (int64_t)kt * B8 + wk + j * 32 + (lane & 31);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int64_t n = n0 + wn + i * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
+        if (n < p.n && k < p.k) {
+          if (p.partial) p.partial[((int64_t)blockIdx.y * p.n + n) * p.k + k] = acc[i][j][e];
+          else ((W*)p.gw)[n * p.k + k] = (W)acc[i][j][e];
+        }
+      }
+    }
+  // gbias: the first block column's workgroups add what they read of gy over the 32 rows, two halves of the columns in turn
+  if (!p.gb || kt != 0) return;
+  float* red = reinterpret_cast<float*>(lds);  // 32 x 64 floats = 8 KiB
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    __syncthreads();
+    if ((c >> 6) == half)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) red[r * 64 + (c & 63) + i] = gsum[i];
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      float s = 0;
+      for (int q = 0; q < WG_ROWS; ++q) s += red[q * 64 + threadIdx.x];
+      const int64_t n = n0 + half * 64 + threadIdx.x;
+      if (n < p.n) {
+        if (p.partial) p.partial[(int64_t)gridDim.y * p.n * p.k + (int64_t)blockIdx.y * p.n + n] = s;
+        else ((W*)p.gb)[n] = (W)s;
+      }
+    }
+  }
+}
+
+template <typename W>
+__global__ __launch_bounds__(256) void wgrad_join_kernel(const float* __restrict__ partial, W* __restrict__ gw,
+                                                         W* __restrict__ gb, int splits, int64_t nk, int64_t n) {
+  const int64_t total = nk + (gb ? n : 0);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const float* src = i < nk ? partial + i : partial + splits * nk + (i - nk);
+    const int64_t step = i < nk ? nk : n;
+    float s = 0;
+    for (int q = 0; q < splits; ++q) s += src[q * step];
+    if (i < nk) gw[i] = (W)s;
+    else gb[i - nk] = (W)s;
+  }
+}
+
+struct WgPlan {
+  int splits, nt, kt;
+  int64_t per_split;
+};
+// three workgroups per compute unit where the batch allows it, at least 256 rows to a split
+WgPlan wg_plan(int64_t m, int64_t n, int64_t k) {
+  WgPlan p;
+  p.nt = (int)((n + B8 - 1) / B8);
+  p.kt = (int)b8_blocks(k);
+  const int64_t tiles = (int64_t)p.nt * p.kt;
+  int64_t s = (768 + tiles - 1) / tiles;
+  if (s > m / 256) s = m / 256;
+  if (s < 1) s = 1;
+  p.per_split = ((m + s - 1) / s + WG_ROWS - 1) / WG_ROWS * WG_ROWS;
+  p.splits = p.per_split > 0 ? (int)((m + p.per_split - 1) / p.per_split) : 1;
+  if (p.splits < 1) p.splits = 1;
+  return p;
+}
+
+int check_operand(const char* what, const char* name, const uint8_t* values, const uint8_t* exps, int64_t exp_pitch,
+                  int tiled, int64_t rows) {
+  VMF_REQUIRE(values && exps, VMF_ERR_BAD_ARG, "%s: %s is null", what, name);
+  VMF_REQUIRE(((uintptr_t)values & 15) == 0 && (tiled || ((uintptr_t)exps & 3) == 0), VMF_ERR_BAD_ARG,
+              "%s: %s is not aligned", what, name);
+  VMF_REQUIRE(tiled ? exp_pitch >= b8_blocks(rows) : exp_pitch >= rows && exp_pitch % 16 == 0, VMF_ERR_BAD_ARG,
+              "%s: exponent pitch %lld of %s", what, (long long)exp_pitch, name);
+  return VMF_OK;
+}
+
+}  // namespace
+
+extern "C" int vmf_blocks8_matmul_workspace(int64_t m, int64_t n, int64_t k, int out_dtype, int64_t* bytes_out) {
+  int rc = b8_check_shape("vmf_blocks8_matmul_workspace", m, k);
+  if (rc != VMF_OK) return rc;
+  rc = b8_check_shape("vmf_blocks8_matmul_workspace", n, k);
+  if (rc != VMF_OK) return rc;
+  VMF_REQUIRE(bytes_out, VMF_ERR_BAD_ARG, "vmf_blocks8_matmul_workspace: null pointer");
+  *bytes_out = 0;
+  if (m == 0 || n == 0) return VMF_OK;
+  const MmPlan pl = mm_plan(m, n, b8_blocks(k), out_dtype == VMF_F32);
+  if (pl.splits > 1) *bytes_out = (int64_t)pl.splits * m * n * 4;
+  return VMF_OK;
+}
+
+extern "C" int vmf_blocks8_matmul(const uint8_t* a, const uint8_t* a_exponents, int64_t a_exp_pitch, int a_tiled,
+                                  const uint8_t* b, const uint8_t* b_exponents, int64_t b_exp_pitch, int b_tiled,
+                                  const void* bias, int bias_dtype, const uint8_t* gate,
+                                  const uint8_t* gate_exponents, int64_t gate_exp_pitch, double beta, void* out,
+                                  int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes,
+                                  int out_dtype, vmf_stream_t stream) {
+  VMF_RANGE("vmf_blocks8_matmul");
+  const char* what = "vmf_blocks8_matmul";
+  int64_t need = 0;
+  int rc = vmf_blocks8_matmul_workspace(m, n, k, out_dtype, &need);
+  if (rc != VMF_OK) return rc;
+  VMF_REQUIRE(out_dtype == VMF_F32 || out_dtype == VMF_F16 || out_dtype == VMF_BF16, VMF_ERR_DTYPE,
+              "%s: out dtype %d is not VMF_F32/VMF_F16/VMF_BF16", what, out_dtype);
+  VMF_REQUIRE(!bias || bias_dtype == VMF_F32 || bias_dtype == VMF_F16 || bias_dtype == VMF_BF16, VMF_ERR_DTYPE,
+              "%s: bias dtype %d", what, bias_dtype);
+  if (m == 0 || n == 0) return VMF_OK;
+  if ((rc = check_operand(what, "a", a, a_exponents, a_exp_pitch, a_tiled, m)) != VMF_OK) return rc;
+  if ((rc = check_operand(what, "b", b, b_exponents, b_exp_pitch, b_tiled, n)) != VMF_OK) return rc;
+  if (gate) {
+    if ((rc = check_operand(what, "gate", gate, gate_exponents, gate_exp_pitch, 0, m)) != VMF_OK) return rc;
+    VMF_REQUIRE(n <= VMF_BLOCKS8_MAX_WIDTH, VMF_ERR_UNSUPPORTED, "%s: n", what);
+    VMF_REQUIRE(beta > 0 && beta <= 1e30 && beta >= 1e-30, VMF_ERR_BAD_ARG, "%s: beta %g", what, beta);
+  }
+  VMF_REQUIRE(out, VMF_ERR_BAD_ARG, "%s: null pointer", what);
+  VMF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), VMF_ERR_BAD_ARG,
+              "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)need);
+  const int64_t blocks = b8_blocks(k);
+  const MmPlan pl = mm_plan(m, n, blocks, out_dtype == VMF_F32);
+  VMF_REQUIRE((int64_t)pl.mt * pl.nt <= 0x7fffffff, VMF_ERR_UNSUPPORTED, "%s: %lld x %lld results", what, (long long)m,
+              (long long)n);
+  MmArgs p;
+  p.a = Operand{a, a_exponents, blocks * B8, a_exp_pitch, m, a_tiled};
+  p.b = Operand{b, b_exponents, blocks * B8, b_exp_pitch, n, b_tiled};
+  p.gate = Operand{gate, gate_exponents, b8_blocks(n) * B8, gate_exp_pitch, m, 0};
+  p.bias = bias;
+  p.bias_code = bias_dtype;
+  p.out = out;
+  p.partial = need ? (float*)workspace : nullptr;
+  p.m = m;
+  p.n = n;
+  p.blocks = (int)blocks;
+  p.blocks_per_split = pl.per_split;
+  p.mt = pl.mt;
+  p.nt = pl.nt;
+  p.beta = (float)beta;
+  hipStream_t st = (hipStream_t)stream;
+  if (out_dtype == VMF_F32) mm_launch<true, float>(pl, p, st);
+  else if (out_dtype == VMF_F16) mm_launch<false, f16_t>(pl, p, st);
+  else mm_launch<false, bf16_t>(pl, p, st);
+  return vmf_check_launch(what);
+}
+
+extern "C" int vmf_blocks8_weight_grad_workspace(int64_t m, int64_t n, int64_t k, int64_t* bytes_out) {
+  int rc = b8_check_shape("vmf_blocks8_weight_grad_workspace", m, k);
+  if (rc != VMF_OK) return rc;
+  VMF_REQUIRE(bytes_out && n >= 0 && n <= VMF_BLOCKS8_MAX_WIDTH, VMF_ERR_BAD_ARG,
+              "vmf_blocks8_weight_grad_workspace: n = %lld or a null pointer", (long long)n);
+  *bytes_out = 0;
+  if (n == 0) return VMF_OK;
+  const WgPlan pl = wg_plan(m, n, k);
+  if (pl.splits > 1) *bytes_out = (int64_t)pl.splits * n * (k + 1) * 4;
+  return VMF_OK;
+}
+
+extern "C" int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const uint8_t* a, const uint8_t* a_exponents,
+                                       int64_t a_exp_pitch, void* gweight, void* gbias, int64_t m, int64_t n,
+                                       int64_t k, void* workspace, int64_t workspace_bytes, int dtype, int out_dtype,
+                                       vmf_stream_t stream) {
+  VMF_RANGE("vmf_blocks8_weight_grad");
+  const char* what = "vmf_blocks8_weight_grad";
+  int64_t need = 0;
+  int rc = vmf_blocks8_weight_grad_workspace(m, n, k, &need);
+  if (rc != VMF_OK) return rc;
+  VMF_REQUIRE(out_dtype == VMF_F32 || out_dtype == dtype, VMF_ERR_DTYPE, "%s: out dtype %d", what, out_dtype);
+  VMF_REQUIRE(gy_stride >= 0, VMF_ERR_BAD_ARG, "%s: negative row stride", what);
+  if (n == 0) return VMF_OK;
+  VMF_REQUIRE(gweight && (m == 0 || gy), VMF_ERR_BAD_ARG, "%s: null pointer", what);
+  if (m > 0 && (rc = check_operand(what, "a", a, a_exponents, a_exp_pitch, 0, m)) != VMF_OK) return rc;
+  VMF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), VMF_ERR_BAD_ARG,
+              "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)need);
+  const WgPlan pl = wg_plan(m, n, k);
+  VMF_REQUIRE((int64_t)pl.nt * pl.kt <= 0x7fffffff, VMF_ERR_UNSUPPORTED, "%s: %lld x %lld results", what, (long long)n,
+              (long long)k);
+  WgArgs p;
+  p.gy = gy;
+  p.gy_stride = gy_stride;
+  p.a = Operand{a, a_exponents, b8_blocks(k) * B8, a_exp_pitch, m, 0};
+  p.gw = gweight;
+  p.gb = gbias;
+  p.partial = need ? (float*)workspace : nullptr;
+  p.m = m;
+  p.n = n;
+  p.k = k;
+  p.rows_per_split = pl.per_split;
+  p.nt = pl.nt;
+  p.kt = pl.kt;
+  const dim3 grid((unsigned)(pl.nt * pl.kt), (unsigned)pl.splits);
+  hipStream_t st = (hipStream_t)stream;
+  LOWP_DISPATCH(dtype, "vmf_blocks8_weight_grad", T, {
+    if (out_dtype == VMF_F32) wgrad_kernel<T, float><<<grid, 256, 0, st>>>(p);
+    else wgrad_kernel<T, T><<<grid, 256, 0, st>>>(p);
+  });
+  rc = vmf_check_launch(what);
+  if (rc != VMF_OK || !need) return rc;
+  LOWP_DISPATCH(out_dtype, "vmf_blocks8_weight_grad", W,
+                (wgrad_join_kernel<W><<<vmf_grid_for(n * (k + 1), 256, 1 << 13), 256, 0, st>>>(
+                    p.partial, (W*)gweight, (W*)gbias, pl.splits, n * k, n)));
+  return vmf_check_launch(what);
+}

@@ -1,0 +1,89 @@
+"""8-bit blocks: what is refused and how results are laid out, without a GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+from medicalimageanalysis_amd import _lib, blocks8
+
+
+def blocks(rows, width, tiled=False):
+    return blocks8.Blocks8(torch.zeros(blocks8.Blocks8.bytes_for(rows, width, tiled), dtype=torch.uint8), (rows, width), tiled)
+
+
+@pytest.mark.parametrize("call,error,match", [
+    (lambda: blocks8.quantize(torch.zeros(())), ValueError, "last dimension"),
+    (lambda: blocks8.quantize(torch.zeros(3, 0)), ValueError, "last dimension"),
+    (lambda: blocks8.quantize(torch.zeros(3, 4, dtype=torch.float64)), TypeError, "float32, float16 or bfloat16"),
+    (lambda: blocks8.quantize(torch.zeros(3, 4), "relu"), ValueError, "activation"),
+    (lambda: blocks8.quantize(torch.zeros(3, 4), "softplus", 0.0), ValueError, "beta"),
+    (lambda: blocks8.quantize(torch.zeros(3, 4), "softplus", float("nan")), ValueError, "beta"),
+    (lambda: blocks8.quantize(torch.zeros(3, 4)), RuntimeError, "HIP device"),
+    (lambda: blocks8.quantize_weight(torch.zeros(4)), ValueError, "matrix"),
+    (lambda: blocks8.quantize_weight(torch.zeros(0, 4)), ValueError, "matrix"),
+    (lambda: blocks8.matmul(torch.zeros(2, 3), blocks(2, 3)), TypeError, "Blocks8"),
+    (lambda: blocks8.matmul(blocks(2, 3), blocks(2, 4)), ValueError, "shapes"),
+    (lambda: blocks8.matmul(blocks(2, 3), blocks(5, 3), torch.zeros(4)), ValueError, r"shape \(5,\)"),
+    (lambda: blocks8.matmul(blocks(2, 3), blocks(5, 3), dtype=torch.float64), TypeError, "float64"),
+    (lambda: blocks8.softplus_grad(torch.zeros(2, 4), blocks(2, 3)), ValueError, "shapes"),
+    (lambda: blocks8.softplus_grad(torch.zeros(2, 3), blocks(2, 3, True)), ValueError, "shapes"),
+    (lambda: blocks8.weight_grad(torch.zeros(3, 5), blocks(2, 3)), ValueError, "shapes"),
+    (lambda: blocks8.weight_grad(torch.zeros(2, 5), blocks(2, 3), dtype=torch.bfloat16), TypeError, "results"),
+    (lambda: blocks8.linear(torch.zeros(2, 3), torch.zeros(5, 4)), ValueError, "weight of shape"),
+    (lambda: blocks8.linear(torch.zeros(2, 3), torch.zeros(3)), ValueError, "matrix"),
+    (lambda: blocks8.linear(torch.zeros(2, 3), torch.zeros(5, 3, dtype=torch.float16)), TypeError, "float16"),
+    (lambda: blocks8.linear(torch.zeros(2, 3, dtype=torch.float64), torch.zeros(5, 3)), TypeError, "float64"),
+    (lambda: blocks8.linear(torch.zeros(2, 3), torch.zeros(5, 3), torch.zeros(3)), ValueError, r"shape \(5,\)"),
+    (lambda: blocks8.linear(torch.zeros(2, 3), torch.zeros(5, 3)), RuntimeError, "HIP device"),
+])
+def test_refusals(call, error, match):
+    with pytest.raises(error, match=match):
+        call()
+
+
+@pytest.mark.parametrize("rows,width,tiled,values,exponents", [
+    (1, 1, False, (1, 128), (1, 16)), (17, 128, False, (17, 128), (1, 32)), (16, 129, False, (16, 256), (2, 16)),
+    (129, 300, True, (129, 384), (3, 2)), (0, 5, False, (0, 128), (1, 16))])
+def test_layout(rows, width, tiled, values, exponents):
+    q = blocks(rows, width, tiled)
+    assert tuple(q.values.shape) == values and tuple(q.exponents.shape) == exponents
+    assert q.storage.numel() % 16 == 0
+
+
+def test_c_entry_refusals():
+    lib = _lib.lib()
+    p, odd = C.c_void_p(256), C.c_void_p(257)
+
+    def quantize(rows=4, width=8, x=p, values=p, pitch=16, act=0, beta=1.0, dtype=0):
+        return lib.vmf_blocks8_quantize(x, 8, values, p, pitch, rows, width, act, beta, dtype, None)
+
+    assert quantize(rows=-1) == -1 and quantize(width=0) == -1 and quantize(width=(1 << 22) + 1) == -4
+    assert quantize(x=None) == -1 and quantize(values=odd) == -1 and quantize(pitch=3) == -1
+    assert quantize(act=2) == -1 and quantize(act=1, beta=0.0) == -1 and quantize(dtype=1) == -2
+    assert quantize(rows=0, x=None) == 0
+    assert lib.vmf_blocks8_quantize_tiles(p, 8, p, p, p, None, 4, 8, 0, None) == -1
+    assert lib.vmf_blocks8_dequantize(p, p, 1, 0, p, 4, 8, 0, None) == -1
+    assert lib.vmf_blocks8_softplus_grad(None, 8, p, p, 16, p, 4, 8, 1.0, 0, None) == -1
+
+    def matmul(m=4, n=4, k=8, a=p, pitch=16, out=p, ws=None, nbytes=0, dtype=0, bias=None, bias_dtype=0, gate=None,
+               beta=1.0):
+        return lib.vmf_blocks8_matmul(a, p, pitch, 0, p, p, 16, 0, bias, bias_dtype, gate, p, 16, beta, out, m, n, k, ws,
+                                      nbytes, dtype, None)
+
+    assert matmul(m=-1) == -1 and matmul(k=0) == -1 and matmul(a=None) == -1 and matmul(a=odd) == -1
+    assert matmul(pitch=8) == -1 and matmul(out=None) == -1 and matmul(dtype=1) == -2
+    assert matmul(bias=p, bias_dtype=1) == -2 and matmul(gate=p, beta=-1.0) == -1
+    assert matmul(m=0) == 0
+    need = C.c_int64(0)
+    assert lib.vmf_blocks8_matmul_workspace(4, 4, 8, 0, need) == 0 and need.value == 0
+    assert lib.vmf_blocks8_matmul_workspace(4, 4, 1 << 16, 0, need) == 0 and need.value > 0
+    assert matmul(k=1 << 16, ws=p, nbytes=need.value - 1) == -1 and b"workspace" in lib.vmf_last_error_string()
+
+    def weight_grad(m=4, n=4, k=8, g=p, gw=p, dtype=0, out_dtype=0, ws=None, nbytes=0):
+        return lib.vmf_blocks8_weight_grad(g, 8, p, p, -(-m // 16) * 16, gw, None, m, n, k, ws, nbytes, dtype, out_dtype,
+                                           None)
+
+    assert weight_grad(m=-1) == -1 and weight_grad(g=None) == -1 and weight_grad(gw=None) == -1
+    assert weight_grad(dtype=3, out_dtype=2) == -2 and weight_grad(n=0) == 0
+    assert lib.vmf_blocks8_weight_grad_workspace(1 << 16, 128, 128, need) == 0 and need.value > 0
+    assert weight_grad(m=1 << 16, n=128, k=128, ws=p, nbytes=need.value - 1) == -1
