@@ -348,11 +348,32 @@ int vmf_blocks8_matmul(const uint8_t* a, const uint8_t* a_exponents, int64_t a_e
                        vmf_stream_t stream);
 /* gweight[n][k] = sum_m gy[m][n] a[m][k], gbias[n] = sum_m gy[m][n] (may be null): gy (m, n) of dtype, a: m rows of width
  * k in blocks by rows, outputs of out_dtype (VMF_F32 or dtype).  Products are exact, sums 32-bit, in a fixed order.
- * m == 0 gives zeros. */
-int vmf_blocks8_weight_grad_workspace(int64_t m, int64_t n, int64_t k, int64_t* bytes_out);
+ * m == 0 gives zeros.  gy_values / gy_exponents (may be null): receive gy's blocks by rows, the bytes that
+ * vmf_blocks8_quantize gives (the operand of the input gradient's product) without another read of gy. */
+int vmf_blocks8_weight_grad_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes_out);
 int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const uint8_t* a, const uint8_t* a_exponents,
-                            int64_t a_exp_pitch, void* gweight, void* gbias, int64_t m, int64_t n, int64_t k,
-                            void* workspace, int64_t workspace_bytes, int dtype, int out_dtype, vmf_stream_t stream);
+                            int64_t a_exp_pitch, void* gweight, void* gbias, uint8_t* gy_values, uint8_t* gy_exponents,
+                            int64_t gy_exp_pitch, int64_t m, int64_t n, int64_t k, void* workspace,
+                            int64_t workspace_bytes, int dtype, int out_dtype, vmf_stream_t stream);
+
+/* A layer's two directions in one call each: y = blocks(activation(x)) tiles(weight)^T + bias, and its gradients.
+ * fwd: weight (n, k) of weight_dtype (dtype or VMF_F32) is quantised in the call, or (null) w_values / w_exponents hold
+ * its tiles already.  a_values / a_exponents receive x's blocks, which bwd takes; wt_values / wt_exponents (may be null)
+ * the transposed weight's tiles, which bwd takes for gx.  y: dense, of dtype.
+ * bwd: gx (may be null; of dtype) = (blocks(gy) tiles(weight)) * softplus slope, gweight (may be null) and gbias (may be
+ * null, comes with gweight) as vmf_blocks8_weight_grad, of weight_dtype.
+ * workspace: the _workspace call's bytes (fwd without a weight: vmf_blocks8_matmul_workspace's), 16-byte aligned. */
+int vmf_blocks8_linear_fwd_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes_out);
+int vmf_blocks8_linear_fwd(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, int weight_dtype,
+                           const uint8_t* w_values, const uint8_t* w_exponents, uint8_t* wt_values,
+                           uint8_t* wt_exponents, const void* bias, int bias_dtype, int activation, double beta,
+                           uint8_t* a_values, uint8_t* a_exponents, int64_t a_exp_pitch, void* y, int64_t m, int64_t n,
+                           int64_t k, void* workspace, int64_t workspace_bytes, int dtype, vmf_stream_t stream);
+int vmf_blocks8_linear_bwd_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes_out);
+int vmf_blocks8_linear_bwd(const void* gy, int64_t gy_stride, const uint8_t* a_values, const uint8_t* a_exponents,
+                           int64_t a_exp_pitch, const uint8_t* wt_values, const uint8_t* wt_exponents, int activation,
+                           double beta, void* gx, void* gweight, void* gbias, int64_t m, int64_t n, int64_t k,
+                           void* workspace, int64_t workspace_bytes, int dtype, int weight_dtype, vmf_stream_t stream);
 
 /* ---- multi-GPU ---------------------------------------------------------------------------------------
  * The path shards by row and exchanges nothing but loss scalars: the `.mean()` / `.sum()` of

@@ -8,6 +8,7 @@ import os
 import threading
 
 import torch
+from torch.autograd.function import once_differentiable
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _DEFAULT = os.path.join(_HERE, "libvmf_hip.so")
@@ -76,8 +77,14 @@ _PROTOS = {
     "vmf_blocks8_matmul_workspace": [_I64, _I64, _I64, _I, _I64P],
     "vmf_blocks8_matmul": [_P, _P, _I64, _I, _P, _P, _I64, _I, _P, _I, _P, _P, _I64, _D, _P, _I64, _I64, _I64, _P, _I64,
                            _I, _P],
-    "vmf_blocks8_weight_grad_workspace": [_I64, _I64, _I64, _I64P],
-    "vmf_blocks8_weight_grad": [_P, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I, _I, _P],
+    "vmf_blocks8_weight_grad_workspace": [_I64, _I64, _I64, _I, _I64P],
+    "vmf_blocks8_weight_grad": [_P, _I64, _P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _I, _I, _P],
+    "vmf_blocks8_linear_fwd_workspace": [_I64, _I64, _I64, _I, _I64P],
+    "vmf_blocks8_linear_fwd": [_P, _I64, _P, _I64, _I, _P, _P, _P, _P, _P, _I, _I, _D, _P, _P, _I64, _P, _I64, _I64, _I64,
+                               _P, _I64, _I, _P],
+    "vmf_blocks8_linear_bwd_workspace": [_I64, _I64, _I64, _I, _I64P],
+    "vmf_blocks8_linear_bwd": [_P, _I64, _P, _P, _I64, _P, _P, _I, _D, _P, _P, _P, _I64, _I64, _I64, _P, _I64, _I, _I,
+                               _P],
 }
 EXPORTS = sorted(list(_PROTOS) + ["vmf_version", "vmf_last_error_string"])
 
@@ -218,6 +225,18 @@ def ptr(t):
 
 def stream_ptr(device):
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def first_order(backward):
+    """A Function's backward that is differentiable once.  Under create_graph=True it goes through torch's
+    once_differentiable, which makes a second derivative an error; otherwise, the usual case, it is called directly: the
+    wrapper's bookkeeping costs more than the calls of a small layer."""
+    checked = once_differentiable(backward)
+
+    def call(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return call
 
 
 def address(t):

@@ -21,7 +21,6 @@ infinities are NaN in blocks.  There is no CPU path.
 import ctypes as C
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -235,13 +234,14 @@ def _weight_grad(g, q, bias, dtype, dev):
     gb = torch.empty(n, device=dev, dtype=dtype) if bias else None
     lib = _lib.lib()
     need = C.c_int64(0)
-    _lib.check(lib.vmf_blocks8_weight_grad_workspace(m, n, k, need), "vmf_blocks8_weight_grad_workspace")
+    code = _lib.FLOAT_CODES[g.dtype]
+    _lib.check(lib.vmf_blocks8_weight_grad_workspace(m, n, k, code, need), "vmf_blocks8_weight_grad_workspace")
     ws = torch.empty(need.value, device=dev, dtype=torch.uint8) if need.value else None
     v, e = q._addresses()
     with _lib.on_device(dev):
-        rc = lib.vmf_blocks8_weight_grad(rows.data_ptr(), stride, v, e, q.exp_pitch, gw.data_ptr(), _lib.address(gb), m,
-                                         n, k, _lib.address(ws), need.value, _lib.FLOAT_CODES[g.dtype],
-                                         _lib.FLOAT_CODES[dtype], _lib.raw_stream(dev))
+        rc = lib.vmf_blocks8_weight_grad(rows.data_ptr(), stride, v, e, q.exp_pitch, gw.data_ptr(), _lib.address(gb), None,
+                                         None, 0, m, n, k, _lib.address(ws), need.value, code, _lib.FLOAT_CODES[dtype],
+                                         _lib.raw_stream(dev))
     _lib.check(rc, "vmf_blocks8_weight_grad")
     return gw, gb
 
@@ -258,42 +258,87 @@ def weight_grad(g, q, bias=True, dtype=torch.float32):
     return _weight_grad(g, q, bias, dtype, _lib.require_hip(g, q.storage))
 
 
+def _linear(x, weight, laid_out, bias, act, beta, dev, columns):
+    """(y, x's blocks, the weight's transposed tiles if `columns`).  The two share an allocation, which a backward pass
+    keeps; the weight's own tiles live in the workspace, and end with the call."""
+    rows, stride = _lib.as_rows(x.detach())
+    m, k = rows.shape
+    code = _lib.FLOAT_CODES[x.dtype]
+    lib = _lib.lib()
+    need = C.c_int64(0)
+    w = wv = we = None
+    w_stride = w_code = 0
+    if laid_out is None:
+        n = weight.shape[0]
+        w, w_stride = _lib.as_rows(weight.detach())
+        w_code = _lib.FLOAT_CODES[w.dtype]
+        _lib.check(lib.vmf_blocks8_linear_fwd_workspace(m, n, k, code, need), "vmf_blocks8_linear_fwd_workspace")
+    else:
+        n = laid_out.rows.rows
+        wv, we = laid_out.rows._addresses()
+        _lib.check(lib.vmf_blocks8_matmul_workspace(m, n, k, code, need), "vmf_blocks8_matmul_workspace")
+    first = Blocks8.bytes_for(m, k)
+    new_columns = columns and laid_out is None
+    kept = torch.empty(first + (Blocks8.bytes_for(k, n, True) if new_columns else 0), device=dev, dtype=torch.uint8)
+    q = Blocks8(kept, x.shape)
+    wt = Blocks8(kept, (k, n), True, first) if new_columns else laid_out.columns if columns else None
+    ws = torch.empty(need.value, device=dev, dtype=torch.uint8) if need.value else None
+    y = torch.empty(x.shape[:-1] + (n,), device=dev, dtype=x.dtype)
+    b = None if bias is None else bias.detach().contiguous()
+    qv, qe = q._addresses()
+    tv, te = wt._addresses() if new_columns else (None, None)
+    with _lib.on_device(dev):
+        rc = lib.vmf_blocks8_linear_fwd(rows.data_ptr(), stride, _lib.address(w), w_stride, w_code, wv, we, tv, te,
+                                        _lib.address(b), 0 if b is None else _lib.FLOAT_CODES[b.dtype], act, beta, qv, qe,
+                                        q.exp_pitch, y.data_ptr(), m, n, k, _lib.address(ws), need.value, code,
+                                        _lib.raw_stream(dev))
+    _lib.check(rc, "vmf_blocks8_linear_fwd")
+    return y, q, wt
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, laid_out, bias, act, beta, dev):
-        need_x, need_w, _, need_b = ctx.needs_input_grad[:4]
-        q = _quantize(x, act, beta, _lib.FLOAT_CODES[x.dtype], dev)
-        w8 = laid_out if weight is None else _quantize_weight(weight, need_x, dev)
-        y = _matmul(q, w8.rows, None if bias is None else bias.detach().contiguous(), None, 1.0, x.dtype, dev)
-        # kept for the backward pass: x in 8 bits and, for its own gradient, the weight in 8 bits
-        keep_q = need_w or need_b or (need_x and act)
-        if need_x and w8.columns is None:
+        need_x = ctx.needs_input_grad[0]
+        if need_x and laid_out is not None and laid_out.columns is None:
             raise ValueError("linear: the laid-out weight has no columns (quantize_weight(..., transpose=True)), which "
                              "the gradient of x reads")
-        ctx.save_for_backward(q.storage if keep_q else None, w8.columns.storage if need_x else None)
-        ctx.meta = (x.shape, (w8.columns.shape, w8.columns.offset) if need_x else None, act, beta,
-                    w8.dtype if weight is None else weight.dtype, None if bias is None else bias.dtype, dev)
+        y, q, wt = _linear(x, weight, laid_out, bias, act, beta, dev, need_x)
+        # kept for the backward pass: x in 8 bits and, for its own gradient, the transposed weight in 8 bits
+        ctx.save_for_backward(q.storage, wt.storage if wt is not None and wt.storage is not q.storage else None)
+        ctx.meta = (x.shape, y.shape[-1], None if wt is None else wt.offset, act, beta,
+                    None if weight is None else weight.dtype, None if bias is None else bias.dtype, dev)
         return y
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, gy):
-        q_storage, w_storage = ctx.saved_tensors
-        shape, columns, act, beta, w_dtype, bias_dtype, dev = ctx.meta
+        kept, other = ctx.saved_tensors
+        shape, n, wt_offset, act, beta, w_dtype, bias_dtype, dev = ctx.meta
         need_x, need_w, _, need_b = ctx.needs_input_grad[:4]
-        q = Blocks8(q_storage, shape) if q_storage is not None else None
-        gx = gw = gb = None
-        if need_x:
-            gq = _quantize(gy, _lib.ACT_NONE, 1.0, _lib.FLOAT_CODES[gy.dtype], dev)
-            w = Blocks8(w_storage, columns[0], True, columns[1])
-            gx = _matmul(gq, w, None, q if act else None, beta, gy.dtype, dev)
-        if need_w or need_b:
-            gw, gb = _weight_grad(gy, q, need_b, w_dtype if w_dtype in (torch.float32, gy.dtype) else torch.float32, dev)
-            if gb is not None and gb.dtype != bias_dtype:
-                gb = gb.to(bias_dtype)
-            if not need_w:
-                gw = None
-        return gx, gw, None, gb, None, None, None
+        q = Blocks8(kept, shape)
+        m, k = q.rows, q.width
+        code = _lib.FLOAT_CODES[gy.dtype]
+        # the weight's gradient in the weight's type; a bias beside a laid-out weight has float32 sums
+        out = w_dtype or torch.float32
+        gx = torch.empty(shape, device=dev, dtype=gy.dtype) if need_x else None
+        gw = torch.empty((n, k), device=dev, dtype=out) if need_w or need_b else None
+        gb = torch.empty(n, device=dev, dtype=out) if need_b else None
+        lib = _lib.lib()
+        need = C.c_int64(0)
+        _lib.check(lib.vmf_blocks8_linear_bwd_workspace(m, n, k, code, need), "vmf_blocks8_linear_bwd_workspace")
+        ws = torch.empty(need.value, device=dev, dtype=torch.uint8)
+        g, stride = _lib.as_rows(gy)
+        qv, qe = q._addresses()
+        tv, te = Blocks8(other if other is not None else kept, (k, n), True, wt_offset)._addresses() if need_x else (None, None)
+        with _lib.on_device(dev):
+            rc = lib.vmf_blocks8_linear_bwd(g.data_ptr(), stride, qv, qe, q.exp_pitch, tv, te, act, beta,
+                                            _lib.address(gx), _lib.address(gw), _lib.address(gb), m, n, k, ws.data_ptr(),
+                                            need.value, code, _lib.FLOAT_CODES[out], _lib.raw_stream(dev))
+        _lib.check(rc, "vmf_blocks8_linear_bwd")
+        if gb is not None and gb.dtype != bias_dtype:
+            gb = gb.to(bias_dtype)
+        return gx, gw if need_w else None, None, gb, None, None, None
 
 
 def linear(x, weight, bias=None, activation=None, beta=1.0):
@@ -318,6 +363,4 @@ def linear(x, weight, bias=None, activation=None, beta=1.0):
     tensor = weight if laid_out is None else None
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, tensor, bias)):
         return _Linear.apply(x, tensor, laid_out, bias, act, beta, dev)
-    q = _quantize(x, act, beta, _lib.FLOAT_CODES[x.dtype], dev)
-    w8 = laid_out if tensor is None else _quantize_weight(tensor, False, dev)
-    return _matmul(q, w8.rows, None if bias is None else bias.detach().contiguous(), None, 1.0, x.dtype, dev)
+    return _linear(x, tensor, laid_out, bias, act, beta, dev, False)[0]

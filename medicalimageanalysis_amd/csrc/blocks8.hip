@@ -9,14 +9,20 @@ __device__ __noinline__ double softplus64(double h, double beta) {
   const double t = beta * h;
   return ((t > 0 ? t : 0) + ::log1p(::exp(-::fabs(t)))) / beta;
 }
-// In 32 bits: off by at most softplus_margin relative to the value.  exp and log1p of the library are within 2 units in
-// the last place, the sum and the product add one each, and beta and t = beta h are rounded: 2 * 2^-24 * |t| in the
-// argument of exp, which counts in full for negative t only (for positive t its share is |t| exp(-t) <= 0.37 of that).
+// In 32 bits, from the hardware's exponential and logarithm (1 unit in the last place each):
+//   log(1 + u), u = exp(-|t|): where 1 + u drops too much of u (u < 1/16), the series to u^6 (the rest is under u^6 / 7
+//   of it); else ln 2 * log2(1 + u), off by 2^-24 / u <= 2^-20.
+// beta, t = beta h and t log2(e) are rounded, 3 * 2^-24 |t| in the exponential's argument, which counts in full for
+// negative t only (for positive t its share is |t| exp(-t) <= 0.37 of that).  Together the result is off by less than
+// softplus_margin relative to its value.
 __device__ __forceinline__ float softplus32(float h, float beta, float inv_beta) {
   const float t = beta * h;
-  return (fmaxf(t, 0.0f) + log1pf(expf(-fabsf(t)))) * inv_beta;
+  const float u = __builtin_amdgcn_exp2f(-fabsf(t) * 1.44269504f);
+  const float few = u * (1.0f + u * (-0.5f + u * (1.0f / 3 + u * (-0.25f + u * (0.2f + u * (-1.0f / 6))))));
+  const float l = u < 0.0625f ? few : 0.69314718f * __builtin_amdgcn_logf(1.0f + u);
+  return (fmaxf(t, 0.0f) + l) * inv_beta;
 }
-__device__ __forceinline__ float softplus_margin(float h, float beta) { return 2e-6f + 3e-7f * fmaxf(-beta * h, 0.0f); }
+__device__ __forceinline__ float softplus_margin(float h, float beta) { return 3e-6f + 3e-7f * fmaxf(-beta * h, 0.0f); }
 
 // a double in [0, 448] -> the float from which a second rounding to fewer bits gives what one rounding of the double
 // would: truncated, with the last bit set if anything was cut off
@@ -30,139 +36,165 @@ __device__ __forceinline__ float round_to_odd(double d) {
   return f;
 }
 
-// Sixteen lanes hold a block, 8 elements each.  ACT: the elements are softplus(h).  Which of two neighbouring 8-bit
-// values is nearest to softplus(h) can hang on its last bits, so a value is computed in 32 bits, and once more in 64 where
-// its 32-bit error could change the result (a few of a million): the bytes are those of the exactly computed softplus.
-template <bool ACT>
-__device__ __forceinline__ uint2 quantize8(float (&h)[8], float beta, float inv_beta, double beta64, int& e_out) {
-  constexpr float INF = __builtin_inff();
-  int e;
-  if constexpr (!ACT) {
-    float top = 0;
+// the exponent and the scaled elements of a block that sixteen lanes hold, 8 elements each
+__device__ __forceinline__ int scale8(float (&h)[8]) {
+  uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float a = fabsf(h[i]);
-      top = a < INF ? fmaxf(top, a) : top;  // false for NaN
-    }
-    e = b8_exponent(lane_max<16>(top));
-    const float inv = b8_pow2(-e);
+  for (int i = 0; i < 8; ++i) top = larger(top, b8_size(h[i]));
+  top = lane_max<16>(top);
+  if (top >= B8_INF) {  // some are not finite: the largest of the others
+    top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = fabsf(h[i]) < INF ? h[i] * inv : __builtin_nanf("");
-    e_out = e;
-    return uint2{b8_pack2(h[0], h[1]) | b8_pack2(h[2], h[3]) << 16, b8_pack2(h[4], h[5]) | b8_pack2(h[6], h[7]) << 16};
-  } else {
-    float top = -INF;  // softplus grows with h: the block's largest comes from the largest h
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = h[i] < INF ? fmaxf(top, h[i]) : top;
+    for (int i = 0; i < 8; ++i) top = b8_size(h[i]) < B8_INF ? larger(top, b8_size(h[i])) : top;
     top = lane_max<16>(top);
-    const float at = softplus32(top, beta, inv_beta), mt = softplus_margin(top, beta);
-    if (at < INF) {
-      e = b8_exponent(at * (1.0f - mt));
-      const int above = b8_exponent(fminf(at * (1.0f + mt), 3.4e38f));
-      if (e != above && softplus64((double)top, beta64) > 448.0 * ::ldexp(1.0, e)) e = above;
-    } else {
-      e = B8_EMAX;
-    }
-    if (top == -INF) e = 0;
-    const float inv = b8_pow2(-e);
-    uint32_t r[4];
+  }
+  const int e = b8_exponent(__uint_as_float(top));
+  const float inv = b8_pow2(-e);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) h[i] *= inv;
+  if (e == B8_EMAX) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = b8_cut(h[i]);
+  }
+  return e;
+}
+
+// One element the exact way: softplus(x) / 2^e, ready for the conversion
+__device__ __noinline__ float softplus_scaled(float x, double beta, int e) {
+  if (!(x < __builtin_inff())) return __builtin_nanf("");
+  return round_to_odd(::fmin(softplus64((double)x, beta) * ::ldexp(1.0, -e), 448.0));
+}
+
+// The block of softplus(h).  Which of two neighbouring 8-bit values is nearest to softplus(h) can hang on its last bits,
+// so a value is computed in 32 bits, and once more in 64 where its 32-bit error could change the result (a few of a
+// million): the bytes are those of the exactly computed softplus.
+__device__ __forceinline__ uint2 softplus8(const float (&h)[8], float beta, float inv_beta, double beta64, int& e_out) {
+  constexpr float INF = __builtin_inff();
+  float top = -INF;  // softplus grows with h: the block's largest comes from the largest h
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = h[i] < INF ? fmaxf(top, h[i]) : top;
+  top = lane_max<16>(top);
+  const float at = softplus32(top, beta, inv_beta), mt = softplus_margin(top, beta);
+  int e = B8_EMAX;
+  if (at < INF) {
+    e = b8_exponent(at * (1.0f - mt));
+    const int above = b8_exponent(fminf(at * (1.0f + mt), 3.4e38f));
+    if (e != above && softplus64((double)top, beta64) > 448.0 * ::ldexp(1.0, e)) e = above;
+  }
+  if (top == -INF) e = 0;
+  e_out = e;
+  const float scale = inv_beta * b8_pow2(-e);
+  float lo[8], hi[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = softplus32(h[i], beta, scale);
+    const float m = fminf(softplus_margin(h[i], beta), 0.5f);  // (-inf, the fill of short rows, has none)
+    lo[i] = fmaf(a, -m, a);
+    hi[i] = fmaf(a, m, a);
+  }
+  uint2 r{b8_pack4(lo), b8_pack4(lo + 4)};
+  if (r.x != b8_pack4(hi) || r.y != b8_pack4(hi + 4) || e == B8_EMAX) {
+    uint32_t w[4];
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-      float lo[2], hi[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float x = h[2 * p + i];
-        const float a = softplus32(x, beta, inv_beta) * inv, m = x == -INF ? 0.0f : softplus_margin(x, beta);
-        lo[i] = x < INF ? a * (1.0f - m) : __builtin_nanf("");
-        hi[i] = x < INF ? a * (1.0f + m) : __builtin_nanf("");
-      }
-      r[p] = b8_pack2(lo[0], lo[1]);
-      if (r[p] != b8_pack2(hi[0], hi[1])) {
-        float v[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float x = h[2 * p + i];
-          v[i] = x < INF ? round_to_odd(::fmin(softplus64((double)x, beta64) * ::ldexp(1.0, -e), 448.0))
-                         : __builtin_nanf("");
-        }
-        r[p] = b8_pack2(v[0], v[1]);
-      }
+      w[p] = b8_pack2(lo[2 * p], lo[2 * p + 1]);
+      if (w[p] != b8_pack2(hi[2 * p], hi[2 * p + 1]) || e == B8_EMAX)
+        w[p] = b8_pack2(softplus_scaled(h[2 * p], beta64, e), softplus_scaled(h[2 * p + 1], beta64, e));
     }
-    e_out = e;
-    return uint2{r[0] | r[1] << 16, r[2] | r[3] << 16};
+    r = uint2{w[0] | w[1] << 16, w[2] | w[3] << 16};
   }
+  return r;
 }
 
 // A workgroup has 16 groups of 16 lanes: 1 << row_bits of them side by side in rows (so that the exponent bytes of
 // neighbouring rows, which lie side by side, leave together), the others in block columns.
+struct RowArgs {
+  const void* x;
+  int64_t x_stride;
+  uint8_t* values;
+  uint8_t* exponents;
+  int64_t exp_pitch, rows, width, blocks;
+  int row_bits, gx, gy;  // workgroups along the rows and along the block columns
+  double beta;
+  float beta32, inv_beta;
+};
 template <typename T, bool ACT>
-__global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, int64_t x_stride,
-                                                       uint8_t* __restrict__ values, int64_t pitch,
-                                                       uint8_t* __restrict__ exponents, int64_t exp_pitch, int64_t rows,
-                                                       int64_t width, int64_t blocks, int row_bits, double beta) {
+__device__ __forceinline__ void quantize_rows(const RowArgs& p, int bx, int by) {
   const int group = threadIdx.x >> 4, lane = threadIdx.x & 15;
-  const int64_t row = ((int64_t)blockIdx.x << row_bits) + (group & ((1 << row_bits) - 1));
-  if (row >= rows) return;
-  const int side = 16 >> row_bits;
-  const float b32 = (float)beta, ib32 = (float)(1.0 / beta);
-  for (int64_t kb = (int64_t)blockIdx.y * side + (group >> row_bits); kb < blocks; kb += (int64_t)gridDim.y * side) {
+  const int64_t row = ((int64_t)bx << p.row_bits) + (group & ((1 << p.row_bits) - 1));
+  if (row >= p.rows) return;
+  const int side = 16 >> p.row_bits;
+  const T* x = (const T*)p.x + row * p.x_stride;
+  for (int64_t kb = (int64_t)by * side + (group >> p.row_bits); kb < p.blocks; kb += (int64_t)p.gy * side) {
     const int64_t col = kb * B8 + lane * 8;
     float h[8];
-    load_some<8>(x + row * x_stride + col, width - col, ACT ? -__builtin_inff() : 0.0f, h);
+    load_some<8>(x + col, p.width - col, ACT ? -__builtin_inff() : 0.0f, h);
     int e;
-    const uint2 v = quantize8<ACT>(h, b32, ib32, beta, e);
-    *reinterpret_cast<uint2*>(values + row * pitch + col) = v;
-    if (lane == 0) exponents[kb * exp_pitch + row] = (uint8_t)(e + 127);
+    uint2 v;
+    if constexpr (ACT) {
+      v = softplus8(h, p.beta32, p.inv_beta, p.beta, e);
+    } else {
+      e = scale8(h);
+      v = uint2{b8_pack4(h), b8_pack4(h + 4)};
+    }
+    *reinterpret_cast<uint2*>(p.values + row * (p.blocks * B8) + col) = v;
+    if (lane == 0) p.exponents[kb * p.exp_pitch + row] = (uint8_t)(e + 127);
   }
+}
+template <typename T, bool ACT>
+__global__ __launch_bounds__(256) void quantize_kernel(RowArgs p) {
+  quantize_rows<T, ACT>(p, blockIdx.x, blockIdx.y);
 }
 
 // One workgroup per 128 x 128 tile of a matrix (n rows, k columns): the tile's bytes in the matrix's order and, through
 // LDS, in the transpose's.
+struct TileArgs {
+  const void* w;
+  int64_t w_stride;
+  uint8_t* values;
+  uint8_t* exps;
+  uint8_t* values_t;
+  uint8_t* exps_t;
+  int64_t n, k, n_tiles, k_tiles;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void quantize_tiles_kernel(const T* __restrict__ w, int64_t w_stride,
-                                                             uint8_t* __restrict__ values, uint8_t* __restrict__ exps,
-                                                             uint8_t* __restrict__ values_t,
-                                                             uint8_t* __restrict__ exps_t, int64_t n, int64_t k) {
-  __shared__ float red[4];
+__device__ __forceinline__ void quantize_tile(const TileArgs& p, int64_t id) {
+  __shared__ uint32_t red[4];
   __shared__ uint8_t tile[B8 * (B8 + 4)];
-  const int64_t nt = blockIdx.y, kt = blockIdx.x;
-  const int64_t n_tiles = gridDim.y, k_tiles = gridDim.x;
+  const int64_t n_tiles = p.n_tiles, k_tiles = p.k_tiles;
+  const int64_t nt = id / k_tiles, kt = id - nt * k_tiles;
   const int group = threadIdx.x >> 4, lane = threadIdx.x & 15;
   float h[8][8];
-  float top = 0;
+  uint32_t top = 0;
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
     const int64_t row = nt * B8 + r * 16 + group, col = kt * B8 + lane * 8;
-    load_some<8>(w + row * w_stride + col, row < n ? k - col : 0, 0.0f, h[r]);
+    load_some<8>((const T*)p.w + row * p.w_stride + col, row < p.n ? p.k - col : 0, 0.0f, h[r]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float a = fabsf(h[r][i]);
-      top = a < __builtin_inff() ? fmaxf(top, a) : top;
-    }
+    for (int i = 0; i < 8; ++i) top = b8_size(h[r][i]) < B8_INF ? larger(top, b8_size(h[r][i])) : top;
   }
   top = lane_max<64>(top);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
   __syncthreads();
-  const int e = b8_exponent(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+  const int e = b8_exponent(__uint_as_float(larger(larger(red[0], red[1]), larger(red[2], red[3]))));
   const float inv = b8_pow2(-e);
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
     const int64_t row = nt * B8 + r * 16 + group;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) h[r][i] = fabsf(h[r][i]) < __builtin_inff() ? h[r][i] * inv : __builtin_nanf("");
-    const uint32_t lo = b8_pack2(h[r][0], h[r][1]) | b8_pack2(h[r][2], h[r][3]) << 16;
-    const uint32_t hi = b8_pack2(h[r][4], h[r][5]) | b8_pack2(h[r][6], h[r][7]) << 16;
-    if (row < n)
-      *reinterpret_cast<uint2*>(values + row * (k_tiles * B8) + kt * B8 + lane * 8) = uint2{lo, hi};
+    for (int i = 0; i < 8; ++i) h[r][i] = e == B8_EMAX ? b8_cut(h[r][i] * inv) : h[r][i] * inv;
+    const uint32_t lo = b8_pack4(h[r]), hi = b8_pack4(h[r] + 4);
+    if (row < p.n)
+      *reinterpret_cast<uint2*>(p.values + row * (k_tiles * B8) + kt * B8 + lane * 8) = uint2{lo, hi};
     uint32_t* t = reinterpret_cast<uint32_t*>(tile + (r * 16 + group) * (B8 + 4) + lane * 8);
     t[0] = lo;
     t[1] = hi;
   }
   if (threadIdx.x == 0) {
-    exps[kt * n_tiles + nt] = (uint8_t)(e + 127);
-    if (exps_t) exps_t[nt * k_tiles + kt] = (uint8_t)(e + 127);
+    p.exps[kt * n_tiles + nt] = (uint8_t)(e + 127);
+    if (p.exps_t) p.exps_t[nt * k_tiles + kt] = (uint8_t)(e + 127);
   }
-  if (!values_t) return;
+  if (!p.values_t) return;
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
@@ -170,7 +202,22 @@ __global__ __launch_bounds__(256) void quantize_tiles_kernel(const T* __restrict
     uint32_t v[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i >> 2] |= (uint32_t)tile[(lane * 8 + i) * (B8 + 4) + r * 16 + group] << (8 * (i & 3));
-    if (row < k) *reinterpret_cast<uint2*>(values_t + row * (n_tiles * B8) + nt * B8 + lane * 8) = uint2{v[0], v[1]};
+    if (row < p.k) *reinterpret_cast<uint2*>(p.values_t + row * (n_tiles * B8) + nt * B8 + lane * 8) = uint2{v[0], v[1]};
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_tiles_kernel(TileArgs p) {
+  quantize_tile<T>(p, blockIdx.x);
+}
+// both in one launch: the tiles' workgroups first
+template <typename T, bool ACT, typename TW>
+__global__ __launch_bounds__(256) void quantize_both_kernel(RowArgs r, TileArgs t) {
+  const int tiles = (int)(t.n_tiles * t.k_tiles), id = (int)blockIdx.x;
+  if (id < tiles) {
+    quantize_tile<TW>(t, id);
+  } else {
+    const int by = (id - tiles) / r.gx;
+    quantize_rows<T, ACT>(r, id - tiles - by * r.gx, by);
   }
 }
 
@@ -211,7 +258,7 @@ Shape shape_for(int64_t rows, int64_t blocks) {
   Shape s;
   s.row_bits = 0;
   while (s.row_bits < 4 && (1 << s.row_bits) < rows) ++s.row_bits;
-  const int64_t gx = (rows + (1 << s.row_bits) - 1) >> s.row_bits;
+  const int64_t gx = rows > 0 ? (rows + (1 << s.row_bits) - 1) >> s.row_bits : 1;
   const int64_t most = (blocks + (16 >> s.row_bits) - 1) / (16 >> s.row_bits);
   int64_t gy = (8192 + gx - 1) / gx;
   if (gy > most) gy = most;
@@ -230,56 +277,116 @@ int b8_check_shape(const char* what, int64_t rows, int64_t width) {
   return VMF_OK;
 }
 
+namespace {
+
+int row_args(const char* what, const void* x, int64_t x_stride, uint8_t* values, uint8_t* exponents, int64_t exp_pitch,
+             int64_t rows, int64_t width, int activation, double beta, RowArgs* out) {
+  int rc = b8_check_shape(what, rows, width);
+  if (rc != VMF_OK) return rc;
+  VMF_REQUIRE(activation == VMF_ACT_NONE || activation == VMF_ACT_SOFTPLUS, VMF_ERR_BAD_ARG, "%s: activation %d", what,
+              activation);
+  VMF_REQUIRE(activation == VMF_ACT_NONE || (beta > 0 && beta <= 1e30 && beta >= 1e-30), VMF_ERR_BAD_ARG,
+              "%s: beta %g", what, beta);
+  VMF_REQUIRE(x_stride >= 0 && exp_pitch >= rows, VMF_ERR_BAD_ARG, "%s: strides", what);
+  if (rows > 0) {
+    VMF_REQUIRE(x && values && exponents, VMF_ERR_BAD_ARG, "%s: null pointer", what);
+    VMF_REQUIRE(((uintptr_t)values & 15) == 0, VMF_ERR_BAD_ARG, "%s: values must be 16-byte aligned", what);
+  }
+  if (activation == VMF_ACT_NONE) beta = 1.0;
+  const int64_t blocks = b8_blocks(width);
+  const Shape s = shape_for(rows, blocks);
+  *out = RowArgs{x, x_stride, values, exponents, exp_pitch, rows, width, blocks, s.row_bits, (int)s.grid.x,
+                 (int)s.grid.y, beta, (float)beta, (float)(1.0 / beta)};
+  return VMF_OK;
+}
+
+int tile_args(const char* what, const void* w, int64_t w_stride, uint8_t* values, uint8_t* exponents,
+              uint8_t* values_t, uint8_t* exponents_t, int64_t rows, int64_t width, TileArgs* out) {
+  int rc = b8_check_shape(what, rows, width);
+  if (rc != VMF_OK) return rc;
+  rc = b8_check_shape(what, width, rows < 1 ? 1 : rows);
+  if (rc != VMF_OK) return rc;
+  VMF_REQUIRE(w_stride >= 0, VMF_ERR_BAD_ARG, "%s: negative row stride", what);
+  VMF_REQUIRE(!values_t == !exponents_t, VMF_ERR_BAD_ARG, "%s: values_t and exponents_t go together", what);
+  if (rows > 0) {
+    VMF_REQUIRE(w && values && exponents, VMF_ERR_BAD_ARG, "%s: null pointer", what);
+    VMF_REQUIRE((((uintptr_t)values | (uintptr_t)values_t) & 15) == 0, VMF_ERR_BAD_ARG,
+                "%s: values must be 16-byte aligned", what);
+  }
+  *out = TileArgs{w, w_stride, values, exponents, values_t, exponents_t, rows, width, b8_blocks(rows), b8_blocks(width)};
+  VMF_REQUIRE(out->n_tiles * out->k_tiles <= 0x7fffffff, VMF_ERR_UNSUPPORTED, "%s: %lld x %lld", what, (long long)rows,
+              (long long)width);
+  return VMF_OK;
+}
+
+int launch_rows(const RowArgs& r, int activation, int dtype, hipStream_t st) {
+  LOWP_DISPATCH(dtype, "vmf_blocks8_quantize", T, {
+    if (activation == VMF_ACT_SOFTPLUS) quantize_kernel<T, true><<<dim3(r.gx, r.gy), 256, 0, st>>>(r);
+    else quantize_kernel<T, false><<<dim3(r.gx, r.gy), 256, 0, st>>>(r);
+  });
+  return vmf_check_launch("vmf_blocks8_quantize");
+}
+
+int launch_tiles(const TileArgs& t, int dtype, hipStream_t st) {
+  LOWP_DISPATCH(dtype, "vmf_blocks8_quantize_tiles", T,
+                (quantize_tiles_kernel<T><<<(unsigned)(t.n_tiles * t.k_tiles), 256, 0, st>>>(t)));
+  return vmf_check_launch("vmf_blocks8_quantize_tiles");
+}
+
+template <typename T, typename TW>
+void launch_both(const RowArgs& r, const TileArgs& t, int activation, hipStream_t st) {
+  const unsigned grid = (unsigned)(t.n_tiles * t.k_tiles + (int64_t)r.gx * r.gy);
+  if (activation == VMF_ACT_SOFTPLUS) quantize_both_kernel<T, true, TW><<<grid, 256, 0, st>>>(r, t);
+  else quantize_both_kernel<T, false, TW><<<grid, 256, 0, st>>>(r, t);
+}
+
+}  // namespace
+
 extern "C" int vmf_blocks8_quantize(const void* x, int64_t x_stride, uint8_t* values, uint8_t* exponents,
                                     int64_t exp_pitch, int64_t rows, int64_t width, int activation, double beta,
                                     int dtype, vmf_stream_t stream) {
   VMF_RANGE("vmf_blocks8_quantize");
-  int rc = b8_check_shape("vmf_blocks8_quantize", rows, width);
-  if (rc != VMF_OK) return rc;
-  VMF_REQUIRE(activation == VMF_ACT_NONE || activation == VMF_ACT_SOFTPLUS, VMF_ERR_BAD_ARG,
-              "vmf_blocks8_quantize: activation %d", activation);
-  VMF_REQUIRE(activation == VMF_ACT_NONE || (beta > 0 && beta <= 1e30 && beta >= 1e-30), VMF_ERR_BAD_ARG,
-              "vmf_blocks8_quantize: beta %g", beta);
-  VMF_REQUIRE(x_stride >= 0 && exp_pitch >= rows, VMF_ERR_BAD_ARG, "vmf_blocks8_quantize: strides");
-  if (rows == 0) return VMF_OK;
-  VMF_REQUIRE(x && values && exponents, VMF_ERR_BAD_ARG, "vmf_blocks8_quantize: null pointer");
-  VMF_REQUIRE(((uintptr_t)values & 15) == 0, VMF_ERR_BAD_ARG, "vmf_blocks8_quantize: values must be 16-byte aligned");
-  const int64_t blocks = b8_blocks(width);
-  const Shape s = shape_for(rows, blocks);
-  hipStream_t st = (hipStream_t)stream;
-  LOWP_DISPATCH(dtype, "vmf_blocks8_quantize", T, {
-    if (activation == VMF_ACT_SOFTPLUS)
-      quantize_kernel<T, true><<<s.grid, 256, 0, st>>>((const T*)x, x_stride, values, blocks * B8, exponents, exp_pitch,
-                                                       rows, width, blocks, s.row_bits, beta);
-    else
-      quantize_kernel<T, false><<<s.grid, 256, 0, st>>>((const T*)x, x_stride, values, blocks * B8, exponents,
-                                                        exp_pitch, rows, width, blocks, s.row_bits, 1.0);
-  });
-  return vmf_check_launch("vmf_blocks8_quantize");
+  RowArgs r;
+  int rc = row_args("vmf_blocks8_quantize", x, x_stride, values, exponents, exp_pitch, rows, width, activation, beta, &r);
+  if (rc != VMF_OK || rows == 0) return rc;
+  return launch_rows(r, activation, dtype, (hipStream_t)stream);
 }
 
 extern "C" int vmf_blocks8_quantize_tiles(const void* w, int64_t w_stride, uint8_t* values, uint8_t* exponents,
                                           uint8_t* values_t, uint8_t* exponents_t, int64_t rows, int64_t width,
                                           int dtype, vmf_stream_t stream) {
   VMF_RANGE("vmf_blocks8_quantize_tiles");
-  int rc = b8_check_shape("vmf_blocks8_quantize_tiles", rows, width);
+  TileArgs t;
+  int rc = tile_args("vmf_blocks8_quantize_tiles", w, w_stride, values, exponents, values_t, exponents_t, rows, width, &t);
+  if (rc != VMF_OK || rows == 0) return rc;
+  return launch_tiles(t, dtype, (hipStream_t)stream);
+}
+
+int b8_quantize_both(const void* x, int64_t x_stride, uint8_t* values, uint8_t* exponents, int64_t exp_pitch, int64_t m,
+                     int64_t k, int activation, double beta, int dtype, const void* w, int64_t w_stride,
+                     uint8_t* w_values, uint8_t* w_exponents, uint8_t* wt_values, uint8_t* wt_exponents, int64_t n,
+                     int w_dtype, vmf_stream_t stream) {
+  const char* what = "vmf_blocks8_linear_fwd";
+  RowArgs r;
+  TileArgs t;
+  int rc = row_args(what, x, x_stride, values, exponents, exp_pitch, m, k, activation, beta, &r);
   if (rc != VMF_OK) return rc;
-  rc = b8_check_shape("vmf_blocks8_quantize_tiles", width, rows < 1 ? 1 : rows);
+  rc = tile_args(what, w, w_stride, w_values, w_exponents, wt_values, wt_exponents, n, k, &t);
   if (rc != VMF_OK) return rc;
-  VMF_REQUIRE(w_stride >= 0, VMF_ERR_BAD_ARG, "vmf_blocks8_quantize_tiles: negative row stride");
-  VMF_REQUIRE(!values_t == !exponents_t, VMF_ERR_BAD_ARG,
-              "vmf_blocks8_quantize_tiles: values_t and exponents_t go together");
-  if (rows == 0) return VMF_OK;
-  VMF_REQUIRE(w && values && exponents, VMF_ERR_BAD_ARG, "vmf_blocks8_quantize_tiles: null pointer");
-  VMF_REQUIRE((((uintptr_t)values | (uintptr_t)values_t) & 15) == 0, VMF_ERR_BAD_ARG,
-              "vmf_blocks8_quantize_tiles: values must be 16-byte aligned");
-  const int64_t n_tiles = b8_blocks(rows);
-  VMF_REQUIRE(n_tiles <= 65535, VMF_ERR_UNSUPPORTED, "vmf_blocks8_quantize_tiles: %lld rows", (long long)rows);
+  VMF_REQUIRE(w_dtype == dtype || w_dtype == VMF_F32, VMF_ERR_DTYPE, "%s: the weight's dtype is x's or VMF_F32, got %d",
+              what, w_dtype);
   hipStream_t st = (hipStream_t)stream;
-  LOWP_DISPATCH(dtype, "vmf_blocks8_quantize_tiles", T,
-                (quantize_tiles_kernel<T><<<dim3((unsigned)b8_blocks(width), (unsigned)n_tiles), 256, 0, st>>>(
-                    (const T*)w, w_stride, values, exponents, values_t, exponents_t, rows, width)));
-  return vmf_check_launch("vmf_blocks8_quantize_tiles");
+  // One launch less is a matter of microseconds; with much of either the rows' workgroups do better without the tiles'
+  // registers and LDS.
+  if (m == 0 || m * k > (1 << 20) || n * k > (1 << 20)) {
+    rc = launch_tiles(t, w_dtype, st);
+    return rc != VMF_OK || m == 0 ? rc : launch_rows(r, activation, dtype, st);
+  }
+  LOWP_DISPATCH(dtype, "vmf_blocks8_linear_fwd", T, {
+    if (w_dtype == VMF_F32) launch_both<T, float>(r, t, activation, st);
+    else launch_both<T, T>(r, t, activation, st);
+  });
+  return vmf_check_launch(what);
 }
 
 static int from_blocks(const char* what, const void* g, int64_t g_stride, const uint8_t* values,

@@ -27,12 +27,25 @@ __device__ __forceinline__ int b8_exponent(float top) {
   const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
   return e < B8_EMIN ? B8_EMIN : e > B8_EMAX ? B8_EMAX : e;
 }
-// two values already divided by 2^e -> two bytes (low half), round to nearest even; NaN stays NaN
+// Two values already divided by the block's 2^e -> two bytes (low half), rounded to nearest even.  Nothing finite is
+// above 448 (1 + 2^-20) then, which the conversion rounds to 448; infinities and NaN become NaN.  (e = 119, the largest,
+// is the exception: b8_pack2_top cuts what is above 448.)
 __device__ __forceinline__ uint32_t b8_pack2(float a, float b) {
-  const float ca = a != a ? a : __builtin_amdgcn_fmed3f(a, -448.0f, 448.0f);
-  const float cb = b != b ? b : __builtin_amdgcn_fmed3f(b, -448.0f, 448.0f);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(ca, cb, 0, false) & 0xffffu;
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu;
 }
+__device__ __forceinline__ float b8_cut(float a) {
+  return fabsf(a) < __builtin_inff() ? fminf(fmaxf(a, -448.0f), 448.0f) : __builtin_nanf("");
+}
+// four values into a word
+__device__ __forceinline__ uint32_t b8_pack4(const float* v) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w, true);
+}
+// the largest finite magnitude of a block of rows' elements: its bits as an integer, which order as the numbers do.
+// Anything at or above the bits of infinity counts as 0.
+__device__ __forceinline__ uint32_t b8_size(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+constexpr uint32_t B8_INF = 0x7f800000u;
+
 // the four elements of a word
 __device__ __forceinline__ void b8_unpack4(uint32_t w, float scale, float* out) {
   out[0] = __builtin_amdgcn_cvt_f32_fp8((int)w, 0) * scale;
@@ -56,3 +69,8 @@ __device__ __forceinline__ void static_for(F&& f) {
 // ---- host side -----------------------------------------------------------------------------------------------
 static inline int64_t b8_blocks(int64_t width) { return (width + B8 - 1) / B8; }
 int b8_check_shape(const char* what, int64_t rows, int64_t width);
+// vmf_blocks8_quantize of x (m, k) and vmf_blocks8_quantize_tiles of w (n, k), in one launch where both are small
+int b8_quantize_both(const void* x, int64_t x_stride, uint8_t* values, uint8_t* exponents, int64_t exp_pitch, int64_t m,
+                     int64_t k, int activation, double beta, int dtype, const void* w, int64_t w_stride,
+                     uint8_t* w_values, uint8_t* w_exponents, uint8_t* wt_values, uint8_t* wt_exponents, int64_t n,
+                     int w_dtype, vmf_stream_t stream);

@@ -121,8 +121,8 @@ __device__ __forceinline__ void finish(const MmArgs& p, int64_t row, int64_t col
 //   one stage is multiplied the next is on its way, one barrier per block column.
 //   A 16-row operand tile takes the rows F * (lane & 15) + i (i = 0 .. F - 1 the tile's number): the exponents of a
 //   lane's F tiles are then one word, and a lane's results are F consecutive columns of a row.
-//   The 16-byte pieces of a row lie at piece ^ (row / F) & 7, so that the eight lanes that are served together read from
-//   all banks.
+//   In LDS the 16 rows of an operand tile lie side by side, the 16-byte pieces of row q at piece ^ (q / 2): the 16 lanes
+//   that read the same piece of the 16 rows then read from all 64 banks (two rows fill the banks once).
 template <int BM, int BN, int WM, int WN, bool WIDE, typename OUT>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p) {
   constexpr int WAVES_N = BN / WN, WAVES = (BM / WM) * WAVES_N;
@@ -154,8 +154,10 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p
   for (int i = 0; i < LOADS; ++i) {
     const int r8 = wave * LOADS + i;  // eight rows of the stage: first A's, then B's
     const bool is_b = r8 >= BM / 8;
-    const int r = (is_b ? r8 - BM / 8 : r8) * 8 + (lane >> 3);
-    const int piece = (lane & 7) ^ ((is_b ? r / FN : r / FM) & 7);
+    const int at = (is_b ? r8 - BM / 8 : r8) * 8 + (lane >> 3), q = at & 15;  // the row's place in LDS
+    const int f = is_b ? FN : FM, tile = at >> 4;
+    const int r = tile / f * (16 * f) + f * q + tile % f;
+    const int piece = (lane & 7) ^ (q >> 1);
     const Operand& o = is_b ? p.b : p.a;
     int64_t row = (is_b ? n0 : m0) + r;
     row = row < o.rows ? row : o.rows - 1;
@@ -182,10 +184,10 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p
 #pragma unroll
     for (int g = 0; g < GN; ++g) eb[slot][g] = load_exps<FN>(p.b, kb, n0 + wn + g * 16 * FN, lane);
   };
-  auto operand = [&](const uint8_t* rows, int row, int f) -> v8i {
-    const int s = (row / f) & 7, c = (lane >> 4) * 2;
-    const v4i lo = *reinterpret_cast<const v4i*>(rows + row * B8 + ((c ^ s) << 4));
-    const v4i hi = *reinterpret_cast<const v4i*>(rows + row * B8 + (((c + 1) ^ s) << 4));
+  auto operand = [&](const uint8_t* tile) -> v8i {  // 16 rows of LDS
+    const int q = lane & 15, c = (lane >> 4) * 2;
+    const v4i lo = *reinterpret_cast<const v4i*>(tile + q * B8 + ((c ^ (q >> 1)) << 4));
+    const v4i hi = *reinterpret_cast<const v4i*>(tile + q * B8 + (((c + 1) ^ (q >> 1)) << 4));
     return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
   auto multiply = [&](int stage, const int* xa, const int* xb) {
@@ -196,12 +198,12 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p
       if constexpr (!WIDE) {
         v8i a[FM];
 #pragma unroll
-        for (int i = 0; i < FM; ++i) a[i] = operand(A, wm + g * 16 * FM + FM * (lane & 15) + i, FM);
+        for (int i = 0; i < FM; ++i) a[i] = operand(A + (wm + (g * FM + i) * 16) * B8);
 #pragma unroll
         for (int h = 0; h < GN; ++h)
           static_for<FN>([&](auto J) {
             constexpr int j = decltype(J)::value;
-            const v8i b = operand(B, wn + h * 16 * FN + FN * (lane & 15) + j, FN);
+            const v8i b = operand(B + (wn + (h * FN + j) * 16) * B8);
             static_for<FM>([&](auto I) {
               constexpr int i = decltype(I)::value;
               v4f& c = acc[g * FM + i][h * FN + j];
@@ -212,12 +214,12 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p
         v8b a[FM][4], b[4];
 #pragma unroll
         for (int i = 0; i < FM; ++i)
-          to_bf16(operand(A, wm + g * 16 * FM + FM * (lane & 15) + i, FM), b8_scale((xa[g] >> (8 * i)) & 0xff), a[i]);
+          to_bf16(operand(A + (wm + (g * FM + i) * 16) * B8), b8_scale((xa[g] >> (8 * i)) & 0xff), a[i]);
 #pragma unroll
         for (int h = 0; h < GN; ++h)
 #pragma unroll
           for (int j = 0; j < FN; ++j) {
-            to_bf16(operand(B, wn + h * 16 * FN + FN * (lane & 15) + j, FN), b8_scale((xb[h] >> (8 * j)) & 0xff), b);
+            to_bf16(operand(B + (wn + (h * FN + j) * 16) * B8), b8_scale((xb[h] >> (8 * j)) & 0xff), b);
 #pragma unroll
             for (int i = 0; i < FM; ++i) acc[g * FM + i][h * FN + j] = mm_step_bf16(a[i], b, acc[g * FM + i][h * FN + j]);
           }
@@ -392,133 +394,250 @@ __device__ __forceinline__ uint32_t cut(float& v) {  // the upper 16 bits; v bec
   return u >> 16;
 }
 
+// the same of two finite values, in one word; `more`: their rests are wanted
+__device__ __forceinline__ uint32_t cut_finite(float& a, float& b, bool more) {
+  const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+  if (more) {
+    a -= __uint_as_float(x & 0xffff0000u);
+    b -= __uint_as_float(y & 0xffff0000u);
+  }
+  return __builtin_amdgcn_perm(y, x, 0x07060302u);
+}
+
 struct WgArgs {
   const void* gy;
   int64_t gy_stride;
   Operand a;
   void* gw;
   void* gb;
-  float* partial;       // [split][n][k] then [split][n]; null with one split
+  float* partial;  // [split][n][k] then [split][n]; null with one split
+  uint8_t* q;      // gy's blocks by rows (null: not wanted)
+  uint8_t* q_exps;
+  int64_t q_pitch, q_exp_pitch;
   int64_t m, n, k;
   int64_t rows_per_split;
   int nt, kt;
 };
 
-// Tile of 128 (n) x 128 (k, one block column), 32 rows of the batch at a time: gy's terms and a's values as bf16 rows in
-// LDS, read back transposed (the rows are the products' inner dimension).  Two stages, one barrier per 32 rows; the next
-// rows are loaded into registers while these are multiplied.
+// Tile of BN (n) x BK (k) over the batch's rows, 32 at a time; waves of WN x WK.
+//   gy's terms and a's values lie in LDS as bf16 rows and are read back transposed (the rows are the products' inner
+//   dimension).  Two stages, one barrier per 32 rows; the rows of two steps ahead are on their way in registers, as they
+//   are in memory (one step's products take 256 to 1024 clocks, a load about 2000).
+//   Bound: a step of the 256 x 256 tile is 1024 clocks of matrix instructions and moves 128 KiB through LDS, 1024 clocks.
+//   The workgroups of the first k tile also add up gbias.  gy's 8-bit blocks (what the input gradient's product reads) are
+//   written on the way too, the k tiles' workgroups taking turns.
 constexpr int WG_ROWS = 32;
-constexpr int WG_PITCH = 2 * B8 + 32;  // bytes; 32 more than the row, so that the rows of a transposed read start 8 banks apart
 
-template <typename T, typename W>
-__global__ __launch_bounds__(256) void wgrad_kernel(WgArgs p) {
+template <typename T, typename W, int BN, int BK, int WN, int WK>
+__global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void wgrad_kernel(WgArgs p) {
+  constexpr int THREADS = (BN / WN) * (BK / WK) * 64;
   constexpr int NT = Terms<T>::count;
-  constexpr int PLANE = WG_ROWS * WG_PITCH;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * (NT + 1) * PLANE];
+  constexpr int E = 16 / (int)sizeof(T);          // elements of gy in a 16-byte piece
+  constexpr int GP = BN / E;                      // pieces per row; divides THREADS, so a thread keeps its columns
+  constexpr int GN = WG_ROWS * GP / THREADS;      // pieces per thread and step
+  constexpr int AP = BK / 16, AN = WG_ROWS * AP / THREADS;
+  constexpr int PITCH_G = 2 * BN + 32, PITCH_A = 2 * BK + 32;  // bytes; 32 more than the row: the rows of a
+                                                               // transposed read start 8 banks apart
+  constexpr int PLANE = WG_ROWS * PITCH_G, STAGE = NT * PLANE + WG_ROWS * PITCH_A;
+  static_assert(THREADS % GP == 0 && THREADS % AP == 0 && GN >= 1 && AN >= 1, "whole pieces");
+  constexpr int FN = WN / 32, FK = WK / 32;
+  typedef typename Pack<T, E>::type Piece;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
+
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int nt = (int)blockIdx.x / p.kt, kt = (int)blockIdx.x % p.kt;
-  const int64_t n0 = (int64_t)nt * B8;
+  const int64_t n0 = (int64_t)nt * BN, k0 = (int64_t)kt * BK;
   const int64_t m0 = (int64_t)blockIdx.y * p.rows_per_split;
   const int64_t m1 = m0 + p.rows_per_split < p.m ? m0 + p.rows_per_split : p.m;
-  const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 16;  // this thread's row of the 32 and its 16 columns
-  const T* gsrc = (const T*)p.gy + n0 + c;
-  const uint8_t* asrc = p.a.values + (int64_t)kt * B8 + c;
-  const uint8_t* esrc = p.a.exps + (int64_t)kt * p.a.exp_pitch;
-  const int64_t left = p.n - n0 - c;
+  const int gr = threadIdx.x / GP, gc = (threadIdx.x % GP) * E;    // row and column of this thread's first piece of gy
+  const int ar = threadIdx.x / AP, ac = (threadIdx.x % AP) * 16;   // and of a
+  const int64_t left = p.n - n0 - gc;
+  const bool a_in = k0 + ac < p.a.pitch;  // the last tile may reach behind a's padded rows
+  const T* gsrc = (const T*)p.gy + n0 + gc;
+  const uint8_t* asrc = p.a.values + k0 + ac;
+  const uint8_t* esrc = p.a.exps + ((k0 + ac) >> 7) * p.a.exp_pitch;
+  const bool sums = kt == 0 && p.gb;
 
-  float g[16];
-  v4i av;
-  uint32_t ae;
-  float gsum[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) gsum[i] = 0;
-  auto fetch = [&](int64_t m) {
-    const int64_t row = m + r;
-    const bool in = row < m1;
-    load_some<8>(gsrc + row * p.gy_stride, in ? left : 0, 0.0f, g);
-    load_some<8>(gsrc + row * p.gy_stride + 8, in ? left - 8 : 0, 0.0f, g + 8);
-    av = v4i{0, 0, 0, 0};
-    ae = 127;
-    if (in) {
-      av = *reinterpret_cast<const v4i*>(asrc + row * p.a.pitch);
-      ae = esrc[row];
-    }
+  struct Step {
+    Piece g[GN];
+    v4i a[AN];
+    uint32_t e[AN];
   };
-  auto put = [&](int stage) {
-    uint8_t* base = lds + stage * (NT + 1) * PLANE + r * WG_PITCH + c * 2;
+  Step ahead[2];
+  float gsum[E];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) gsum[i] += g[i];
+  for (int i = 0; i < E; ++i) gsum[i] = 0;
+  auto fetch = [&](int64_t m, Step& s) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      uint32_t w[8];
+    for (int i = 0; i < GN; ++i) {
+      const int64_t row = m + gr + i * (THREADS / GP);
+      const T* src = gsrc + row * p.gy_stride;
+      Piece v;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t lo = cut(g[2 * i]), hi = cut(g[2 * i + 1]);
-        w[i] = lo | hi << 16;
+      for (int j = 0; j < E; ++j) v[j] = (T)0;
+      if (row < m1) {
+        if (left >= E) {
+          v = *reinterpret_cast<const Piece*>(src);
+        } else {
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            if (j < left) v[j] = src[j];
+        }
       }
-      uint4* d = reinterpret_cast<uint4*>(base + t * PLANE);
-      d[0] = uint4{w[0], w[1], w[2], w[3]};
-      d[1] = uint4{w[4], w[5], w[6], w[7]};
+      s.g[i] = v;
     }
-    const float scale = b8_scale(ae);
-    v2b* d = reinterpret_cast<v2b*>(base + NT * PLANE);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      d[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(av[i], scale, false);
-      d[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(av[i], scale, true);
+    for (int i = 0; i < AN; ++i) {
+      const int64_t row = m + ar + i * (THREADS / AP);
+      s.a[i] = v4i{0, 0, 0, 0};
+      s.e[i] = 127;
+      if (row < m1 && a_in) {
+        s.a[i] = *reinterpret_cast<const v4i*>(asrc + row * p.a.pitch);
+        s.e[i] = esrc[row];
+      }
     }
   };
-  // 32 columns from `col` of the 16 rows from `row` of a plane, as the operand of a 32 x 32 x 16 product: lane l gets
-  // column l % 32, rows 8 * (l / 32) .. + 7
-  auto transposed = [&](const uint8_t* plane, int row, int col) -> v8b {
+  auto put = [&](int64_t m, const Step& s, int stage, bool blocks) {
+    uint8_t* base = lds + stage * STAGE;
+#pragma unroll
+    for (int i = 0; i < GN; ++i) {
+      const int r = gr + i * (THREADS / GP);
+      float v[E];
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = (float)s.g[i][j];
+      if (sums)
+#pragma unroll
+        for (int j = 0; j < E; ++j) gsum[j] += v[j];
+      uint32_t top = 0;
+      if (blocks || NT > 1)
+#pragma unroll
+        for (int j = 0; j < E; ++j) top = larger(top, b8_size(v[j]));
+      uint8_t* d = base + r * PITCH_G + gc * 2;
+      if constexpr (NT == 1) {
+        *reinterpret_cast<Piece*>(__builtin_assume_aligned(d, 16)) = s.g[i];
+      } else {
+        float u[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) u[j] = v[j];
+        const bool fine = top < B8_INF;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          uint32_t w[E / 2];
+          if (fine) {
+#pragma unroll
+            for (int j = 0; j < E / 2; ++j) w[j] = cut_finite(u[2 * j], u[2 * j + 1], t < NT - 1);
+          } else {
+#pragma unroll
+            for (int j = 0; j < E / 2; ++j) {
+              const uint32_t lo = cut(u[2 * j]), hi = cut(u[2 * j + 1]);
+              w[j] = lo | hi << 16;
+            }
+          }
+          if constexpr (E == 8) *reinterpret_cast<uint4*>(d + t * PLANE) = uint4{w[0], w[1], w[2], w[3]};
+          else *reinterpret_cast<uint2*>(d + t * PLANE) = uint2{w[0], w[1]};
+        }
+      }
+      if (blocks) {  // 128 / E neighbouring lanes hold a block
+        top = lane_max<B8 / E>(top);
+        if (top >= B8_INF) {
+          top = 0;
+#pragma unroll
+          for (int j = 0; j < E; ++j) top = b8_size(v[j]) < B8_INF ? larger(top, b8_size(v[j])) : top;
+          top = lane_max<B8 / E>(top);
+        }
+        const int e = b8_exponent(__uint_as_float(top));
+        const float inv = b8_pow2(-e);
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[j] *= inv;
+        if (e == B8_EMAX)
+#pragma unroll
+          for (int j = 0; j < E; ++j) v[j] = b8_cut(v[j]);
+        const int64_t row = m + r, col = n0 + gc;
+        if (row < m1 && col < p.q_pitch) {
+          uint8_t* q = p.q + row * p.q_pitch + col;
+          if constexpr (E == 8) *reinterpret_cast<uint2*>(q) = uint2{b8_pack4(v), b8_pack4(v + 4)};
+          else *reinterpret_cast<uint32_t*>(q) = b8_pack4(v);
+          if ((gc & (B8 - 1)) == 0) p.q_exps[(col >> 7) * p.q_exp_pitch + row] = (uint8_t)(e + 127);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < AN; ++i) {
+      const float scale = b8_scale(s.e[i]);
+      union {
+        v2b h[8];
+        uint4 w[2];
+      } u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        u.h[2 * j] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(s.a[i][j], scale, false);
+        u.h[2 * j + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(s.a[i][j], scale, true);
+      }
+      uint4* d = reinterpret_cast<uint4*>(base + NT * PLANE + (ar + i * (THREADS / AP)) * PITCH_A + ac * 2);
+      d[0] = u.w[0];
+      d[1] = u.w[1];
+    }
+  };
+  // 32 columns from `col` of the 16 rows from `row`, as the operand of a 32 x 32 x 16 product: lane l gets column l % 32,
+  // rows 8 * (l / 32) .. + 7
+  auto transposed = [&](const uint8_t* plane, int pitch, int row, int col) -> v8b {
     const int q = lane & 15, grp = lane >> 4;
-    const uint8_t* s = plane + (row + (grp >> 1) * 8 + (q >> 2)) * WG_PITCH + (col + (grp & 1) * 16 + (q & 3) * 4) * 2;
+    const uint8_t* s = plane + (row + (grp >> 1) * 8 + (q >> 2)) * pitch + (col + (grp & 1) * 16 + (q & 3) * 4) * 2;
     union {
       v4s h[2];
       v8b v;
     } u;
     u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(v4s, s));
-    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(v4s, s + 4 * WG_PITCH));
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(v4s, s + 4 * pitch));
     return u.v;
   };
-  const int wn = (wave >> 1) * 64, wk = (wave & 1) * 64;
-  v16f acc[2][2];
+  const int wn = (wave / (BK / WK)) * WN, wk = (wave % (BK / WK)) * WK;
+  v16f acc[FN][FK];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < FN; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < FK; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
 
-  int stage = 0;
-  if (m0 < m1) fetch(m0);
-  for (int64_t m = m0; m < m1; m += WG_ROWS) {
-    put(stage);
-    if (m + WG_ROWS < m1) fetch(m + WG_ROWS);
-    // one barrier is enough: the stage written next was read before the previous barrier
-    __syncthreads();
-    const uint8_t* base = lds + stage * (NT + 1) * PLANE;
+  int turn = 0;  // which k tile's workgroup writes gy's blocks of this step
+  if (m0 < m1) fetch(m0, ahead[0]);
+  if (m0 + WG_ROWS < m1) fetch(m0 + WG_ROWS, ahead[1]);
+  for (int64_t mm = m0; mm < m1; mm += 2 * WG_ROWS) {
 #pragma unroll
-    for (int s = 0; s < WG_ROWS; s += 16) {
-      const v8b b0 = transposed(base + NT * PLANE, s, wk), b1 = transposed(base + NT * PLANE, s, wk + 32);
+    for (int half = 0; half < 2; ++half) {
+      const int64_t m = mm + half * WG_ROWS;
+      if (m < m1) {
+        put(m, ahead[half], half, p.q && turn == kt);
+        turn = turn + 1 == p.kt ? 0 : turn + 1;
+        if (m + 2 * WG_ROWS < m1) fetch(m + 2 * WG_ROWS, ahead[half]);
+        // one barrier is enough: this stage was last read before the previous one
+        __syncthreads();
+        const uint8_t* base = lds + half * STAGE;
 #pragma unroll
-      for (int t = NT - 1; t >= 0; --t) {
-        const v8b a0 = transposed(base + t * PLANE, s, wn), a1 = transposed(base + t * PLANE, s, wn + 32);
-        acc[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0, b0, acc[0][0], 0, 0, 0);
-        acc[0][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0, b1, acc[0][1], 0, 0, 0);
-        acc[1][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1, b0, acc[1][0], 0, 0, 0);
-        acc[1][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1, b1, acc[1][1], 0, 0, 0);
+        for (int s = 0; s < WG_ROWS; s += 16) {
+          v8b b[FK];
+#pragma unroll
+          for (int j = 0; j < FK; ++j) b[j] = transposed(base + NT * PLANE, PITCH_A, s, wk + 32 * j);
+#pragma unroll
+          for (int t = NT - 1; t >= 0; --t)
+#pragma unroll
+            for (int i = 0; i < FN; ++i) {
+              const v8b a = transposed(base + t * PLANE, PITCH_G, s, wn + 32 * i);
+#pragma unroll
+              for (int j = 0; j < FK; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[j], acc[i][j], 0, 0, 0);
+            }
+        }
       }
     }
-    stage ^= 1;
   }
 
   // D: column (k) lane % 32, rows (n) (e & 3) + 8 (e >> 2) + 4 (lane / 32)
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < FN; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int64_t k = (int64_t)kt * B8 + wk + j * 32 + (lane & 31);
+    for (int j = 0; j < FK; ++j) {
+      const int64_t k = k0 + wk + j * 32 + (lane & 31);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int64_t n = n0 + wn + i * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
@@ -528,24 +647,23 @@ __global__ __launch_bounds__(256) void wgrad_kernel(WgArgs p) {
         }
       }
     }
-  // gbias: the first block column's workgroups add what they read of gy over the 32 rows, two halves of the columns in turn
-  if (!p.gb || kt != 0) return;
-  float* red = reinterpret_cast<float*>(lds);  // 32 x 64 floats = 8 KiB
+  if (!sums) return;
+  // gbias: the threads that share columns add their sums in order
+  constexpr int SHARE = THREADS / GP;
+  float* red = reinterpret_cast<float*>(lds);
+  static_assert(SHARE * BN * 4 <= 2 * STAGE, "the sums fit the stages");
+  __syncthreads();
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    __syncthreads();
-    if ((c >> 6) == half)
+  for (int i = 0; i < E; ++i) red[gr * BN + gc + i] = gsum[i];
+  __syncthreads();
+  if (threadIdx.x < BN) {
+    float s = 0;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) red[r * 64 + (c & 63) + i] = gsum[i];
-    __syncthreads();
-    if (threadIdx.x < 64) {
-      float s = 0;
-      for (int q = 0; q < WG_ROWS; ++q) s += red[q * 64 + threadIdx.x];
-      const int64_t n = n0 + half * 64 + threadIdx.x;
-      if (n < p.n) {
-        if (p.partial) p.partial[(int64_t)gridDim.y * p.n * p.k + (int64_t)blockIdx.y * p.n + n] = s;
-        else ((W*)p.gb)[n] = (W)s;
-      }
+    for (int q = 0; q < SHARE; ++q) s += red[q * BN + threadIdx.x];
+    const int64_t n = n0 + threadIdx.x;
+    if (n < p.n) {
+      if (p.partial) p.partial[(int64_t)gridDim.y * p.n * p.k + (int64_t)blockIdx.y * p.n + n] = s;
+      else ((W*)p.gb)[n] = (W)s;
     }
   }
 }
@@ -558,6 +676,7 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(const float* __restrict
     const float* src = i < nk ? partial + i : partial + splits * nk + (i - nk);
     const int64_t step = i < nk ? nk : n;
     float s = 0;
+#pragma unroll 8
     for (int q = 0; q < splits; ++q) s += src[q * step];
     if (i < nk) gw[i] = (W)s;
     else gb[i - nk] = (W)s;
@@ -565,22 +684,35 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(const float* __restrict
 }
 
 struct WgPlan {
-  int splits, nt, kt;
+  int splits, nt, kt, tile;
   int64_t per_split;
 };
-// three workgroups per compute unit where the batch allows it, at least 256 rows to a split
-WgPlan wg_plan(int64_t m, int64_t n, int64_t k) {
+// Tiles of 256 x 256 for the 16-bit types where the result has several; the batch is split until there is a workgroup
+// (of the small tile: two) for every compute unit, at least 256 rows to a split.
+WgPlan wg_plan(int64_t m, int64_t n, int64_t k, int dtype) {
   WgPlan p;
-  p.nt = (int)((n + B8 - 1) / B8);
-  p.kt = (int)b8_blocks(k);
+  p.tile = dtype != VMF_F32 && n > 256 && k > 256 ? 256 : 128;
+  p.nt = (int)((n + p.tile - 1) / p.tile);
+  p.kt = (int)((k + p.tile - 1) / p.tile);
   const int64_t tiles = (int64_t)p.nt * p.kt;
-  int64_t s = (768 + tiles - 1) / tiles;
+  int64_t s = (p.tile == 256 ? 256 : 512) / tiles;
   if (s > m / 256) s = m / 256;
   if (s < 1) s = 1;
   p.per_split = ((m + s - 1) / s + WG_ROWS - 1) / WG_ROWS * WG_ROWS;
   p.splits = p.per_split > 0 ? (int)((m + p.per_split - 1) / p.per_split) : 1;
-  if (p.splits < 1) p.splits = 1;
   return p;
+}
+
+template <typename T, typename W>
+void wgrad_launch(const WgPlan& pl, const WgArgs& p, hipStream_t st) {
+  const dim3 grid((unsigned)(pl.nt * pl.kt), (unsigned)pl.splits);
+  if constexpr (sizeof(T) == 2) {
+    if (pl.tile == 256) {
+      wgrad_kernel<T, W, 256, 256, 128, 64><<<grid, 512, 0, st>>>(p);
+      return;
+    }
+  }
+  wgrad_kernel<T, W, 128, 128, 64, 64><<<grid, 256, 0, st>>>(p);
 }
 
 int check_operand(const char* what, const char* name, const uint8_t* values, const uint8_t* exps, int64_t exp_pitch,
@@ -660,35 +792,38 @@ extern "C" int vmf_blocks8_matmul(const uint8_t* a, const uint8_t* a_exponents, 
   return vmf_check_launch(what);
 }
 
-extern "C" int vmf_blocks8_weight_grad_workspace(int64_t m, int64_t n, int64_t k, int64_t* bytes_out) {
+extern "C" int vmf_blocks8_weight_grad_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes_out) {
   int rc = b8_check_shape("vmf_blocks8_weight_grad_workspace", m, k);
   if (rc != VMF_OK) return rc;
   VMF_REQUIRE(bytes_out && n >= 0 && n <= VMF_BLOCKS8_MAX_WIDTH, VMF_ERR_BAD_ARG,
               "vmf_blocks8_weight_grad_workspace: n = %lld or a null pointer", (long long)n);
   *bytes_out = 0;
   if (n == 0) return VMF_OK;
-  const WgPlan pl = wg_plan(m, n, k);
+  const WgPlan pl = wg_plan(m, n, k, dtype);
   if (pl.splits > 1) *bytes_out = (int64_t)pl.splits * n * (k + 1) * 4;
   return VMF_OK;
 }
 
 extern "C" int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const uint8_t* a, const uint8_t* a_exponents,
-                                       int64_t a_exp_pitch, void* gweight, void* gbias, int64_t m, int64_t n,
-                                       int64_t k, void* workspace, int64_t workspace_bytes, int dtype, int out_dtype,
+                                       int64_t a_exp_pitch, void* gweight, void* gbias, uint8_t* gy_values,
+                                       uint8_t* gy_exponents, int64_t gy_exp_pitch, int64_t m, int64_t n, int64_t k,
+                                       void* workspace, int64_t workspace_bytes, int dtype, int out_dtype,
                                        vmf_stream_t stream) {
   VMF_RANGE("vmf_blocks8_weight_grad");
   const char* what = "vmf_blocks8_weight_grad";
   int64_t need = 0;
-  int rc = vmf_blocks8_weight_grad_workspace(m, n, k, &need);
+  int rc = vmf_blocks8_weight_grad_workspace(m, n, k, dtype, &need);
   if (rc != VMF_OK) return rc;
   VMF_REQUIRE(out_dtype == VMF_F32 || out_dtype == dtype, VMF_ERR_DTYPE, "%s: out dtype %d", what, out_dtype);
   VMF_REQUIRE(gy_stride >= 0, VMF_ERR_BAD_ARG, "%s: negative row stride", what);
   if (n == 0) return VMF_OK;
   VMF_REQUIRE(gweight && (m == 0 || gy), VMF_ERR_BAD_ARG, "%s: null pointer", what);
   if (m > 0 && (rc = check_operand(what, "a", a, a_exponents, a_exp_pitch, 0, m)) != VMF_OK) return rc;
+  if (gy_values && (rc = check_operand(what, "gy's blocks", gy_values, gy_exponents, gy_exp_pitch, 0, m)) != VMF_OK)
+    return rc;
   VMF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), VMF_ERR_BAD_ARG,
               "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)need);
-  const WgPlan pl = wg_plan(m, n, k);
+  const WgPlan pl = wg_plan(m, n, k, dtype);
   VMF_REQUIRE((int64_t)pl.nt * pl.kt <= 0x7fffffff, VMF_ERR_UNSUPPORTED, "%s: %lld x %lld results", what, (long long)n,
               (long long)k);
   WgArgs p;
@@ -698,17 +833,20 @@ extern "C" int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const 
   p.gw = gweight;
   p.gb = gbias;
   p.partial = need ? (float*)workspace : nullptr;
+  p.q = gy_values;
+  p.q_exps = gy_exponents;
+  p.q_pitch = b8_blocks(n) * B8;
+  p.q_exp_pitch = gy_exp_pitch;
   p.m = m;
   p.n = n;
   p.k = k;
   p.rows_per_split = pl.per_split;
   p.nt = pl.nt;
   p.kt = pl.kt;
-  const dim3 grid((unsigned)(pl.nt * pl.kt), (unsigned)pl.splits);
   hipStream_t st = (hipStream_t)stream;
   LOWP_DISPATCH(dtype, "vmf_blocks8_weight_grad", T, {
-    if (out_dtype == VMF_F32) wgrad_kernel<T, float><<<grid, 256, 0, st>>>(p);
-    else wgrad_kernel<T, T><<<grid, 256, 0, st>>>(p);
+    if (out_dtype == VMF_F32) wgrad_launch<T, float>(pl, p, st);
+    else wgrad_launch<T, T>(pl, p, st);
   });
   rc = vmf_check_launch(what);
   if (rc != VMF_OK || !need) return rc;
@@ -716,4 +854,91 @@ extern "C" int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const 
                 (wgrad_join_kernel<W><<<vmf_grid_for(n * (k + 1), 256, 1 << 13), 256, 0, st>>>(
                     p.partial, (W*)gweight, (W*)gbias, pl.splits, n * k, n)));
   return vmf_check_launch(what);
+}
+
+// ---- a layer's two directions --------------------------------------------------------------------------------------
+
+namespace {
+int64_t up16(int64_t v) { return (v + 15) / 16 * 16; }
+int64_t exp_rows(int64_t rows) { return rows < 16 ? 16 : up16(rows); }
+int64_t row_block_bytes(int64_t rows, int64_t width) { return b8_blocks(width) * (rows * B8 + exp_rows(rows)); }
+int64_t tile_bytes(int64_t rows, int64_t width) { return up16(b8_blocks(width) * (rows * B8 + b8_blocks(rows))); }
+}  // namespace
+
+extern "C" int vmf_blocks8_linear_fwd_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes_out) {
+  int rc = vmf_blocks8_matmul_workspace(m, n, k, dtype, bytes_out);
+  if (rc == VMF_OK) *bytes_out = up16(*bytes_out) + tile_bytes(n, k);
+  return rc;
+}
+
+extern "C" int vmf_blocks8_linear_fwd(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                                      int weight_dtype, const uint8_t* w_values, const uint8_t* w_exponents,
+                                      uint8_t* wt_values, uint8_t* wt_exponents, const void* bias, int bias_dtype,
+                                      int activation, double beta, uint8_t* a_values, uint8_t* a_exponents,
+                                      int64_t a_exp_pitch, void* y, int64_t m, int64_t n, int64_t k, void* workspace,
+                                      int64_t workspace_bytes, int dtype, vmf_stream_t stream) {
+  VMF_RANGE("vmf_blocks8_linear_fwd");
+  const char* what = "vmf_blocks8_linear_fwd";
+  int64_t need = 0;
+  int rc = vmf_blocks8_matmul_workspace(m, n, k, dtype, &need);
+  if (rc != VMF_OK) return rc;
+  const int64_t front = up16(need), all = weight ? front + tile_bytes(n, k) : need;
+  VMF_REQUIRE(n >= 1, VMF_ERR_BAD_ARG, "%s: n = %lld", what, (long long)n);
+  VMF_REQUIRE(all == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= all), VMF_ERR_BAD_ARG,
+              "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)all);
+  if (weight) {
+    uint8_t* v = (uint8_t*)workspace + front;
+    w_values = v;
+    w_exponents = v + n * b8_blocks(k) * B8;
+    rc = b8_quantize_both(x, x_stride, a_values, a_exponents, a_exp_pitch, m, k, activation, beta, dtype, weight,
+                          weight_stride, v, v + n * b8_blocks(k) * B8, wt_values, wt_exponents, n, weight_dtype, stream);
+  } else {
+    rc = vmf_blocks8_quantize(x, x_stride, a_values, a_exponents, a_exp_pitch, m, k, activation, beta, dtype, stream);
+  }
+  if (rc != VMF_OK) return rc;
+  return vmf_blocks8_matmul(a_values, a_exponents, a_exp_pitch, 0, w_values, w_exponents, b8_blocks(n), 1, bias,
+                            bias_dtype, nullptr, nullptr, 0, 1.0, y, m, n, k, workspace, need, dtype, stream);
+}
+
+extern "C" int vmf_blocks8_linear_bwd_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes_out) {
+  int64_t mm = 0, wg = 0;
+  int rc = n >= 1 ? vmf_blocks8_matmul_workspace(m, k, n, dtype, &mm) : VMF_ERR_BAD_ARG;
+  VMF_REQUIRE(n >= 1, VMF_ERR_BAD_ARG, "vmf_blocks8_linear_bwd_workspace: n = %lld", (long long)n);
+  if (rc != VMF_OK) return rc;
+  rc = vmf_blocks8_weight_grad_workspace(m, n, k, dtype, &wg);
+  if (rc != VMF_OK) return rc;
+  VMF_REQUIRE(bytes_out, VMF_ERR_BAD_ARG, "vmf_blocks8_linear_bwd_workspace: null pointer");
+  *bytes_out = up16(mm > wg ? mm : wg) + row_block_bytes(m, n);
+  return VMF_OK;
+}
+
+extern "C" int vmf_blocks8_linear_bwd(const void* gy, int64_t gy_stride, const uint8_t* a_values,
+                                      const uint8_t* a_exponents, int64_t a_exp_pitch, const uint8_t* wt_values,
+                                      const uint8_t* wt_exponents, int activation, double beta, void* gx, void* gweight,
+                                      void* gbias, int64_t m, int64_t n, int64_t k, void* workspace,
+                                      int64_t workspace_bytes, int dtype, int weight_dtype, vmf_stream_t stream) {
+  VMF_RANGE("vmf_blocks8_linear_bwd");
+  const char* what = "vmf_blocks8_linear_bwd";
+  int64_t need = 0;
+  int rc = vmf_blocks8_linear_bwd_workspace(m, n, k, dtype, &need);
+  if (rc != VMF_OK) return rc;
+  VMF_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need, VMF_ERR_BAD_ARG,
+              "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)need);
+  VMF_REQUIRE(gweight || !gbias, VMF_ERR_BAD_ARG, "%s: gbias comes with gweight", what);
+  VMF_REQUIRE(!gx || wt_values, VMF_ERR_BAD_ARG, "%s: gx needs the transposed weight", what);
+  // gy's blocks lie in front, what the products add up in parts behind them: one after the other, on one stream
+  uint8_t* q = (uint8_t*)workspace;
+  uint8_t* q_exps = q + m * b8_blocks(n) * B8;
+  uint8_t* parts = q + row_block_bytes(m, n);
+  const int64_t left = workspace_bytes - row_block_bytes(m, n);
+  if (gweight)
+    rc = vmf_blocks8_weight_grad(gy, gy_stride, a_values, a_exponents, a_exp_pitch, gweight, gbias, gx ? q : nullptr,
+                                 q_exps, exp_rows(m), m, n, k, parts, left, dtype, weight_dtype, stream);
+  else if (gx)
+    rc = vmf_blocks8_quantize(gy, gy_stride, q, q_exps, exp_rows(m), m, n, VMF_ACT_NONE, 1.0, dtype, stream);
+  if (rc != VMF_OK || !gx) return rc;
+  const bool gate = activation == VMF_ACT_SOFTPLUS;
+  return vmf_blocks8_matmul(q, q_exps, exp_rows(m), 0, wt_values, wt_exponents, b8_blocks(k), 1, nullptr, 0,
+                            gate ? a_values : nullptr, a_exponents, a_exp_pitch, beta, gx, m, k, n, parts, left, dtype,
+                            stream);
 }

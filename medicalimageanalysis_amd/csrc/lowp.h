@@ -67,19 +67,49 @@ __device__ __forceinline__ void store_some(T* p, int64_t left, const A* in) {
   }
 }
 
-// sum over groups of G consecutive lanes (G a power of two <= 64), the same value in every lane
-template <int G, typename A>
-__device__ __forceinline__ A lane_sum(A v) {
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+// Reductions over groups of G consecutive lanes (G a power of two, 16 .. 64), the same bits in every lane: inside 16 lanes
+// by rotations in the vector unit (a rotation by half the distance left pairs every lane with one whose sum is over the
+// complementary lanes), across them through the LDS crossbar.
+template <int N, typename A>
+__device__ __forceinline__ A rotated16(A v) {
+  if constexpr (sizeof(A) == 4) {
+    union {
+      A a;
+      int i;
+    } u;
+    u.a = v;
+    u.i = __builtin_amdgcn_update_dpp(0, u.i, 0x120 + N, 0xf, 0xf, true);
+    return u.a;
+  } else {
+    union {
+      A a;
+      int i[2];
+    } u;
+    u.a = v;
+    u.i[0] = __builtin_amdgcn_update_dpp(0, u.i[0], 0x120 + N, 0xf, 0xf, true);
+    u.i[1] = __builtin_amdgcn_update_dpp(0, u.i[1], 0x120 + N, 0xf, 0xf, true);
+    return u.a;
+  }
 }
 template <int G, typename A>
-__device__ __forceinline__ A lane_max(A v) {
+__device__ __forceinline__ A lane_sum(A v) {
+  v += rotated16<8>(v);
+  v += rotated16<4>(v);
+  v += rotated16<2>(v);
+  v += rotated16<1>(v);
 #pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) {
-    const A u = __shfl_xor(v, o, 64);
-    v = u > v ? u : v;
-  }
+  for (int o = 16; o < G; o <<= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+template <typename A>
+__device__ __forceinline__ A larger(A a, A b) { return b > a ? b : a; }
+template <int G, typename A>
+__device__ __forceinline__ A lane_max(A v) {
+  v = larger(v, rotated16<8>(v));
+  v = larger(v, rotated16<4>(v));
+  v = larger(v, rotated16<2>(v));
+  v = larger(v, rotated16<1>(v));
+#pragma unroll
+  for (int o = 16; o < G; o <<= 1) v = larger(v, (A)__shfl_xor(v, o, 64));
   return v;
 }

@@ -10,7 +10,6 @@ views are copied.  There is no CPU path.
 import ctypes as C
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -41,11 +40,14 @@ def _forward(x, weight, bias, eps, dev, code, wcode, keep):
     w = None if weight is None else weight.detach().contiguous()
     b = None if bias is None else bias.detach().contiguous()
     y = torch.empty(x.shape, device=dev, dtype=x.dtype)
-    stats = torch.empty((2, n), device=dev, dtype=torch.float64 if x.dtype == torch.float64 else torch.float32) if keep else None
+    stats = mean = rstd = None
+    if keep:  # the rows' means, then their reciprocal deviations
+        stats = torch.empty(2 * n, device=dev, dtype=torch.float64 if code == _lib.VMF_F64 else torch.float32)
+        mean = stats.data_ptr()
+        rstd = mean + n * stats.element_size()
     with _lib.on_device(dev):
-        rc = _lib.lib().vmf_layer_norm_fwd(_lib.ptr(rows), stride, _lib.ptr(w), _lib.ptr(b), _lib.ptr(y),
-                                           _lib.ptr(stats[0]) if keep else None, _lib.ptr(stats[1]) if keep else None,
-                                           n, width, eps, code, wcode, _lib.stream_ptr(dev))
+        rc = _lib.lib().vmf_layer_norm_fwd(rows.data_ptr(), stride, _lib.address(w), _lib.address(b), y.data_ptr(),
+                                           mean, rstd, n, width, eps, code, wcode, _lib.raw_stream(dev))
     _lib.check(rc, "vmf_layer_norm_fwd")
     return y, rows, stride, w, stats
 
@@ -55,33 +57,31 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps, dev, code, wcode):
         y, rows, stride, w, stats = _forward(x, weight, bias, eps, dev, code, wcode, True)
         ctx.save_for_backward(rows, w, stats)
-        ctx.meta = (x.shape, stride, None if bias is None else bias.dtype, code, wcode)
+        ctx.meta = (x.shape, stride, None if bias is None else bias.dtype, code, wcode, dev)
         return y
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, gy):
         rows, w, stats = ctx.saved_tensors
-        shape, x_stride, bias_dtype, code, wcode = ctx.meta
-        dev = rows.device
+        shape, x_stride, bias_dtype, code, wcode, dev = ctx.meta
         g, g_stride = _lib.as_rows(gy)
         n, width = rows.shape
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         gx = torch.empty(shape, device=dev, dtype=rows.dtype) if need_x else None
         gw = torch.empty(width, device=dev, dtype=w.dtype) if need_w else None
         gb = torch.empty(width, device=dev, dtype=bias_dtype) if need_b else None
-        ws, ws_bytes = None, 0
         lib = _lib.lib()
+        ws, need = None, C.c_int64(0)
         if need_w or need_b:
-            nb = C.c_int64(0)
-            _lib.check(lib.vmf_layer_norm_bwd_workspace(n, width, code, C.byref(nb)), "vmf_layer_norm_bwd_workspace")
-            ws_bytes = nb.value
-            ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+            _lib.check(lib.vmf_layer_norm_bwd_workspace(n, width, code, need), "vmf_layer_norm_bwd_workspace")
+            ws = torch.empty(need.value, device=dev, dtype=torch.uint8)
+        mean = stats.data_ptr()
         with _lib.on_device(dev):
-            rc = lib.vmf_layer_norm_bwd(_lib.ptr(rows), x_stride, _lib.ptr(g), g_stride, _lib.ptr(w),
-                                        _lib.ptr(stats[0]), _lib.ptr(stats[1]), _lib.ptr(gx), _lib.ptr(gw),
-                                        _lib.ptr(gb), n, width, _lib.ptr(ws), ws_bytes, code, wcode,
-                                        _lib.stream_ptr(dev))
+            rc = lib.vmf_layer_norm_bwd(rows.data_ptr(), x_stride, g.data_ptr(), g_stride, _lib.address(w), mean,
+                                        mean + n * stats.element_size(), _lib.address(gx), _lib.address(gw),
+                                        _lib.address(gb), n, width, _lib.address(ws), need.value, code, wcode,
+                                        _lib.raw_stream(dev))
         _lib.check(rc, "vmf_layer_norm_bwd")
         return gx, gw, gb, None, None, None, None
 

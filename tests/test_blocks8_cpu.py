@@ -80,10 +80,35 @@ def test_c_entry_refusals():
     assert matmul(k=1 << 16, ws=p, nbytes=need.value - 1) == -1 and b"workspace" in lib.vmf_last_error_string()
 
     def weight_grad(m=4, n=4, k=8, g=p, gw=p, dtype=0, out_dtype=0, ws=None, nbytes=0):
-        return lib.vmf_blocks8_weight_grad(g, 8, p, p, -(-m // 16) * 16, gw, None, m, n, k, ws, nbytes, dtype, out_dtype,
+        return lib.vmf_blocks8_weight_grad(g, 8, p, p, -(-m // 16) * 16, gw, None, None, None, 0, m, n, k, ws, nbytes, dtype, out_dtype,
                                            None)
 
     assert weight_grad(m=-1) == -1 and weight_grad(g=None) == -1 and weight_grad(gw=None) == -1
     assert weight_grad(dtype=3, out_dtype=2) == -2 and weight_grad(n=0) == 0
-    assert lib.vmf_blocks8_weight_grad_workspace(1 << 16, 128, 128, need) == 0 and need.value > 0
+    assert lib.vmf_blocks8_weight_grad_workspace(1 << 16, 128, 128, 0, need) == 0 and need.value > 0
     assert weight_grad(m=1 << 16, n=128, k=128, ws=p, nbytes=need.value - 1) == -1
+
+
+def test_layer_entry_refusals():
+    lib = _lib.lib()
+    p = C.c_void_p(256)
+    need = C.c_int64(0)
+    assert lib.vmf_blocks8_linear_fwd_workspace(4, 4, 8, 0, need) == 0 and need.value > 0
+
+    def fwd(m=4, n=4, k=8, weight=p, dtype=0, w_dtype=0, act=0, nbytes=need.value, ws=p, wt=None, wte=None):
+        return lib.vmf_blocks8_linear_fwd(p, 8, weight, 8, w_dtype, None, None, wt, wte, None, 0, act, 1.0, p, p, 16, p, m, n,
+                                          k, ws, nbytes, dtype, None)
+
+    assert fwd(m=-1) == -1 and fwd(n=0) == -1 and fwd(k=0) == -1 and fwd(act=3) == -1
+    assert fwd(nbytes=need.value - 1) == -1 and fwd(ws=C.c_void_p(264)) == -1 and fwd(wt=p) == -1
+    assert fwd(dtype=3, w_dtype=2) == -2
+    assert fwd(m=0, weight=None) == 0  # no rows and no weight to lay out: nothing to do
+    assert lib.vmf_blocks8_linear_bwd_workspace(4, 4, 8, 0, need) == 0 and need.value > 0
+    assert lib.vmf_blocks8_linear_bwd_workspace(4, 0, 8, 0, need) == -1
+    assert lib.vmf_blocks8_linear_bwd_workspace(4, 4, 8, 0, need) == 0
+
+    def bwd(m=4, n=4, k=8, gx=p, gw=p, gb=p, wt=p, nbytes=need.value, w_dtype=0):
+        return lib.vmf_blocks8_linear_bwd(p, 8, p, p, 16, wt, p, 0, 1.0, gx, gw, gb, m, n, k, p, nbytes, 0, w_dtype, None)
+
+    assert bwd(m=-1) == -1 and bwd(gw=None) == -1 and bwd(wt=None) == -1 and bwd(nbytes=need.value - 1) == -1
+    assert bwd(w_dtype=2) == -2

@@ -296,7 +296,7 @@ def layer_formula(x, w, b, gy, activation, beta):
 @pytest.mark.parametrize("x_type,w_type", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
                                            (torch.float16, torch.float32)])
 @pytest.mark.parametrize("activation,beta", [(None, 1.0), ("softplus", 1.0), ("softplus", 3.0)])
-@pytest.mark.parametrize("m,n,k", [(1, 64, 200), (33, 129, 100), (128, 128, 128), (1500, 300, 260), (2048, 2100, 300)])
+@pytest.mark.parametrize("m,n,k", [(1, 64, 200), (33, 129, 100), (37, 785, 1000), (128, 128, 128), (1500, 300, 260), (2048, 2100, 300)])
 def test_linear(m, n, k, activation, beta, x_type, w_type):
     x = normal(m, k, seed=1, scale=2.0).to(x_type).requires_grad_()
     w = normal(n, k, seed=2, scale=k ** -0.5).to(w_type).requires_grad_()
