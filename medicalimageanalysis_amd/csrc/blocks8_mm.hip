@@ -46,14 +46,15 @@ struct MmArgs {
 };
 
 // F exponent bytes of the rows row0 + F * (lane & 15) + 0..F-1, in one word.  Rows behind the last one get some byte of
-// the array (their products are dropped).
+// the array (their products are dropped).  A tile's one byte is repeated by spread_exps, later: an operation on the loaded
+// value would wait for every load before it, the next stage's among them.
 template <int F>
 __device__ __forceinline__ int load_exps(const Operand& o, int64_t kb, int64_t row0, int lane) {
   const uint8_t* e = o.exps + kb * o.exp_pitch;
   if (o.tiled) {
     int64_t r = row0 >> 7;
     r = r < o.exp_pitch ? r : o.exp_pitch - 1;
-    return (int)e[r] * 0x01010101;
+    return e[r];
   }
   int64_t r = row0 + F * (lane & 15);
   const int64_t last = o.exp_pitch - F;
@@ -62,6 +63,7 @@ __device__ __forceinline__ int load_exps(const Operand& o, int64_t kb, int64_t r
   if constexpr (F == 2) return *reinterpret_cast<const uint16_t*>(e + r);
   return e[r];
 }
+__device__ __forceinline__ int spread_exps(const Operand& o, int raw) { return o.tiled ? raw * 0x01010101 : raw; }
 
 // acc += A B for one block column of a 16 x 16 tile; IA, IB: which byte of the exponent words
 template <int IA, int IB>
@@ -116,6 +118,61 @@ __device__ __forceinline__ void finish(const MmArgs& p, int64_t row, int64_t col
   store_some<NC>((OUT*)p.out + row * p.n + col, p.n - col, v);
 }
 
+// Workgroup b runs on XCD b % 8: give each XCD a contiguous run of tiles, and walk the run in columns of 8 row tiles, so
+// that the rows and columns in use at a time fit its L2.
+__device__ __forceinline__ void tile_of(const MmArgs& p, int id, int& mt, int& nt) {
+  const int tiles = p.mt * p.nt, q = tiles >> 3, r = tiles & 7, x = id & 7;
+  id = x * q + (x < r ? x : r) + (id >> 3);
+  const int group = id / (8 * p.nt), first = group * 8, high = p.mt - first < 8 ? p.mt - first : 8;
+  const int in_group = id - group * 8 * p.nt;
+  mt = first + in_group % high;
+  nt = in_group / high;
+}
+// The row of an operand whose 16-byte pieces lie at place `at` of a stage's part for it (F: row tiles that share an
+// exponent word), and the piece that lies there.
+template <int F>
+__device__ __forceinline__ int row_at(int at) {
+  const int tile = at >> 4;
+  return tile / F * (16 * F) + F * (at & 15) + tile % F;
+}
+// a 16-row operand tile from LDS: lane l gets row l % 16, the 32 bytes of quarter l / 16
+__device__ __forceinline__ v8i operand(const uint8_t* tile, int lane) {
+  const int q = lane & 15, c = (lane >> 4) * 2;
+  const v4i lo = *reinterpret_cast<const v4i*>(tile + q * B8 + ((c ^ (q >> 1)) << 4));
+  const v4i hi = *reinterpret_cast<const v4i*>(tile + q * B8 + (((c + 1) ^ (q >> 1)) << 4));
+  return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+}
+// what a wave holds of the result: lane l has rows FM * (4 * (l / 16) + r) + i, columns FN * (l % 16) + 0 .. FN - 1 of
+// each group of 16 FM rows and 16 FN columns
+template <int FM, int FN, int GM, int GN, typename OUT>
+__device__ __forceinline__ void write_tile(const MmArgs& p, const v4f (&acc)[GM * FM][GN * FN], int64_t row0, int64_t col0,
+                                           int lane) {
+#pragma unroll
+  for (int h = 0; h < GN; ++h) {
+    const int64_t col = col0 + h * 16 * FN + FN * (lane & 15);
+    if (col >= p.n) continue;
+    float bias[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) bias[j] = p.bias && !p.partial && col + j < p.n ? load_bias(p.bias, p.bias_code, col + j) : 0.0f;
+#pragma unroll
+    for (int g = 0; g < GM; ++g)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+          const int64_t row = row0 + g * 16 * FM + FM * (4 * (lane >> 4) + r) + i;
+          if (row >= p.m) continue;
+          float v[FN];
+#pragma unroll
+          for (int j = 0; j < FN; ++j) v[j] = acc[g * FM + i][h * FN + j][r];
+          if (p.partial)
+            store_some<FN>(p.partial + ((int64_t)blockIdx.y * p.m + row) * p.n + col, p.n - col, v);
+          else
+            finish<FN, OUT>(p, row, col, bias, v);
+        }
+  }
+}
+
 // Tile of BM x BN over the block columns, waves of WM x WN side by side.
 //   LDS: two stages of the tile's rows of 128 bytes, filled by loads that go from global memory straight into LDS; while
 //   one stage is multiplied the next is on its way, one barrier per block column.
@@ -134,17 +191,9 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // Workgroup b runs on XCD b % 8: give each XCD a contiguous run of tiles, and walk the run in columns of 8 row tiles, so
-  // that the rows and columns in use at a time fit its L2.
-  const int tiles = p.mt * p.nt;
-  int id = (int)blockIdx.x;
-  {
-    const int q = tiles >> 3, r = tiles & 7, x = id & 7;
-    id = x * q + (x < r ? x : r) + (id >> 3);
-  }
-  const int group = id / (8 * p.nt), first = group * 8, high = p.mt - first < 8 ? p.mt - first : 8;
-  const int in_group = id - group * 8 * p.nt;
-  const int64_t m0 = (int64_t)(first + in_group % high) * BM, n0 = (int64_t)(in_group / high) * BN;
+  int mt, nt;
+  tile_of(p, (int)blockIdx.x, mt, nt);
+  const int64_t m0 = (int64_t)mt * BM, n0 = (int64_t)nt * BN;
   const int kb0 = (int)blockIdx.y * p.blocks_per_split;
   const int kb1 = kb0 + p.blocks_per_split < p.blocks ? kb0 + p.blocks_per_split : p.blocks;
 
@@ -155,8 +204,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p
     const int r8 = wave * LOADS + i;  // eight rows of the stage: first A's, then B's
     const bool is_b = r8 >= BM / 8;
     const int at = (is_b ? r8 - BM / 8 : r8) * 8 + (lane >> 3), q = at & 15;  // the row's place in LDS
-    const int f = is_b ? FN : FM, tile = at >> 4;
-    const int r = tile / f * (16 * f) + f * q + tile % f;
+    const int r = is_b ? row_at<FN>(at) : row_at<FM>(at);
     const int piece = (lane & 7) ^ (q >> 1);
     const Operand& o = is_b ? p.b : p.a;
     int64_t row = (is_b ? n0 : m0) + r;
@@ -184,13 +232,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p
 #pragma unroll
     for (int g = 0; g < GN; ++g) eb[slot][g] = load_exps<FN>(p.b, kb, n0 + wn + g * 16 * FN, lane);
   };
-  auto operand = [&](const uint8_t* tile) -> v8i {  // 16 rows of LDS
-    const int q = lane & 15, c = (lane >> 4) * 2;
-    const v4i lo = *reinterpret_cast<const v4i*>(tile + q * B8 + ((c ^ (q >> 1)) << 4));
-    const v4i hi = *reinterpret_cast<const v4i*>(tile + q * B8 + (((c + 1) ^ (q >> 1)) << 4));
-    return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-  };
-  auto multiply = [&](int stage, const int* xa, const int* xb) {
+  auto multiply = [&](int stage, const int* xa, const int* xb, auto&& then) {
     const uint8_t* A = lds + stage * STAGE;
     const uint8_t* B = A + BM * B8;
 #pragma unroll
@@ -198,12 +240,13 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p
       if constexpr (!WIDE) {
         v8i a[FM];
 #pragma unroll
-        for (int i = 0; i < FM; ++i) a[i] = operand(A + (wm + (g * FM + i) * 16) * B8);
+        for (int i = 0; i < FM; ++i) a[i] = operand(A + (wm + (g * FM + i) * 16) * B8, lane);
+        if (g == 0) then();
 #pragma unroll
         for (int h = 0; h < GN; ++h)
           static_for<FN>([&](auto J) {
             constexpr int j = decltype(J)::value;
-            const v8i b = operand(B + (wn + (h * FN + j) * 16) * B8);
+            const v8i b = operand(B + (wn + (h * FN + j) * 16) * B8, lane);
             static_for<FM>([&](auto I) {
               constexpr int i = decltype(I)::value;
               v4f& c = acc[g * FM + i][h * FN + j];
@@ -214,12 +257,13 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p
         v8b a[FM][4], b[4];
 #pragma unroll
         for (int i = 0; i < FM; ++i)
-          to_bf16(operand(A + (wm + (g * FM + i) * 16) * B8), b8_scale((xa[g] >> (8 * i)) & 0xff), a[i]);
+          to_bf16(operand(A + (wm + (g * FM + i) * 16) * B8, lane), b8_scale((xa[g] >> (8 * i)) & 0xff), a[i]);
+        if (g == 0) then();
 #pragma unroll
         for (int h = 0; h < GN; ++h)
 #pragma unroll
           for (int j = 0; j < FN; ++j) {
-            to_bf16(operand(B + (wn + (h * FN + j) * 16) * B8), b8_scale((xb[h] >> (8 * j)) & 0xff), b);
+            to_bf16(operand(B + (wn + (h * FN + j) * 16) * B8, lane), b8_scale((xb[h] >> (8 * j)) & 0xff), b);
 #pragma unroll
             for (int i = 0; i < FM; ++i) acc[g * FM + i][h * FN + j] = mm_step_bf16(a[i], b, acc[g * FM + i][h * FN + j]);
           }
@@ -238,40 +282,155 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p
         // this wave's share of the stage has arrived; after the barrier everyone's has, and the other stage is free
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (kb + half + 1 < kb1) {
-          fetch(kb + half + 1, half ^ 1);
-          fetch_exps(kb + half + 1, half ^ 1);
-        }
-        multiply(half, ea[half], eb[half]);
+        int xa[GM], xb[GN];
+#pragma unroll
+        for (int g = 0; g < GM; ++g) xa[g] = spread_exps(p.a, ea[half][g]);
+#pragma unroll
+        for (int g = 0; g < GN; ++g) xb[g] = spread_exps(p.b, eb[half][g]);
+        multiply(half, xa, xb, [&] {  // (behind the first operand reads, which would wait in the queue otherwise)
+          if (kb + half + 1 < kb1) {
+            fetch(kb + half + 1, half ^ 1);
+            fetch_exps(kb + half + 1, half ^ 1);
+          }
+        });
       }
     }
   }
 
-  // lane: rows FM * (4 * (lane / 16) + r) + i, columns FN * (lane % 16) + 0 .. FN - 1 of each group
+  write_tile<FM, FN, GM, GN, OUT>(p, acc, m0 + wm, n0 + wn, lane);
+}
+
+// The same for large 16-bit results: tile of 256 x 256, eight waves of 128 x 64, a block column's 32 products per wave in
+// four phases of two row tiles and all four column tiles.  What a phase multiplies was read from LDS in the phase before,
+// also across block columns: the barrier that makes the next stage readable, and the stage read last writable, stands
+// before the last phase's products, whose operands are in registers by then.  The loads into LDS are spread over three
+// phases, so that they do not stand before the operand reads in the queue.
+// Bound: 2048 clocks of matrix instructions per block column and CU, against 1536 + 512 clocks of LDS reads and writes.
+// a by rows, b by tiles, as a layer has them.
+template <typename OUT>
+__global__ __launch_bounds__(512, 2) void mm_large_kernel(MmArgs p) {
+  constexpr int BM = 256, BN = 256, STAGE = (BM + BN) * B8;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int mt, nt;
+  tile_of(p, (int)blockIdx.x, mt, nt);
+  const int64_t m0 = (int64_t)mt * BM, n0 = (int64_t)nt * BN;
+  const int kb0 = (int)blockIdx.y * p.blocks_per_split;
+  const int kb1 = kb0 + p.blocks_per_split < p.blocks ? kb0 + p.blocks_per_split : p.blocks;
+  const int wm = (wave >> 2) * 128, wn = (wave & 3) * 64;
+
+  // waves 0 - 3 load A's rows, 4 - 7 B's, 64 each; offsets from the tile's first row fit 32 bits (rows of up to 2^22)
+  const Operand& mine = wave < 4 ? p.a : p.b;
+  const int64_t first = wave < 4 ? m0 : n0;
+  const uint8_t* base = mine.values + first * mine.pitch;
+  const int64_t last = mine.rows - 1 - first;
+  uint32_t off[8];
 #pragma unroll
-  for (int h = 0; h < GN; ++h) {
-    const int64_t col = n0 + wn + h * 16 * FN + FN * (lane & 15);
-    if (col >= p.n) continue;
-    float bias[FN];
-#pragma unroll
-    for (int j = 0; j < FN; ++j) bias[j] = p.bias && !p.partial && col + j < p.n ? load_bias(p.bias, p.bias_code, col + j) : 0.0f;
-#pragma unroll
-    for (int g = 0; g < GM; ++g)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int i = 0; i < FM; ++i) {
-          const int64_t row = m0 + wm + g * 16 * FM + FM * (4 * (lane >> 4) + r) + i;
-          if (row >= p.m) continue;
-          float v[FN];
-#pragma unroll
-          for (int j = 0; j < FN; ++j) v[j] = acc[g * FM + i][h * FN + j][r];
-          if (p.partial)
-            store_some<FN>(p.partial + ((int64_t)blockIdx.y * p.m + row) * p.n + col, p.n - col, v);
-          else
-            finish<FN, OUT>(p, row, col, bias, v);
-        }
+  for (int i = 0; i < 8; ++i) {
+    const int at = (wave & 3) * 64 + i * 8 + (lane >> 3), r = row_at<4>(at);
+    off[i] = (uint32_t)((r < last ? r : last) * mine.pitch) + (((lane & 7) ^ ((at & 15) >> 1)) << 4);
   }
+  auto load = [&](int kb, int stage, int i) {
+    __builtin_amdgcn_global_load_lds(GLOBAL_PTR(base + (int64_t)kb * B8 + off[i]),
+                                     LDS_PTR(void, lds + stage * STAGE + (wave * 8 + i) * 1024), 16, 0, 0);
+  };
+  // the exponents of this lane's 8 row tiles, in two words, and the byte of the wave's column tile
+  struct Exps {
+    int a0, a1, b;
+  };
+  const int64_t end = p.a.exp_pitch - 4, r0 = m0 + wm + 4 * (lane & 15), r1 = r0 + 64;
+  const uint8_t* ea0 = p.a.exps + (r0 < end ? r0 : end);
+  const uint8_t* ea1 = p.a.exps + (r1 < end ? r1 : end);
+  const int64_t ct = (n0 + wn) >> 7;
+  const uint8_t* eb = p.b.exps + (ct < p.b.exp_pitch ? ct : p.b.exp_pitch - 1);
+  auto load_exps_of = [&](int kb) {
+    return Exps{*reinterpret_cast<const int*>(ea0 + kb * p.a.exp_pitch), *reinterpret_cast<const int*>(ea1 + kb * p.a.exp_pitch),
+                eb[kb * p.b.exp_pitch]};
+  };
+
+  v4f acc[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = v4f{0, 0, 0, 0};
+  v8i a[2][2], b[4];
+  auto read_a = [&](int stage, int pair, v8i(&to)[2]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) to[i] = operand(lds + stage * STAGE + (wm + (2 * pair + i) * 16) * B8, lane);
+  };
+  auto read_b = [&](int stage, int j) { b[j] = operand(lds + stage * STAGE + (BM + wn + j * 16) * B8, lane); };
+  // row tiles 2 PAIR, 2 PAIR + 1 with column tile J
+  auto multiply = [&](const v8i(&row)[2], auto PAIR, auto J, const Exps& e) {
+    constexpr int j = decltype(J)::value, t = 2 * decltype(PAIR)::value;
+    const int xa = t < 4 ? e.a0 : e.a1;
+    acc[t][j] = mm_step<t % 4, j>(row[0], b[j], acc[t][j], xa, e.b);
+    acc[t + 1][j] = mm_step<t % 4 + 1, j>(row[1], b[j], acc[t + 1][j], xa, e.b);
+  };
+
+  // One block column.  MORE: how many follow (2: at least two).  No branch inside: products and reads keep their order.
+  Exps now, raw;
+  auto step = [&](int kb, int stage, auto MORE) {
+    constexpr int more = decltype(MORE)::value;
+    static_for<3>([&](auto P) {
+      constexpr int ph = decltype(P)::value;
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(a[ph & 1], P, std::integral_constant<int, 0>{}, now);
+      __builtin_amdgcn_sched_barrier(0);
+      read_a(stage, ph + 1, a[(ph + 1) & 1]);
+      if constexpr (more > 0 && ph < 2) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) load(kb + 1, stage ^ 1, 2 + 3 * ph + i);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      static_for<3>([&](auto J) { multiply(a[ph & 1], P, std::integral_constant<int, decltype(J)::value + 1>{}, now); });
+    });
+    __builtin_amdgcn_sched_barrier(0);
+    Exps then = now;
+    if constexpr (more > 0) {
+      // this wave's share of the next stage has arrived; after the barrier everyone's has, and everyone has read the
+      // last of this stage
+      // (the exponents pass through the wait, so that their first use does not bring one of its own)
+      asm volatile("s_waitcnt vmcnt(0)" : "+v"(raw.a0), "+v"(raw.a1), "+v"(raw.b) : : "memory");
+      __syncthreads();
+      then = Exps{raw.a0, raw.a1, raw.b * 0x01010101};
+      if constexpr (more > 1) {
+        raw = load_exps_of(kb + 2);
+        load(kb + 2, stage, 0);
+        load(kb + 2, stage, 1);
+      }
+      read_a(stage ^ 1, 0, a[0]);
+    }
+    static_for<4>([&](auto J) {
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(a[1], std::integral_constant<int, 3>{}, J, now);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (more > 0) read_b(stage ^ 1, decltype(J)::value);
+    });
+    __builtin_amdgcn_sched_barrier(0);
+    now = then;
+  };
+  if (kb0 < kb1) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) load(kb0, 0, i);
+    now = load_exps_of(kb0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    now.b *= 0x01010101;
+    read_a(0, 0, a[0]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) read_b(0, j);
+    int kb = kb0;
+    if (kb + 1 < kb1) {
+      raw = load_exps_of(kb0 + 1);
+      load(kb0 + 1, 1, 0);
+      load(kb0 + 1, 1, 1);
+      for (; kb + 2 < kb1; ++kb) step(kb, (kb - kb0) & 1, std::integral_constant<int, 2>{});
+      step(kb, (kb - kb0) & 1, std::integral_constant<int, 1>{});
+      ++kb;
+    }
+    step(kb, (kb - kb0) & 1, std::integral_constant<int, 0>{});
+  }
+  write_tile<4, 4, 2, 1, OUT>(p, acc, m0 + wm, n0 + wn, lane);
 }
 
 // Up to 16 rows: the weight's bytes are what there is to move.  A workgroup takes 16 columns, its eight waves share the
@@ -338,9 +497,9 @@ struct MmPlan {
   MmKind kind;
   int splits, per_split, mt, nt;
 };
-// The largest tile that still gives every compute unit (256) a workgroup; where even the smallest does not, the block
+// The largest tile (`large`: 256 x 256 among them) that still gives every compute unit (256) a workgroup; where even the smallest does not, the block
 // columns are split, at least four of them to a split.
-MmPlan mm_plan(int64_t m, int64_t n, int64_t blocks, bool wide) {
+MmPlan mm_plan(int64_t m, int64_t n, int64_t blocks, bool large) {
   MmPlan p;
   auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
   int64_t groups;
@@ -350,7 +509,7 @@ MmPlan mm_plan(int64_t m, int64_t n, int64_t blocks, bool wide) {
     p.nt = (int)((n + 15) / 16);
     groups = p.nt;
   } else {
-    const int t = !wide && tiles(256) >= 256 ? 256 : tiles(128) >= 256 ? 128 : 64;
+    const int t = large && tiles(256) >= 256 ? 256 : tiles(128) >= 256 ? 128 : 64;
     p.kind = t == 256 ? MM_256 : t == 128 ? MM_128 : MM_64;
     p.mt = (int)((m + t - 1) / t);
     p.nt = (int)((n + t - 1) / t);
@@ -371,7 +530,7 @@ void mm_launch(const MmPlan& pl, const MmArgs& a, hipStream_t st) {
   if (pl.kind == MM_FEW) mm_few_kernel<WIDE, OUT><<<grid, 512, 0, st>>>(a);
   else if (pl.kind == MM_64) mm_kernel<64, 64, 32, 32, WIDE, OUT><<<grid, 256, 0, st>>>(a);
   else if (pl.kind == MM_128) mm_kernel<128, 128, 64, 64, WIDE, OUT><<<grid, 256, 0, st>>>(a);
-  else if constexpr (!WIDE) mm_kernel<256, 256, 128, 64, false, OUT><<<grid, 512, 0, st>>>(a);
+  else if constexpr (!WIDE) mm_large_kernel<OUT><<<grid, 512, 0, st>>>(a);
   if (a.partial) mm_join_kernel<OUT><<<vmf_grid_for(a.m * a.n, 256, 1 << 14), 256, 0, st>>>(a, pl.splits);
 }
 
@@ -601,33 +760,44 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void wgrad_kernel(Wg
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
 
   int turn = 0;  // which k tile's workgroup writes gy's blocks of this step
-  if (m0 < m1) fetch(m0, ahead[0]);
-  if (m0 + WG_ROWS < m1) fetch(m0 + WG_ROWS, ahead[1]);
+  auto put_next = [&](int64_t m, const Step& st, int stage) {
+    put(m, st, stage, p.q && turn == kt);
+    turn = turn + 1 == p.kt ? 0 : turn + 1;
+  };
+  auto products = [&](const uint8_t* base, int s) {
+    v8b b[FK];
+#pragma unroll
+    for (int j = 0; j < FK; ++j) b[j] = transposed(base + NT * PLANE, PITCH_A, s, wk + 32 * j);
+#pragma unroll
+    for (int t = NT - 1; t >= 0; --t)
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        const v8b a = transposed(base + t * PLANE, PITCH_G, s, wn + 32 * i);
+#pragma unroll
+        for (int j = 0; j < FK; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[j], acc[i][j], 0, 0, 0);
+      }
+  };
+  // Between the two halves of a step's products the next step's rows go into the other stage (read last before the
+  // barrier), while the matrix unit still works on the first half.
+  if (m0 < m1) {
+    fetch(m0, ahead[0]);
+    put_next(m0, ahead[0], 0);
+    if (m0 + WG_ROWS < m1) fetch(m0 + WG_ROWS, ahead[1]);
+    if (m0 + 2 * WG_ROWS < m1) fetch(m0 + 2 * WG_ROWS, ahead[0]);
+  }
   for (int64_t mm = m0; mm < m1; mm += 2 * WG_ROWS) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int64_t m = mm + half * WG_ROWS;
       if (m < m1) {
-        put(m, ahead[half], half, p.q && turn == kt);
-        turn = turn + 1 == p.kt ? 0 : turn + 1;
-        if (m + 2 * WG_ROWS < m1) fetch(m + 2 * WG_ROWS, ahead[half]);
-        // one barrier is enough: this stage was last read before the previous one
         __syncthreads();
         const uint8_t* base = lds + half * STAGE;
-#pragma unroll
-        for (int s = 0; s < WG_ROWS; s += 16) {
-          v8b b[FK];
-#pragma unroll
-          for (int j = 0; j < FK; ++j) b[j] = transposed(base + NT * PLANE, PITCH_A, s, wk + 32 * j);
-#pragma unroll
-          for (int t = NT - 1; t >= 0; --t)
-#pragma unroll
-            for (int i = 0; i < FN; ++i) {
-              const v8b a = transposed(base + t * PLANE, PITCH_G, s, wn + 32 * i);
-#pragma unroll
-              for (int j = 0; j < FK; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[j], acc[i][j], 0, 0, 0);
-            }
+        products(base, 0);
+        if (m + WG_ROWS < m1) {
+          put_next(m + WG_ROWS, ahead[half ^ 1], half ^ 1);
+          if (m + 3 * WG_ROWS < m1) fetch(m + 3 * WG_ROWS, ahead[half ^ 1]);
         }
+        products(base, 16);
       }
     }
   }
@@ -735,7 +905,8 @@ extern "C" int vmf_blocks8_matmul_workspace(int64_t m, int64_t n, int64_t k, int
   VMF_REQUIRE(bytes_out, VMF_ERR_BAD_ARG, "vmf_blocks8_matmul_workspace: null pointer");
   *bytes_out = 0;
   if (m == 0 || n == 0) return VMF_OK;
-  const MmPlan pl = mm_plan(m, n, b8_blocks(k), out_dtype == VMF_F32);
+  // (no kind of operand makes a difference where the block columns are split)
+  const MmPlan pl = mm_plan(m, n, b8_blocks(k), false);
   if (pl.splits > 1) *bytes_out = (int64_t)pl.splits * m * n * 4;
   return VMF_OK;
 }
@@ -767,7 +938,7 @@ extern "C" int vmf_blocks8_matmul(const uint8_t* a, const uint8_t* a_exponents, 
   VMF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), VMF_ERR_BAD_ARG,
               "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)need);
   const int64_t blocks = b8_blocks(k);
-  const MmPlan pl = mm_plan(m, n, blocks, out_dtype == VMF_F32);
+  const MmPlan pl = mm_plan(m, n, blocks, out_dtype != VMF_F32 && !a_tiled && b_tiled);
   VMF_REQUIRE((int64_t)pl.mt * pl.nt <= 0x7fffffff, VMF_ERR_UNSUPPORTED, "%s: %lld x %lld results", what, (long long)m,
               (long long)n);
   MmArgs p;
