@@ -10,6 +10,8 @@
 // K = 8192 (the products of one instruction are aligned to the largest of them).  That is a hundredth of a step of a
 // 16-bit result, and it is used for those.  A 32-bit result is computed with the bf16 instruction instead: an element of
 // a block is exact in bf16, so are the products, and the sums are 32-bit (4e-8 at K = 1024).
+#include <type_traits>
+
 #include "blocks8_dev.h"
 
 namespace {
@@ -578,6 +580,100 @@ struct WgArgs {
   int nt, kt;
 };
 
+// 32 columns of the 16 rows that start at `rows`, as the operand of a 32 x 32 x 16 product: lane l gets column l % 32 of
+// rows 8 * (l / 32) .. + 7.  `at(row)` is where the row's 32 columns start.
+template <typename F>
+__device__ __forceinline__ v8b transposed(int lane, F&& at) {
+  const int q = lane & 15, grp = lane >> 4;
+  const int row = (grp >> 1) * 8 + (q >> 2), col = ((grp & 1) * 16 + (q & 3) * 4) * 2;
+  union {
+    v4s h[2];
+    v8b v;
+  } u;
+  u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(v4s, at(row) + col));
+  u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(v4s, at(row + 4) + col));
+  return u.v;
+}
+// a wave's part of the result: D of a product has column (k) lane % 32, rows (n) (e & 3) + 8 (e >> 2) + 4 (lane / 32)
+template <typename W, int FN, int FK>
+__device__ __forceinline__ void write_wgrad(const WgArgs& p, const v16f (&acc)[FN][FK], int64_t n0, int64_t k0, int lane) {
+#pragma unroll
+  for (int i = 0; i < FN; ++i)
+#pragma unroll
+    for (int j = 0; j < FK; ++j) {
+      const int64_t k = k0 + j * 32 + (lane & 31);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int64_t n = n0 + i * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
+        if (n < p.n && k < p.k) {
+          if (p.partial) p.partial[((int64_t)blockIdx.y * p.n + n) * p.k + k] = acc[i][j][e];
+          else ((W*)p.gw)[n * p.k + k] = (W)acc[i][j][e];
+        }
+      }
+    }
+}
+// gbias: SHARE threads have sums of the same BN columns (thread: row `share`, E columns from `col`); added in order
+template <typename W, int BN, int SHARE, int E>
+__device__ __forceinline__ void write_gbias(const WgArgs& p, uint8_t* lds, const float (&sum)[E], int share, int col,
+                                            int64_t n0) {
+  float* red = reinterpret_cast<float*>(lds);  // SHARE * BN floats
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < E; ++i) red[share * BN + col + i] = sum[i];
+  __syncthreads();
+  if (threadIdx.x < BN) {
+    float s = 0;
+#pragma unroll
+    for (int q = 0; q < SHARE; ++q) s += red[q * BN + threadIdx.x];
+    const int64_t n = n0 + threadIdx.x;
+    if (n < p.n) {
+      if (p.partial) p.partial[(int64_t)gridDim.y * p.n * p.k + (int64_t)blockIdx.y * p.n + n] = s;
+      else ((W*)p.gb)[n] = (W)s;
+    }
+  }
+}
+// E consecutive elements of gy's row `row` from column `col`, of a block that 128 / E neighbouring lanes hold: into gy's
+// 8-bit blocks.  `in`: the row is one of the batch.  top: the largest of the lane's sizes.
+template <int E>
+__device__ __forceinline__ void write_gy_block(const WgArgs& p, float (&v)[E], uint32_t top, int64_t row, int64_t col,
+                                               bool in) {
+  top = lane_max<B8 / E>(top);
+  if (top >= B8_INF) {
+    top = 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j) top = b8_size(v[j]) < B8_INF ? larger(top, b8_size(v[j])) : top;
+    top = lane_max<B8 / E>(top);
+  }
+  const int e = b8_exponent(__uint_as_float(top));
+  const float inv = b8_pow2(-e);
+#pragma unroll
+  for (int j = 0; j < E; ++j) v[j] *= inv;
+  if (e == B8_EMAX)
+#pragma unroll
+    for (int j = 0; j < E; ++j) v[j] = b8_cut(v[j]);
+  if (in && col < p.q_pitch) {
+    uint8_t* q = p.q + row * p.q_pitch + col;
+    if constexpr (E == 8) *reinterpret_cast<uint2*>(q) = uint2{b8_pack4(v), b8_pack4(v + 4)};
+    else *reinterpret_cast<uint32_t*>(q) = b8_pack4(v);
+    if ((col & (B8 - 1)) == 0) p.q_exps[(col >> 7) * p.q_exp_pitch + row] = (uint8_t)(e + 127);
+  }
+}
+// 16 elements of a as bf16
+__device__ __forceinline__ void expand16(v4i a, uint32_t exp_byte, uint4* out) {
+  const float scale = b8_scale(exp_byte);
+  union {
+    v2b h[8];
+    uint4 w[2];
+  } u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    u.h[2 * j] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a[j], scale, false);
+    u.h[2 * j + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a[j], scale, true);
+  }
+  out[0] = u.w[0];
+  out[1] = u.w[1];
+}
+
 // Tile of BN (n) x BK (k) over the batch's rows, 32 at a time; waves of WN x WK.
 //   gy's terms and a's values lie in LDS as bf16 rows and are read back transposed (the rows are the products' inner
 //   dimension).  Two stages, one barrier per 32 rows; the rows of two steps ahead are on their way in registers, as they
@@ -595,8 +691,8 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void wgrad_kernel(Wg
   constexpr int GP = BN / E;                      // pieces per row; divides THREADS, so a thread keeps its columns
   constexpr int GN = WG_ROWS * GP / THREADS;      // pieces per thread and step
   constexpr int AP = BK / 16, AN = WG_ROWS * AP / THREADS;
-  constexpr int PITCH_G = 2 * BN + 32, PITCH_A = 2 * BK + 32;  // bytes; 32 more than the row: the rows of a
-                                                               // transposed read start 8 banks apart
+  constexpr int PITCH_G = 2 * BN + 64, PITCH_A = 2 * BK + 64;  // bytes; 64 more than the row: the four rows of a
+                                                               // transposed read lie in different banks
   constexpr int PLANE = WG_ROWS * PITCH_G, STAGE = NT * PLANE + WG_ROWS * PITCH_A;
   static_assert(THREADS % GP == 0 && THREADS % AP == 0 && GN >= 1 && AN >= 1, "whole pieces");
   constexpr int FN = WN / 32, FK = WK / 32;
@@ -696,59 +792,11 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void wgrad_kernel(Wg
           else *reinterpret_cast<uint2*>(d + t * PLANE) = uint2{w[0], w[1]};
         }
       }
-      if (blocks) {  // 128 / E neighbouring lanes hold a block
-        top = lane_max<B8 / E>(top);
-        if (top >= B8_INF) {
-          top = 0;
-#pragma unroll
-          for (int j = 0; j < E; ++j) top = b8_size(v[j]) < B8_INF ? larger(top, b8_size(v[j])) : top;
-          top = lane_max<B8 / E>(top);
-        }
-        const int e = b8_exponent(__uint_as_float(top));
-        const float inv = b8_pow2(-e);
-#pragma unroll
-        for (int j = 0; j < E; ++j) v[j] *= inv;
-        if (e == B8_EMAX)
-#pragma unroll
-          for (int j = 0; j < E; ++j) v[j] = b8_cut(v[j]);
-        const int64_t row = m + r, col = n0 + gc;
-        if (row < m1 && col < p.q_pitch) {
-          uint8_t* q = p.q + row * p.q_pitch + col;
-          if constexpr (E == 8) *reinterpret_cast<uint2*>(q) = uint2{b8_pack4(v), b8_pack4(v + 4)};
-          else *reinterpret_cast<uint32_t*>(q) = b8_pack4(v);
-          if ((gc & (B8 - 1)) == 0) p.q_exps[(col >> 7) * p.q_exp_pitch + row] = (uint8_t)(e + 127);
-        }
-      }
+      if (blocks) write_gy_block<E>(p, v, top, m + r, n0 + gc, m + r < m1);
     }
 #pragma unroll
-    for (int i = 0; i < AN; ++i) {
-      const float scale = b8_scale(s.e[i]);
-      union {
-        v2b h[8];
-        uint4 w[2];
-      } u;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        u.h[2 * j] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(s.a[i][j], scale, false);
-        u.h[2 * j + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(s.a[i][j], scale, true);
-      }
-      uint4* d = reinterpret_cast<uint4*>(base + NT * PLANE + (ar + i * (THREADS / AP)) * PITCH_A + ac * 2);
-      d[0] = u.w[0];
-      d[1] = u.w[1];
-    }
-  };
-  // 32 columns from `col` of the 16 rows from `row`, as the operand of a 32 x 32 x 16 product: lane l gets column l % 32,
-  // rows 8 * (l / 32) .. + 7
-  auto transposed = [&](const uint8_t* plane, int pitch, int row, int col) -> v8b {
-    const int q = lane & 15, grp = lane >> 4;
-    const uint8_t* s = plane + (row + (grp >> 1) * 8 + (q >> 2)) * pitch + (col + (grp & 1) * 16 + (q & 3) * 4) * 2;
-    union {
-      v4s h[2];
-      v8b v;
-    } u;
-    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(v4s, s));
-    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(v4s, s + 4 * pitch));
-    return u.v;
+    for (int i = 0; i < AN; ++i)
+      expand16(s.a[i], s.e[i], reinterpret_cast<uint4*>(base + NT * PLANE + (ar + i * (THREADS / AP)) * PITCH_A + ac * 2));
   };
   const int wn = (wave / (BK / WK)) * WN, wk = (wave % (BK / WK)) * WK;
   v16f acc[FN][FK];
@@ -767,12 +815,12 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void wgrad_kernel(Wg
   auto products = [&](const uint8_t* base, int s) {
     v8b b[FK];
 #pragma unroll
-    for (int j = 0; j < FK; ++j) b[j] = transposed(base + NT * PLANE, PITCH_A, s, wk + 32 * j);
+    for (int j = 0; j < FK; ++j) b[j] = transposed(lane, [&](int r) { return base + NT * PLANE + (s + r) * PITCH_A + (wk + 32 * j) * 2; });
 #pragma unroll
     for (int t = NT - 1; t >= 0; --t)
 #pragma unroll
       for (int i = 0; i < FN; ++i) {
-        const v8b a = transposed(base + t * PLANE, PITCH_G, s, wn + 32 * i);
+        const v8b a = transposed(lane, [&](int r) { return base + t * PLANE + (s + r) * PITCH_G + (wn + 32 * i) * 2; });
 #pragma unroll
         for (int j = 0; j < FK; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[j], acc[i][j], 0, 0, 0);
       }
@@ -802,40 +850,163 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void wgrad_kernel(Wg
     }
   }
 
-  // D: column (k) lane % 32, rows (n) (e & 3) + 8 (e >> 2) + 4 (lane / 32)
-#pragma unroll
-  for (int i = 0; i < FN; ++i)
-#pragma unroll
-    for (int j = 0; j < FK; ++j) {
-      const int64_t k = k0 + wk + j * 32 + (lane & 31);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int64_t n = n0 + wn + i * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
-        if (n < p.n && k < p.k) {
-          if (p.partial) p.partial[((int64_t)blockIdx.y * p.n + n) * p.k + k] = acc[i][j][e];
-          else ((W*)p.gw)[n * p.k + k] = (W)acc[i][j][e];
-        }
+  write_wgrad<W, FN, FK>(p, acc, n0 + wn, k0 + wk, lane);
+  static_assert(THREADS / GP * BN * 4 <= 2 * STAGE, "the sums fit the stages");
+  if (sums) write_gbias<W, BN, THREADS / GP, E>(p, lds, gsum, gr, gc, n0);
+}
+
+// The same for bf16 gradients in whole aligned 16-byte pieces (n, the row stride and the address are multiples of 8
+// elements): tile of 256 x 256, eight waves of 128 x 64.  Each half of a step's products has its operands read while the
+// half before it is multiplied, across the barrier as well; the next step's rows go from registers into the other stage
+// between, and the rows after that are asked for.
+// Bound: 1024 clocks of matrix instructions per step and CU, against 640 + 256 clocks of LDS reads and writes.
+template <typename W>
+__global__ __launch_bounds__(512, 2) void wgrad_large_kernel(WgArgs p) {
+  constexpr int BN = 256, BK = 256, PITCH = 2 * 256 + 64, PLANE = WG_ROWS * PITCH, STAGE = 2 * PLANE;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // workgroup b runs on XCD b % 8: neighbouring tiles, which share gy's columns, on the same one
+  int id = (int)blockIdx.x;
+  {
+    const int tiles = p.nt * p.kt, q = tiles >> 3, r = tiles & 7, x = id & 7;
+    id = x * q + (x < r ? x : r) + (id >> 3);
+  }
+  const int nt = id / p.kt, kt = id % p.kt;
+  const int64_t n0 = (int64_t)nt * BN, k0 = (int64_t)kt * BK;
+  const int64_t m0 = (int64_t)blockIdx.y * p.rows_per_split;
+  const int rows = (int)(m0 + p.rows_per_split < p.m ? p.rows_per_split : p.m - m0);
+  const int steps = (rows + WG_ROWS - 1) / WG_ROWS;
+  const int wn = (wave >> 2) * 128, wk = (wave & 3) * 64;
+
+  // gy: the 8 values from gc of rows gr and gr + 16 of a step; a: the 16 values from ac of row ar.  Where a tile reaches
+  // behind the last column the first columns are read instead (their results are dropped).
+  const int gr = threadIdx.x >> 5, gc = (threadIdx.x & 31) * 8;
+  const int ar = threadIdx.x >> 4, ac = (threadIdx.x & 15) * 16;
+  const bool g_in = n0 + gc < p.n, a_in = k0 + ac < p.a.pitch;
+  const uint8_t* gsrc = (const uint8_t*)p.gy + ((m0 + gr) * p.gy_stride + n0 + (g_in ? gc : 0)) * 2;
+  const uint8_t* asrc = p.a.values + (m0 + ar) * p.a.pitch + k0 + (a_in ? ac : 0);
+  const uint8_t* esrc = p.a.exps + ((k0 + (a_in ? ac : 0)) >> 7) * p.a.exp_pitch + m0 + ar;
+  const int64_t g_half = 16 * p.gy_stride * 2, g_step = 2 * g_half, a_step = WG_ROWS * p.a.pitch;
+  v4i g[2], av;
+  uint32_t ae;
+  // the next step's rows; `left`: how many there are (32: no test)
+  auto load = [&](auto WHOLE, int left) {
+    if (decltype(WHOLE)::value) {
+      g[0] = *reinterpret_cast<const v4i*>(gsrc);
+      g[1] = *reinterpret_cast<const v4i*>(gsrc + g_half);
+      av = *reinterpret_cast<const v4i*>(asrc);
+      ae = *esrc;
+    } else {
+      g[0] = g[1] = av = v4i{0, 0, 0, 0};
+      ae = 127;
+      if (gr < left) g[0] = *reinterpret_cast<const v4i*>(gsrc);
+      if (gr + 16 < left) g[1] = *reinterpret_cast<const v4i*>(gsrc + g_half);
+      if (ar < left) {
+        av = *reinterpret_cast<const v4i*>(asrc);
+        ae = *esrc;
       }
     }
-  if (!sums) return;
-  // gbias: the threads that share columns add their sums in order
-  constexpr int SHARE = THREADS / GP;
-  float* red = reinterpret_cast<float*>(lds);
-  static_assert(SHARE * BN * 4 <= 2 * STAGE, "the sums fit the stages");
-  __syncthreads();
+    gsrc += g_step;
+    asrc += a_step;
+    esrc += WG_ROWS;
+  };
+  uint8_t* const g_to = lds + gr * PITCH + gc * 2;
+  uint8_t* const a_to = lds + PLANE + ar * PITCH + ac * 2;
+  auto put = [&](int stage) {
+    *reinterpret_cast<v4i*>(g_to + stage * STAGE) = g[0];
+    *reinterpret_cast<v4i*>(g_to + stage * STAGE + 16 * PITCH) = g[1];
+    expand16(av, ae, reinterpret_cast<uint4*>(a_to + stage * STAGE));
+  };
+  // gbias and gy's blocks, from the rows in registers (those of step t)
+  const bool sums = kt == 0 && p.gb;
+  float gsum[8];
 #pragma unroll
-  for (int i = 0; i < E; ++i) red[gr * BN + gc + i] = gsum[i];
-  __syncthreads();
-  if (threadIdx.x < BN) {
-    float s = 0;
+  for (int i = 0; i < 8; ++i) gsum[i] = 0;
+  int turn = 0;  // which k tile's workgroup writes the blocks of this step
+  auto side = [&](int t) {
+    const bool blocks = p.q && turn == kt;
+    turn = turn + 1 == p.kt ? 0 : turn + 1;
+    if (!sums && !blocks) return;
 #pragma unroll
-    for (int q = 0; q < SHARE; ++q) s += red[q * BN + threadIdx.x];
-    const int64_t n = n0 + threadIdx.x;
-    if (n < p.n) {
-      if (p.partial) p.partial[(int64_t)gridDim.y * p.n * p.k + (int64_t)blockIdx.y * p.n + n] = s;
-      else ((W*)p.gb)[n] = (W)s;
+    for (int i = 0; i < 2; ++i) {
+      float v[8];
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = __uint_as_float(j & 1 ? (uint32_t)g[i][j >> 1] & 0xffff0000u : (uint32_t)g[i][j >> 1] << 16);
+        if (!g_in) v[j] = 0;
+        gsum[j] += v[j];
+        top = larger(top, b8_size(v[j]));
+      }
+      const int r = t * WG_ROWS + gr + 16 * i;
+      if (blocks) write_gy_block<8>(p, v, top, m0 + r, n0 + gc, r < rows);
     }
+  };
+
+  struct Half {
+    v8b g[4], a[2];
+  };
+  auto read_half = [&](int stage, int s, Half& h) {
+    const uint8_t* G = lds + stage * STAGE + s * PITCH + wn * 2;
+    const uint8_t* A = lds + stage * STAGE + PLANE + s * PITCH + wk * 2;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) h.a[j] = transposed(lane, [&](int r) { return A + r * PITCH + j * 64; });
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h.g[i] = transposed(lane, [&](int r) { return G + r * PITCH + i * 64; });
+  };
+  v16f acc[4][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+  auto multiply = [&](const Half& h, int from, int to) {
+#pragma unroll
+    for (int i = from; i < to; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(h.g[i], h.a[j], acc[i][j], 0, 0, 0);
+  };
+
+  Half h0, h1;
+  // MORE: how many steps follow (3: at least three)
+  auto step = [&](int t, auto MORE) {
+    constexpr int more = decltype(MORE)::value;
+    const int stage = t & 1;
+    if constexpr (more > 0) side(t + 1);
+    read_half(stage, 16, h1);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(h0, 0, 2);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (more > 0) put(stage ^ 1);
+    if constexpr (more > 2) load(std::true_type{}, 0);
+    if constexpr (more == 2) load(std::false_type{}, rows - (t + 2) * WG_ROWS);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(h0, 2, 4);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (more > 0) {
+      __syncthreads();  // the next step's rows are there, and this step's have been read
+      read_half(stage ^ 1, 0, h0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(h1, 0, 4);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (steps > 0) {
+    load(std::false_type{}, rows);
+    side(0);
+    put(0);
+    if (steps > 1) load(std::false_type{}, rows - WG_ROWS);
+    __syncthreads();
+    read_half(0, 0, h0);
+    int t = 0;
+    for (; t + 3 < steps; ++t) step(t, std::integral_constant<int, 3>{});
+    if (t + 2 < steps) step(t++, std::integral_constant<int, 2>{});
+    if (t + 1 < steps) step(t++, std::integral_constant<int, 1>{});
+    step(t, std::integral_constant<int, 0>{});
   }
+  write_wgrad<W, 4, 2>(p, acc, n0 + wn, k0 + wk, lane);
+  if (sums) write_gbias<W, BN, 16, 8>(p, lds, gsum, gr, gc, n0);
 }
 
 template <typename W>
@@ -876,6 +1047,12 @@ WgPlan wg_plan(int64_t m, int64_t n, int64_t k, int dtype) {
 template <typename T, typename W>
 void wgrad_launch(const WgPlan& pl, const WgArgs& p, hipStream_t st) {
   const dim3 grid((unsigned)(pl.nt * pl.kt), (unsigned)pl.splits);
+  if constexpr (std::is_same<T, bf16_t>::value) {
+    if (pl.tile == 256 && p.n % 8 == 0 && p.gy_stride % 8 == 0 && ((uintptr_t)p.gy & 15) == 0) {
+      wgrad_large_kernel<W><<<grid, 512, 0, st>>>(p);
+      return;
+    }
+  }
   if constexpr (sizeof(T) == 2) {
     if (pl.tile == 256) {
       wgrad_kernel<T, W, 256, 256, 128, 64><<<grid, 512, 0, st>>>(p);
