@@ -4,11 +4,6 @@
 
 namespace {
 
-// softplus in 64 bits, for the few values that lie next to a rounding border (see below)
-__device__ __noinline__ double softplus64(double h, double beta) {
-  const double t = beta * h;
-  return ((t > 0 ? t : 0) + ::log1p(::exp(-::fabs(t)))) / beta;
-}
 // In 32 bits, from the hardware's exponential and logarithm (1 unit in the last place each):
 //   log(1 + u), u = exp(-|t|): where 1 + u drops too much of u (u < 1/16), the series to u^6 (the rest is under u^6 / 7
 //   of it); else ln 2 * log2(1 + u), off by 2^-24 / u <= 2^-20.
@@ -23,6 +18,43 @@ __device__ __forceinline__ float softplus32(float h, float beta, float inv_beta)
   return (fmaxf(t, 0.0f) + l) * inv_beta;
 }
 __device__ __forceinline__ float softplus_margin(float h, float beta) { return 3e-6f + 3e-7f * fmaxf(-beta * h, 0.0f); }
+
+// exp in 64 bits: t = n ln 2 + r, |r| <= 0.35, and the power series of exp(r) to r^13 (the next term is under 5e-18)
+__device__ __forceinline__ double exp64(double t) {
+  const double n = ::rint(t * 1.4426950408889634);
+  const double r = ::fma(-n, 2.3190468138462996e-17, ::fma(-n, 0.69314718055994531, t));
+  double s = 1.0 / 6227020800.0;
+  s = ::fma(s, r, 1.0 / 479001600.0);
+  s = ::fma(s, r, 1.0 / 39916800.0);
+  s = ::fma(s, r, 1.0 / 3628800.0);
+  s = ::fma(s, r, 1.0 / 362880.0);
+  s = ::fma(s, r, 1.0 / 40320.0);
+  s = ::fma(s, r, 1.0 / 5040.0);
+  s = ::fma(s, r, 1.0 / 720.0);
+  s = ::fma(s, r, 1.0 / 120.0);
+  s = ::fma(s, r, 1.0 / 24.0);
+  s = ::fma(s, r, 1.0 / 6.0);
+  s = ::fma(s, r, 0.5);
+  s = ::fma(s, r, 1.0);
+  s = ::fma(s, r, 1.0);
+  return ::ldexp(s, n < -1100 ? -1100 : (int)n);
+}
+// softplus to 40 bits and more, for the few values that lie next to a rounding border (see softplus8).
+// l = log(1 + u), u = exp(-|t|): for small u its series; else from the 32-bit l0, with d = (1 + u) exp(-l0) - 1 under 1e-5,
+// l = l0 + log(1 + d) = l0 + d - d^2 / 2 + d^3 / 3.
+__device__ __noinline__ double softplus64(double h, double beta) {
+  const double t = beta * h;
+  const double u = exp64(-::fabs(t));
+  double l;
+  if (u < 1.0 / 4096) {
+    l = u * ::fma(u, ::fma(u, ::fma(u, -0.25, 1.0 / 3), -0.5), 1.0);
+  } else {
+    const double l0 = (double)(0.69314718f * __builtin_amdgcn_logf((float)(1.0 + u)));
+    const double d = ::fma(1.0 + u, exp64(-l0), -1.0);
+    l = l0 + d * ::fma(d, ::fma(d, 1.0 / 3, -0.5), 1.0);
+  }
+  return ((t > 0 ? t : 0) + l) / beta;
+}
 
 // a double in [0, 448] -> the float from which a second rounding to fewer bits gives what one rounding of the double
 // would: truncated, with the last bit set if anything was cut off
@@ -92,18 +124,19 @@ __device__ __forceinline__ uint2 softplus8(const float (&h)[8], float beta, floa
     lo[i] = fmaf(a, -m, a);
     hi[i] = fmaf(a, m, a);
   }
-  uint2 r{b8_pack4(lo), b8_pack4(lo + 4)};
-  if (r.x != b8_pack4(hi) || r.y != b8_pack4(hi + 4) || e == B8_EMAX) {
-    uint32_t w[4];
+  uint32_t w[2] = {b8_pack4(lo), b8_pack4(lo + 4)};
+  const uint32_t x[2] = {w[0] ^ b8_pack4(hi), w[1] ^ b8_pack4(hi + 4)};
+  if ((x[0] | x[1]) != 0 || e == B8_EMAX) {
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      w[p] = b8_pack2(lo[2 * p], lo[2 * p + 1]);
-      if (w[p] != b8_pack2(hi[2 * p], hi[2 * p + 1]) || e == B8_EMAX)
-        w[p] = b8_pack2(softplus_scaled(h[2 * p], beta64, e), softplus_scaled(h[2 * p + 1], beta64, e));
+    for (int i = 0; i < 8; ++i) {
+      const int at = 8 * (i & 3);
+      if ((x[i >> 2] >> at & 0xff) != 0 || e == B8_EMAX) {
+        const float v = softplus_scaled(h[i], beta64, e);
+        w[i >> 2] = (w[i >> 2] & ~(0xffu << at)) | (b8_pack2(v, v) & 0xff) << at;
+      }
     }
-    r = uint2{w[0] | w[1] << 16, w[2] | w[3] << 16};
   }
-  return r;
+  return uint2{w[0], w[1]};
 }
 
 // A workgroup has 16 groups of 16 lanes: 1 << row_bits of them side by side in rows (so that the exponent bytes of

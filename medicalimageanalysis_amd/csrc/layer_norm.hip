@@ -133,20 +133,21 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__
   }
 }
 
-// Backward.  A lane keeps the same columns for every row it sees, so gw and gb grow in its registers; a workgroup
-// leaves one partial row of each (after adding its rows side by side in LDS), and ln_reduce_kernel adds the
-// workgroups' partials in a fixed order: the same bits on every run.
-template <typename T, typename W, int TPR, int NCH>
-__global__ __launch_bounds__(TPR > THREADS ? TPR : THREADS) void ln_bwd_kernel(
-    const T* __restrict__ x, int64_t x_stride, const T* __restrict__ gy, int64_t gy_stride, const W* __restrict__ w,
-    const typename AccOf<T>::type* __restrict__ mean_in, const typename AccOf<T>::type* __restrict__ rstd_in,
-    T* __restrict__ gx, typename AccOf<T>::type* __restrict__ partial, int64_t n, int width) {
+// The backward pass of the rows that a workgroup of NT threads takes (TPR to a row, the workgroup's rows `step` apart).
+// A lane keeps the same columns for every row it sees, so gw and gb grow in its registers (SUMS); at the end the rows
+// side by side are added in LDS, in order, into one partial row of each per workgroup.
+template <typename T, typename W, int NT, int TPR, int NCH, bool SUMS>
+__device__ __forceinline__ void ln_bwd_rows(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ gy,
+                                            int64_t gy_stride, const W* __restrict__ w,
+                                            const typename AccOf<T>::type* __restrict__ mean_in,
+                                            const typename AccOf<T>::type* __restrict__ rstd_in, T* __restrict__ gx,
+                                            typename AccOf<T>::type* __restrict__ partial, int64_t n, int width,
+                                            int64_t first, int64_t step) {
   using A = typename AccOf<T>::type;
   constexpr int V = LnVec<T>::value;
-  constexpr int NT = TPR > THREADS ? TPR : THREADS;
   constexpr int ROWS = NT / TPR;
   __shared__ A red[2 * (TPR > 64 ? TPR / 64 : 1)];
-  __shared__ A side[ROWS > 1 ? (ROWS - 1) * TPR * V : 1];
+  __shared__ A side[SUMS && ROWS > 1 ? (ROWS - 1) * TPR * V : 1];
   int flip = 0;
   const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   const A inv = (A)1 / (A)width;
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(TPR > THREADS ? TPR : THREADS) void ln_bwd_kernel(
       gw[c][i] = gb[c][i] = 0;
     }
   }
-  for (int64_t row = (int64_t)blockIdx.x * ROWS + sub; row < n; row += (int64_t)gridDim.x * ROWS) {
+  for (int64_t row = first + sub; row < n; row += step) {
     const T* xr = x + row * x_stride;
     const T* gr = gy + row * gy_stride;
     const A mean = mean_in[row], rstd = rstd_in[row];
@@ -178,8 +179,10 @@ __global__ __launch_bounds__(TPR > THREADS ? TPR : THREADS) void ln_bwd_kernel(
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         xh[c][i] = (xh[c][i] - mean) * rstd;
-        gw[c][i] += h[c][i] * xh[c][i];
-        gb[c][i] += h[c][i];
+        if constexpr (SUMS) {
+          gw[c][i] += h[c][i] * xh[c][i];
+          gb[c][i] += h[c][i];
+        }
         h[c][i] *= wv[c][i];
         s1 += h[c][i];
         s2 += h[c][i] * xh[c][i];
@@ -197,27 +200,81 @@ __global__ __launch_bounds__(TPR > THREADS ? TPR : THREADS) void ln_bwd_kernel(
       }
     }
   }
-  if (!partial) return;
-  A* out = partial + (int64_t)blockIdx.x * 2 * width;
+  if constexpr (SUMS) {
+    if (!partial) return;
 #pragma unroll
-  for (int which = 0; which < 2; ++which)
+    for (int which = 0; which < 2; ++which)
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-      A(&g)[V] = which ? gb[c] : gw[c];
-      if constexpr (ROWS > 1) {
-        __syncthreads();
-        if (sub > 0)
+      for (int c = 0; c < NCH; ++c) {
+        A(&g)[V] = which ? gb[c] : gw[c];
+        if constexpr (ROWS > 1) {
+          __syncthreads();
+          if (sub > 0)
 #pragma unroll
-          for (int i = 0; i < V; ++i) side[((sub - 1) * TPR + lane) * V + i] = g[i];
-        __syncthreads();
-        if (sub == 0)
-          for (int r = 0; r < ROWS - 1; ++r)
+            for (int i = 0; i < V; ++i) side[((sub - 1) * TPR + lane) * V + i] = g[i];
+          __syncthreads();
+          if (sub == 0)
+            for (int r = 0; r < ROWS - 1; ++r)
 #pragma unroll
-            for (int i = 0; i < V; ++i) g[i] += side[(r * TPR + lane) * V + i];
+              for (int i = 0; i < V; ++i) g[i] += side[(r * TPR + lane) * V + i];
+        }
+        const int col = (c * TPR + lane) * V;
+        if (sub == 0) store_some<V>(partial + (int64_t)which * width + col, (int64_t)width - col, g);
       }
-      const int col = (c * TPR + lane) * V;
-      if (sub == 0) store_some<V>(out + (int64_t)which * width + col, (int64_t)width - col, g);
+  }
+}
+// One partial row of gw and gb per workgroup; ln_reduce_kernel adds them in order: the same bits on every run.
+template <typename T, typename W, int NT, int TPR, int NCH>
+__global__ __launch_bounds__(NT) void ln_bwd_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ gy,
+                                                    int64_t gy_stride, const W* __restrict__ w,
+                                                    const typename AccOf<T>::type* __restrict__ mean_in,
+                                                    const typename AccOf<T>::type* __restrict__ rstd_in,
+                                                    T* __restrict__ gx, typename AccOf<T>::type* __restrict__ partial,
+                                                    int64_t n, int width) {
+  constexpr int ROWS = NT / TPR;
+  ln_bwd_rows<T, W, NT, TPR, NCH, true>(x, x_stride, gy, gy_stride, w, mean_in, rstd_in, gx,
+                                        partial ? partial + (int64_t)blockIdx.x * 2 * width : nullptr, n, width,
+                                        (int64_t)blockIdx.x * ROWS, (int64_t)gridDim.x * ROWS);
+}
+// Few rows: both results in one launch and without partials.  The first workgroups take the rows, the others 16 columns
+// each, which 16 threads share; x and gy are read twice, the second time out of the L2.
+template <typename T, typename W, int TPR, int NCH>
+__global__ __launch_bounds__(THREADS) void ln_bwd_few_kernel(const T* __restrict__ x, int64_t x_stride,
+                                                             const T* __restrict__ gy, int64_t gy_stride,
+                                                             const W* __restrict__ w,
+                                                             const typename AccOf<T>::type* __restrict__ mean_in,
+                                                             const typename AccOf<T>::type* __restrict__ rstd_in,
+                                                             T* __restrict__ gx, W* __restrict__ gw,
+                                                             W* __restrict__ gb, int n, int width, int row_groups) {
+  using A = typename AccOf<T>::type;
+  constexpr int ROWS = THREADS / TPR;
+  if ((int)blockIdx.x < row_groups) {
+    ln_bwd_rows<T, W, THREADS, TPR, NCH, false>(x, x_stride, gy, gy_stride, w, mean_in, rstd_in, gx, nullptr, n, width,
+                                                (int64_t)blockIdx.x * ROWS, (int64_t)row_groups * ROWS);
+    return;
+  }
+  __shared__ A sums[2][16][17];
+  const int c = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+  const int col = ((int)blockIdx.x - row_groups) * 16 + c;
+  A a = 0, b = 0;
+  if (col < width)
+#pragma unroll 4
+    for (int r = r0; r < n; r += 16) {
+      const A g = (A)gy[r * gy_stride + col];
+      a += g * (((A)x[r * x_stride + col] - mean_in[r]) * rstd_in[r]);
+      b += g;
     }
+  sums[0][r0][c] = a;
+  sums[1][r0][c] = b;
+  __syncthreads();
+  if (threadIdx.x < 32 && col < width) {  // threads 0 - 15: gw, 16 - 31: gb
+    const int which = threadIdx.x >> 4;
+    A s = 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s += sums[which][r][c];
+    W* out = which ? gb : gw;
+    if (out) out[col] = (W)s;
+  }
 }
 
 // Rows that do not fit: gx alone, a workgroup per row ...
@@ -304,12 +361,6 @@ __global__ __launch_bounds__(256) void ln_reduce_kernel(const A* __restrict__ pa
   }
 }
 
-// How many workgroups of the backward pass leave a partial: enough to fill 256 compute units, and no more than there
-// are rows to share (each partial costs 2 * width values written and read back).
-int bwd_groups(int64_t n, int rows_per_group) {
-  const int64_t g = (n + rows_per_group - 1) / rows_per_group;
-  return (int)(g < 512 ? (g < 1 ? 1 : g) : 512);
-}
 // lanes per row by the width in vectors of 16 bytes: as few as hold the row in at most `chunks` registers' worth each
 int lanes_for(int64_t vectors, int chunks) {
   for (int tpr = 16; tpr <= 1024; tpr *= tpr == 64 ? 4 : tpr == 256 ? 4 : 2)
@@ -331,7 +382,7 @@ void run_fwd(const void* x, int64_t xs, const void* w, const void* b, void* y, v
              int64_t width, double eps, hipStream_t st) {
   using A = typename AccOf<T>::type;
   constexpr int V = LnVec<T>::value;
-  constexpr int MAXC = 32 / V;  // 32 values per lane
+  constexpr int MAXC = 32 / V;  // 32 values per lane (64 in one wave instead of 16 in four: 65536x4096 bf16 0.36 ms against 0.26)
   const int64_t vectors = (width + V - 1) / V;
 #define LN_FWD(TPR, NCH) \
   if (vectors <= (int64_t)(TPR) * (NCH)) return launch_fwd<T, W, TPR, NCH>(x, xs, w, b, y, mean, rstd, n, width, eps, st)
@@ -351,13 +402,34 @@ void run_fwd(const void* x, int64_t xs, const void* w, const void* b, void* y, v
 
 template <typename T> constexpr int bwd_chunks() { return 16 / LnVec<T>::value; }  // 16 values per lane
 
-// partial rows of the backward pass (host arithmetic shared with the workspace query)
+// How the backward pass is launched (host arithmetic shared with the workspace query).
+struct BwdPlan {
+  int tpr;      // lanes per row; 0: rows that do not fit the registers
+  int threads;  // of a workgroup
+  int parts;    // workgroups, each leaving a partial row of gw and gb; 0: none are left (few rows)
+};
+// Few rows (up to 512, rows of up to 256 lanes): one launch.  Otherwise two workgroups for each of 256 compute units (four
+// where a row is four waves, whose barriers others then fill: 65536x4096 bf16 0.57 -> 0.36 ms; 1048576x784 fp32, a wave
+// to a row, 1.95 with two, 2.05 with four), but no more than have 32 rows each, since each leaves 2 * width values that are
+// written and read again.
 template <typename T>
-int bwd_parts(int64_t n, int64_t width) {
+BwdPlan bwd_plan(int64_t n, int64_t width) {
   constexpr int V = LnVec<T>::value;
-  const int tpr = lanes_for((width + V - 1) / V, bwd_chunks<T>());
-  if (tpr == 0) return bwd_groups(n, 64);
-  return bwd_groups(n, tpr < THREADS ? THREADS / tpr : 1);
+  BwdPlan p;
+  p.tpr = lanes_for((width + V - 1) / V, bwd_chunks<T>());
+  p.threads = p.tpr == 0 ? 256 : p.tpr > THREADS ? p.tpr : THREADS;
+  if (p.tpr != 0 && p.tpr <= THREADS && n <= 512) {
+    p.parts = 0;
+    return p;
+  }
+  const int64_t most = p.tpr == THREADS ? 1024 : 512;
+  // rows to a workgroup: 32, or as many as it has side by side, or fewer where that leaves compute units without one
+  const int64_t at_once = p.tpr == 0 ? 1 : p.threads / p.tpr;
+  const int64_t rows = at_once > 32 ? at_once : 32;
+  int64_t g = (n + rows - 1) / rows;
+  if (g < 256) g = (n + at_once - 1) / at_once < 256 ? (n + at_once - 1) / at_once : 256;
+  p.parts = (int)(g < 1 ? 1 : g > most ? most : g);
+  return p;
 }
 
 template <typename T, typename W>
@@ -366,36 +438,53 @@ int run_bwd(const void* x, int64_t xs, const void* gy, int64_t gs, const void* w
   using A = typename AccOf<T>::type;
   constexpr int V = LnVec<T>::value;
   constexpr int C = bwd_chunks<T>();
-  const int parts = bwd_parts<T>(n, width);
+  const BwdPlan pl = bwd_plan<T>(n, width);
   A* partial = gw || gb ? (A*)ws : nullptr;
   const int64_t vectors = (width + V - 1) / V;
-  const int tpr = lanes_for(vectors, C);
-#define LN_BWD(TPR, NCH)                                                                                        \
-  ln_bwd_kernel<T, W, TPR, NCH><<<parts, TPR > THREADS ? TPR : THREADS, 0, st>>>(                                \
-      (const T*)x, xs, (const T*)gy, gs, (const W*)w, (const A*)mean, (const A*)rstd, (T*)gx, partial, n, (int)width)
-  if (tpr == 16) {
-    if (vectors <= 16) LN_BWD(16, 1);
-    else LN_BWD(16, C);
-  } else if (tpr == 32) {
-    LN_BWD(32, C);
-  } else if (tpr == 64) {
-    LN_BWD(64, C);
-  } else if (tpr == 256) {
-    LN_BWD(256, C);
-  } else if (tpr == 1024) {
-    LN_BWD(1024, C);
+  if (pl.tpr != 0 && pl.parts == 0) {
+    const int rows = THREADS / pl.tpr;
+    const int row_groups = gx ? (int)((n + rows - 1) / rows) : 0;
+    const int grid = row_groups + (gw || gb ? (int)((width + 15) / 16) : 0);
+#define LN_FEW(TPR, NCH)                                                                                      \
+  ln_bwd_few_kernel<T, W, TPR, NCH><<<grid, THREADS, 0, st>>>((const T*)x, xs, (const T*)gy, gs, (const W*)w, \
+                                                              (const A*)mean, (const A*)rstd, (T*)gx, (W*)gw, \
+                                                              (W*)gb, (int)n, (int)width, row_groups)
+    if (grid > 0) {
+      if (pl.tpr == 16) LN_FEW(16, C);
+      else if (pl.tpr == 32) LN_FEW(32, C);
+      else if (pl.tpr == 64) LN_FEW(64, C);
+      else LN_FEW(256, C);
+    }
+#undef LN_FEW
+    return vmf_check_launch("vmf_layer_norm_bwd");
+  }
+#define LN_BWD(NT, TPR, NCH)                                                                                    \
+  ln_bwd_kernel<T, W, NT, TPR, NCH><<<pl.parts, NT, 0, st>>>((const T*)x, xs, (const T*)gy, gs, (const W*)w,      \
+                                                             (const A*)mean, (const A*)rstd, (T*)gx, partial, n, \
+                                                             (int)width)
+  if (pl.tpr == 16) {
+    if (vectors <= 16) LN_BWD(THREADS, 16, 1);
+    else LN_BWD(THREADS, 16, C);
+  } else if (pl.tpr == 32) {
+    LN_BWD(THREADS, 32, C);
+  } else if (pl.tpr == 64) {
+    LN_BWD(THREADS, 64, C);
+  } else if (pl.tpr == 256) {
+    LN_BWD(256, 256, C);
+  } else if (pl.tpr == 1024) {
+    LN_BWD(1024, 1024, C);
   } else {
     if (gx)
       ln_bwd_long_kernel<T, W><<<vmf_grid_for(n, 1, 1 << 16), 1024, 0, st>>>(
           (const T*)x, xs, (const T*)gy, gs, (const W*)w, (const A*)mean, (const A*)rstd, (T*)gx, n, width);
     if (partial)
-      ln_cols_kernel<T><<<dim3((unsigned)((width + 255) / 256), (unsigned)parts), 256, 0, st>>>(
+      ln_cols_kernel<T><<<dim3((unsigned)((width + 255) / 256), (unsigned)pl.parts), 256, 0, st>>>(
           (const T*)x, xs, (const T*)gy, gs, (const A*)mean, (const A*)rstd, partial, n, width);
   }
 #undef LN_BWD
   int rc = vmf_check_launch("vmf_layer_norm_bwd");
   if (rc != VMF_OK || !partial) return rc;
-  ln_reduce_kernel<A, W><<<(unsigned)((2 * width + 15) / 16), 256, 0, st>>>(partial, (W*)gw, (W*)gb, parts, width);
+  ln_reduce_kernel<A, W><<<(unsigned)((2 * width + 15) / 16), 256, 0, st>>>(partial, (W*)gw, (W*)gb, pl.parts, width);
   return vmf_check_launch("vmf_layer_norm_bwd sums");
 }
 
@@ -447,9 +536,9 @@ extern "C" int vmf_layer_norm_bwd_workspace(int64_t n, int64_t width, int dtype,
   if (rc != VMF_OK) return rc;
   VMF_REQUIRE(bytes_out, VMF_ERR_BAD_ARG, "vmf_layer_norm_bwd_workspace: null pointer");
   int parts;
-  if (dtype == VMF_F32) parts = bwd_parts<float>(n, width);
-  else if (dtype == VMF_F64) parts = bwd_parts<double>(n, width);
-  else parts = bwd_parts<f16_t>(n, width);
+  if (dtype == VMF_F32) parts = bwd_plan<float>(n, width).parts;
+  else if (dtype == VMF_F64) parts = bwd_plan<double>(n, width).parts;
+  else parts = bwd_plan<f16_t>(n, width).parts;
   *bytes_out = (int64_t)parts * 2 * width * (dtype == VMF_F64 ? 8 : 4);
   return VMF_OK;
 }
@@ -466,7 +555,7 @@ extern "C" int vmf_layer_norm_bwd(const void* x, int64_t x_stride, const void* g
   if (gweight || gbias) {
     int64_t need = 0;
     vmf_layer_norm_bwd_workspace(n, width, dtype, &need);
-    VMF_REQUIRE(workspace && workspace_bytes >= need, VMF_ERR_BAD_ARG,
+    VMF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), VMF_ERR_BAD_ARG,
                 "vmf_layer_norm_bwd: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   } else if (!gx || n == 0) {
     return VMF_OK;

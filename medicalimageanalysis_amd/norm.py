@@ -75,7 +75,7 @@ class _LayerNorm(torch.autograd.Function):
         ws, need = None, C.c_int64(0)
         if need_w or need_b:
             _lib.check(lib.vmf_layer_norm_bwd_workspace(n, width, code, need), "vmf_layer_norm_bwd_workspace")
-            ws = torch.empty(need.value, device=dev, dtype=torch.uint8)
+            ws = torch.empty(need.value, device=dev, dtype=torch.uint8) if need.value else None
         mean = stats.data_ptr()
         with _lib.on_device(dev):
             rc = lib.vmf_layer_norm_bwd(rows.data_ptr(), x_stride, g.data_ptr(), g_stride, _lib.address(w), mean,
