@@ -10,6 +10,7 @@ import torch.nn.functional as F
 
 from ..sampler.spherical_uniform import HypersphericalUniform
 from ..sampler.von_mises_fisher import VonMisesFisher, vmf_rsample_from_heads
+from . import hidden as _hidden
 
 
 class HypersphericalVAE(nn.Module):
@@ -29,11 +30,10 @@ class HypersphericalVAE(nn.Module):
         self.decoder_function = nn.Linear(self.latent_dim, dw, device=dev)
         self.decoder_linear_layers = nn.ModuleList([nn.Linear(dw, dw, device=dev) for _ in range(config["decoder_depth"])])
         self.function_x_mu = nn.Linear(dw, self.extrinsic_dim, device=dev)
+        _hidden.prepare(self)
 
     def encode(self, x):
-        h = F.softplus(self.encoder_function(x), beta=self.sftbeta)
-        for layer in self.encoder_linear_layers:
-            h = F.softplus(layer(h), beta=self.sftbeta)
+        h = _hidden.encode(self, x)
         z_mu = F.normalize(self.function_z_mu(h), dim=-1)
         z_kappa = F.softplus(self.function_z_logvar(h)).squeeze(-1) + 1
         return z_mu, z_kappa
@@ -43,19 +43,14 @@ class HypersphericalVAE(nn.Module):
         return VonMisesFisher(z_mu, z_kappa, validate_args=False).rsample()
 
     def decode(self, z):
-        h = F.softplus(self.decoder_function(z), beta=self.sftbeta)
-        for layer in self.decoder_linear_layers:
-            h = F.softplus(layer(h), beta=self.sftbeta)
-        return self.function_x_mu(h)
+        return _hidden.decode(self, z)
 
     def forward(self, x):
         """encode -> sample -> decode.  The sampler takes the raw outputs of BOTH heads: it normalises the mean rows and
         evaluates kappa = softplus(.) + 1 inside its kernels (forward and backward), so neither the (B, latent_dim)
         normalisation pass nor the softplus / add passes and their backward launches exist; the posterior parameters
         returned are the same (unit z_mu, kappa) that encode() gives."""
-        h = F.softplus(self.encoder_function(x), beta=self.sftbeta)
-        for layer in self.encoder_linear_layers:
-            h = F.softplus(layer(h), beta=self.sftbeta)
+        h = _hidden.encode(self, x)
         raw = self.function_z_mu(h)
         z, z_kappa = vmf_rsample_from_heads(raw, self.function_z_logvar(h).squeeze(-1))
         with torch.no_grad():  # reporting only: the KL term depends on kappa alone

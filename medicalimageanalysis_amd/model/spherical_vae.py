@@ -12,6 +12,7 @@ from ..sampler.spherical_uniform import SphericalUniform
 from ..sampler.von_mises_fisher import VonMisesFisher3D, vmf3_rsample_from_heads
 from .. import kl as _kl
 from .. import losses as _losses
+from . import hidden as _hidden
 
 
 class SphericalVAE(nn.Module):
@@ -40,13 +41,12 @@ class SphericalVAE(nn.Module):
             [nn.Linear(self.decoder_width, self.decoder_width, device=dev) for _ in range(self.decoder_depth)])
         self.function_x_mu = nn.Linear(self.decoder_width, self.extrinsic_dim, device=dev)
         self.dropout = nn.Dropout(p=self.dropout_p)
+        _hidden.prepare(self)
 
     def encode(self, x):
         """(z_mu, z_kappa): un-normalised mean direction (B, latent_dim) and kappa = softplus(.) + 1 of shape (B, 1)
         (model/spherical_vae.py:51-72)"""
-        h = F.softplus(self.encoder_function(x), beta=self.sftbeta)
-        for layer in self.encoder_linear_layers:
-            h = F.softplus(layer(h), beta=self.sftbeta)
+        h = _hidden.encode(self, x)
         z_mu = self.function_z_mu(h)
         z_kappa = F.softplus(self.function_z_logvar(h)) + 1
         return z_mu, z_kappa
@@ -58,19 +58,14 @@ class SphericalVAE(nn.Module):
         return q_z.rsample()
 
     def decode(self, z):
-        h = F.softplus(self.decoder_function(z), beta=self.sftbeta)
-        for layer in self.decoder_linear_layers:
-            h = F.softplus(layer(h), beta=self.sftbeta)
-        return self.function_x_mu(h)
+        return _hidden.decode(self, z)
 
     def forward(self, x):
         """encode -> reparemetrize -> decode with the values and the noise order of model/spherical_vae.py:103-117.  The
         sampler kernel takes the RAW output of the concentration head and evaluates kappa = softplus(.) + 1 itself
         (handing kappa back for the KL term), so the head's softplus / add passes and their backward launches are
         gone; encode() and reparemetrize() remain for callers that use them separately."""
-        h = F.softplus(self.encoder_function(x), beta=self.sftbeta)
-        for layer in self.encoder_linear_layers:
-            h = F.softplus(layer(h), beta=self.sftbeta)
+        h = _hidden.encode(self, x)
         z_mu = self.function_z_mu(h)
         z, z_kappa = vmf3_rsample_from_heads(z_mu, self.function_z_logvar(h))
         x_mu = self.decode(z)

@@ -11,6 +11,7 @@ from ..sampler.spherical_uniform import SphericalUniform
 from ..sampler.von_mises_fisher import VonMisesFisher3D, vmf3_rsample_from_heads
 from .. import kl as _kl
 from .. import losses as _losses
+from . import hidden as _hidden
 
 
 class ToroidalVAE(nn.Module):
@@ -42,6 +43,7 @@ class ToroidalVAE(nn.Module):
             [nn.Linear(self.decoder_width, self.decoder_width, device=dev) for _ in range(self.decoder_depth)])
         self.function_x_mu = nn.Linear(self.decoder_width, self.extrinsic_dim, device=dev)
         self.dropout = nn.Dropout(p=self.dropout_p)
+        _hidden.prepare(self)
 
     def _build_torus(self, z_theta, z_phi):
         """model/torus_vae.py:60-81: the first two components of each sphere sample act as (cos, sin);
@@ -49,9 +51,7 @@ class ToroidalVAE(nn.Module):
         return _losses.build_torus(z_theta, z_phi, self.longest_radius, self.shortes_radius)
 
     def encode(self, x):
-        h = F.softplus(self.encoder_function(x), beta=self.sftbeta)
-        for layer in self.encoder_linear_layers:
-            h = F.softplus(layer(h), beta=self.sftbeta)
+        h = _hidden.encode(self, x)
         z_theta_mu = self.function_z_theta_mu(h)
         z_theta_logvar = F.softplus(self.function_z_theta_logvar(h)) + 1
         z_phi_mu = self.function_z_phi_mu(h)
@@ -68,17 +68,12 @@ class ToroidalVAE(nn.Module):
         return self._build_torus(z_theta, z_phi)
 
     def decode(self, z):
-        h = F.softplus(self.decoder_function(z), beta=self.sftbeta)
-        for layer in self.decoder_linear_layers:
-            h = F.softplus(layer(h), beta=self.sftbeta)
-        return self.function_x_mu(h)
+        return _hidden.decode(self, z)
 
     def forward(self, x):
         """encode -> reparemetrize -> decode (model/torus_vae.py:144-158); kappa = softplus(.) + 1 of both heads is
         evaluated inside the sampler kernels (see SphericalVAE.forward).  Draw order: theta, then phi."""
-        h = F.softplus(self.encoder_function(x), beta=self.sftbeta)
-        for layer in self.encoder_linear_layers:
-            h = F.softplus(layer(h), beta=self.sftbeta)
+        h = _hidden.encode(self, x)
         z_theta_mu, z_phi_mu = self.function_z_theta_mu(h), self.function_z_phi_mu(h)
         z_theta, z_theta_kappa = vmf3_rsample_from_heads(z_theta_mu, self.function_z_theta_logvar(h))
         z_phi, z_phi_kappa = vmf3_rsample_from_heads(z_phi_mu, self.fucntion_z_phi_logvar(h))

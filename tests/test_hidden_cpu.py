@@ -1,0 +1,40 @@
+"""The VAEs' optional hidden layers: configuration, without a GPU."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+from medicalimageanalysis_amd.model.hyperspherical_vae import HypersphericalVAE
+from medicalimageanalysis_amd.model.spherical_vae import SphericalVAE
+from medicalimageanalysis_amd.model.torus_vae import ToroidalVAE
+
+CONFIG = dict(extrinsic_dim=12, latent_dim=3, sftbeta=4.5, encoder_width=16, encoder_depth=2, decoder_width=20,
+              decoder_depth=1, dropout_p=0.1, device="cpu", gamma=1.0, beta=0.01, longest_radius=2.0, shortest_radius=1.0)
+MODELS = [HypersphericalVAE, SphericalVAE, ToroidalVAE]
+
+
+@pytest.mark.parametrize("model", MODELS)
+def test_keys_change_nothing_unless_they_are_set(model):
+    torch.manual_seed(0)
+    plain = model(CONFIG)
+    assert not any("norm" in k for k in plain.state_dict())
+    h = F.softplus(plain.decoder_function(torch.ones(5, 3)), beta=4.5)
+    for layer in plain.decoder_linear_layers:
+        h = F.softplus(layer(h), beta=4.5)
+    assert torch.equal(plain.decode(torch.ones(5, 3)), plain.function_x_mu(h))
+    eight = model(dict(CONFIG, hidden="blocks8"))
+    eight.load_state_dict(plain.state_dict())  # the same parameters
+    normed = model(dict(CONFIG, layer_norm=True))
+    extra = set(normed.state_dict()) - set(plain.state_dict())
+    assert extra == {f"{s}_norms.{i}.{p}" for s, d in (("encoder", 3), ("decoder", 2)) for i in range(d)
+                     for p in ("weight", "bias")}
+
+
+@pytest.mark.parametrize("model", MODELS)
+def test_unknown_kind_is_refused(model):
+    with pytest.raises(ValueError, match="blocks8"):
+        model(dict(CONFIG, hidden="fp4"))
+
+
+def test_eight_bit_layers_need_a_hip_device():
+    with pytest.raises(RuntimeError, match="HIP device"):
+        HypersphericalVAE(dict(CONFIG, hidden="blocks8")).decode(torch.ones(5, 3))
