@@ -358,12 +358,13 @@ int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const uint8_t* a,
 
 /* A layer's two directions in one call each: y = blocks(activation(x)) tiles(weight)^T + bias, and its gradients.
  * fwd: weight (n, k) of weight_dtype (dtype or VMF_F32) is quantised in the call, or (null) w_values / w_exponents hold
- * its tiles already.  a_values / a_exponents receive x's blocks, which bwd takes; wt_values / wt_exponents (may be null)
- * the transposed weight's tiles, which bwd takes for gx.  y: dense, of dtype.
+ * its tiles already.  a_values / a_exponents (may be null: not kept) receive x's blocks, which bwd takes; wt_values /
+ * wt_exponents (may be null) the transposed weight's tiles, which bwd takes for gx.  y: dense, of dtype.
  * bwd: gx (may be null; of dtype) = (blocks(gy) tiles(weight)) * softplus slope, gweight (may be null) and gbias (may be
  * null, comes with gweight) as vmf_blocks8_weight_grad, of weight_dtype.
- * workspace: the _workspace call's bytes (fwd without a weight: vmf_blocks8_matmul_workspace's), 16-byte aligned. */
-int vmf_blocks8_linear_fwd_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes_out);
+ * workspace: the _workspace call's bytes (laid_out: weight is null, kept: a_values is not), 16-byte aligned. */
+int vmf_blocks8_linear_fwd_workspace(int64_t m, int64_t n, int64_t k, int laid_out, int kept, int dtype,
+                                     int64_t* bytes_out);
 int vmf_blocks8_linear_fwd(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, int weight_dtype,
                            const uint8_t* w_values, const uint8_t* w_exponents, uint8_t* wt_values,
                            uint8_t* wt_exponents, const void* bias, int bias_dtype, int activation, double beta,

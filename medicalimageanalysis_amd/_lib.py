@@ -79,7 +79,7 @@ _PROTOS = {
                            _I, _P],
     "vmf_blocks8_weight_grad_workspace": [_I64, _I64, _I64, _I, _I64P],
     "vmf_blocks8_weight_grad": [_P, _I64, _P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _I, _I, _P],
-    "vmf_blocks8_linear_fwd_workspace": [_I64, _I64, _I64, _I, _I64P],
+    "vmf_blocks8_linear_fwd_workspace": [_I64, _I64, _I64, _I, _I, _I, _I64P],
     "vmf_blocks8_linear_fwd": [_P, _I64, _P, _I64, _I, _P, _P, _P, _P, _P, _I, _I, _D, _P, _P, _I64, _P, _I64, _I64, _I64,
                                _P, _I64, _I, _P],
     "vmf_blocks8_linear_bwd_workspace": [_I64, _I64, _I64, _I, _I64P],
@@ -237,6 +237,11 @@ def first_order(backward):
         return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return call
+
+
+def dense(t):
+    """a vector (or None) whose elements lie side by side"""
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def address(t):

@@ -258,42 +258,49 @@ def weight_grad(g, q, bias=True, dtype=torch.float32):
     return _weight_grad(g, q, bias, dtype, _lib.require_hip(g, q.storage))
 
 
-def _linear(x, weight, laid_out, bias, act, beta, dev, columns):
-    """(y, x's blocks, the weight's transposed tiles if `columns`).  The two share an allocation, which a backward pass
-    keeps; the weight's own tiles live in the workspace, and end with the call."""
-    rows, stride = _lib.as_rows(x.detach())
+def _linear(x, weight, laid_out, bias, act, beta, dev, keep, columns):
+    """(y, kept, wt, sizes).  keep: kept holds x's blocks and, if `columns`, those of the transposed weight from wt[0] on
+    (wt: where its values and its exponents start; None without).  What is not kept lives in the workspace, and ends with
+    the call."""
+    rows, stride = _lib.as_rows(x)
     m, k = rows.shape
     code = _lib.FLOAT_CODES[x.dtype]
     lib = _lib.lib()
     need = C.c_int64(0)
-    w = wv = we = None
-    w_stride = w_code = 0
+    w = wv = we = kept = wt = base = base_e = tv = te = None
+    w_stride = w_code = pitch = 0
     if laid_out is None:
         n = weight.shape[0]
-        w, w_stride = _lib.as_rows(weight.detach())
+        w, w_stride = _lib.as_rows(weight)
         w_code = _lib.FLOAT_CODES[w.dtype]
-        _lib.check(lib.vmf_blocks8_linear_fwd_workspace(m, n, k, code, need), "vmf_blocks8_linear_fwd_workspace")
     else:
         n = laid_out.rows.rows
         wv, we = laid_out.rows._addresses()
-        _lib.check(lib.vmf_blocks8_matmul_workspace(m, n, k, code, need), "vmf_blocks8_matmul_workspace")
-    first = Blocks8.bytes_for(m, k)
-    new_columns = columns and laid_out is None
-    kept = torch.empty(first + (Blocks8.bytes_for(k, n, True) if new_columns else 0), device=dev, dtype=torch.uint8)
-    q = Blocks8(kept, x.shape)
-    wt = Blocks8(kept, (k, n), True, first) if new_columns else laid_out.columns if columns else None
+    _lib.check(lib.vmf_blocks8_linear_fwd_workspace(m, n, k, laid_out is not None, keep, code, need),
+               "vmf_blocks8_linear_fwd_workspace")
+    if keep:
+        kp = _up(k, BLOCK)
+        pitch = max(16, _up(m, 16))
+        size = _up(m * kp + kp // BLOCK * pitch, 16)  # Blocks8.bytes_for(m, k)
+        if columns and laid_out is None:
+            wt = (size, size + k * _up(n, BLOCK))
+            size += Blocks8.bytes_for(k, n, True)
+        kept = torch.empty(size, device=dev, dtype=torch.uint8)
+        base = kept.data_ptr()
+        base_e = base + m * kp
+        if wt is not None:
+            tv, te = base + wt[0], base + wt[1]
     ws = torch.empty(need.value, device=dev, dtype=torch.uint8) if need.value else None
     y = torch.empty(x.shape[:-1] + (n,), device=dev, dtype=x.dtype)
-    b = None if bias is None else bias.detach().contiguous()
-    qv, qe = q._addresses()
-    tv, te = wt._addresses() if new_columns else (None, None)
+    b = _lib.dense(bias)
     with _lib.on_device(dev):
         rc = lib.vmf_blocks8_linear_fwd(rows.data_ptr(), stride, _lib.address(w), w_stride, w_code, wv, we, tv, te,
-                                        _lib.address(b), 0 if b is None else _lib.FLOAT_CODES[b.dtype], act, beta, qv, qe,
-                                        q.exp_pitch, y.data_ptr(), m, n, k, _lib.address(ws), need.value, code,
+                                        _lib.address(b), 0 if b is None else _lib.FLOAT_CODES[b.dtype], act, beta, base,
+                                        base_e, pitch, y.data_ptr(), m, n, k, _lib.address(ws), need.value, code,
                                         _lib.raw_stream(dev))
-    _lib.check(rc, "vmf_blocks8_linear_fwd")
-    return y, q, wt
+    if rc:
+        _lib.check(rc, "vmf_blocks8_linear_fwd")
+    return y, kept, wt, (m, n, k)
 
 
 class _Linear(torch.autograd.Function):
@@ -303,21 +310,23 @@ class _Linear(torch.autograd.Function):
         if need_x and laid_out is not None and laid_out.columns is None:
             raise ValueError("linear: the laid-out weight has no columns (quantize_weight(..., transpose=True)), which "
                              "the gradient of x reads")
-        y, q, wt = _linear(x, weight, laid_out, bias, act, beta, dev, need_x)
+        y, kept, wt, sizes = _linear(x, weight, laid_out, bias, act, beta, dev, True, need_x)
         # kept for the backward pass: x in 8 bits and, for its own gradient, the transposed weight in 8 bits
-        ctx.save_for_backward(q.storage, wt.storage if wt is not None and wt.storage is not q.storage else None)
-        ctx.meta = (x.shape, y.shape[-1], None if wt is None else wt.offset, act, beta,
-                    None if weight is None else weight.dtype, None if bias is None else bias.dtype, dev)
+        other = None
+        if need_x and laid_out is not None:
+            columns = laid_out.columns
+            other, wt = columns.storage, (columns.offset, columns.exp_offset)
+        ctx.save_for_backward(kept, other)
+        ctx.meta = (x.shape, sizes, wt, act, beta, None if weight is None else weight.dtype,
+                    None if bias is None else bias.dtype, dev)
         return y
 
     @staticmethod
     @_lib.first_order
     def backward(ctx, gy):
         kept, other = ctx.saved_tensors
-        shape, n, wt_offset, act, beta, w_dtype, bias_dtype, dev = ctx.meta
+        shape, (m, n, k), wt, act, beta, w_dtype, bias_dtype, dev = ctx.meta
         need_x, need_w, _, need_b = ctx.needs_input_grad[:4]
-        q = Blocks8(kept, shape)
-        m, k = q.rows, q.width
         code = _lib.FLOAT_CODES[gy.dtype]
         # the weight's gradient in the weight's type; a bias beside a laid-out weight has float32 sums
         out = w_dtype or torch.float32
@@ -329,13 +338,17 @@ class _Linear(torch.autograd.Function):
         _lib.check(lib.vmf_blocks8_linear_bwd_workspace(m, n, k, code, need), "vmf_blocks8_linear_bwd_workspace")
         ws = torch.empty(need.value, device=dev, dtype=torch.uint8)
         g, stride = _lib.as_rows(gy)
-        qv, qe = q._addresses()
-        tv, te = Blocks8(other if other is not None else kept, (k, n), True, wt_offset)._addresses() if need_x else (None, None)
+        base = kept.data_ptr()
+        tv = te = None
+        if need_x:
+            at = base if other is None else other.data_ptr()
+            tv, te = at + wt[0], at + wt[1]
         with _lib.on_device(dev):
-            rc = lib.vmf_blocks8_linear_bwd(g.data_ptr(), stride, qv, qe, q.exp_pitch, tv, te, act, beta,
-                                            _lib.address(gx), _lib.address(gw), _lib.address(gb), m, n, k, ws.data_ptr(),
-                                            need.value, code, _lib.FLOAT_CODES[out], _lib.raw_stream(dev))
-        _lib.check(rc, "vmf_blocks8_linear_bwd")
+            rc = lib.vmf_blocks8_linear_bwd(g.data_ptr(), stride, base, base + m * _up(k, BLOCK), max(16, _up(m, 16)), tv,
+                                            te, act, beta, _lib.address(gx), _lib.address(gw), _lib.address(gb), m, n, k,
+                                            ws.data_ptr(), need.value, code, _lib.FLOAT_CODES[out], _lib.raw_stream(dev))
+        if rc:
+            _lib.check(rc, "vmf_blocks8_linear_bwd")
         if gb is not None and gb.dtype != bias_dtype:
             gb = gb.to(bias_dtype)
         return gx, gw if need_w else None, None, gb, None, None, None
@@ -361,6 +374,7 @@ def linear(x, weight, bias=None, activation=None, beta=1.0):
     _check_bias(bias, n, "linear")
     dev = _lib.require_hip(x, weight if laid_out is None else laid_out.rows.storage, bias)
     tensor = weight if laid_out is None else None
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, tensor, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or (tensor is not None and tensor.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
         return _Linear.apply(x, tensor, laid_out, bias, act, beta, dev)
-    return _linear(x, tensor, laid_out, bias, act, beta, dev, False)[0]
+    return _linear(x, tensor, laid_out, bias, act, beta, dev, False, False)[0]

@@ -4,141 +4,6 @@
 
 namespace {
 
-// In 32 bits, from the hardware's exponential and logarithm (1 unit in the last place each):
-//   log(1 + u), u = exp(-|t|): where 1 + u drops too much of u (u < 1/16), the series to u^6 (the rest is under u^6 / 7
-//   of it); else ln 2 * log2(1 + u), off by 2^-24 / u <= 2^-20.
-// beta, t = beta h and t log2(e) are rounded, 3 * 2^-24 |t| in the exponential's argument, which counts in full for
-// negative t only (for positive t its share is |t| exp(-t) <= 0.37 of that).  Together the result is off by less than
-// softplus_margin relative to its value.
-__device__ __forceinline__ float softplus32(float h, float beta, float inv_beta) {
-  const float t = beta * h;
-  const float u = __builtin_amdgcn_exp2f(-fabsf(t) * 1.44269504f);
-  const float few = u * (1.0f + u * (-0.5f + u * (1.0f / 3 + u * (-0.25f + u * (0.2f + u * (-1.0f / 6))))));
-  const float l = u < 0.0625f ? few : 0.69314718f * __builtin_amdgcn_logf(1.0f + u);
-  return (fmaxf(t, 0.0f) + l) * inv_beta;
-}
-__device__ __forceinline__ float softplus_margin(float h, float beta) { return 3e-6f + 3e-7f * fmaxf(-beta * h, 0.0f); }
-
-// exp in 64 bits: t = n ln 2 + r, |r| <= 0.35, and the power series of exp(r) to r^13 (the next term is under 5e-18)
-__device__ __forceinline__ double exp64(double t) {
-  const double n = ::rint(t * 1.4426950408889634);
-  const double r = ::fma(-n, 2.3190468138462996e-17, ::fma(-n, 0.69314718055994531, t));
-  double s = 1.0 / 6227020800.0;
-  s = ::fma(s, r, 1.0 / 479001600.0);
-  s = ::fma(s, r, 1.0 / 39916800.0);
-  s = ::fma(s, r, 1.0 / 3628800.0);
-  s = ::fma(s, r, 1.0 / 362880.0);
-  s = ::fma(s, r, 1.0 / 40320.0);
-  s = ::fma(s, r, 1.0 / 5040.0);
-  s = ::fma(s, r, 1.0 / 720.0);
-  s = ::fma(s, r, 1.0 / 120.0);
-  s = ::fma(s, r, 1.0 / 24.0);
-  s = ::fma(s, r, 1.0 / 6.0);
-  s = ::fma(s, r, 0.5);
-  s = ::fma(s, r, 1.0);
-  s = ::fma(s, r, 1.0);
-  return ::ldexp(s, n < -1100 ? -1100 : (int)n);
-}
-// softplus to 40 bits and more, for the few values that lie next to a rounding border (see softplus8).
-// l = log(1 + u), u = exp(-|t|): for small u its series; else from the 32-bit l0, with d = (1 + u) exp(-l0) - 1 under 1e-5,
-// l = l0 + log(1 + d) = l0 + d - d^2 / 2 + d^3 / 3.
-__device__ __noinline__ double softplus64(double h, double beta) {
-  const double t = beta * h;
-  const double u = exp64(-::fabs(t));
-  double l;
-  if (u < 1.0 / 4096) {
-    l = u * ::fma(u, ::fma(u, ::fma(u, -0.25, 1.0 / 3), -0.5), 1.0);
-  } else {
-    const double l0 = (double)(0.69314718f * __builtin_amdgcn_logf((float)(1.0 + u)));
-    const double d = ::fma(1.0 + u, exp64(-l0), -1.0);
-    l = l0 + d * ::fma(d, ::fma(d, 1.0 / 3, -0.5), 1.0);
-  }
-  return ((t > 0 ? t : 0) + l) / beta;
-}
-
-// a double in [0, 448] -> the float from which a second rounding to fewer bits gives what one rounding of the double
-// would: truncated, with the last bit set if anything was cut off
-__device__ __forceinline__ float round_to_odd(double d) {
-  float f = (float)d;
-  if ((double)f != d) {
-    uint32_t u = __float_as_uint(f);
-    if ((double)f > d) --u;
-    f = __uint_as_float(u | 1u);
-  }
-  return f;
-}
-
-// the exponent and the scaled elements of a block that sixteen lanes hold, 8 elements each
-__device__ __forceinline__ int scale8(float (&h)[8]) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = larger(top, b8_size(h[i]));
-  top = lane_max<16>(top);
-  if (top >= B8_INF) {  // some are not finite: the largest of the others
-    top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = b8_size(h[i]) < B8_INF ? larger(top, b8_size(h[i])) : top;
-    top = lane_max<16>(top);
-  }
-  const int e = b8_exponent(__uint_as_float(top));
-  const float inv = b8_pow2(-e);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) h[i] *= inv;
-  if (e == B8_EMAX) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = b8_cut(h[i]);
-  }
-  return e;
-}
-
-// One element the exact way: softplus(x) / 2^e, ready for the conversion
-__device__ __noinline__ float softplus_scaled(float x, double beta, int e) {
-  if (!(x < __builtin_inff())) return __builtin_nanf("");
-  return round_to_odd(::fmin(softplus64((double)x, beta) * ::ldexp(1.0, -e), 448.0));
-}
-
-// The block of softplus(h).  Which of two neighbouring 8-bit values is nearest to softplus(h) can hang on its last bits,
-// so a value is computed in 32 bits, and once more in 64 where its 32-bit error could change the result (a few of a
-// million): the bytes are those of the exactly computed softplus.
-__device__ __forceinline__ uint2 softplus8(const float (&h)[8], float beta, float inv_beta, double beta64, int& e_out) {
-  constexpr float INF = __builtin_inff();
-  float top = -INF;  // softplus grows with h: the block's largest comes from the largest h
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = h[i] < INF ? fmaxf(top, h[i]) : top;
-  top = lane_max<16>(top);
-  const float at = softplus32(top, beta, inv_beta), mt = softplus_margin(top, beta);
-  int e = B8_EMAX;
-  if (at < INF) {
-    e = b8_exponent(at * (1.0f - mt));
-    const int above = b8_exponent(fminf(at * (1.0f + mt), 3.4e38f));
-    if (e != above && softplus64((double)top, beta64) > 448.0 * ::ldexp(1.0, e)) e = above;
-  }
-  if (top == -INF) e = 0;
-  e_out = e;
-  const float scale = inv_beta * b8_pow2(-e);
-  float lo[8], hi[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = softplus32(h[i], beta, scale);
-    const float m = fminf(softplus_margin(h[i], beta), 0.5f);  // (-inf, the fill of short rows, has none)
-    lo[i] = fmaf(a, -m, a);
-    hi[i] = fmaf(a, m, a);
-  }
-  uint32_t w[2] = {b8_pack4(lo), b8_pack4(lo + 4)};
-  const uint32_t x[2] = {w[0] ^ b8_pack4(hi), w[1] ^ b8_pack4(hi + 4)};
-  if ((x[0] | x[1]) != 0 || e == B8_EMAX) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int at = 8 * (i & 3);
-      if ((x[i >> 2] >> at & 0xff) != 0 || e == B8_EMAX) {
-        const float v = softplus_scaled(h[i], beta64, e);
-        w[i >> 2] = (w[i >> 2] & ~(0xffu << at)) | (b8_pack2(v, v) & 0xff) << at;
-      }
-    }
-  }
-  return uint2{w[0], w[1]};
-}
-
 // A workgroup has 16 groups of 16 lanes: 1 << row_bits of them side by side in rows (so that the exponent bytes of
 // neighbouring rows, which lie side by side, leave together), the others in block columns.
 struct RowArgs {

@@ -435,6 +435,27 @@ __global__ __launch_bounds__(512, 2) void mm_large_kernel(MmArgs p) {
   write_tile<4, 4, 2, 1, OUT>(p, acc, m0 + wm, n0 + wn, lane);
 }
 
+// the eight waves' sums of 16 rows and 16 columns, added in their order
+template <typename OUT>
+__device__ __forceinline__ void few_result(const MmArgs& p, float (&sums)[8][16][17], v4f acc, int64_t n0, int lane,
+                                           int wave) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) sums[wave][4 * (lane >> 4) + r][lane & 15] = acc[r];
+  __syncthreads();
+  if (threadIdx.x >= 256) return;
+  const int64_t row = threadIdx.x >> 4, col = n0 + (threadIdx.x & 15);
+  if (row >= p.m || col >= p.n) return;
+  float v = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) v += sums[w][threadIdx.x >> 4][threadIdx.x & 15];
+  if (p.partial) {
+    p.partial[((int64_t)blockIdx.y * p.m + row) * p.n + col] = v;
+  } else {
+    const float bias = p.bias ? load_bias(p.bias, p.bias_code, col) : 0.0f;
+    finish<1, OUT>(p, row, col, &bias, &v);
+  }
+}
+
 // Up to 16 rows: the weight's bytes are what there is to move.  A workgroup takes 16 columns, its eight waves share the
 // block columns and read both operands straight into registers; their sums are added through LDS.
 template <bool WIDE, typename OUT>
@@ -464,21 +485,88 @@ __global__ __launch_bounds__(512) void mm_few_kernel(MmArgs p) {
       acc = mm_step_bf16(aw, bw, acc);
     }
   }
+  few_result<OUT>(p, sums, acc, n0, lane, wave);
+}
+
+// The same in one launch with x's quantisation, for a row or a few through a weight that was laid out before (and no
+// blocks of x to keep): every workgroup quantises its rows for itself into LDS, at most two blocks per 16 lanes, while
+// the weight's bytes are on their way into registers.
+constexpr int FEW_AHEAD = 4;        // block columns of the weight that a wave asks for in advance
+constexpr int FEW_MAX_BLOCKS = 64;  // blocks of x per workgroup
+struct FewArgs {
+  const void* x;
+  int64_t x_stride, width;
+  float beta, inv_beta;
+  double beta64;
+};
+template <typename T, bool ACT>
+__global__ __launch_bounds__(512) void linear_few_kernel(MmArgs p, FewArgs f) {
+  constexpr bool WIDE = std::is_same<T, float>::value;
+  constexpr int PAD = 16;  // after every row: the rows of an operand lie in different banks
+  __shared__ float sums[8][16][17];
+  __shared__ __attribute__((aligned(16))) uint8_t rows[FEW_MAX_BLOCKS * B8 + 16 * PAD];
+  __shared__ uint8_t exps[FEW_MAX_BLOCKS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int kb0 = (int)blockIdx.y * p.blocks_per_split;
+  const int kb1 = kb0 + p.blocks_per_split < p.blocks ? kb0 + p.blocks_per_split : p.blocks;
+  const int count = kb1 - kb0, pitch = count * B8 + PAD;
+  const int64_t rb = n0 + (lane & 15) < p.n ? n0 + (lane & 15) : p.n - 1;
+  const uint8_t* B = p.b.values + rb * p.b.pitch + (lane >> 4) * 32;
+  const uint8_t* eb = p.b.exps + (p.b.tiled ? rb >> 7 : rb);
+  v8i b[FEW_AHEAD];
+  int xb[FEW_AHEAD];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) sums[wave][4 * (lane >> 4) + r][lane & 15] = acc[r];
-  __syncthreads();
-  if (threadIdx.x >= 256) return;
-  const int64_t row = threadIdx.x >> 4, col = n0 + (threadIdx.x & 15);
-  if (row >= p.m || col >= p.n) return;
-  float v = 0;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) v += sums[w][threadIdx.x >> 4][threadIdx.x & 15];
-  if (p.partial) {
-    p.partial[((int64_t)blockIdx.y * p.m + row) * p.n + col] = v;
-  } else {
-    const float bias = p.bias ? load_bias(p.bias, p.bias_code, col) : 0.0f;
-    finish<1, OUT>(p, row, col, &bias, &v);
+  for (int i = 0; i < FEW_AHEAD; ++i) {
+    const int kb = kb0 + wave + 8 * i;
+    if (kb < kb1) {
+      b[i] = *reinterpret_cast<const v8i_at16*>(B + (int64_t)kb * B8);
+      xb[i] = eb[(int64_t)kb * p.b.exp_pitch];
+    }
   }
+  {  // x's blocks: 32 groups of 16 lanes
+    const int group = threadIdx.x >> 4, part = threadIdx.x & 15;
+    for (int id = group; id < (int)p.m * count; id += 32) {
+      const int row = id / count, c = id - row * count;
+      const int64_t col = (int64_t)(kb0 + c) * B8 + part * 8;
+      float h[8];
+      load_some<8>((const T*)f.x + row * f.x_stride + col, f.width - col, ACT ? -__builtin_inff() : 0.0f, h);
+      int e;
+      uint2 v;
+      if constexpr (ACT) {
+        v = softplus8(h, f.beta, f.inv_beta, f.beta64, e);
+      } else {
+        e = scale8(h);
+        v = uint2{b8_pack4(h), b8_pack4(h + 4)};
+      }
+      *reinterpret_cast<uint2*>(rows + row * pitch + c * B8 + part * 8) = v;
+      if (part == 0) exps[id] = (uint8_t)(e + 127);
+    }
+  }
+  __syncthreads();
+  const int ra = (lane & 15) < p.m ? (lane & 15) : (int)p.m - 1;
+  const uint8_t* A = rows + ra * pitch + (lane >> 4) * 32;
+  v4f acc = {0, 0, 0, 0};
+  auto product = [&](int kb, v8i bv, int be) {
+    const v8i a = *reinterpret_cast<const v8i_at16*>(A + (kb - kb0) * B8);
+    const int ae = exps[ra * count + kb - kb0];
+    if constexpr (!WIDE) {
+      acc = mm_step<0, 0>(a, bv, acc, ae, be);
+    } else {
+      v8b aw[4], bw[4];
+      to_bf16(a, b8_scale(ae), aw);
+      to_bf16(bv, b8_scale(be), bw);
+      acc = mm_step_bf16(aw, bw, acc);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < FEW_AHEAD; ++i) {
+    const int kb = kb0 + wave + 8 * i;
+    if (kb < kb1) product(kb, b[i], xb[i]);
+  }
+  for (int kb = kb0 + wave + 8 * FEW_AHEAD; kb < kb1; kb += 8)
+    product(kb, *reinterpret_cast<const v8i_at16*>(B + (int64_t)kb * B8), eb[(int64_t)kb * p.b.exp_pitch]);
+  few_result<T>(p, sums, acc, n0, lane, wave);
 }
 
 // the splits' sums in their order, then what the tile would have done
@@ -1090,13 +1178,12 @@ extern "C" int vmf_blocks8_matmul_workspace(int64_t m, int64_t n, int64_t k, int
   return VMF_OK;
 }
 
-extern "C" int vmf_blocks8_matmul(const uint8_t* a, const uint8_t* a_exponents, int64_t a_exp_pitch, int a_tiled,
-                                  const uint8_t* b, const uint8_t* b_exponents, int64_t b_exp_pitch, int b_tiled,
-                                  const void* bias, int bias_dtype, const uint8_t* gate,
-                                  const uint8_t* gate_exponents, int64_t gate_exp_pitch, double beta, void* out,
-                                  int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes,
-                                  int out_dtype, vmf_stream_t stream) {
-  VMF_RANGE("vmf_blocks8_matmul");
+// vmf_blocks8_matmul; few: not null, a are the rows there, quantised by the same launch (one that few_fits)
+static int matmul(const FewArgs* few, int activation, const uint8_t* a, const uint8_t* a_exponents, int64_t a_exp_pitch, int a_tiled,
+                  const uint8_t* b, const uint8_t* b_exponents, int64_t b_exp_pitch, int b_tiled, const void* bias,
+                  int bias_dtype, const uint8_t* gate, const uint8_t* gate_exponents, int64_t gate_exp_pitch,
+                  double beta, void* out, int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes,
+                  int out_dtype, vmf_stream_t stream) {
   const char* what = "vmf_blocks8_matmul";
   int64_t need = 0;
   int rc = vmf_blocks8_matmul_workspace(m, n, k, out_dtype, &need);
@@ -1106,7 +1193,7 @@ extern "C" int vmf_blocks8_matmul(const uint8_t* a, const uint8_t* a_exponents, 
   VMF_REQUIRE(!bias || bias_dtype == VMF_F32 || bias_dtype == VMF_F16 || bias_dtype == VMF_BF16, VMF_ERR_DTYPE,
               "%s: bias dtype %d", what, bias_dtype);
   if (m == 0 || n == 0) return VMF_OK;
-  if ((rc = check_operand(what, "a", a, a_exponents, a_exp_pitch, a_tiled, m)) != VMF_OK) return rc;
+  if (!few && (rc = check_operand(what, "a", a, a_exponents, a_exp_pitch, a_tiled, m)) != VMF_OK) return rc;
   if ((rc = check_operand(what, "b", b, b_exponents, b_exp_pitch, b_tiled, n)) != VMF_OK) return rc;
   if (gate) {
     if ((rc = check_operand(what, "gate", gate, gate_exponents, gate_exp_pitch, 0, m)) != VMF_OK) return rc;
@@ -1136,10 +1223,31 @@ extern "C" int vmf_blocks8_matmul(const uint8_t* a, const uint8_t* a_exponents, 
   p.nt = pl.nt;
   p.beta = (float)beta;
   hipStream_t st = (hipStream_t)stream;
+  if (few) {
+    const dim3 grid((unsigned)pl.nt, (unsigned)pl.splits);
+    LOWP_DISPATCH(out_dtype, "vmf_blocks8_linear_fwd", T, {
+      if (activation == VMF_ACT_SOFTPLUS) linear_few_kernel<T, true><<<grid, 512, 0, st>>>(p, *few);
+      else linear_few_kernel<T, false><<<grid, 512, 0, st>>>(p, *few);
+      if (p.partial) mm_join_kernel<T><<<vmf_grid_for(m * n, 256, 1 << 14), 256, 0, st>>>(p, pl.splits);
+    });
+    return vmf_check_launch("vmf_blocks8_linear_fwd");
+  }
   if (out_dtype == VMF_F32) mm_launch<true, float>(pl, p, st);
   else if (out_dtype == VMF_F16) mm_launch<false, f16_t>(pl, p, st);
   else mm_launch<false, bf16_t>(pl, p, st);
   return vmf_check_launch(what);
+}
+
+extern "C" int vmf_blocks8_matmul(const uint8_t* a, const uint8_t* a_exponents, int64_t a_exp_pitch, int a_tiled,
+                                  const uint8_t* b, const uint8_t* b_exponents, int64_t b_exp_pitch, int b_tiled,
+                                  const void* bias, int bias_dtype, const uint8_t* gate,
+                                  const uint8_t* gate_exponents, int64_t gate_exp_pitch, double beta, void* out,
+                                  int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes,
+                                  int out_dtype, vmf_stream_t stream) {
+  VMF_RANGE("vmf_blocks8_matmul");
+  return matmul(nullptr, VMF_ACT_NONE, a, a_exponents, a_exp_pitch, a_tiled, b, b_exponents, b_exp_pitch, b_tiled, bias,
+                bias_dtype, gate, gate_exponents, gate_exp_pitch, beta, out, m, n, k, workspace, workspace_bytes,
+                out_dtype, stream);
 }
 
 extern "C" int vmf_blocks8_weight_grad_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes_out) {
@@ -1215,10 +1323,23 @@ int64_t row_block_bytes(int64_t rows, int64_t width) { return b8_blocks(width) *
 int64_t tile_bytes(int64_t rows, int64_t width) { return up16(b8_blocks(width) * (rows * B8 + b8_blocks(rows))); }
 }  // namespace
 
-extern "C" int vmf_blocks8_linear_fwd_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes_out) {
+// Whether x's rows are few enough for linear_few_kernel: at most 64 blocks for a workgroup to quantise (two per 16 lanes,
+// about a microsecond, as long as the weight's bytes take to come).
+static bool few_fits(int64_t m, int64_t n, int64_t k) {
+  if (m < 1 || m > 16) return false;
+  const MmPlan pl = mm_plan(m, n, b8_blocks(k), false);
+  return m * pl.per_split <= FEW_MAX_BLOCKS;
+}
+
+extern "C" int vmf_blocks8_linear_fwd_workspace(int64_t m, int64_t n, int64_t k, int laid_out, int kept, int dtype,
+                                                int64_t* bytes_out) {
   int rc = vmf_blocks8_matmul_workspace(m, n, k, dtype, bytes_out);
-  if (rc == VMF_OK) *bytes_out = up16(*bytes_out) + tile_bytes(n, k);
-  return rc;
+  if (rc != VMF_OK) return rc;
+  VMF_REQUIRE(n >= 1, VMF_ERR_BAD_ARG, "vmf_blocks8_linear_fwd_workspace: n = %lld", (long long)n);
+  *bytes_out = up16(*bytes_out);
+  if (!laid_out) *bytes_out += tile_bytes(n, k);
+  if (!kept && !(laid_out && few_fits(m, n, k))) *bytes_out += row_block_bytes(m, k);
+  return VMF_OK;
 }
 
 extern "C" int vmf_blocks8_linear_fwd(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
@@ -1229,19 +1350,35 @@ extern "C" int vmf_blocks8_linear_fwd(const void* x, int64_t x_stride, const voi
                                       int64_t workspace_bytes, int dtype, vmf_stream_t stream) {
   VMF_RANGE("vmf_blocks8_linear_fwd");
   const char* what = "vmf_blocks8_linear_fwd";
-  int64_t need = 0;
-  int rc = vmf_blocks8_matmul_workspace(m, n, k, dtype, &need);
+  int64_t all = 0, need = 0;
+  int rc = vmf_blocks8_linear_fwd_workspace(m, n, k, weight == nullptr, a_values != nullptr, dtype, &all);
   if (rc != VMF_OK) return rc;
-  const int64_t front = up16(need), all = weight ? front + tile_bytes(n, k) : need;
-  VMF_REQUIRE(n >= 1, VMF_ERR_BAD_ARG, "%s: n = %lld", what, (long long)n);
+  vmf_blocks8_matmul_workspace(m, n, k, dtype, &need);
   VMF_REQUIRE(all == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= all), VMF_ERR_BAD_ARG,
               "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)all);
+  uint8_t* at = (uint8_t*)workspace + up16(need);
+  if (!a_values && !weight && few_fits(m, n, k)) {
+    VMF_REQUIRE(x && x_stride >= 0, VMF_ERR_BAD_ARG, "%s: x", what);
+    VMF_REQUIRE(activation == VMF_ACT_NONE || activation == VMF_ACT_SOFTPLUS, VMF_ERR_BAD_ARG, "%s: activation %d", what,
+                activation);
+    if (activation == VMF_ACT_NONE) beta = 1.0;
+    VMF_REQUIRE(beta > 0 && beta <= 1e30 && beta >= 1e-30, VMF_ERR_BAD_ARG, "%s: beta %g", what, beta);
+    const FewArgs f{x, x_stride, k, (float)beta, (float)(1.0 / beta), beta};
+    return matmul(&f, activation, nullptr, nullptr, 0, 0, w_values, w_exponents, b8_blocks(n), 1, bias, bias_dtype,
+                  nullptr, nullptr, 0, 1.0, y, m, n, k, workspace, need, dtype, stream);
+  }
+  if (!a_values) {
+    a_values = at;
+    a_exponents = at + m * b8_blocks(k) * B8;
+    a_exp_pitch = exp_rows(m);
+    at += row_block_bytes(m, k);
+  }
   if (weight) {
-    uint8_t* v = (uint8_t*)workspace + front;
-    w_values = v;
-    w_exponents = v + n * b8_blocks(k) * B8;
+    uint8_t* e = at + n * b8_blocks(k) * B8;
     rc = b8_quantize_both(x, x_stride, a_values, a_exponents, a_exp_pitch, m, k, activation, beta, dtype, weight,
-                          weight_stride, v, v + n * b8_blocks(k) * B8, wt_values, wt_exponents, n, weight_dtype, stream);
+                          weight_stride, at, e, wt_values, wt_exponents, n, weight_dtype, stream);
+    w_values = at;
+    w_exponents = e;
   } else {
     rc = vmf_blocks8_quantize(x, x_stride, a_values, a_exponents, a_exp_pitch, m, k, activation, beta, dtype, stream);
   }

@@ -14,41 +14,47 @@ import torch
 from . import _lib
 
 
+_ROWS = (torch.float32, torch.float64, torch.float16, torch.bfloat16)
+
+
 def _check(x, weight, bias):
     if x.dim() < 1:
         raise ValueError("layer_norm: x needs at least one dimension")
     width = x.shape[-1]
     if width < 1:
         raise ValueError("layer_norm: the last dimension is empty")
-    code = _lib.float_code(x, "layer_norm", (torch.float32, torch.float64, torch.float16, torch.bfloat16))
-    params = [p for p in (weight, bias) if p is not None]
-    for p in params:
-        if tuple(p.shape) != (width,):
+    code = wcode = _lib.float_code(x, "layer_norm", _ROWS)
+    first = None
+    for p in (weight, bias):
+        if p is None:
+            continue
+        if p.dim() != 1 or p.shape[0] != width:
             raise ValueError(f"layer_norm: weight and bias must have shape ({width},), got {tuple(p.shape)}")
-        if p.dtype != params[0].dtype:
-            raise TypeError(f"layer_norm: weight and bias differ in type ({params[0].dtype}, {p.dtype})")
-        if p.dtype != x.dtype and not (p.dtype == torch.float32 and x.dtype in (torch.float16, torch.bfloat16)):
+        if first is not None and p.dtype != first:
+            raise TypeError(f"layer_norm: weight and bias differ in type ({first}, {p.dtype})")
+        first = p.dtype
+        wcode = _lib.FLOAT_CODES.get(first, -1)
+        if wcode != code and not (wcode == _lib.VMF_F32 and code in (_lib.VMF_F16, _lib.VMF_BF16)):
             raise TypeError(f"layer_norm: weight and bias of {x.dtype} rows are {x.dtype}"
-                            f"{' or float32' if x.dtype in (torch.float16, torch.bfloat16) else ''}, got {p.dtype}")
-    wcode = _lib.FLOAT_CODES[params[0].dtype] if params else code
+                            f"{' or float32' if code in (_lib.VMF_F16, _lib.VMF_BF16) else ''}, got {first}")
     return _lib.require_hip(x, weight, bias), code, wcode
 
 
-def _forward(x, weight, bias, eps, dev, code, wcode, keep):
-    rows, stride = _lib.as_rows(x.detach())
+def _forward(x, w, b, eps, dev, code, wcode, keep):
+    rows, stride = _lib.as_rows(x)
     n, width = rows.shape
-    w = None if weight is None else weight.detach().contiguous()
-    b = None if bias is None else bias.detach().contiguous()
+    w, b = _lib.dense(w), _lib.dense(b)
     y = torch.empty(x.shape, device=dev, dtype=x.dtype)
     stats = mean = rstd = None
     if keep:  # the rows' means, then their reciprocal deviations
         stats = torch.empty(2 * n, device=dev, dtype=torch.float64 if code == _lib.VMF_F64 else torch.float32)
         mean = stats.data_ptr()
-        rstd = mean + n * stats.element_size()
+        rstd = mean + n * (8 if code == _lib.VMF_F64 else 4)
     with _lib.on_device(dev):
         rc = _lib.lib().vmf_layer_norm_fwd(rows.data_ptr(), stride, _lib.address(w), _lib.address(b), y.data_ptr(),
                                            mean, rstd, n, width, eps, code, wcode, _lib.raw_stream(dev))
-    _lib.check(rc, "vmf_layer_norm_fwd")
+    if rc:
+        _lib.check(rc, "vmf_layer_norm_fwd")
     return y, rows, stride, w, stats
 
 
@@ -57,32 +63,33 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps, dev, code, wcode):
         y, rows, stride, w, stats = _forward(x, weight, bias, eps, dev, code, wcode, True)
         ctx.save_for_backward(rows, w, stats)
-        ctx.meta = (x.shape, stride, None if bias is None else bias.dtype, code, wcode, dev)
+        ctx.meta = (x.shape, rows.shape, stride, code, wcode, dev, None if bias is None else bias.dtype)
         return y
 
     @staticmethod
     @_lib.first_order
     def backward(ctx, gy):
         rows, w, stats = ctx.saved_tensors
-        shape, x_stride, bias_dtype, code, wcode, dev = ctx.meta
+        shape, (n, width), x_stride, code, wcode, dev, p_dtype = ctx.meta
         g, g_stride = _lib.as_rows(gy)
-        n, width = rows.shape
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        gx = torch.empty(shape, device=dev, dtype=rows.dtype) if need_x else None
+        gx = torch.empty(shape, device=dev, dtype=gy.dtype) if need_x else None
         gw = torch.empty(width, device=dev, dtype=w.dtype) if need_w else None
-        gb = torch.empty(width, device=dev, dtype=bias_dtype) if need_b else None
+        gb = torch.empty(width, device=dev, dtype=p_dtype) if need_b else None
         lib = _lib.lib()
         ws, need = None, C.c_int64(0)
         if need_w or need_b:
             _lib.check(lib.vmf_layer_norm_bwd_workspace(n, width, code, need), "vmf_layer_norm_bwd_workspace")
-            ws = torch.empty(need.value, device=dev, dtype=torch.uint8) if need.value else None
+            if need.value:
+                ws = torch.empty(need.value, device=dev, dtype=torch.uint8)
         mean = stats.data_ptr()
         with _lib.on_device(dev):
             rc = lib.vmf_layer_norm_bwd(rows.data_ptr(), x_stride, g.data_ptr(), g_stride, _lib.address(w), mean,
-                                        mean + n * stats.element_size(), _lib.address(gx), _lib.address(gw),
-                                        _lib.address(gb), n, width, _lib.address(ws), need.value, code, wcode,
-                                        _lib.raw_stream(dev))
-        _lib.check(rc, "vmf_layer_norm_bwd")
+                                        mean + n * (8 if code == _lib.VMF_F64 else 4), _lib.address(gx),
+                                        _lib.address(gw), _lib.address(gb), n, width, _lib.address(ws), need.value, code,
+                                        wcode, _lib.raw_stream(dev))
+        if rc:
+            _lib.check(rc, "vmf_layer_norm_bwd")
         return gx, gw, gb, None, None, None, None
 
 
@@ -90,7 +97,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x."""
     dev, code, wcode = _check(x, weight, bias)
     eps = float(eps)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, eps, dev, code, wcode)
     return _forward(x, weight, bias, eps, dev, code, wcode, False)[0]
 

@@ -93,7 +93,7 @@ def test_layer_entry_refusals():
     lib = _lib.lib()
     p = C.c_void_p(256)
     need = C.c_int64(0)
-    assert lib.vmf_blocks8_linear_fwd_workspace(4, 4, 8, 0, need) == 0 and need.value > 0
+    assert lib.vmf_blocks8_linear_fwd_workspace(4, 4, 8, 0, 1, 0, need) == 0 and need.value > 0
 
     def fwd(m=4, n=4, k=8, weight=p, dtype=0, w_dtype=0, act=0, nbytes=need.value, ws=p, wt=None, wte=None):
         return lib.vmf_blocks8_linear_fwd(p, 8, weight, 8, w_dtype, None, None, wt, wte, None, 0, act, 1.0, p, p, 16, p, m, n,
@@ -103,6 +103,10 @@ def test_layer_entry_refusals():
     assert fwd(nbytes=need.value - 1) == -1 and fwd(ws=C.c_void_p(264)) == -1 and fwd(wt=p) == -1
     assert fwd(dtype=3, w_dtype=2) == -2
     assert fwd(m=0, weight=None) == 0  # no rows and no weight to lay out: nothing to do
+    few = C.c_int64(-1)
+    assert lib.vmf_blocks8_linear_fwd_workspace(1, 4096, 4096, 1, 0, 0, few) == 0 and few.value == 0  # one launch
+    assert lib.vmf_blocks8_linear_fwd_workspace(17, 4096, 4096, 1, 0, 0, few) == 0 and few.value > 0
+    assert lib.vmf_blocks8_linear_fwd_workspace(1, 0, 4096, 1, 0, 0, few) == -1
     assert lib.vmf_blocks8_linear_bwd_workspace(4, 4, 8, 0, need) == 0 and need.value > 0
     assert lib.vmf_blocks8_linear_bwd_workspace(4, 0, 8, 0, need) == -1
     assert lib.vmf_blocks8_linear_bwd_workspace(4, 4, 8, 0, need) == 0

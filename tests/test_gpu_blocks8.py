@@ -308,8 +308,26 @@ def test_linear(m, n, k, activation, beta, x_type, w_type):
         want = layer_formula(x, w, b, gy, activation, beta)
         for name, terms in (("y", k + 8), ("gx", n + 16), ("gw", m / 16 + 64), ("gb", m / 16 + 64)):
             near(got[name], *want[name], terms)
-        # the same layer with the weight laid out beforehand
+        # the same layer with the weight laid out beforehand, and without anything to keep
         assert torch.equal(blocks8.linear(x, blocks8.quantize_weight(w), b, activation, beta), y)
+    xs = x.detach().requires_grad_()
+    assert torch.equal(blocks8.linear(xs, blocks8.quantize_weight(w), b, activation, beta), y)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("activation", [None, "softplus"])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 17, 300), (1, 784, 128), (1, 4096, 8192), (1, 40, 20000), (2, 100, 4000),
+                                   (3, 130, 129), (7, 33, 1000), (16, 50, 512), (16, 4096, 500), (16, 64, 3000)])
+def test_linear_of_few_rows(m, n, k, activation, dtype):
+    """a row or a few through a laid-out weight, whether or not the quantisation is part of the product's launch"""
+    wide = normal(m, k + 5, seed=1, scale=2.0).to(dtype)
+    x, w, b = wide[:, 2:2 + k], normal(n, k, seed=2, scale=k ** -0.5), normal(n, seed=3)
+    w8 = blocks8.quantize_weight(w)
+    got = blocks8.linear(x, w8, b, activation, 1.5)
+    q = blocks8.quantize(x, activation, 1.5)
+    a, wd = q.dequantize().double(), w8.rows.dequantize().double()
+    assert torch.equal(a, by_blocks(softplus(x, 1.5) if activation else x.double()))
+    near(got, a @ wd.t() + b, a.abs() @ wd.abs().t() + b.abs(), k + 8)
 
 
 def test_linear_leading_dimensions_and_which_gradients_are_asked_for():
