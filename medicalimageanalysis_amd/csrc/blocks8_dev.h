@@ -190,8 +190,20 @@ __device__ __forceinline__ uint2 softplus8(const float (&h)[8], float beta, floa
   return uint2{w[0], w[1]};
 }
 
-// d softplus / dh from the kept a = softplus(h): sigmoid(beta h) = 1 - exp(-beta a)
-__device__ __forceinline__ float b8_softplus_slope(float a, float beta) { return -expm1f(-beta * a); }
+// d softplus / dh from the kept a = softplus(h): sigmoid(beta h) = 1 - exp(-z), z = beta a.  For z under 1/2 the series
+// to z^8 (the rest is under 2e-8 of it), else from the hardware's exponential, whose unit in the last place is 2^-24 of
+// at most 0.6 against a result of at least 0.39.
+__device__ __forceinline__ float b8_softplus_slope(float a, float beta) {
+  const float z = beta * a;
+  float s = fmaf(z, -1.0f / 40320, 1.0f / 5040);
+  s = fmaf(z, -s, 1.0f / 720);
+  s = fmaf(z, -s, 1.0f / 120);
+  s = fmaf(z, -s, 1.0f / 24);
+  s = fmaf(z, -s, 1.0f / 6);
+  s = fmaf(z, -s, 0.5f);
+  s = fmaf(z, -s, 1.0f);
+  return z < 0.5f ? z * s : 1.0f - __builtin_amdgcn_exp2f(z * -1.44269504f);
+}
 
 // f(integral_constant<int, 0>), ..., f(integral_constant<int, N - 1>)
 template <typename F, int... I>

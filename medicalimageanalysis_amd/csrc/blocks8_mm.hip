@@ -97,27 +97,16 @@ __device__ __forceinline__ float load_bias(const void* bias, int code, int64_t i
                          : code == VMF_F16 ? (float)((const f16_t*)bias)[i] : (float)((const bf16_t*)bias)[i];
 }
 
-// bias, gate and rounding of NC consecutive columns of one row
-template <int NC, typename OUT>
-__device__ __forceinline__ void finish(const MmArgs& p, int64_t row, int64_t col, const float* bias, float* v) {
-#pragma unroll
-  for (int j = 0; j < NC; ++j) v[j] += bias[j];
+// bias, gate and rounding of one element
+template <typename OUT>
+__device__ __forceinline__ void finish1(const MmArgs& p, int64_t row, int64_t col, float v) {
+  if (p.bias) v += load_bias(p.bias, p.bias_code, col);
   if (p.gate.values) {
-    const uint8_t* q = p.gate.values + row * p.gate.pitch + col;
-    const float scale = b8_scale(p.gate.exps[(col >> 7) * p.gate.exp_pitch + row]);
     float a[4];
-    if constexpr (NC == 4) {
-      b8_unpack4(*reinterpret_cast<const uint32_t*>(q), scale, a);
-    } else {
-      uint32_t w = 0;
-#pragma unroll
-      for (int j = 0; j < NC; ++j) w |= (uint32_t)q[j] << (8 * j);
-      b8_unpack4(w, scale, a);
-    }
-#pragma unroll
-    for (int j = 0; j < NC; ++j) v[j] *= b8_softplus_slope(a[j], p.beta);
+    b8_unpack4(p.gate.values[row * p.gate.pitch + col], b8_scale(p.gate.exps[(col >> 7) * p.gate.exp_pitch + row]), a);
+    v *= b8_softplus_slope(a[0], p.beta);
   }
-  store_some<NC>((OUT*)p.out + row * p.n + col, p.n - col, v);
+  ((OUT*)p.out)[row * p.n + col] = (OUT)v;
 }
 
 // Workgroup b runs on XCD b % 8: give each XCD a contiguous run of tiles, and walk the run in columns of 8 row tiles, so
@@ -144,34 +133,66 @@ __device__ __forceinline__ v8i operand(const uint8_t* tile, int lane) {
   const v4i hi = *reinterpret_cast<const v4i*>(tile + q * B8 + (((c + 1) ^ (q >> 1)) << 4));
   return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
-// what a wave holds of the result: lane l has rows FM * (4 * (l / 16) + r) + i, columns FN * (l % 16) + 0 .. FN - 1 of
-// each group of 16 FM rows and 16 FN columns
-template <int FM, int FN, int GM, int GN, typename OUT>
+// What a wave holds of the result: lane l has the rows 4 FM * (l / 16) + t (t = FM * r + i: element r of row tile i) and
+// the columns FN * (l % 16) + 0 .. FN - 1 of each group of 16 FM rows and 16 FN columns.  GATE: the 4 FM rows' kept
+// values are all asked for before the first is used.
+template <int FM, int FN, int GM, int GN, bool GATE, typename OUT>
 __device__ __forceinline__ void write_tile(const MmArgs& p, const v4f (&acc)[GM * FM][GN * FN], int64_t row0, int64_t col0,
                                            int lane) {
+  constexpr int R = 4 * FM;
+  const bool whole = row0 + GM * 16 * FM <= p.m && col0 + GN * 16 * FN <= p.n;
 #pragma unroll
   for (int h = 0; h < GN; ++h) {
     const int64_t col = col0 + h * 16 * FN + FN * (lane & 15);
-    if (col >= p.n) continue;
+    if (!whole && col >= p.n) continue;
+    const int left = whole || p.n - col >= FN ? FN : (int)(p.n - col);
     float bias[FN];
 #pragma unroll
-    for (int j = 0; j < FN; ++j) bias[j] = p.bias && !p.partial && col + j < p.n ? load_bias(p.bias, p.bias_code, col + j) : 0.0f;
+    for (int j = 0; j < FN; ++j) bias[j] = p.bias && !p.partial && j < left ? load_bias(p.bias, p.bias_code, col + j) : 0.0f;
 #pragma unroll
-    for (int g = 0; g < GM; ++g)
+    for (int g = 0; g < GM; ++g) {
+      const int64_t row = row0 + g * 16 * FM + R * (lane >> 4);
+      const int rows = whole || p.m - row >= R ? R : (int)(p.m - row);
+      if (rows <= 0) continue;
+      uint32_t code[GATE ? R : 1], ex[GATE ? R / 4 : 1];
+      if constexpr (GATE) {
+        const uint8_t* q = p.gate.values + row * p.gate.pitch + col;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+        for (int t = 0; t < R; ++t) {
+          const uint8_t* at = q + (t < rows ? t : rows - 1) * p.gate.pitch;
+          code[t] = FN == 4 ? *reinterpret_cast<const uint32_t*>(at) : *reinterpret_cast<const uint16_t*>(at);
+        }
+        // (the exponents of rows come in sixteens, so these words are all there)
+        const uint32_t* e = reinterpret_cast<const uint32_t*>(p.gate.exps + (col >> 7) * p.gate.exp_pitch + row);
 #pragma unroll
-        for (int i = 0; i < FM; ++i) {
-          const int64_t row = row0 + g * 16 * FM + FM * (4 * (lane >> 4) + r) + i;
-          if (row >= p.m) continue;
+        for (int t = 0; t < R / 4; ++t) ex[t] = e[t];
+      }
+      OUT* out = (OUT*)p.out + row * p.n + col;
+      float* part = p.partial + ((int64_t)blockIdx.y * p.m + row) * p.n + col;
+#pragma unroll
+      for (int t = 0; t < R; ++t) {
+        if (t < rows) {
           float v[FN];
 #pragma unroll
-          for (int j = 0; j < FN; ++j) v[j] = acc[g * FM + i][h * FN + j][r];
-          if (p.partial)
-            store_some<FN>(p.partial + ((int64_t)blockIdx.y * p.m + row) * p.n + col, p.n - col, v);
-          else
-            finish<FN, OUT>(p, row, col, bias, v);
+          for (int j = 0; j < FN; ++j) v[j] = acc[g * FM + t % FM][h * FN + j][t / FM];
+          if (p.partial) {
+            store_some<FN>(part, left, v);
+          } else {
+#pragma unroll
+            for (int j = 0; j < FN; ++j) v[j] += bias[j];
+            if constexpr (GATE) {
+              float a[4];
+              b8_unpack4(code[t], b8_scale(ex[t / 4] >> (8 * (t % 4)) & 0xff), a);
+#pragma unroll
+              for (int j = 0; j < FN; ++j) v[j] *= b8_softplus_slope(a[j], p.beta);
+            }
+            store_some<FN>(out, left, v);
+          }
         }
+        out += p.n;
+        part += p.n;
+      }
+    }
   }
 }
 
@@ -182,7 +203,7 @@ __device__ __forceinline__ void write_tile(const MmArgs& p, const v4f (&acc)[GM 
 //   lane's F tiles are then one word, and a lane's results are F consecutive columns of a row.
 //   In LDS the 16 rows of an operand tile lie side by side, the 16-byte pieces of row q at piece ^ (q / 2): the 16 lanes
 //   that read the same piece of the 16 rows then read from all 64 banks (two rows fill the banks once).
-template <int BM, int BN, int WM, int WN, bool WIDE, typename OUT>
+template <int BM, int BN, int WM, int WN, bool WIDE, bool GATE, typename OUT>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p) {
   constexpr int WAVES_N = BN / WN, WAVES = (BM / WM) * WAVES_N;
   constexpr int FM = WM / 16 < 4 ? WM / 16 : 4, FN = WN / 16 < 4 ? WN / 16 : 4;  // tiles that share an exponent word
@@ -299,7 +320,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p
     }
   }
 
-  write_tile<FM, FN, GM, GN, OUT>(p, acc, m0 + wm, n0 + wn, lane);
+  write_tile<FM, FN, GM, GN, GATE, OUT>(p, acc, m0 + wm, n0 + wn, lane);
 }
 
 // The same for large 16-bit results: tile of 256 x 256, eight waves of 128 x 64, a block column's 32 products per wave in
@@ -309,7 +330,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p
 // phases, so that they do not stand before the operand reads in the queue.
 // Bound: 2048 clocks of matrix instructions per block column and CU, against 1536 + 512 clocks of LDS reads and writes.
 // a by rows, b by tiles, as a layer has them.
-template <typename OUT>
+template <bool GATE, typename OUT>
 __global__ __launch_bounds__(512, 2) void mm_large_kernel(MmArgs p) {
   constexpr int BM = 256, BN = 256, STAGE = (BM + BN) * B8;
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
@@ -432,7 +453,7 @@ __global__ __launch_bounds__(512, 2) void mm_large_kernel(MmArgs p) {
     }
     step(kb, (kb - kb0) & 1, std::integral_constant<int, 0>{});
   }
-  write_tile<4, 4, 2, 1, OUT>(p, acc, m0 + wm, n0 + wn, lane);
+  write_tile<4, 4, 2, 1, GATE, OUT>(p, acc, m0 + wm, n0 + wn, lane);
 }
 
 // the eight waves' sums of 16 rows and 16 columns, added in their order
@@ -451,8 +472,7 @@ __device__ __forceinline__ void few_result(const MmArgs& p, float (&sums)[8][16]
   if (p.partial) {
     p.partial[((int64_t)blockIdx.y * p.m + row) * p.n + col] = v;
   } else {
-    const float bias = p.bias ? load_bias(p.bias, p.bias_code, col) : 0.0f;
-    finish<1, OUT>(p, row, col, &bias, &v);
+    finish1<OUT>(p, row, col, v);
   }
 }
 
@@ -577,8 +597,7 @@ __global__ __launch_bounds__(256) void mm_join_kernel(MmArgs p, int splits) {
     float v = 0;
     for (int s = 0; s < splits; ++s) v += p.partial[s * total + i];
     const int64_t row = i / p.n, col = i - row * p.n;
-    const float bias = p.bias ? load_bias(p.bias, p.bias_code, col) : 0.0f;
-    finish<1, OUT>(p, row, col, &bias, &v);
+    finish1<OUT>(p, row, col, v);
   }
 }
 
@@ -614,13 +633,18 @@ MmPlan mm_plan(int64_t m, int64_t n, int64_t blocks, bool large) {
   return p;
 }
 
+template <bool WIDE, bool GATE, typename OUT>
+void mm_launch_tiles(const MmPlan& pl, const MmArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)(pl.mt * pl.nt), (unsigned)pl.splits);
+  if (pl.kind == MM_64) mm_kernel<64, 64, 32, 32, WIDE, GATE, OUT><<<grid, 256, 0, st>>>(a);
+  else if (pl.kind == MM_128) mm_kernel<128, 128, 64, 64, WIDE, GATE, OUT><<<grid, 256, 0, st>>>(a);
+  else if constexpr (!WIDE) mm_large_kernel<GATE, OUT><<<grid, 512, 0, st>>>(a);
+}
 template <bool WIDE, typename OUT>
 void mm_launch(const MmPlan& pl, const MmArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)(pl.mt * pl.nt), (unsigned)pl.splits);
-  if (pl.kind == MM_FEW) mm_few_kernel<WIDE, OUT><<<grid, 512, 0, st>>>(a);
-  else if (pl.kind == MM_64) mm_kernel<64, 64, 32, 32, WIDE, OUT><<<grid, 256, 0, st>>>(a);
-  else if (pl.kind == MM_128) mm_kernel<128, 128, 64, 64, WIDE, OUT><<<grid, 256, 0, st>>>(a);
-  else if constexpr (!WIDE) mm_large_kernel<OUT><<<grid, 512, 0, st>>>(a);
+  if (pl.kind == MM_FEW) mm_few_kernel<WIDE, OUT><<<dim3((unsigned)pl.nt, (unsigned)pl.splits), 512, 0, st>>>(a);
+  else if (a.gate.values && !a.partial) mm_launch_tiles<WIDE, true, OUT>(pl, a, st);
+  else mm_launch_tiles<WIDE, false, OUT>(pl, a, st);
   if (a.partial) mm_join_kernel<OUT><<<vmf_grid_for(a.m * a.n, 256, 1 << 14), 256, 0, st>>>(a, pl.splits);
 }
 
