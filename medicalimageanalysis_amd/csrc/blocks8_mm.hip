@@ -788,194 +788,30 @@ __device__ __forceinline__ void expand16(v4i a, uint32_t exp_byte, uint4* out) {
 
 // Tile of BN (n) x BK (k) over the batch's rows, 32 at a time; waves of WN x WK.
 //   gy's terms and a's values lie in LDS as bf16 rows and are read back transposed (the rows are the products' inner
-//   dimension).  Two stages, one barrier per 32 rows; the rows of two steps ahead are on their way in registers, as they
-//   are in memory (one step's products take 256 to 1024 clocks, a load about 2000).
-//   Bound: a step of the 256 x 256 tile is 1024 clocks of matrix instructions and moves 128 KiB through LDS, 1024 clocks.
+//   dimension).  Each half of a step's products has its operands read while the half before it is multiplied, across the
+//   step's one barrier as well; the next step's rows go from registers into the other stage between, and the rows after
+//   that are asked for.
+//   WHOLE: gy comes in whole aligned 16-byte pieces (n, the row stride and the address are multiples of them).
 //   The workgroups of the first k tile also add up gbias.  gy's 8-bit blocks (what the input gradient's product reads) are
 //   written on the way too, the k tiles' workgroups taking turns.
+// Bound: per step and CU the 256 x 256 tile (bf16) takes 1024 clocks of matrix instructions against 640 + 256 of LDS reads
+// and writes; the 128 x 256 tile 1024 (fp16) and 1536 (fp32), where the vector work of taking gy apart comes next, which
+// is why this tile is wide in k.
 constexpr int WG_ROWS = 32;
 
-template <typename T, typename W, int BN, int BK, int WN, int WK>
+template <typename T, typename W, int BN, int BK, int WN, int WK, bool WHOLE>
 __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void wgrad_kernel(WgArgs p) {
-  constexpr int THREADS = (BN / WN) * (BK / WK) * 64;
+  constexpr int WAVES_K = BK / WK, THREADS = (BN / WN) * WAVES_K * 64;
   constexpr int NT = Terms<T>::count;
-  constexpr int E = 16 / (int)sizeof(T);          // elements of gy in a 16-byte piece
-  constexpr int GP = BN / E;                      // pieces per row; divides THREADS, so a thread keeps its columns
-  constexpr int GN = WG_ROWS * GP / THREADS;      // pieces per thread and step
-  constexpr int AP = BK / 16, AN = WG_ROWS * AP / THREADS;
-  // bytes; 64 more than the row: the four rows of a transposed read lie in different banks.  (Half of that where two terms
-  // and the large tile leave no registers for the addresses that 64 takes: 1.1 -> 1.0 ms for fp16 16384x4096x4096.)
-  constexpr int PAD = NT == 2 && BN == 256 ? 32 : 64, PITCH_G = 2 * BN + PAD, PITCH_A = 2 * BK + PAD;
-  constexpr int PLANE = WG_ROWS * PITCH_G, STAGE = NT * PLANE + WG_ROWS * PITCH_A;
-  static_assert(THREADS % GP == 0 && THREADS % AP == 0 && GN >= 1 && AN >= 1, "whole pieces");
+  constexpr int E = 16 / (int)sizeof(T);                     // elements of gy in a 16-byte piece
+  constexpr int GP = BN / E, GROWS = THREADS / GP;           // pieces per row, rows per pass of the workgroup
+  constexpr int GN = WG_ROWS / GROWS;                        // passes
   constexpr int FN = WN / 32, FK = WK / 32;
-  typedef typename Pack<T, E>::type Piece;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
-
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int nt = (int)blockIdx.x / p.kt, kt = (int)blockIdx.x % p.kt;
-  const int64_t n0 = (int64_t)nt * BN, k0 = (int64_t)kt * BK;
-  const int64_t m0 = (int64_t)blockIdx.y * p.rows_per_split;
-  const int64_t m1 = m0 + p.rows_per_split < p.m ? m0 + p.rows_per_split : p.m;
-  const int gr = threadIdx.x / GP, gc = (threadIdx.x % GP) * E;    // row and column of this thread's first piece of gy
-  const int ar = threadIdx.x / AP, ac = (threadIdx.x % AP) * 16;   // and of a
-  const int64_t left = p.n - n0 - gc;
-  const bool a_in = k0 + ac < p.a.pitch;  // the last tile may reach behind a's padded rows
-  const T* gsrc = (const T*)p.gy + n0 + gc;
-  const uint8_t* asrc = p.a.values + k0 + ac;
-  const uint8_t* esrc = p.a.exps + ((k0 + ac) >> 7) * p.a.exp_pitch;
-  const bool sums = kt == 0 && p.gb;
-
-  struct Step {
-    Piece g[GN];
-    v4i a[AN];
-    uint32_t e[AN];
-  };
-  Step ahead[2];
-  float gsum[E];
-#pragma unroll
-  for (int i = 0; i < E; ++i) gsum[i] = 0;
-  auto fetch = [&](int64_t m, Step& s) {
-#pragma unroll
-    for (int i = 0; i < GN; ++i) {
-      const int64_t row = m + gr + i * (THREADS / GP);
-      const T* src = gsrc + row * p.gy_stride;
-      Piece v;
-#pragma unroll
-      for (int j = 0; j < E; ++j) v[j] = (T)0;
-      if (row < m1) {
-        if (left >= E) {
-          v = *reinterpret_cast<const Piece*>(src);
-        } else {
-#pragma unroll
-          for (int j = 0; j < E; ++j)
-            if (j < left) v[j] = src[j];
-        }
-      }
-      s.g[i] = v;
-    }
-#pragma unroll
-    for (int i = 0; i < AN; ++i) {
-      const int64_t row = m + ar + i * (THREADS / AP);
-      s.a[i] = v4i{0, 0, 0, 0};
-      s.e[i] = 127;
-      if (row < m1 && a_in) {
-        s.a[i] = *reinterpret_cast<const v4i*>(asrc + row * p.a.pitch);
-        s.e[i] = esrc[row];
-      }
-    }
-  };
-  auto put = [&](int64_t m, const Step& s, int stage, bool blocks) {
-    uint8_t* base = lds + stage * STAGE;
-#pragma unroll
-    for (int i = 0; i < GN; ++i) {
-      const int r = gr + i * (THREADS / GP);
-      float v[E];
-#pragma unroll
-      for (int j = 0; j < E; ++j) v[j] = (float)s.g[i][j];
-      if (sums)
-#pragma unroll
-        for (int j = 0; j < E; ++j) gsum[j] += v[j];
-      uint32_t top = 0;
-      if (blocks || NT > 1)
-#pragma unroll
-        for (int j = 0; j < E; ++j) top = larger(top, b8_size(v[j]));
-      uint8_t* d = base + r * PITCH_G + gc * 2;
-      if constexpr (NT == 1) {
-        *reinterpret_cast<Piece*>(__builtin_assume_aligned(d, 16)) = s.g[i];
-      } else {
-        float u[E];
-#pragma unroll
-        for (int j = 0; j < E; ++j) u[j] = v[j];
-        const bool fine = top < B8_INF;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          uint32_t w[E / 2];
-          if (fine) {
-#pragma unroll
-            for (int j = 0; j < E / 2; ++j) w[j] = cut_finite(u[2 * j], u[2 * j + 1], t < NT - 1);
-          } else {
-#pragma unroll
-            for (int j = 0; j < E / 2; ++j) {
-              const uint32_t lo = cut(u[2 * j]), hi = cut(u[2 * j + 1]);
-              w[j] = lo | hi << 16;
-            }
-          }
-          if constexpr (E == 8) *reinterpret_cast<uint4*>(d + t * PLANE) = uint4{w[0], w[1], w[2], w[3]};
-          else *reinterpret_cast<uint2*>(d + t * PLANE) = uint2{w[0], w[1]};
-        }
-      }
-      if (blocks) write_gy_block<E>(p, v, top, m + r, n0 + gc, m + r < m1);
-    }
-#pragma unroll
-    for (int i = 0; i < AN; ++i)
-      expand16(s.a[i], s.e[i], reinterpret_cast<uint4*>(base + NT * PLANE + (ar + i * (THREADS / AP)) * PITCH_A + ac * 2));
-  };
-  const int wn = (wave / (BK / WK)) * WN, wk = (wave % (BK / WK)) * WK;
-  v16f acc[FN][FK];
-#pragma unroll
-  for (int i = 0; i < FN; ++i)
-#pragma unroll
-    for (int j = 0; j < FK; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
-
-  int turn = 0;  // which k tile's workgroup writes gy's blocks of this step
-  auto put_next = [&](int64_t m, const Step& st, int stage) {
-    put(m, st, stage, p.q && turn == kt);
-    turn = turn + 1 == p.kt ? 0 : turn + 1;
-  };
-  auto products = [&](const uint8_t* base, int s) {
-    v8b b[FK];
-#pragma unroll
-    for (int j = 0; j < FK; ++j) b[j] = transposed(lane, [&](int r) { return base + NT * PLANE + (s + r) * PITCH_A + (wk + 32 * j) * 2; });
-#pragma unroll
-    for (int t = NT - 1; t >= 0; --t)
-#pragma unroll
-      for (int i = 0; i < FN; ++i) {
-        const v8b a = transposed(lane, [&](int r) { return base + t * PLANE + (s + r) * PITCH_G + (wn + 32 * i) * 2; });
-#pragma unroll
-        for (int j = 0; j < FK; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[j], acc[i][j], 0, 0, 0);
-      }
-  };
-  // Between the two halves of a step's products the next step's rows go into the other stage (read last before the
-  // barrier), while the matrix unit still works on the first half.
-  if (m0 < m1) {
-    fetch(m0, ahead[0]);
-    put_next(m0, ahead[0], 0);
-    if (m0 + WG_ROWS < m1) fetch(m0 + WG_ROWS, ahead[1]);
-    if (m0 + 2 * WG_ROWS < m1) fetch(m0 + 2 * WG_ROWS, ahead[0]);
-  }
-  for (int64_t mm = m0; mm < m1; mm += 2 * WG_ROWS) {
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int64_t m = mm + half * WG_ROWS;
-      if (m < m1) {
-        __syncthreads();
-        const uint8_t* base = lds + half * STAGE;
-        products(base, 0);
-        if (m + WG_ROWS < m1) {
-          put_next(m + WG_ROWS, ahead[half ^ 1], half ^ 1);
-          if (m + 3 * WG_ROWS < m1) fetch(m + 3 * WG_ROWS, ahead[half ^ 1]);
-        }
-        products(base, 16);
-      }
-    }
-  }
-
-  write_wgrad<W, FN, FK>(p, acc, n0 + wn, k0 + wk, lane);
-  static_assert(THREADS / GP * BN * 4 <= 2 * STAGE, "the sums fit the stages");
-  if (sums) write_gbias<W, BN, THREADS / GP, E>(p, lds, gsum, gr, gc, n0);
-}
-
-// The same for bf16 gradients in whole aligned 16-byte pieces (n, the row stride and the address are multiples of 8
-// elements): tile of 256 x 256, eight waves of 128 x 64.  Each half of a step's products has its operands read while the
-// half before it is multiplied, across the barrier as well; the next step's rows go from registers into the other stage
-// between, and the rows after that are asked for.
-// Bound: 1024 clocks of matrix instructions per step and CU, against 640 + 256 clocks of LDS reads and writes.
-template <typename W>
-__global__ __launch_bounds__(512, 2) void wgrad_large_kernel(WgArgs p) {
-  constexpr int BN = 256, BK = 256, PITCH = 2 * 256 + 64, PLANE = WG_ROWS * PITCH, STAGE = 2 * PLANE;
+  // bytes; 64 more than the row: the four rows of a transposed read lie in different banks
+  constexpr int PITCH_G = 2 * BN + 64, PITCH_A = 2 * BK + 64;
+  constexpr int PLANE = WG_ROWS * PITCH_G, STAGE = NT * PLANE + WG_ROWS * PITCH_A;
+  static_assert(THREADS % GP == 0 && GN >= 1 && THREADS == WG_ROWS * (BK / 16), "whole pieces");
+  static_assert(GROWS * BN * 4 <= 2 * STAGE, "gbias's sums fit the stages");
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // workgroup b runs on XCD b % 8: neighbouring tiles, which share gy's columns, on the same one
@@ -989,31 +825,56 @@ __global__ __launch_bounds__(512, 2) void wgrad_large_kernel(WgArgs p) {
   const int64_t m0 = (int64_t)blockIdx.y * p.rows_per_split;
   const int rows = (int)(m0 + p.rows_per_split < p.m ? p.rows_per_split : p.m - m0);
   const int steps = (rows + WG_ROWS - 1) / WG_ROWS;
-  const int wn = (wave >> 2) * 128, wk = (wave & 3) * 64;
+  const int wn = wave / WAVES_K * WN, wk = wave % WAVES_K * WK;
 
-  // gy: the 8 values from gc of rows gr and gr + 16 of a step; a: the 16 values from ac of row ar.  Where a tile reaches
-  // behind the last column the first columns are read instead (their results are dropped).
-  const int gr = threadIdx.x >> 5, gc = (threadIdx.x & 31) * 8;
-  const int ar = threadIdx.x >> 4, ac = (threadIdx.x & 15) * 16;
+  // gy: the E values from gc of rows gr, gr + GROWS ... of a step; a: the 16 values from ac of row ar.  Where a tile
+  // reaches behind the last column other ones are read instead, or none (their results are dropped).
+  const int gr = threadIdx.x / GP, gc = threadIdx.x % GP * E;
+  const int ar = threadIdx.x / (BK / 16), ac = threadIdx.x % (BK / 16) * 16;
   const bool g_in = n0 + gc < p.n, a_in = k0 + ac < p.a.pitch;
-  const uint8_t* gsrc = (const uint8_t*)p.gy + ((m0 + gr) * p.gy_stride + n0 + (g_in ? gc : 0)) * 2;
+  const int g_left = p.n - n0 - gc >= E ? E : g_in ? (int)(p.n - n0 - gc) : 0;
+  const uint8_t* gsrc = (const uint8_t*)p.gy + ((m0 + gr) * p.gy_stride + n0 + (g_in ? gc : 0)) * (int64_t)sizeof(T);
   const uint8_t* asrc = p.a.values + (m0 + ar) * p.a.pitch + k0 + (a_in ? ac : 0);
   const uint8_t* esrc = p.a.exps + ((k0 + (a_in ? ac : 0)) >> 7) * p.a.exp_pitch + m0 + ar;
-  const int64_t g_half = 16 * p.gy_stride * 2, g_step = 2 * g_half, a_step = WG_ROWS * p.a.pitch;
-  v4i g[2], av;
+  const int64_t g_pass = GROWS * p.gy_stride * (int64_t)sizeof(T), g_step = GN * g_pass, a_step = WG_ROWS * p.a.pitch;
+  v4i g[GN], av;
   uint32_t ae;
-  // the next step's rows; `left`: how many there are (32: no test)
-  auto load = [&](auto WHOLE, int left) {
-    if (decltype(WHOLE)::value) {
-      g[0] = *reinterpret_cast<const v4i*>(gsrc);
-      g[1] = *reinterpret_cast<const v4i*>(gsrc + g_half);
+  auto load_piece = [&](const uint8_t* src) -> v4i {
+    if constexpr (WHOLE) {
+      return *reinterpret_cast<const v4i*>(src);
+    } else {
+      union {
+        T e[E];
+        v4i v;
+      } u;
+      u.v = v4i{0, 0, 0, 0};
+      if (g_left == E) {
+        const typename Pack<T, E>::type w = *reinterpret_cast<const typename Pack<T, E>::type*>(src);
+#pragma unroll
+        for (int j = 0; j < E; ++j) u.e[j] = w[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (j < g_left) u.e[j] = reinterpret_cast<const T*>(src)[j];
+      }
+      return u.v;
+    }
+  };
+  // the next step's rows; ALL: all 32 are there, else `left` of them
+  auto load = [&](auto ALL, int left) {
+    if constexpr (decltype(ALL)::value) {
+#pragma unroll
+      for (int i = 0; i < GN; ++i) g[i] = load_piece(gsrc + i * g_pass);
       av = *reinterpret_cast<const v4i*>(asrc);
       ae = *esrc;
     } else {
-      g[0] = g[1] = av = v4i{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < GN; ++i) {
+        g[i] = v4i{0, 0, 0, 0};
+        if (gr + i * GROWS < left) g[i] = load_piece(gsrc + i * g_pass);
+      }
+      av = v4i{0, 0, 0, 0};
       ae = 127;
-      if (gr < left) g[0] = *reinterpret_cast<const v4i*>(gsrc);
-      if (gr + 16 < left) g[1] = *reinterpret_cast<const v4i*>(gsrc + g_half);
       if (ar < left) {
         av = *reinterpret_cast<const v4i*>(asrc);
         ae = *esrc;
@@ -1023,62 +884,119 @@ __global__ __launch_bounds__(512, 2) void wgrad_large_kernel(WgArgs p) {
     asrc += a_step;
     esrc += WG_ROWS;
   };
-  uint8_t* const g_to = lds + gr * PITCH + gc * 2;
-  uint8_t* const a_to = lds + PLANE + ar * PITCH + ac * 2;
+  auto unpack = [&](v4i piece, float(&v)[E]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = __int_as_float(piece[j]);
+    } else {
+      union {
+        v4i i;
+        T e[E];
+      } u;
+      u.i = piece;
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = (float)u.e[j];
+    }
+  };
+  uint8_t* const g_to = lds + gr * PITCH_G + gc * 2;
+  uint8_t* const a_to = lds + NT * PLANE + ar * PITCH_A + ac * 2;
   auto put = [&](int stage) {
-    *reinterpret_cast<v4i*>(g_to + stage * STAGE) = g[0];
-    *reinterpret_cast<v4i*>(g_to + stage * STAGE + 16 * PITCH) = g[1];
+    uint8_t* to = g_to + stage * STAGE;
+    if constexpr (NT == 1) {
+#pragma unroll
+      for (int i = 0; i < GN; ++i) *reinterpret_cast<v4i*>(to + i * GROWS * PITCH_G) = g[i];
+    } else {
+      float v[GN][E];
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < GN; ++i) {
+        unpack(g[i], v[i]);
+#pragma unroll
+        for (int j = 0; j < E; ++j) top = larger(top, b8_size(v[i][j]));
+      }
+      auto write = [&](int t, int i, const uint32_t(&w)[E / 2]) {
+        uint8_t* d = to + t * PLANE + i * GROWS * PITCH_G;
+        if constexpr (E == 8) *reinterpret_cast<uint4*>(d) = uint4{w[0], w[1], w[2], w[3]};
+        else *reinterpret_cast<uint2*>(d) = uint2{w[0], w[1]};
+      };
+      if (__all(top < B8_INF)) {
+#pragma unroll
+        for (int i = 0; i < GN; ++i)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            uint32_t w[E / 2];
+#pragma unroll
+            for (int j = 0; j < E / 2; ++j) w[j] = cut_finite(v[i][2 * j], v[i][2 * j + 1], t < NT - 1);
+            write(t, i, w);
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < GN; ++i)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            uint32_t w[E / 2];
+#pragma unroll
+            for (int j = 0; j < E / 2; ++j) {
+              const uint32_t lo = cut(v[i][2 * j]), hi = cut(v[i][2 * j + 1]);
+              w[j] = lo | hi << 16;
+            }
+            write(t, i, w);
+          }
+      }
+    }
     expand16(av, ae, reinterpret_cast<uint4*>(a_to + stage * STAGE));
   };
   // gbias and gy's blocks, from the rows in registers (those of step t)
   const bool sums = kt == 0 && p.gb;
-  float gsum[8];
+  float gsum[E];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) gsum[i] = 0;
+  for (int i = 0; i < E; ++i) gsum[i] = 0;
   int turn = 0;  // which k tile's workgroup writes the blocks of this step
   auto side = [&](int t) {
     const bool blocks = p.q && turn == kt;
     turn = turn + 1 == p.kt ? 0 : turn + 1;
     if (!sums && !blocks) return;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float v[8];
+    for (int i = 0; i < GN; ++i) {
+      float v[E];
       uint32_t top = 0;
+      unpack(g[i], v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[j] = __uint_as_float(j & 1 ? (uint32_t)g[i][j >> 1] & 0xffff0000u : (uint32_t)g[i][j >> 1] << 16);
-        if (!g_in) v[j] = 0;
+      for (int j = 0; j < E; ++j) {
+        if (WHOLE && !g_in) v[j] = 0;
         gsum[j] += v[j];
         top = larger(top, b8_size(v[j]));
       }
-      const int r = t * WG_ROWS + gr + 16 * i;
-      if (blocks) write_gy_block<8>(p, v, top, m0 + r, n0 + gc, r < rows);
+      const int r = t * WG_ROWS + gr + i * GROWS;
+      if (blocks) write_gy_block<E>(p, v, top, m0 + r, n0 + gc, r < rows);
     }
   };
 
   struct Half {
-    v8b g[4], a[2];
+    v8b g[NT * FN], a[FK];
   };
   auto read_half = [&](int stage, int s, Half& h) {
-    const uint8_t* G = lds + stage * STAGE + s * PITCH + wn * 2;
-    const uint8_t* A = lds + stage * STAGE + PLANE + s * PITCH + wk * 2;
+    const uint8_t* G = lds + stage * STAGE + s * PITCH_G + wn * 2;
+    const uint8_t* A = lds + stage * STAGE + NT * PLANE + s * PITCH_A + wk * 2;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) h.a[j] = transposed(lane, [&](int r) { return A + r * PITCH + j * 64; });
+    for (int j = 0; j < FK; ++j) h.a[j] = transposed(lane, [&](int r) { return A + r * PITCH_A + j * 64; });
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h.g[i] = transposed(lane, [&](int r) { return G + r * PITCH + i * 64; });
+    for (int i = 0; i < NT * FN; ++i)  // the smallest terms first
+      h.g[i] = transposed(lane, [&](int r) { return G + (NT - 1 - i / FN) * PLANE + r * PITCH_G + i % FN * 64; });
   };
-  v16f acc[4][2];
+  v16f acc[FN][FK];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < FN; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < FK; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
   auto multiply = [&](const Half& h, int from, int to) {
 #pragma unroll
     for (int i = from; i < to; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(h.g[i], h.a[j], acc[i][j], 0, 0, 0);
+      for (int j = 0; j < FK; ++j)
+        acc[i % FN][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(h.g[i], h.a[j], acc[i % FN][j], 0, 0, 0);
   };
 
   Half h0, h1;
@@ -1089,20 +1007,20 @@ __global__ __launch_bounds__(512, 2) void wgrad_large_kernel(WgArgs p) {
     if constexpr (more > 0) side(t + 1);
     read_half(stage, 16, h1);
     __builtin_amdgcn_sched_barrier(0);
-    multiply(h0, 0, 2);
+    multiply(h0, 0, NT * FN / 2);
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (more > 0) put(stage ^ 1);
     if constexpr (more > 2) load(std::true_type{}, 0);
     if constexpr (more == 2) load(std::false_type{}, rows - (t + 2) * WG_ROWS);
     __builtin_amdgcn_sched_barrier(0);
-    multiply(h0, 2, 4);
+    multiply(h0, NT * FN / 2, NT * FN);
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (more > 0) {
       __syncthreads();  // the next step's rows are there, and this step's have been read
       read_half(stage ^ 1, 0, h0);
     }
     __builtin_amdgcn_sched_barrier(0);
-    multiply(h1, 0, 4);
+    multiply(h1, 0, NT * FN);
     __builtin_amdgcn_sched_barrier(0);
   };
   if (steps > 0) {
@@ -1118,8 +1036,8 @@ __global__ __launch_bounds__(512, 2) void wgrad_large_kernel(WgArgs p) {
     if (t + 1 < steps) step(t++, std::integral_constant<int, 1>{});
     step(t, std::integral_constant<int, 0>{});
   }
-  write_wgrad<W, 4, 2>(p, acc, n0 + wn, k0 + wk, lane);
-  if (sums) write_gbias<W, BN, 16, 8>(p, lds, gsum, gr, gc, n0);
+  write_wgrad<W, FN, FK>(p, acc, n0 + wn, k0 + wk, lane);
+  if (sums) write_gbias<W, BN, GROWS, E>(p, lds, gsum, gr, gc, n0);
 }
 
 template <typename W>
@@ -1138,19 +1056,21 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(const float* __restrict
 }
 
 struct WgPlan {
-  int splits, nt, kt, tile;
+  int splits, nt, kt, bn, bk;
   int64_t per_split;
 };
-// Tiles of 256 x 256 for the 16-bit types where the result has several (fp16, 16384x4096x4096: 1.0 ms, in tiles of 128
-// 1.3); the batch is split until there is a workgroup
-// (of the small tile: two) for every compute unit, at least 256 rows to a split.
+// Tiles of 256 x 256 (bf16) or 128 x 256 (fp16 and fp32, whose two and three terms take the registers and LDS) where the
+// result is that large, of 128 x 128 else.  The batch is split until there is a workgroup (of the small tile: two) for
+// every compute unit, at least 256 rows to a split.
 WgPlan wg_plan(int64_t m, int64_t n, int64_t k, int dtype) {
   WgPlan p;
-  p.tile = dtype != VMF_F32 && n > 256 && k > 256 ? 256 : 128;
-  p.nt = (int)((n + p.tile - 1) / p.tile);
-  p.kt = (int)((k + p.tile - 1) / p.tile);
+  p.bk = k > 256 || (dtype != VMF_BF16 && k > 128) ? 256 : 128;
+  p.bn = dtype == VMF_BF16 && n > 256 ? 256 : 128;
+  if (dtype == VMF_BF16 && (p.bk != 256 || p.bn != 256)) p.bk = p.bn = 128;
+  p.nt = (int)((n + p.bn - 1) / p.bn);
+  p.kt = (int)((k + p.bk - 1) / p.bk);
   const int64_t tiles = (int64_t)p.nt * p.kt;
-  int64_t s = (p.tile == 256 ? 256 : 512) / tiles;
+  int64_t s = (p.bk == 256 ? 256 : 512) / tiles;
   if (s > m / 256) s = m / 256;
   if (s < 1) s = 1;
   p.per_split = ((m + s - 1) / s + WG_ROWS - 1) / WG_ROWS * WG_ROWS;
@@ -1158,22 +1078,22 @@ WgPlan wg_plan(int64_t m, int64_t n, int64_t k, int dtype) {
   return p;
 }
 
-template <typename T, typename W>
-void wgrad_launch(const WgPlan& pl, const WgArgs& p, hipStream_t st) {
+template <typename T, typename W, bool WHOLE>
+void wgrad_launch_tiles(const WgPlan& pl, const WgArgs& p, hipStream_t st) {
   const dim3 grid((unsigned)(pl.nt * pl.kt), (unsigned)pl.splits);
   if constexpr (std::is_same<T, bf16_t>::value) {
-    if (pl.tile == 256 && p.n % 8 == 0 && p.gy_stride % 8 == 0 && ((uintptr_t)p.gy & 15) == 0) {
-      wgrad_large_kernel<W><<<grid, 512, 0, st>>>(p);
-      return;
-    }
+    if (pl.bn == 256) wgrad_kernel<T, W, 256, 256, 128, 64, WHOLE><<<grid, 512, 0, st>>>(p);
+    else wgrad_kernel<T, W, 128, 128, 64, 64, WHOLE><<<grid, 256, 0, st>>>(p);
+  } else {
+    if (pl.bk == 256) wgrad_kernel<T, W, 128, 256, 64, 64, WHOLE><<<grid, 512, 0, st>>>(p);
+    else wgrad_kernel<T, W, 128, 128, 64, 64, WHOLE><<<grid, 256, 0, st>>>(p);
   }
-  if constexpr (sizeof(T) == 2) {
-    if (pl.tile == 256) {
-      wgrad_kernel<T, W, 256, 256, 128, 64><<<grid, 512, 0, st>>>(p);
-      return;
-    }
-  }
-  wgrad_kernel<T, W, 128, 128, 64, 64><<<grid, 256, 0, st>>>(p);
+}
+template <typename T, typename W>
+void wgrad_launch(const WgPlan& pl, const WgArgs& p, hipStream_t st) {
+  constexpr int E = 16 / (int)sizeof(T);
+  if (p.n % E == 0 && p.gy_stride % E == 0 && ((uintptr_t)p.gy & 15) == 0) wgrad_launch_tiles<T, W, true>(pl, p, st);
+  else wgrad_launch_tiles<T, W, false>(pl, p, st);
 }
 
 int check_operand(const char* what, const char* name, const uint8_t* values, const uint8_t* exps, int64_t exp_pitch,
