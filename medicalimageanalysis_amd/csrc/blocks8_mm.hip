@@ -109,11 +109,15 @@ __device__ __forceinline__ void finish1(const MmArgs& p, int64_t row, int64_t co
   ((OUT*)p.out)[row * p.n + col] = (OUT)v;
 }
 
-// Workgroup b runs on XCD b % 8: give each XCD a contiguous run of tiles, and walk the run in columns of 8 row tiles, so
-// that the rows and columns in use at a time fit its L2.
+// Workgroup b of `all` runs on XCD b % 8: the place of b where each XCD has a contiguous run
+__device__ __forceinline__ int xcd_run(int b, int all) {
+  const int q = all >> 3, r = all & 7, x = b & 7;
+  return x * q + (x < r ? x : r) + (b >> 3);
+}
+// Each XCD gets a contiguous run of tiles, and the run is walked in columns of 8 row tiles, so that the rows and columns
+// in use at a time fit its L2.
 __device__ __forceinline__ void tile_of(const MmArgs& p, int id, int& mt, int& nt) {
-  const int tiles = p.mt * p.nt, q = tiles >> 3, r = tiles & 7, x = id & 7;
-  id = x * q + (x < r ? x : r) + (id >> 3);
+  id = xcd_run(id, p.mt * p.nt);
   const int group = id / (8 * p.nt), first = group * 8, high = p.mt - first < 8 ? p.mt - first : 8;
   const int in_group = id - group * 8 * p.nt;
   mt = first + in_group % high;
@@ -689,7 +693,7 @@ struct WgArgs {
   int64_t q_pitch, q_exp_pitch;
   int64_t m, n, k;
   int64_t rows_per_split;
-  int nt, kt;
+  int nt, kt, splits;
 };
 
 // 32 columns of the 16 rows that start at `rows`, as the operand of a 32 x 32 x 16 product: lane l gets column l % 32 of
@@ -708,7 +712,7 @@ __device__ __forceinline__ v8b transposed(int lane, F&& at) {
 }
 // a wave's part of the result: D of a product has column (k) lane % 32, rows (n) (e & 3) + 8 (e >> 2) + 4 (lane / 32)
 template <typename W, int FN, int FK>
-__device__ __forceinline__ void write_wgrad(const WgArgs& p, const v16f (&acc)[FN][FK], int64_t n0, int64_t k0, int lane) {
+__device__ __forceinline__ void write_wgrad(const WgArgs& p, const v16f (&acc)[FN][FK], int split, int64_t n0, int64_t k0, int lane) {
 #pragma unroll
   for (int i = 0; i < FN; ++i)
 #pragma unroll
@@ -718,7 +722,7 @@ __device__ __forceinline__ void write_wgrad(const WgArgs& p, const v16f (&acc)[F
       for (int e = 0; e < 16; ++e) {
         const int64_t n = n0 + i * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
         if (n < p.n && k < p.k) {
-          if (p.partial) p.partial[((int64_t)blockIdx.y * p.n + n) * p.k + k] = acc[i][j][e];
+          if (p.partial) p.partial[((int64_t)split * p.n + n) * p.k + k] = acc[i][j][e];
           else ((W*)p.gw)[n * p.k + k] = (W)acc[i][j][e];
         }
       }
@@ -727,7 +731,7 @@ __device__ __forceinline__ void write_wgrad(const WgArgs& p, const v16f (&acc)[F
 // gbias: SHARE threads have sums of the same BN columns (thread: row `share`, E columns from `col`); added in order
 template <typename W, int BN, int SHARE, int E>
 __device__ __forceinline__ void write_gbias(const WgArgs& p, uint8_t* lds, const float (&sum)[E], int share, int col,
-                                            int64_t n0) {
+                                            int split, int64_t n0) {
   float* red = reinterpret_cast<float*>(lds);  // SHARE * BN floats
   __syncthreads();
 #pragma unroll
@@ -739,7 +743,7 @@ __device__ __forceinline__ void write_gbias(const WgArgs& p, uint8_t* lds, const
     for (int q = 0; q < SHARE; ++q) s += red[q * BN + threadIdx.x];
     const int64_t n = n0 + threadIdx.x;
     if (n < p.n) {
-      if (p.partial) p.partial[(int64_t)gridDim.y * p.n * p.k + (int64_t)blockIdx.y * p.n + n] = s;
+      if (p.partial) p.partial[(int64_t)p.splits * p.n * p.k + (int64_t)split * p.n + n] = s;
       else ((W*)p.gb)[n] = (W)s;
     }
   }
@@ -814,15 +818,12 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void wgrad_kernel(Wg
   static_assert(GROWS * BN * 4 <= 2 * STAGE, "gbias's sums fit the stages");
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // workgroup b runs on XCD b % 8: neighbouring tiles, which share gy's columns, on the same one
-  int id = (int)blockIdx.x;
-  {
-    const int tiles = p.nt * p.kt, q = tiles >> 3, r = tiles & 7, x = id & 7;
-    id = x * q + (x < r ? x : r) + (id >> 3);
-  }
-  const int nt = id / p.kt, kt = id % p.kt;
+  // workgroup b runs on XCD b % 8: the tiles of a split, which read the same rows, on the same one
+  const int tiles = p.nt * p.kt;
+  const int id = xcd_run((int)blockIdx.x, tiles * p.splits), split = id / tiles, tile = id - split * tiles;
+  const int nt = tile / p.kt, kt = tile - nt * p.kt;
   const int64_t n0 = (int64_t)nt * BN, k0 = (int64_t)kt * BK;
-  const int64_t m0 = (int64_t)blockIdx.y * p.rows_per_split;
+  const int64_t m0 = (int64_t)split * p.rows_per_split;
   const int rows = (int)(m0 + p.rows_per_split < p.m ? p.rows_per_split : p.m - m0);
   const int steps = (rows + WG_ROWS - 1) / WG_ROWS;
   const int wn = wave / WAVES_K * WN, wk = wave % WAVES_K * WK;
@@ -1036,8 +1037,8 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void wgrad_kernel(Wg
     if (t + 1 < steps) step(t++, std::integral_constant<int, 1>{});
     step(t, std::integral_constant<int, 0>{});
   }
-  write_wgrad<W, FN, FK>(p, acc, n0 + wn, k0 + wk, lane);
-  if (sums) write_gbias<W, BN, GROWS, E>(p, lds, gsum, gr, gc, n0);
+  write_wgrad<W, FN, FK>(p, acc, split, n0 + wn, k0 + wk, lane);
+  if (sums) write_gbias<W, BN, GROWS, E>(p, lds, gsum, gr, gc, split, n0);
 }
 
 template <typename W>
@@ -1060,8 +1061,8 @@ struct WgPlan {
   int64_t per_split;
 };
 // Tiles of 256 x 256 (bf16) or 128 x 256 (fp16 and fp32, whose two and three terms take the registers and LDS) where the
-// result is that large, of 128 x 128 else.  The batch is split until there is a workgroup (of the small tile: two) for
-// every compute unit, at least 256 rows to a split.
+// result is that large, of 128 x 128 else.  The batch is split until there is a workgroup for
+// every compute unit (two of the small tile for each measure the same), at least 256 rows to a split.
 WgPlan wg_plan(int64_t m, int64_t n, int64_t k, int dtype) {
   WgPlan p;
   p.bk = k > 256 || (dtype != VMF_BF16 && k > 128) ? 256 : 128;
@@ -1070,7 +1071,7 @@ WgPlan wg_plan(int64_t m, int64_t n, int64_t k, int dtype) {
   p.nt = (int)((n + p.bn - 1) / p.bn);
   p.kt = (int)((k + p.bk - 1) / p.bk);
   const int64_t tiles = (int64_t)p.nt * p.kt;
-  int64_t s = (p.bk == 256 ? 256 : 512) / tiles;
+  int64_t s = 256 / tiles;
   if (s > m / 256) s = m / 256;
   if (s < 1) s = 1;
   p.per_split = ((m + s - 1) / s + WG_ROWS - 1) / WG_ROWS * WG_ROWS;
@@ -1080,7 +1081,7 @@ WgPlan wg_plan(int64_t m, int64_t n, int64_t k, int dtype) {
 
 template <typename T, typename W, bool WHOLE>
 void wgrad_launch_tiles(const WgPlan& pl, const WgArgs& p, hipStream_t st) {
-  const dim3 grid((unsigned)(pl.nt * pl.kt), (unsigned)pl.splits);
+  const unsigned grid = (unsigned)(pl.nt * pl.kt * pl.splits);
   if constexpr (std::is_same<T, bf16_t>::value) {
     if (pl.bn == 256) wgrad_kernel<T, W, 256, 256, 128, 64, WHOLE><<<grid, 512, 0, st>>>(p);
     else wgrad_kernel<T, W, 128, 128, 64, 64, WHOLE><<<grid, 256, 0, st>>>(p);
@@ -1226,8 +1227,8 @@ extern "C" int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const 
   VMF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), VMF_ERR_BAD_ARG,
               "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)need);
   const WgPlan pl = wg_plan(m, n, k, dtype);
-  VMF_REQUIRE((int64_t)pl.nt * pl.kt <= 0x7fffffff, VMF_ERR_UNSUPPORTED, "%s: %lld x %lld results", what, (long long)n,
-              (long long)k);
+  VMF_REQUIRE((int64_t)pl.nt * pl.kt * pl.splits <= 0x7fffffff, VMF_ERR_UNSUPPORTED, "%s: %lld x %lld results", what,
+              (long long)n, (long long)k);
   WgArgs p;
   p.gy = gy;
   p.gy_stride = gy_stride;
@@ -1245,6 +1246,7 @@ extern "C" int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const 
   p.rows_per_split = pl.per_split;
   p.nt = pl.nt;
   p.kt = pl.kt;
+  p.splits = pl.splits;
   hipStream_t st = (hipStream_t)stream;
   LOWP_DISPATCH(dtype, "vmf_blocks8_weight_grad", T, {
     if (out_dtype == VMF_F32) wgrad_launch<T, float>(pl, p, st);
