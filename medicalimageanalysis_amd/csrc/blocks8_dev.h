@@ -19,13 +19,11 @@ __device__ __forceinline__ float b8_pow2(int e) { return __uint_as_float((uint32
 // the stored byte is the exponent field of 2^e
 __device__ __forceinline__ float b8_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-// top: a finite magnitude
+// top: a finite magnitude.  448 = 1.75 * 2^8: a mantissa above 0x600000 carries into the exponent field.
 __device__ __forceinline__ int b8_exponent(float top) {
   const uint32_t u = __float_as_uint(top);
-  if (u == 0) return 0;
-  // 448 = 1.75 * 2^8
-  const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return e < B8_EMIN ? B8_EMIN : e > B8_EMAX ? B8_EMAX : e;
+  const int e = (int)((u + 0x1fffffu) >> 23) - 127 - 8;
+  return u == 0 ? 0 : e < B8_EMIN ? B8_EMIN : e > B8_EMAX ? B8_EMAX : e;
 }
 // Two values already divided by the block's 2^e -> two bytes (low half), rounded to nearest even.  Nothing finite is
 // above 448 (1 + 2^-20) then, which the conversion rounds to 448; infinities and NaN become NaN.  (e = 119, the largest,
@@ -55,20 +53,28 @@ __device__ __forceinline__ void b8_unpack4(uint32_t w, float scale, float* out) 
 }
 // ---- softplus into blocks -----------------------------------------------------------------------------------------
 
-// In 32 bits, from the hardware's exponential and logarithm (1 unit in the last place each):
-//   log(1 + u), u = exp(-|t|): where 1 + u drops too much of u (u < 1/16), the series to u^6 (the rest is under u^6 / 7
-//   of it); else ln 2 * log2(1 + u), off by 2^-24 / u <= 2^-20.
+// In 32 bits: log(1 + u), u = exp(-|t|) from the hardware's exponential (1 unit in the last place), as u times a polynomial
+// of degree 7 in u: the best one on [0, 1] by relative error (an exchange fit), 2e-7, with its roundings 3.4e-7.
 // beta, t = beta h and t log2(e) are rounded, 3 * 2^-24 |t| in the exponential's argument, which counts in full for
 // negative t only (for positive t its share is |t| exp(-t) <= 0.37 of that).  Together the result is off by less than
 // softplus_margin relative to its value.
 __device__ __forceinline__ float softplus32(float h, float beta, float inv_beta) {
   const float t = beta * h;
   const float u = __builtin_amdgcn_exp2f(-fabsf(t) * 1.44269504f);
-  const float few = u * (1.0f + u * (-0.5f + u * (1.0f / 3 + u * (-0.25f + u * (0.2f + u * (-1.0f / 6))))));
-  const float l = u < 0.0625f ? few : 0.69314718f * __builtin_amdgcn_logf(1.0f + u);
-  return (fmaxf(t, 0.0f) + l) * inv_beta;
+  float s = -0.00853920821f;
+  s = fmaf(s, u, 0.044089634f);
+  s = fmaf(s, u, -0.107681714f);
+  s = fmaf(s, u, 0.177452415f);
+  s = fmaf(s, u, -0.244954631f);
+  s = fmaf(s, u, 0.332754791f);
+  s = fmaf(s, u, -0.499974042f);
+  s = fmaf(s, u, 0.999999821f);
+  return fmaf(u, s, __builtin_amdgcn_fmed3f(t, 0.0f, __builtin_inff())) * inv_beta;  // (a NaN is in u)
 }
-__device__ __forceinline__ float softplus_margin(float h, float beta) { return 3e-6f + 3e-7f * fmaxf(-beta * h, 0.0f); }
+// (at most 0.48, also for -inf, the fill of short rows)
+__device__ __forceinline__ float softplus_margin(float h, float beta) {
+  return fmaf(__builtin_amdgcn_fmed3f(-beta * h, 0.0f, 1.6e6f), 3e-7f, 2e-6f);
+}
 
 // exp in 64 bits: t = n ln 2 + r, |r| <= 0.35, and the power series of exp(r) to r^13 (the next term is under 5e-18)
 __device__ __forceinline__ double exp64(double t) {
@@ -153,17 +159,24 @@ static __device__ __noinline__ float softplus_scaled(float x, double beta, int e
 // million): the bytes are those of the exactly computed softplus.
 __device__ __forceinline__ uint2 softplus8(const float (&h)[8], float beta, float inv_beta, double beta64, int& e_out) {
   constexpr float INF = __builtin_inff();
-  float top = -INF;  // softplus grows with h: the block's largest comes from the largest h
+  // softplus grows with h: the block's largest comes from the largest h.  As integers the bits of floats order like them
+  // from zero up; if none is there, the largest is the negative one with the smallest bits.
+  int most = INT32_MIN;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = h[i] < INF ? fmaxf(top, h[i]) : top;
-  top = lane_max<16>(top);
-  const float at = softplus32(top, beta, inv_beta), mt = softplus_margin(top, beta);
-  int e = B8_EMAX;
-  if (at < INF) {
-    e = b8_exponent(at * (1.0f - mt));
-    const int above = b8_exponent(fminf(at * (1.0f + mt), 3.4e38f));
-    if (e != above && softplus64((double)top, beta64) > 448.0 * ::ldexp(1.0, e)) e = above;
+  for (int i = 0; i < 8; ++i) most = larger(most, __float_as_int(h[i]));
+  most = lane_max<16>(most);
+  float top = __int_as_float(most);
+  if (most < 0 || most >= (int)B8_INF) {
+    top = -INF;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = h[i] < INF && h[i] > top ? h[i] : top;  // (neither infinity nor NaN)
+    top = lane_max<16>(top);
   }
+  const float at = softplus32(top, beta, inv_beta), mt = softplus_margin(top, beta);
+  const float most32 = 3.4e38f;
+  int e = b8_exponent(at < most32 ? at * (1.0f - mt) : most32);
+  const int above = b8_exponent(at < most32 ? at * (1.0f + mt) : most32);
+  if (e != above && softplus64((double)top, beta64) > 448.0 * ::ldexp(1.0, e)) e = above;
   if (top == -INF) e = 0;
   e_out = e;
   const float scale = inv_beta * b8_pow2(-e);
@@ -171,7 +184,7 @@ __device__ __forceinline__ uint2 softplus8(const float (&h)[8], float beta, floa
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float a = softplus32(h[i], beta, scale);
-    const float m = fminf(softplus_margin(h[i], beta), 0.5f);  // (-inf, the fill of short rows, has none)
+    const float m = softplus_margin(h[i], beta);
     lo[i] = fmaf(a, -m, a);
     hi[i] = fmaf(a, m, a);
   }
