@@ -16,7 +16,8 @@ operand of the next layer's product and as the checkpoint that the backward pass
 linear's gradients: gx = (blocks(gy) tiles(weight)) * softplus slope, gw = gy^T blocks(activation(x)), gb = the sum of
 gy's rows; the roundings to 8 bits pass their gradient on as it is.  float32 results come from 32-bit sums, float16 and
 bfloat16 ones from the faster 8-bit matrix instruction (1.3e-5 relative, a hundredth of their own rounding).  NaN and
-infinities are NaN in blocks.  There is no CPU path.
+infinities are NaN in blocks.  Only linear takes part in autograd: the other functions' results carry no gradient.  There
+is no CPU path.
 """
 import ctypes as C
 

@@ -14,14 +14,21 @@ from .. import blocks8
 from ..norm import LayerNorm
 
 
+def _option(config, key, default):
+    try:
+        return config[key]
+    except KeyError:
+        return default
+
+
 def prepare(model):
     """reads the two keys of model.config and adds the norms; called at the end of a model's constructor"""
     config = model.config
-    hidden = config.get("hidden")
+    hidden = _option(config, "hidden", None)
     if hidden not in (None, "blocks8"):
         raise ValueError(f"config['hidden'] must be absent, None or 'blocks8', got {hidden!r}")
     model._hidden_kind = hidden
-    if config.get("layer_norm", False):
+    if _option(config, "layer_norm", False):
         for side in ("encoder", "decoder"):
             setattr(model, side + "_norms", nn.ModuleList(
                 [LayerNorm(config[side + "_width"], device=model.device) for _ in range(config[side + "_depth"] + 1)]))

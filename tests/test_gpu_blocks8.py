@@ -215,6 +215,19 @@ def test_matmul_of_two_sets_of_rows(m, n, k, dtype):
     near(blocks8.matmul(a, b, dtype=dtype), ad @ bd.t(), ad.abs() @ bd.abs().t(), k)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n", [(3, 20), (70, 90), (4096, 4096)])
+def test_matmul_of_very_small_and_very_large_blocks(m, n, dtype):
+    """exponents at both ends of their range: 2^-110 times 2^100, and rows of zeros"""
+    k = 256
+    x, w = normal(m, k, seed=1) * 2.0 ** -112, normal(n, k, seed=2) * 2.0 ** 95
+    x[1], w[2] = 0.0, 0.0
+    x[0] *= 2.0 ** -12  # below what a block can hold: mostly zeros
+    a, b = blocks8.quantize(x), blocks8.quantize_weight(w).rows
+    ad, bd = a.dequantize().double(), b.dequantize().double()
+    near(blocks8.matmul(a, b, dtype=dtype), ad @ bd.t(), ad.abs() @ bd.abs().t(), k)
+
+
 def test_matmul_with_the_weight_on_the_left():
     w = blocks8.quantize_weight(normal(200, 260, seed=1)).rows
     b = blocks8.quantize(normal(90, 260, seed=2))
@@ -351,6 +364,31 @@ def test_linear_leading_dimensions_and_which_gradients_are_asked_for():
     summed = [t.clone().requires_grad_() for t in (x, w, b)]
     blocks8.linear(*summed).sum().backward()  # the gradient of a sum is one element, expanded
     assert summed[2].grad.eq(15).all()
+
+
+def test_linear_is_differentiable_once():
+    leaves = [t.requires_grad_() for t in (normal(9, 40, seed=1), normal(30, 40, seed=2), normal(30, seed=3))]
+    gy = normal(9, 30, seed=4)
+    plain = torch.autograd.grad(blocks8.linear(*leaves, "softplus"), leaves, gy)
+    graph = torch.autograd.grad(blocks8.linear(*leaves, "softplus"), leaves, gy, create_graph=True)
+    for p, q in zip(plain, graph):
+        assert torch.equal(p, q)
+    with pytest.raises(RuntimeError, match="once_differentiable|twice|does not require grad"):
+        torch.autograd.grad(graph[0].sum(), leaves)
+
+
+@pytest.mark.parametrize("stride,offset", [(140, 0), (144, 8), (139, 3)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_with_strides_and_offsets(dtype, stride, offset):
+    """gy's rows at aligned and unaligned addresses: the same results"""
+    x, w = normal(333, 300, seed=1).to(dtype).requires_grad_(), normal(130, 300, seed=2).to(dtype).requires_grad_()
+    gy = normal(333, 130, seed=3).to(dtype)
+    want = torch.autograd.grad(blocks8.linear(x, w, None, "softplus"), (x, w), gy)
+    wide = torch.full((333, stride + 8), math.nan, device=DEV, dtype=dtype)
+    wide[:, offset:offset + 130] = gy
+    got = torch.autograd.grad(blocks8.linear(x, w, None, "softplus"), (x, w), wide[:, offset:offset + 130])
+    for p, q in zip(got, want):
+        assert torch.equal(p, q)
 
 
 def test_linear_of_no_rows():

@@ -120,12 +120,35 @@ def test_strides_views_and_leading_dimensions():
     assert (wide[:, :3] == 7).all() and (wide[:, 103:] == 7).all()
 
 
-def test_no_rows():
-    x = torch.empty(0, 12, device=DEV, requires_grad=True)
-    w, b = torch.ones(12, device=DEV, requires_grad=True), torch.zeros(12, device=DEV, requires_grad=True)
+@pytest.mark.parametrize("width", [12, 9000, 40000])
+def test_no_rows(width):
+    x = torch.empty(0, width, device=DEV, requires_grad=True)
+    w, b = torch.ones(width, device=DEV, requires_grad=True), torch.zeros(width, device=DEV, requires_grad=True)
     y = norm.layer_norm(x, w, b)
-    gx, gw, gb = torch.autograd.grad(y, (x, w, b), torch.empty(0, 12, device=DEV))
-    assert y.shape == gx.shape == (0, 12) and not gw.any() and not gb.any()
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), torch.empty(0, width, device=DEV))
+    assert y.shape == gx.shape == (0, width) and not gw.any() and not gb.any()
+
+
+@pytest.mark.parametrize("n,width", [(5, 40), (2000, 300), (700, 5000), (6, 40000)])
+def test_each_gradient_alone(n, width):
+    x, w, b, gy = data(n, width, torch.float32, seed=n)
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    full = torch.autograd.grad(norm.layer_norm(*leaves), leaves, gy)
+    for i in range(3):
+        some = [t.detach().requires_grad_(j == i) for j, t in enumerate((x, w, b))]
+        got, = torch.autograd.grad(norm.layer_norm(*some), some[i], gy)
+        assert torch.equal(got, full[i])
+
+
+def test_differentiable_once():
+    x, w, b, gy = data(4, 30, torch.float32)
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    plain = torch.autograd.grad(norm.layer_norm(*leaves), leaves, gy)
+    graph = torch.autograd.grad(norm.layer_norm(*leaves), leaves, gy, create_graph=True)
+    for p, q in zip(plain, graph):
+        assert torch.equal(p, q)
+    with pytest.raises(RuntimeError, match="once_differentiable|twice|does not require grad"):
+        torch.autograd.grad(graph[0].sum(), leaves)
 
 
 def test_constant_rows_and_large_means():
