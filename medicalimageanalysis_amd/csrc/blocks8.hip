@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256) void from_blocks_kernel(const T* __restrict__ 
       float gv[8];
       load_some<8>(g + row * g_stride + col, width - col, 0.0f, gv);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] = gv[i] * b8_softplus_slope(a[i], beta);
+      for (int i = 0; i < 8; ++i) a[i] = gv[i] * b8_softplus_slope<sizeof(T) == 2>(a[i], beta);
     }
     store_some<8>(out + row * width + col, width - col, a);
   }

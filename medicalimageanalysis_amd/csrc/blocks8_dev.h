@@ -203,19 +203,24 @@ __device__ __forceinline__ uint2 softplus8(const float (&h)[8], float beta, floa
   return uint2{w[0], w[1]};
 }
 
-// d softplus / dh from the kept a = softplus(h): sigmoid(beta h) = 1 - exp(-z), z = beta a.  For z under 1/2 the series
-// to z^8 (the rest is under 2e-8 of it), else from the hardware's exponential, whose unit in the last place is 2^-24 of
-// at most 0.6 against a result of at least 0.39.
+// d softplus / dh from the kept a = softplus(h): sigmoid(beta h) = 1 - exp(-z), z = beta a.  For small z a series, else
+// from the hardware's exponential (a unit in the last place is 2^-24).  For 32-bit results the series runs to z^8 under
+// 1/2 (the rest is under 2e-8 of it) and the difference is at least 0.39; SHORT, for results of 11 bits and fewer: to z^4
+// under 1/16 (2e-7), the difference at least 0.06 (1e-6 off at most).
+template <bool SHORT>
 __device__ __forceinline__ float b8_softplus_slope(float a, float beta) {
   const float z = beta * a;
-  float s = fmaf(z, -1.0f / 40320, 1.0f / 5040);
-  s = fmaf(z, -s, 1.0f / 720);
-  s = fmaf(z, -s, 1.0f / 120);
-  s = fmaf(z, -s, 1.0f / 24);
+  float s = 1.0f / 24;
+  if constexpr (!SHORT) {
+    s = fmaf(z, -1.0f / 40320, 1.0f / 5040);
+    s = fmaf(z, -s, 1.0f / 720);
+    s = fmaf(z, -s, 1.0f / 120);
+    s = fmaf(z, -s, 1.0f / 24);
+  }
   s = fmaf(z, -s, 1.0f / 6);
   s = fmaf(z, -s, 0.5f);
   s = fmaf(z, -s, 1.0f);
-  return z < 0.5f ? z * s : 1.0f - __builtin_amdgcn_exp2f(z * -1.44269504f);
+  return z < (SHORT ? 0.0625f : 0.5f) ? z * s : 1.0f - __builtin_amdgcn_exp2f(z * -1.44269504f);
 }
 
 // f(integral_constant<int, 0>), ..., f(integral_constant<int, N - 1>)

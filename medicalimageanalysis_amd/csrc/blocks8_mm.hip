@@ -104,7 +104,7 @@ __device__ __forceinline__ void finish1(const MmArgs& p, int64_t row, int64_t co
   if (p.gate.values) {
     float a[4];
     b8_unpack4(p.gate.values[row * p.gate.pitch + col], b8_scale(p.gate.exps[(col >> 7) * p.gate.exp_pitch + row]), a);
-    v *= b8_softplus_slope(a[0], p.beta);
+    v *= b8_softplus_slope<sizeof(OUT) == 2>(a[0], p.beta);
   }
   ((OUT*)p.out)[row * p.n + col] = (OUT)v;
 }
@@ -188,7 +188,7 @@ __device__ __forceinline__ void write_tile(const MmArgs& p, const v4f (&acc)[GM 
               float a[4];
               b8_unpack4(code[t], b8_scale(ex[t / 4] >> (8 * (t % 4)) & 0xff), a);
 #pragma unroll
-              for (int j = 0; j < FN; ++j) v[j] *= b8_softplus_slope(a[j], p.beta);
+              for (int j = 0; j < FN; ++j) v[j] *= b8_softplus_slope<sizeof(OUT) == 2>(a[j], p.beta);
             }
             store_some<FN>(out, left, v);
           }
@@ -1041,18 +1041,29 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void wgrad_kernel(Wg
   if (sums) write_gbias<W, BN, GROWS, E>(p, lds, gsum, gr, gc, split, n0);
 }
 
+// the splits' sums in their order: four elements of gweight to a thread, then gbias's
 template <typename W>
 __global__ __launch_bounds__(256) void wgrad_join_kernel(const float* __restrict__ partial, W* __restrict__ gw,
                                                          W* __restrict__ gb, int splits, int64_t nk, int64_t n) {
-  const int64_t total = nk + (gb ? n : 0);
+  const int64_t quads = (nk + 3) / 4, total = quads + (gb ? n : 0);
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const float* src = i < nk ? partial + i : partial + splits * nk + (i - nk);
-    const int64_t step = i < nk ? nk : n;
-    float s = 0;
+    float s[4] = {0, 0, 0, 0};
+    if (i < quads) {
+      const int64_t left = nk - 4 * i;
+#pragma unroll 4
+      for (int q = 0; q < splits; ++q) {
+        float v[4];
+        load_some<4>(partial + q * nk + 4 * i, left, 0.0f, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] += v[j];
+      }
+      store_some<4>(gw + 4 * i, left, s);
+    } else {
+      const float* src = partial + splits * nk + (i - quads);
 #pragma unroll 8
-    for (int q = 0; q < splits; ++q) s += src[q * step];
-    if (i < nk) gw[i] = (W)s;
-    else gb[i - nk] = (W)s;
+      for (int q = 0; q < splits; ++q) s[0] += src[q * n];
+      gb[i - quads] = (W)s[0];
+    }
   }
 }
 
@@ -1255,7 +1266,7 @@ extern "C" int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const 
   rc = vmf_check_launch(what);
   if (rc != VMF_OK || !need) return rc;
   LOWP_DISPATCH(out_dtype, "vmf_blocks8_weight_grad", W,
-                (wgrad_join_kernel<W><<<vmf_grid_for(n * (k + 1), 256, 1 << 13), 256, 0, st>>>(
+                (wgrad_join_kernel<W><<<vmf_grid_for((n * k + 3) / 4 + n, 256, 1 << 13), 256, 0, st>>>(
                     p.partial, (W*)gweight, (W*)gbias, pl.splits, n * k, n)));
   return vmf_check_launch(what);
 }

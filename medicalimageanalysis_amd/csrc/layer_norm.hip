@@ -347,6 +347,7 @@ __global__ __launch_bounds__(256) void ln_reduce_kernel(const A* __restrict__ pa
   const int64_t col = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);  // 0 .. 2 width
   A s = 0;
   if (col < 2 * width)
+#pragma unroll 8
     for (int p = threadIdx.x >> 4; p < parts; p += 16) s += partial[(int64_t)p * 2 * width + col];
   red[threadIdx.x] = s;
   __syncthreads();
