@@ -383,7 +383,11 @@ void run_fwd(const void* x, int64_t xs, const void* w, const void* b, void* y, v
              int64_t width, double eps, hipStream_t st) {
   using A = typename AccOf<T>::type;
   constexpr int V = LnVec<T>::value;
-  constexpr int MAXC = 32 / V;  // 32 values per lane (64 in one wave instead of 16 in four: 65536x4096 bf16 0.36 ms against 0.26)
+  // The fewest lanes that hold the row in 32 values each, and for them the shortest of these rows: 65536x128 bf16 with 16
+  // lanes 8.1 us, with 32 13.5, with 64 22.6; 65536x784 bf16 in two vectors to a lane 45 us, in four 75; 16384x4096 bf16 in
+  // 256 lanes 47 us, in four vectors to a lane 83, in 1024 lanes 398.  (64 values in one wave instead of 16 in four:
+  // 65536x4096 bf16 0.36 ms against 0.26.)
+  constexpr int MAXC = 32 / V;
   const int64_t vectors = (width + V - 1) / V;
 #define LN_FWD(TPR, NCH) \
   if (vectors <= (int64_t)(TPR) * (NCH)) return launch_fwd<T, W, TPR, NCH>(x, xs, w, b, y, mean, rstd, n, width, eps, st)
@@ -409,10 +413,12 @@ struct BwdPlan {
   int threads;  // of a workgroup
   int parts;    // workgroups, each leaving a partial row of gw and gb; 0: none are left (few rows)
 };
-// Few rows (up to 512, rows of up to 256 lanes): one launch.  Otherwise two workgroups for each of 256 compute units (four
-// where a row is four waves, whose barriers others then fill: 65536x4096 bf16 0.57 -> 0.36 ms; 1048576x784 fp32, a wave
-// to a row, 1.95 with two, 2.05 with four), but no more than have 32 rows each, since each leaves 2 * width values that are
-// written and read again.
+// Few rows (up to 512, rows of up to 256 lanes): one launch (512x784 fp32 4.1 us, with partials 7.5; 2048x784 17.2 and 10.0).
+// Otherwise two workgroups for each of 256 compute units (1048576x784 fp32, a wave to a row, 1.88 ms, with four 2.00), four
+// where the other waves have more to fill: rows of 16 bits, whose loads are half as many (1048576x784 bf16 1.14 ms, with two
+// 1.88), and rows of four waves, which wait at barriers (65536x4096 bf16 0.33 ms, with two 0.50).  No more than have 32
+// rows each, since each leaves 2 * width values that are written and read again; 16 where a wave or more works on one row
+// (16384x4096 bf16 98 us, with 32 136; 8192x128 bf16, 16 lanes to a row, 8.2 us, with 32 7.8).
 template <typename T>
 BwdPlan bwd_plan(int64_t n, int64_t width) {
   constexpr int V = LnVec<T>::value;
@@ -423,10 +429,10 @@ BwdPlan bwd_plan(int64_t n, int64_t width) {
     p.parts = 0;
     return p;
   }
-  const int64_t most = p.tpr == THREADS ? 1024 : 512;
-  // rows to a workgroup: 32, or as many as it has side by side, or fewer where that leaves compute units without one
+  const int64_t most = sizeof(T) == 2 || p.tpr == THREADS ? 1024 : 512;
+  // rows to a workgroup: those, or as many as it has side by side, or fewer where that leaves compute units without one
   const int64_t at_once = p.tpr == 0 ? 1 : p.threads / p.tpr;
-  const int64_t rows = at_once > 32 ? at_once : 32;
+  const int64_t few = p.tpr == 0 || p.tpr >= 64 ? 16 : 32, rows = at_once > few ? at_once : few;
   int64_t g = (n + rows - 1) / rows;
   if (g < 256) g = (n + at_once - 1) / at_once < 256 ? (n + at_once - 1) / at_once : 256;
   p.parts = (int)(g < 1 ? 1 : g > most ? most : g);
