@@ -610,8 +610,14 @@ struct MmPlan {
   MmKind kind;
   int splits, per_split, mt, nt;
 };
-// The largest tile (`large`: 256 x 256 among them) that still gives every compute unit (256) a workgroup; where even the smallest does not, the block
-// columns are split, at least four of them to a split.
+// Up to 16 rows: mm_few_kernel (1 x 4096 x 4096 bf16 4.7 us, in 64 x 64 tiles 8.2; 16 x 4096 x 4096 6.0 and 9.2).
+// Else the largest tile that still gives the 256 compute units enough workgroups:
+//   256 x 256 (`large`: a 16-bit result of rows and tiles) from 256 of them on: 4096 x 4096 x 1024 21.9 us, 128 x 128 29.4,
+//     64 x 64 36.7; at 128 of them (4096 x 2048 x 2048) 43.0 us against 25.5;
+//   128 x 128 from 384 on: at 400 (2560 x 2560 x 2048) 24.4 us, 64 x 64 27.8; at 256 (2048^3) 19.2 and 16.9.
+// Where even the smallest tile leaves compute units without one the block columns are split, at least 8 to a split
+// (128 x 128 x 16384 12.3 us, 4 to a split 15.8, unsplit 42); up to 16 rows at least 16 (1 x 128 x 16384 6.8 us,
+// unsplit 10.8), and none up to 32 block columns (1 x 128 x 4096 4.1 us, split in two 5.0).
 MmPlan mm_plan(int64_t m, int64_t n, int64_t blocks, bool large) {
   MmPlan p;
   auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
@@ -622,13 +628,13 @@ MmPlan mm_plan(int64_t m, int64_t n, int64_t blocks, bool large) {
     p.nt = (int)((n + 15) / 16);
     groups = p.nt;
   } else {
-    const int t = large && tiles(256) >= 256 ? 256 : tiles(128) >= 256 ? 128 : 64;
+    const int t = large && tiles(256) >= 256 ? 256 : tiles(128) >= 384 ? 128 : 64;
     p.kind = t == 256 ? MM_256 : t == 128 ? MM_128 : MM_64;
     p.mt = (int)((m + t - 1) / t);
     p.nt = (int)((n + t - 1) / t);
     groups = (int64_t)p.mt * p.nt;
   }
-  const int64_t least = p.kind == MM_FEW ? 16 : 4;
+  const int64_t least = p.kind != MM_FEW ? 8 : blocks > 32 ? 16 : blocks;
   int64_t s = (256 + groups - 1) / groups;
   if (s > blocks / least) s = blocks / least;
   if (s < 1) s = 1;
@@ -1007,21 +1013,32 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void wgrad_kernel(Wg
     const int stage = t & 1;
     if constexpr (more > 0) side(t + 1);
     read_half(stage, 16, h1);
-    __builtin_amdgcn_sched_barrier(0);
     multiply(h0, 0, NT * FN / 2);
-    __builtin_amdgcn_sched_barrier(0);
     if constexpr (more > 0) put(stage ^ 1);
     if constexpr (more > 2) load(std::true_type{}, 0);
     if constexpr (more == 2) load(std::false_type{}, rows - (t + 2) * WG_ROWS);
-    __builtin_amdgcn_sched_barrier(0);
     multiply(h0, NT * FN / 2, NT * FN);
+    // between two products: operand reads, the vector work of the next rows, their writes, the loads of those after
+#pragma unroll
+    for (int q = 0; q < NT * FN * FK; ++q) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix instruction
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
+      __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // vector instructions
+      __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);  // LDS write
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // load
+    }
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (more > 0) {
       __syncthreads();  // the next step's rows are there, and this step's have been read
       read_half(stage ^ 1, 0, h0);
     }
-    __builtin_amdgcn_sched_barrier(0);
     multiply(h1, 0, NT * FN);
+#pragma unroll
+    for (int q = 0; q < NT * FN * FK; ++q) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+      __builtin_amdgcn_sched_group_barrier(0x002, 4, 1);
+    }
     __builtin_amdgcn_sched_barrier(0);
   };
   if (steps > 0) {
@@ -1071,19 +1088,27 @@ struct WgPlan {
   int splits, nt, kt, bn, bk;
   int64_t per_split;
 };
-// Tiles of 256 x 256 (bf16) or 128 x 256 (fp16 and fp32, whose two and three terms take the registers and LDS) where the
-// result is that large, of 128 x 128 else.  The batch is split until there is a workgroup for
-// every compute unit (two of the small tile for each measure the same), at least 256 rows to a split.
+// The large tile is 256 x 256 for bf16, 128 x 256 for fp16 and fp32, whose two and three terms take the registers and LDS.
+// It reads less for a product but fills a compute unit by itself, where two workgroups of the 128 x 128 tile hide each
+// other's start, barriers and end: it is taken from 2^34 products on (bf16: 65536x512x512 60.6 us, small 61.2;
+// 16384x512x512 40.5 and 29.7; 4096^3 128 and 176), for the others from 2^31 on (fp32: 16384x512x512 39.0 and 43.7,
+// 16384x128x784 35.4 and 33.8).
+// The batch is split until every compute unit has a workgroup, at least 256 rows to a split (fp32 16384x1024x1024 95.6 us,
+// unsplit 515; bf16 4096x256x256 15.4 us, with 128 rows 19.1), in up to 16 splits 128 rows (fp32 1000x257x257 16.1 us, with
+// 256 22.5); the small tile until there are two for each, at least 512 rows to a split (bf16 4096x1024x1024 28.5 us, with
+// one 32.0; 2048x1024x1024, where that is 256 rows, 26.3 and 23.4).
 WgPlan wg_plan(int64_t m, int64_t n, int64_t k, int dtype) {
   WgPlan p;
-  p.bk = k > 256 || (dtype != VMF_BF16 && k > 128) ? 256 : 128;
-  p.bn = dtype == VMF_BF16 && n > 256 ? 256 : 128;
-  if (dtype == VMF_BF16 && (p.bk != 256 || p.bn != 256)) p.bk = p.bn = 128;
+  const bool bf16 = dtype == VMF_BF16;
+  const bool large = (double)m * n * k >= (bf16 ? 0x1p34 : 0x1p31) && k > 128 && (!bf16 || n > 128);
+  p.bk = large ? 256 : 128;
+  p.bn = large && bf16 ? 256 : 128;
   p.nt = (int)((n + p.bn - 1) / p.bn);
   p.kt = (int)((k + p.bk - 1) / p.bk);
   const int64_t tiles = (int64_t)p.nt * p.kt;
-  int64_t s = 256 / tiles;
-  if (s > m / 256) s = m / 256;
+  auto least = [](int64_t a, int64_t b) { return a < b ? a : b; };
+  int64_t s = least(256 / tiles, m / 256 > 16 ? m / 256 : least(m / 128, 16));
+  if (!large && least(512 / tiles, m / 512) > s) s = least(512 / tiles, m / 512);
   if (s < 1) s = 1;
   p.per_split = ((m + s - 1) / s + WG_ROWS - 1) / WG_ROWS * WG_ROWS;
   p.splits = p.per_split > 0 ? (int)((m + p.per_split - 1) / p.per_split) : 1;
@@ -1280,12 +1305,14 @@ int64_t row_block_bytes(int64_t rows, int64_t width) { return b8_blocks(width) *
 int64_t tile_bytes(int64_t rows, int64_t width) { return up16(b8_blocks(width) * (rows * B8 + b8_blocks(rows))); }
 }  // namespace
 
-// Whether x's rows are few enough for linear_few_kernel: at most 64 blocks for a workgroup to quantise (two per 16 lanes,
-// about a microsecond, as long as the weight's bytes take to come).
+// Whether linear_few_kernel pays: at most 64 blocks for a workgroup to quantise (two per 16 lanes, about a microsecond, as
+// long as the weight's bytes take to come) and at most two workgroups for a compute unit, since every one does it again.
+// bf16, softplus, the launches one after the other: 1 x 4096 x 4096 6.5 us, in two launches 7.8; 4 x 1024 x 1024 5.2 and 6.2;
+// 1 x 8192 x 4096 11.1 and 10.2 (where a call alone still gains the launch, 3 us); 1 x 16384 x 4096 26.8 and 21.0.
 static bool few_fits(int64_t m, int64_t n, int64_t k) {
   if (m < 1 || m > 16) return false;
   const MmPlan pl = mm_plan(m, n, b8_blocks(k), false);
-  return m * pl.per_split <= FEW_MAX_BLOCKS;
+  return m * pl.per_split <= FEW_MAX_BLOCKS && (int64_t)pl.nt * pl.splits <= 512;
 }
 
 extern "C" int vmf_blocks8_linear_fwd_workspace(int64_t m, int64_t n, int64_t k, int laid_out, int kept, int dtype,
