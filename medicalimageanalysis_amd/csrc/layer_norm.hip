@@ -35,6 +35,11 @@ __device__ __forceinline__ A row_sum(A v, A* red, int& flip) {
   }
 }
 
+// Whether a workgroup keeps weight and bias in registers and has its next row's loads under way while it works on one.  For
+// 16-bit rows, whose loads are half as many (1048576x784 bf16 0.95 -> 0.69 ms, 65536x8192 0.60 -> 0.54); fp32 rows keep the
+// memory busy without (1048576x784 1.22 ms, with it 1.35), and 1024 lanes to a row have no registers left for it.
+template <typename T, int TPR> constexpr bool ahead() { return sizeof(T) == 2 && TPR <= THREADS; }
+
 template <typename T, typename W, int TPR, int NCH>
 __global__ __launch_bounds__(TPR > THREADS ? TPR : THREADS) void ln_fwd_kernel(
     const T* __restrict__ x, int64_t x_stride, const W* __restrict__ w, const W* __restrict__ b, T* __restrict__ y,
@@ -44,21 +49,53 @@ __global__ __launch_bounds__(TPR > THREADS ? TPR : THREADS) void ln_fwd_kernel(
   constexpr int V = LnVec<T>::value;
   constexpr int NT = TPR > THREADS ? TPR : THREADS;
   constexpr int ROWS = NT / TPR;
+  constexpr bool AHEAD = ahead<T, TPR>();
+  constexpr int KEPT = AHEAD ? NCH : 1;
   __shared__ A red[2 * (TPR > 64 ? TPR / 64 : 1)];
   int flip = 0;
   const int lane = threadIdx.x % TPR;
   const A inv = (A)1 / (A)width;
-  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR; row < n; row += (int64_t)gridDim.x * ROWS) {
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  A v[NCH][V], next[KEPT][V], wv[KEPT][V], bv[KEPT][V];
+  auto load_row = [&](int64_t row, auto& to) {
     const T* xr = x + row * x_stride;
-    A v[NCH][V];
-    A s = 0;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       const int col = (c * TPR + lane) * V;
-      load_some<V>(xr + col, (int64_t)width - col, (A)0, v[c]);
+      load_some<V>(xr + col, (int64_t)width - col, (A)0, to[c]);
+    }
+  };
+  auto load_affine = [&](int c, int to) {
+    const int col = (c * TPR + lane) * V;
+    if (w) load_some<V>(w + col, (int64_t)width - col, (A)0, wv[to]);
+    if (b) load_some<V>(b + col, (int64_t)width - col, (A)0, bv[to]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (!w) wv[to][i] = (A)1;
+      if (!b) bv[to][i] = (A)0;
+    }
+  };
+  int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+  if constexpr (AHEAD) {
+    if (row < n) load_row(row, next);
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) load_affine(c, c);
+  }
+  for (; row < n; row += step) {
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int c = 0; c < NCH; ++c)
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[c][i] = next[c][i];
+      if (row + step < n) load_row(row + step, next);
+    } else {
+      load_row(row, v);
+    }
+    A s = 0;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c)
 #pragma unroll
       for (int i = 0; i < V; ++i) s += v[c][i];
-    }
     const A mean = row_sum<TPR>(s, red, flip) * inv;
     s = 0;
 #pragma unroll
@@ -78,12 +115,10 @@ __global__ __launch_bounds__(TPR > THREADS ? TPR : THREADS) void ln_fwd_kernel(
     T* yr = y + row * (int64_t)width;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      const int col = (c * TPR + lane) * V;
-      A wv[V], bv[V];
-      if (w) load_some<V>(w + col, (int64_t)width - col, (A)0, wv);
-      if (b) load_some<V>(b + col, (int64_t)width - col, (A)0, bv);
+      const int col = (c * TPR + lane) * V, at = AHEAD ? c : 0;
+      if constexpr (!AHEAD) load_affine(c, 0);
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[c][i] = v[c][i] * rstd * (w ? wv[i] : (A)1) + (b ? bv[i] : (A)0);
+      for (int i = 0; i < V; ++i) v[c][i] = v[c][i] * rstd * wv[at][i] + bv[at][i];
       store_some<V>(yr + col, (int64_t)width - col, v[c]);
     }
   }
@@ -374,7 +409,8 @@ void launch_fwd(const void* x, int64_t xs, const void* w, const void* b, void* y
                 int64_t width, double eps, hipStream_t st) {
   using A = typename AccOf<T>::type;
   constexpr int NT = TPR > THREADS ? TPR : THREADS;
-  const int grid = vmf_grid_for(n, NT / TPR, 1 << 16);
+  // (four workgroups to a compute unit where a workgroup gains from going on: 65536x4096 bf16 0.20 ms, with 65536 0.26)
+  const int grid = vmf_grid_for(n, NT / TPR, ahead<T, TPR>() ? 1024 : 1 << 16);
   ln_fwd_kernel<T, W, TPR, NCH><<<grid, NT, 0, st>>>((const T*)x, xs, (const W*)w, (const W*)b, (T*)y, (A*)mean,
                                                       (A*)rstd, n, (int)width, eps);
 }
@@ -385,7 +421,7 @@ void run_fwd(const void* x, int64_t xs, const void* w, const void* b, void* y, v
   constexpr int V = LnVec<T>::value;
   // The fewest lanes that hold the row in 32 values each, and for them the shortest of these rows: 65536x128 bf16 with 16
   // lanes 8.1 us, with 32 13.5, with 64 22.6; 65536x784 bf16 in two vectors to a lane 45 us, in four 75; 16384x4096 bf16 in
-  // 256 lanes 47 us, in four vectors to a lane 83, in 1024 lanes 398.  (64 values in one wave instead of 16 in four:
+  // 256 lanes 47 us, in four vectors to a lane 83, in 1024 lanes 398 (without the rows ahead).  (64 values in one wave instead of 16 in four:
   // 65536x4096 bf16 0.36 ms against 0.26.)
   constexpr int MAXC = 32 / V;
   const int64_t vectors = (width + V - 1) / V;
