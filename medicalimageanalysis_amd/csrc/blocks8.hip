@@ -119,31 +119,41 @@ __global__ __launch_bounds__(256) void quantize_both_kernel(RowArgs r, TileArgs 
   }
 }
 
-// out = value * 2^e (GRAD: out = g * slope of the softplus at the kept value)
+// out = value * 2^e (GRAD: out = g * slope of the softplus at the kept value).  A lane has as many elements as fill the 16
+// bytes of a store: 8 of 16 bits and, so that the lanes' stores lie side by side, 4 of 32.
 template <typename T, bool GRAD>
 __global__ __launch_bounds__(256) void from_blocks_kernel(const T* __restrict__ g, int64_t g_stride,
                                                           const uint8_t* __restrict__ values, int64_t pitch,
                                                           const uint8_t* __restrict__ exponents, int64_t exp_pitch,
                                                           int exp_shift, T* __restrict__ out, int64_t rows,
                                                           int64_t width, int64_t blocks, int row_bits, float beta) {
-  const int group = threadIdx.x >> 4, lane = threadIdx.x & 15;
+  constexpr int E = 16 / (int)sizeof(T), LANES = B8 / E, GROUPS = 256 / LANES;
+  const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
   const int64_t row = ((int64_t)blockIdx.x << row_bits) + (group & ((1 << row_bits) - 1));
   if (row >= rows) return;
-  const int side = 16 >> row_bits;
+  const int side = GROUPS >> row_bits;
   for (int64_t kb = (int64_t)blockIdx.y * side + (group >> row_bits); kb < blocks; kb += (int64_t)gridDim.y * side) {
-    const int64_t col = kb * B8 + lane * 8;
-    const uint2 v = *reinterpret_cast<const uint2*>(values + row * pitch + col);
+    const int64_t col = kb * B8 + lane * E;
     const float scale = b8_scale(exponents[kb * exp_pitch + (row >> exp_shift)]);
-    float a[8];
-    b8_unpack4(v.x, scale, a);
-    b8_unpack4(v.y, scale, a + 4);
-    if constexpr (GRAD) {
-      float gv[8];
-      load_some<8>(g + row * g_stride + col, width - col, 0.0f, gv);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] = gv[i] * b8_softplus_slope<sizeof(T) == 2>(a[i], beta);
+    const uint32_t* v = reinterpret_cast<const uint32_t*>(values + row * pitch + col);
+    uint32_t w[E / 4];
+    float a[E];
+    if constexpr (E == 8) {
+      const uint2 both = *reinterpret_cast<const uint2*>(v);
+      w[0] = both.x;
+      w[1] = both.y;
+    } else {
+      w[0] = *v;
     }
-    store_some<8>(out + row * width + col, width - col, a);
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i) b8_unpack4(w[i], scale, a + 4 * i);
+    if constexpr (GRAD) {
+      float gv[E];
+      load_some<E>(g + row * g_stride + col, width - col, 0.0f, gv);
+#pragma unroll
+      for (int i = 0; i < E; ++i) a[i] = gv[i] * b8_softplus_slope<sizeof(T) == 2>(a[i], beta);
+    }
+    store_some<E>(out + row * width + col, width - col, a);
   }
 }
 
@@ -151,13 +161,14 @@ struct Shape {
   dim3 grid;
   int row_bits;
 };
-// as many rows side by side as there are, up to 16; block columns are walked in a loop once there are enough groups
-Shape shape_for(int64_t rows, int64_t blocks) {
+// A workgroup's 1 << group_bits groups: as many rows side by side as there are; block columns are walked in a loop once
+// there are enough workgroups
+Shape shape_for(int64_t rows, int64_t blocks, int group_bits) {
   Shape s;
   s.row_bits = 0;
-  while (s.row_bits < 4 && (1 << s.row_bits) < rows) ++s.row_bits;
+  while (s.row_bits < group_bits && (1 << s.row_bits) < rows) ++s.row_bits;
   const int64_t gx = rows > 0 ? (rows + (1 << s.row_bits) - 1) >> s.row_bits : 1;
-  const int64_t most = (blocks + (16 >> s.row_bits) - 1) / (16 >> s.row_bits);
+  const int64_t side = (1 << group_bits) >> s.row_bits, most = (blocks + side - 1) / side;
   int64_t gy = (8192 + gx - 1) / gx;
   if (gy > most) gy = most;
   s.grid = dim3((unsigned)gx, (unsigned)(gy < 1 ? 1 : gy > 65535 ? 65535 : gy));
@@ -192,7 +203,7 @@ int row_args(const char* what, const void* x, int64_t x_stride, uint8_t* values,
   }
   if (activation == VMF_ACT_NONE) beta = 1.0;
   const int64_t blocks = b8_blocks(width);
-  const Shape s = shape_for(rows, blocks);
+  const Shape s = shape_for(rows, blocks, 4);
   *out = RowArgs{x, x_stride, values, exponents, exp_pitch, rows, width, blocks, s.row_bits, (int)s.grid.x,
                  (int)s.grid.y, beta, (float)beta, (float)(1.0 / beta)};
   return VMF_OK;
@@ -300,7 +311,7 @@ static int from_blocks(const char* what, const void* g, int64_t g_stride, const 
   VMF_REQUIRE(values && exponents && out && (g || !grad), VMF_ERR_BAD_ARG, "%s: null pointer", what);
   VMF_REQUIRE(((uintptr_t)values & 15) == 0, VMF_ERR_BAD_ARG, "%s: values must be 16-byte aligned", what);
   const int64_t blocks = b8_blocks(width);
-  const Shape s = shape_for(rows, blocks);
+  const Shape s = shape_for(rows, blocks, dtype == VMF_F32 ? 3 : 4);
   hipStream_t st = (hipStream_t)stream;
   LOWP_DISPATCH(dtype, "vmf_blocks8", T, {
     if (grad)
