@@ -319,7 +319,7 @@ int vmf_layer_norm_bwd(const void* x, int64_t x_stride, const void* gy, int64_t 
  *   exponents  bytes e + 127, [ceil(width / 128)][exp_pitch]: by rows exp_pitch >= rows (products: a multiple of 16,
  *              so that the array's end is a multiple of 16 too), by tiles exp_pitch = ceil(rows / 128)
  * x, g, out: VMF_F32, VMF_F16 or VMF_BF16, row strides in elements as in the layer norm; out is dense. */
-#define VMF_BLOCKS8_MAX_ROWS ((int64_t)1 << 30)
+#define VMF_BLOCKS8_MAX_ROWS ((int64_t)1 << 26)
 #define VMF_BLOCKS8_MAX_WIDTH ((int64_t)1 << 22)
 enum vmf_activation { VMF_ACT_NONE = 0, VMF_ACT_SOFTPLUS = 1 };
 /* blocks of x, or of softplus(x) = log(1 + exp(beta x)) / beta: the bytes of its exact value, whatever x's type */

@@ -44,11 +44,18 @@ class Blocks8:
     __slots__ = ("storage", "shape", "rows", "width", "tiled", "exp_pitch", "exp_offset", "offset")
 
     def __init__(self, storage, shape, tiled=False, offset=0):
-        self.storage, self.shape, self.tiled, self.offset = storage, torch.Size(shape), tiled, offset
+        self.storage, self.shape, self.tiled, self.offset = storage, torch.Size(shape), bool(tiled), offset
+        if len(self.shape) < 1 or self.shape[-1] < 1 or (tiled and len(self.shape) != 2):
+            raise ValueError(f"Blocks8: shape {tuple(self.shape)}")
         self.width = self.shape[-1]
         self.rows = self.shape.numel() // self.width
         self.exp_pitch = max(1, _up(self.rows, BLOCK) // BLOCK) if tiled else max(16, _up(self.rows, 16))
         self.exp_offset = offset + self.rows * _up(self.width, BLOCK)
+        if (storage.dtype != torch.uint8 or storage.dim() != 1 or not storage.is_contiguous() or offset < 0 or offset % 16
+                or storage.numel() < offset + self.bytes_for(self.rows, self.width, tiled)):
+            raise ValueError(f"Blocks8: {tuple(self.shape)} needs {self.bytes_for(self.rows, self.width, tiled)} bytes of a "
+                             f"dense uint8 tensor from a multiple of 16 on, got {storage.dtype} of {tuple(storage.shape)} "
+                             f"from {offset} on")
 
     @staticmethod
     def bytes_for(rows, width, tiled=False):
@@ -96,6 +103,9 @@ class Weight8:
     __slots__ = ("rows", "columns", "dtype")
 
     def __init__(self, rows, columns, dtype):
+        if not rows.tiled or (columns is not None and (not columns.tiled or columns.shape != rows.shape[::-1]
+                                                       or columns.device != rows.device)):
+            raise ValueError(f"Weight8: {rows} and {columns} are not the tiles of a matrix and of its transpose")
         self.rows, self.columns, self.dtype = rows, columns, dtype
 
     @property

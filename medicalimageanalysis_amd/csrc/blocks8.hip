@@ -223,7 +223,8 @@ int tile_args(const char* what, const void* w, int64_t w_stride, uint8_t* values
                 "%s: values must be 16-byte aligned", what);
   }
   *out = TileArgs{w, w_stride, values, exponents, values_t, exponents_t, rows, width, b8_blocks(rows), b8_blocks(width)};
-  VMF_REQUIRE(out->n_tiles * out->k_tiles <= 0x7fffffff, VMF_ERR_UNSUPPORTED, "%s: %lld x %lld", what, (long long)rows,
+  // (a launch has fewer than 2^32 threads)
+  VMF_REQUIRE(out->n_tiles * out->k_tiles < (1 << 24), VMF_ERR_UNSUPPORTED, "%s: %lld x %lld", what, (long long)rows,
               (long long)width);
   return VMF_OK;
 }

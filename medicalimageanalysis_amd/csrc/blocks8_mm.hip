@@ -1186,7 +1186,8 @@ static int matmul(const FewArgs* few, int activation, const uint8_t* a, const ui
               "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)need);
   const int64_t blocks = b8_blocks(k);
   const MmPlan pl = mm_plan(m, n, blocks, out_dtype != VMF_F32 && !a_tiled && b_tiled);
-  VMF_REQUIRE((int64_t)pl.mt * pl.nt <= 0x7fffffff, VMF_ERR_UNSUPPORTED, "%s: %lld x %lld results", what, (long long)m,
+  // (a launch has fewer than 2^32 threads)
+  VMF_REQUIRE((int64_t)pl.mt * pl.nt < (1 << 23), VMF_ERR_UNSUPPORTED, "%s: %lld x %lld results", what, (long long)m,
               (long long)n);
   MmArgs p;
   p.a = Operand{a, a_exponents, blocks * B8, a_exp_pitch, m, a_tiled};
@@ -1263,7 +1264,7 @@ extern "C" int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const 
   VMF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), VMF_ERR_BAD_ARG,
               "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)need);
   const WgPlan pl = wg_plan(m, n, k, dtype);
-  VMF_REQUIRE((int64_t)pl.nt * pl.kt * pl.splits <= 0x7fffffff, VMF_ERR_UNSUPPORTED, "%s: %lld x %lld results", what,
+  VMF_REQUIRE((int64_t)pl.nt * pl.kt * pl.splits < (1 << 23), VMF_ERR_UNSUPPORTED, "%s: %lld x %lld results", what,
               (long long)n, (long long)k);
   WgArgs p;
   p.gy = gy;

@@ -12,6 +12,12 @@ def blocks(rows, width, tiled=False):
 
 
 @pytest.mark.parametrize("call,error,match", [
+    (lambda: blocks8.Blocks8(torch.zeros(143, dtype=torch.uint8), (1, 5)), ValueError, "144 bytes"),
+    (lambda: blocks8.Blocks8(torch.zeros(144, dtype=torch.uint8), (1, 5), offset=16), ValueError, "144 bytes"),
+    (lambda: blocks8.Blocks8(torch.zeros(200, dtype=torch.uint8), (1, 5), offset=8), ValueError, "multiple of 16"),
+    (lambda: blocks8.Blocks8(torch.zeros(288, dtype=torch.uint8)[::2], (1, 5)), ValueError, "dense"),
+    (lambda: blocks8.Blocks8(torch.zeros(144), (1, 5)), ValueError, "uint8"),
+    (lambda: blocks8.Blocks8(torch.zeros(144, dtype=torch.uint8), (3, 0)), ValueError, "shape"),
     (lambda: blocks8.quantize(torch.zeros(())), ValueError, "last dimension"),
     (lambda: blocks8.quantize(torch.zeros(3, 0)), ValueError, "last dimension"),
     (lambda: blocks8.quantize(torch.zeros(3, 4, dtype=torch.float64)), TypeError, "float32, float16 or bfloat16"),
@@ -19,6 +25,8 @@ def blocks(rows, width, tiled=False):
     (lambda: blocks8.quantize(torch.zeros(3, 4), "softplus", 0.0), ValueError, "beta"),
     (lambda: blocks8.quantize(torch.zeros(3, 4), "softplus", float("nan")), ValueError, "beta"),
     (lambda: blocks8.quantize(torch.zeros(3, 4)), RuntimeError, "HIP device"),
+    (lambda: blocks8.Weight8(blocks(3, 5), None, torch.float32), ValueError, "tiles"),
+    (lambda: blocks8.Weight8(blocks(3, 5, True), blocks(5, 4, True), torch.float32), ValueError, "transpose"),
     (lambda: blocks8.quantize_weight(torch.zeros(4)), ValueError, "matrix"),
     (lambda: blocks8.quantize_weight(torch.zeros(0, 4)), ValueError, "matrix"),
     (lambda: blocks8.matmul(torch.zeros(2, 3), blocks(2, 3)), TypeError, "Blocks8"),
@@ -57,6 +65,7 @@ def test_c_entry_refusals():
     def quantize(rows=4, width=8, x=p, values=p, pitch=16, act=0, beta=1.0, dtype=0):
         return lib.vmf_blocks8_quantize(x, 8, values, p, pitch, rows, width, act, beta, dtype, None)
 
+    assert quantize(rows=(1 << 26) + 1, pitch=1 << 27) == -4  # a launch has fewer than 2^32 threads
     assert quantize(rows=-1) == -1 and quantize(width=0) == -1 and quantize(width=(1 << 22) + 1) == -4
     assert quantize(x=None) == -1 and quantize(values=odd) == -1 and quantize(pitch=3) == -1
     assert quantize(act=2) == -1 and quantize(act=1, beta=0.0) == -1 and quantize(dtype=1) == -2
@@ -70,6 +79,9 @@ def test_c_entry_refusals():
         return lib.vmf_blocks8_matmul(a, p, pitch, 0, p, p, 16, 0, bias, bias_dtype, gate, p, 16, beta, out, m, n, k, ws,
                                       nbytes, dtype, None)
 
+    assert matmul(m=1 << 26, n=1 << 26, pitch=1 << 26) == -1  # (b's exponent pitch)
+    assert lib.vmf_blocks8_matmul(p, p, 1 << 26, 0, p, p, 1 << 26, 0, None, 0, None, p, 16, 1.0, p, 1 << 26, 1 << 26, 8, None,
+                                  0, 0, None) == -4
     assert matmul(m=-1) == -1 and matmul(k=0) == -1 and matmul(a=None) == -1 and matmul(a=odd) == -1
     assert matmul(pitch=8) == -1 and matmul(out=None) == -1 and matmul(dtype=1) == -2
     assert matmul(bias=p, bias_dtype=1) == -2 and matmul(gate=p, beta=-1.0) == -1

@@ -194,7 +194,7 @@ SHAPES = [(1, 1, 1), (1, 784, 128), (1, 4096, 4096), (3, 100, 129), (16, 33, 210
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("m,n,k", SHAPES + [(4097, 4100, 384), (4096, 4096, 128)])
+@pytest.mark.parametrize("m,n,k", SHAPES + [(4097, 4100, 384), (4096, 4096, 128), (2500, 2601, 300)])
 def test_matmul(m, n, k, dtype):
     a = blocks8.quantize(normal(m, k, seed=1) * torch.exp(normal(m, 1, seed=2)))
     w = blocks8.quantize_weight(normal(n, k, seed=3), transpose=False).rows
@@ -206,7 +206,7 @@ def test_matmul(m, n, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("m,n,k", [(5, 40, 300), (100, 140, 300), (2048, 2048, 128)])
+@pytest.mark.parametrize("m,n,k", [(5, 40, 300), (100, 140, 300), (2048, 2048, 128), (2560, 2561, 129)])
 def test_matmul_of_two_sets_of_rows(m, n, k, dtype):
     """both sides with an exponent per row and block, of very different sizes"""
     a = blocks8.quantize(normal(m, k, seed=1) * torch.exp(3 * normal(m, 1, seed=2)))
@@ -246,7 +246,8 @@ def test_matmul_non_finite_rows_stay_theirs():
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 128, 784), (31, 5, 129), (128, 128, 128), (1000, 300, 200), (5000, 130, 1000),
-                                   (16384, 784, 128), (70000, 16, 16)])
+                                   (16384, 784, 128), (70000, 16, 16), (600, 257, 257), (1100, 1400, 1504),
+                                   (1101, 1401, 1500), (2100, 2050, 4001)])
 def test_weight_grad(m, n, k, dtype):
     g = (normal(m, n, seed=1) * torch.exp(normal(m, 1, seed=2))).to(dtype)
     q = blocks8.quantize(normal(m, k, seed=3), "softplus")
@@ -309,7 +310,8 @@ def layer_formula(x, w, b, gy, activation, beta):
 @pytest.mark.parametrize("x_type,w_type", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
                                            (torch.float16, torch.float32)])
 @pytest.mark.parametrize("activation,beta", [(None, 1.0), ("softplus", 1.0), ("softplus", 3.0)])
-@pytest.mark.parametrize("m,n,k", [(1, 64, 200), (33, 129, 100), (37, 785, 1000), (128, 128, 128), (1500, 300, 260), (2048, 2100, 300)])
+@pytest.mark.parametrize("m,n,k", [(1, 64, 200), (33, 129, 100), (37, 785, 1000), (128, 128, 128), (1500, 300, 260), (2048, 2100, 300), (2500, 300, 2601),
+                                   (16300, 150, 1000)])
 def test_linear(m, n, k, activation, beta, x_type, w_type):
     x = normal(m, k, seed=1, scale=2.0).to(x_type).requires_grad_()
     w = normal(n, k, seed=2, scale=k ** -0.5).to(w_type).requires_grad_()
