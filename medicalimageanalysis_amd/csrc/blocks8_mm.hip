@@ -599,6 +599,7 @@ __global__ __launch_bounds__(256) void mm_join_kernel(MmArgs p, int splits) {
   const int64_t total = p.m * p.n;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     float v = 0;
+#pragma unroll 8
     for (int s = 0; s < splits; ++s) v += p.partial[s * total + i];
     const int64_t row = i / p.n, col = i - row * p.n;
     finish1<OUT>(p, row, col, v);
@@ -838,9 +839,13 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void wgrad_kernel(Wg
   // reaches behind the last column other ones are read instead, or none (their results are dropped).
   const int gr = threadIdx.x / GP, gc = threadIdx.x % GP * E;
   const int ar = threadIdx.x / (BK / 16), ac = threadIdx.x % (BK / 16) * 16;
+  // No piece reaches behind its row: a column behind the last whole piece reads that, and where the row ends inside the
+  // piece (not WHOLE) it is moved into place by g_back elements.
   const bool g_in = n0 + gc < p.n, a_in = k0 + ac < p.a.pitch;
-  const int g_left = p.n - n0 - gc >= E ? E : g_in ? (int)(p.n - n0 - gc) : 0;
-  const uint8_t* gsrc = (const uint8_t*)p.gy + ((m0 + gr) * p.gy_stride + n0 + (g_in ? gc : 0)) * (int64_t)sizeof(T);
+  const bool ragged = !WHOLE && n0 + BN > p.n, tiny = !WHOLE && p.n < E;
+  const int64_t g_col = tiny ? 0 : n0 + gc + E > p.n ? p.n - E : n0 + gc;
+  const int g_back = g_in ? (int)(n0 + gc - g_col) : 0;
+  const uint8_t* gsrc = (const uint8_t*)p.gy + ((m0 + gr) * p.gy_stride + g_col) * (int64_t)sizeof(T);
   const uint8_t* asrc = p.a.values + (m0 + ar) * p.a.pitch + k0 + (a_in ? ac : 0);
   const uint8_t* esrc = p.a.exps + ((k0 + (a_in ? ac : 0)) >> 7) * p.a.exp_pitch + m0 + ar;
   const int64_t g_pass = GROWS * p.gy_stride * (int64_t)sizeof(T), g_step = GN * g_pass, a_step = WG_ROWS * p.a.pitch;
@@ -852,19 +857,32 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void wgrad_kernel(Wg
     } else {
       union {
         T e[E];
+        typename Pack<T, E>::type w;
         v4i v;
       } u;
-      u.v = v4i{0, 0, 0, 0};
-      if (g_left == E) {
-        const typename Pack<T, E>::type w = *reinterpret_cast<const typename Pack<T, E>::type*>(src);
-#pragma unroll
-        for (int j = 0; j < E; ++j) u.e[j] = w[j];
-      } else {
+      if (!tiny) {
+        u.w = *reinterpret_cast<const typename Pack<T, E>::type*>(src);
+      } else {  // fewer columns than a piece has
+        u.v = v4i{0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < E; ++j)
-          if (j < g_left) u.e[j] = reinterpret_cast<const T*>(src)[j];
+          if (g_in && j < p.n) u.e[j] = reinterpret_cast<const T*>(src)[j];
       }
       return u.v;
+    }
+  };
+  auto place = [&] {  // what has arrived, in a tile that reaches behind the last column
+    if (ragged && !tiny) {
+#pragma unroll
+      for (int i = 0; i < GN; ++i) {
+        union {
+          v4i v;
+          unsigned __int128 bits;
+        } u;
+        u.v = g[i];
+        u.bits = g_in ? u.bits >> (8 * (int)sizeof(T) * g_back) : 0;
+        g[i] = u.v;
+      }
     }
   };
   // the next step's rows; ALL: all 32 are there, else `left` of them
@@ -1011,7 +1029,10 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void wgrad_kernel(Wg
   auto step = [&](int t, auto MORE) {
     constexpr int more = decltype(MORE)::value;
     const int stage = t & 1;
-    if constexpr (more > 0) side(t + 1);
+    if constexpr (more > 0) {
+      place();
+      side(t + 1);
+    }
     read_half(stage, 16, h1);
     multiply(h0, 0, NT * FN / 2);
     if constexpr (more > 0) put(stage ^ 1);
@@ -1043,6 +1064,7 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void wgrad_kernel(Wg
   };
   if (steps > 0) {
     load(std::false_type{}, rows);
+    place();
     side(0);
     put(0);
     if (steps > 1) load(std::false_type{}, rows - WG_ROWS);
@@ -1058,29 +1080,50 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void wgrad_kernel(Wg
   if (sums) write_gbias<W, BN, GROWS, E>(p, lds, gsum, gr, gc, split, n0);
 }
 
-// the splits' sums in their order: four elements of gweight to a thread, then gbias's
-template <typename W>
+// The splits' sums in a fixed order: gweight and gbias in fours, which PARTS threads of a workgroup share (each adds every
+// PARTS-th split, the results are added in LDS).  A sum is a chain of loads that wait for memory: with one thread to a four,
+// 36 splits of 128 x 784 took as long as the product itself.
+template <typename W, int PARTS>
 __global__ __launch_bounds__(256) void wgrad_join_kernel(const float* __restrict__ partial, W* __restrict__ gw,
                                                          W* __restrict__ gb, int splits, int64_t nk, int64_t n) {
-  const int64_t quads = (nk + 3) / 4, total = quads + (gb ? n : 0);
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+  constexpr int FOURS = 256 / PARTS;
+  __shared__ float red[PARTS > 1 ? PARTS : 1][FOURS][4];
+  const int at = threadIdx.x % FOURS, part = threadIdx.x / FOURS;
+  const int64_t w_fours = (nk + 3) / 4, total = w_fours + (gb ? (n + 3) / 4 : 0);
+  for (int64_t first = (int64_t)blockIdx.x * FOURS; first < total; first += (int64_t)gridDim.x * FOURS) {
+    int64_t i = first + at, size = nk;
+    const float* src = partial;
+    W* out = gw;
+    if (i >= w_fours) {
+      i -= w_fours;
+      src += splits * nk;
+      size = n;
+      out = gb;
+    }
+    const int64_t left = first + at < total ? size - 4 * i : 0;
     float s[4] = {0, 0, 0, 0};
-    if (i < quads) {
-      const int64_t left = nk - 4 * i;
-#pragma unroll 4
-      for (int q = 0; q < splits; ++q) {
+    if (left > 0) {
+#pragma unroll 8
+      for (int q = part; q < splits; q += PARTS) {
         float v[4];
-        load_some<4>(partial + q * nk + 4 * i, left, 0.0f, v);
+        load_some<4>(src + q * size + 4 * i, left, 0.0f, v);
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[j] += v[j];
       }
-      store_some<4>(gw + 4 * i, left, s);
-    } else {
-      const float* src = partial + splits * nk + (i - quads);
-#pragma unroll 8
-      for (int q = 0; q < splits; ++q) s[0] += src[q * n];
-      gb[i - quads] = (W)s[0];
     }
+    if constexpr (PARTS > 1) {
+      __syncthreads();  // (the last round's sums have been read)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) red[part][at][j] = s[j];
+      __syncthreads();
+      if (part == 0) {
+#pragma unroll
+        for (int q = 1; q < PARTS; ++q)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[j] += red[q][at][j];
+      }
+    }
+    if (part == 0) store_some<4>(out + 4 * i, left, s);
   }
 }
 
@@ -1291,9 +1334,15 @@ extern "C" int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const 
   });
   rc = vmf_check_launch(what);
   if (rc != VMF_OK || !need) return rc;
-  LOWP_DISPATCH(out_dtype, "vmf_blocks8_weight_grad", W,
-                (wgrad_join_kernel<W><<<vmf_grid_for((n * k + 3) / 4 + n, 256, 1 << 13), 256, 0, st>>>(
-                    p.partial, (W*)gweight, (W*)gbias, pl.splits, n * k, n)));
+  const int64_t fours = (n * k + 3) / 4 + (n + 3) / 4;
+  LOWP_DISPATCH(out_dtype, "vmf_blocks8_weight_grad", W, {
+    if (pl.splits > 8)
+      wgrad_join_kernel<W, 8><<<vmf_grid_for(fours, 32, 1 << 13), 256, 0, st>>>(p.partial, (W*)gweight, (W*)gbias,
+                                                                               pl.splits, n * k, n);
+    else
+      wgrad_join_kernel<W, 1><<<vmf_grid_for(fours, 256, 1 << 13), 256, 0, st>>>(p.partial, (W*)gweight, (W*)gbias,
+                                                                                pl.splits, n * k, n);
+  });
   return vmf_check_launch(what);
 }
 

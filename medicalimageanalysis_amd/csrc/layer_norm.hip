@@ -374,21 +374,22 @@ __global__ __launch_bounds__(256) void ln_cols_kernel(const T* __restrict__ x, i
   partial[((int64_t)blockIdx.y * 2 + 1) * width + col] = gb;
 }
 
-// gw / gb from `parts` partial rows of 2 * width values: a workgroup takes 16 columns, 16 threads share one
+// gw / gb from `parts` partial rows of 2 * width values: a workgroup takes 16 columns, 32 threads share one
+constexpr int REDUCE_SHARE = 32;
 template <typename A, typename W>
-__global__ __launch_bounds__(256) void ln_reduce_kernel(const A* __restrict__ partial, W* __restrict__ gw,
+__global__ __launch_bounds__(16 * REDUCE_SHARE) void ln_reduce_kernel(const A* __restrict__ partial, W* __restrict__ gw,
                                                         W* __restrict__ gb, int parts, int64_t width) {
-  __shared__ A red[256];
+  __shared__ A red[16 * REDUCE_SHARE];
   const int64_t col = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);  // 0 .. 2 width
   A s = 0;
   if (col < 2 * width)
 #pragma unroll 8
-    for (int p = threadIdx.x >> 4; p < parts; p += 16) s += partial[(int64_t)p * 2 * width + col];
+    for (int p = threadIdx.x >> 4; p < parts; p += REDUCE_SHARE) s += partial[(int64_t)p * 2 * width + col];
   red[threadIdx.x] = s;
   __syncthreads();
   if (threadIdx.x < 16 && col < 2 * width) {
 #pragma unroll
-    for (int r = 1; r < 16; ++r) s += red[r * 16 + threadIdx.x];
+    for (int r = 1; r < REDUCE_SHARE; ++r) s += red[r * 16 + threadIdx.x];
     if (col < width) {
       if (gw) gw[col] = (W)s;
     } else if (gb) {
@@ -527,7 +528,8 @@ int run_bwd(const void* x, int64_t xs, const void* gy, int64_t gs, const void* w
 #undef LN_BWD
   int rc = vmf_check_launch("vmf_layer_norm_bwd");
   if (rc != VMF_OK || !partial) return rc;
-  ln_reduce_kernel<A, W><<<(unsigned)((2 * width + 15) / 16), 256, 0, st>>>(partial, (W*)gw, (W*)gb, pl.parts, width);
+  ln_reduce_kernel<A, W><<<(unsigned)((2 * width + 15) / 16), 16 * REDUCE_SHARE, 0, st>>>(partial, (W*)gw, (W*)gb,
+                                                                                         pl.parts, width);
   return vmf_check_launch("vmf_layer_norm_bwd sums");
 }
 
