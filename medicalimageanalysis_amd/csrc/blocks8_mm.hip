@@ -616,9 +616,10 @@ struct MmPlan {
 //   256 x 256 (`large`: a 16-bit result of rows and tiles) from 256 of them on: 4096 x 4096 x 1024 21.9 us, 128 x 128 29.4,
 //     64 x 64 36.7; at 128 of them (4096 x 2048 x 2048) 43.0 us against 25.5;
 //   128 x 128 from 384 on: at 400 (2560 x 2560 x 2048) 24.4 us, 64 x 64 27.8; at 256 (2048^3) 19.2 and 16.9.
-// Where even the smallest tile leaves compute units without one the block columns are split, at least 8 to a split
-// (128 x 128 x 16384 12.3 us, 4 to a split 15.8, unsplit 42); up to 16 rows at least 16 (1 x 128 x 16384 6.8 us,
-// unsplit 10.8), and none up to 32 block columns (1 x 128 x 4096 4.1 us, split in two 5.0).
+// Where even the smallest tile leaves compute units without one the block columns are split, at least 4 to a split
+// (256 x 256 x 4096 7.4 us, 8 to a split 8.9, unsplit 13.2), and none up to 16 of them (256 x 1024 x 1024 6.0 us, split in
+// two 7.9); up to 16 rows at least 8 (16 x 512 x 8192 5.1 us, 16 to a split 6.8, unsplit 9.1), and none up to 32
+// (1 x 128 x 4096 4.1 us, split in two 5.1).
 MmPlan mm_plan(int64_t m, int64_t n, int64_t blocks, bool large) {
   MmPlan p;
   auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
@@ -635,7 +636,7 @@ MmPlan mm_plan(int64_t m, int64_t n, int64_t blocks, bool large) {
     p.nt = (int)((n + t - 1) / t);
     groups = (int64_t)p.mt * p.nt;
   }
-  const int64_t least = p.kind != MM_FEW ? 8 : blocks > 32 ? 16 : blocks;
+  const int64_t least = p.kind == MM_FEW ? (blocks > 32 ? 8 : blocks) : blocks > 16 ? 4 : blocks;
   int64_t s = (256 + groups - 1) / groups;
   if (s > blocks / least) s = blocks / least;
   if (s < 1) s = 1;
@@ -1082,7 +1083,8 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void wgrad_kernel(Wg
 
 // The splits' sums in a fixed order: gweight and gbias in fours, which PARTS threads of a workgroup share (each adds every
 // PARTS-th split, the results are added in LDS).  A sum is a chain of loads that wait for memory: with one thread to a four,
-// 36 splits of 128 x 784 took as long as the product itself.
+// 36 splits of 128 x 784 took as long as the product itself (16384x128x784 fp32 with eight threads 27.8 us, with one 34.2).
+// One does where there are many fours and few splits (16384x1024x2048 fp32, 8 splits: 172.7 us, with eight threads 177).
 template <typename W, int PARTS>
 __global__ __launch_bounds__(256) void wgrad_join_kernel(const float* __restrict__ partial, W* __restrict__ gw,
                                                          W* __restrict__ gb, int splits, int64_t nk, int64_t n) {
@@ -1133,17 +1135,18 @@ struct WgPlan {
 };
 // The large tile is 256 x 256 for bf16, 128 x 256 for fp16 and fp32, whose two and three terms take the registers and LDS.
 // It reads less for a product but fills a compute unit by itself, where two workgroups of the 128 x 128 tile hide each
-// other's start, barriers and end: it is taken from 2^34 products on (bf16: 65536x512x512 60.6 us, small 61.2;
-// 16384x512x512 40.5 and 29.7; 4096^3 128 and 176), for the others from 2^31 on (fp32: 16384x512x512 39.0 and 43.7,
-// 16384x128x784 35.4 and 33.8).
-// The batch is split until every compute unit has a workgroup, at least 256 rows to a split (fp32 16384x1024x1024 95.6 us,
-// unsplit 515; bf16 4096x256x256 15.4 us, with 128 rows 19.1), in up to 16 splits 128 rows (fp32 1000x257x257 16.1 us, with
-// 256 22.5); the small tile until there are two for each, at least 512 rows to a split (bf16 4096x1024x1024 28.5 us, with
-// one 32.0; 2048x1024x1024, where that is 256 rows, 26.3 and 23.4).
+// other's start, barriers and end: it is taken above 2^33 products (bf16: 65536x512x512 53.7 us, small 57.4; 16384x512x512
+// 33.8 and 27.7; 4096^3 126 and 173), for the others above 2^30 (fp32: 16384x128x784 24.5 us, small 27.8; 4096^3 328 and
+// 391; 1024^3 25.4 and 24.2).
+// The batch is split until every compute unit has a workgroup, at least 256 rows to a split (fp32 16384x512x512 36 us,
+// unsplit over 500; bf16 4096x256x256 13.0 us, with 64 rows 17.9), in up to 16 splits 128 rows (fp32 1000x257x257 15.1 us,
+// with 256 19.9); the small tile until there are two for each, at least 512 rows to a split and in up to 128 splits (bf16
+// 16384x512x512 27.7 us, with one 30.8; 2048x1024x1024, where that is 256 rows, 26.5 and 23.7; 262144x128x128, where that is
+// 512 splits, 43.0 and 37.2).
 WgPlan wg_plan(int64_t m, int64_t n, int64_t k, int dtype) {
   WgPlan p;
   const bool bf16 = dtype == VMF_BF16;
-  const bool large = (double)m * n * k >= (bf16 ? 0x1p34 : 0x1p31) && k > 128 && (!bf16 || n > 128);
+  const bool large = (double)m * n * k > (bf16 ? 0x1p33 : 0x1p30) && k > 128 && (!bf16 || n > 128);
   p.bk = large ? 256 : 128;
   p.bn = large && bf16 ? 256 : 128;
   p.nt = (int)((n + p.bn - 1) / p.bn);
@@ -1151,7 +1154,8 @@ WgPlan wg_plan(int64_t m, int64_t n, int64_t k, int dtype) {
   const int64_t tiles = (int64_t)p.nt * p.kt;
   auto least = [](int64_t a, int64_t b) { return a < b ? a : b; };
   int64_t s = least(256 / tiles, m / 256 > 16 ? m / 256 : least(m / 128, 16));
-  if (!large && least(512 / tiles, m / 512) > s) s = least(512 / tiles, m / 512);
+  const int64_t two = least(least(512 / tiles, m / 512), 128);
+  if (!large && two > s) s = two;
   if (s < 1) s = 1;
   p.per_split = ((m + s - 1) / s + WG_ROWS - 1) / WG_ROWS * WG_ROWS;
   p.splits = p.per_split > 0 ? (int)((m + p.per_split - 1) / p.per_split) : 1;
@@ -1336,7 +1340,7 @@ extern "C" int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const 
   if (rc != VMF_OK || !need) return rc;
   const int64_t fours = (n * k + 3) / 4 + (n + 3) / 4;
   LOWP_DISPATCH(out_dtype, "vmf_blocks8_weight_grad", W, {
-    if (pl.splits > 8)
+    if (pl.splits > 8 || fours <= 1 << 16)
       wgrad_join_kernel<W, 8><<<vmf_grid_for(fours, 32, 1 << 13), 256, 0, st>>>(p.partial, (W*)gweight, (W*)gbias,
                                                                                pl.splits, n * k, n);
     else

@@ -246,8 +246,8 @@ def test_matmul_non_finite_rows_stay_theirs():
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 128, 784), (31, 5, 129), (128, 128, 128), (1000, 300, 200), (5000, 130, 1000),
-                                   (16384, 784, 128), (70000, 16, 16), (600, 257, 257), (1100, 1400, 1504),
-                                   (1101, 1401, 1500), (2100, 2050, 4001)])
+                                   (16384, 784, 128), (70000, 16, 16), (600, 257, 257), (900, 1000, 1504),
+                                   (901, 1001, 1500), (1100, 2050, 4001), (20000, 3, 300)])
 def test_weight_grad(m, n, k, dtype):
     g = (normal(m, n, seed=1) * torch.exp(normal(m, 1, seed=2))).to(dtype)
     q = blocks8.quantize(normal(m, k, seed=3), "softplus")
