@@ -296,13 +296,13 @@ def _linear(x, weight, laid_out, bias, act, beta, dev, keep, columns):
         if columns and laid_out is None:
             wt = (size, size + k * _up(n, BLOCK))
             size += Blocks8.bytes_for(k, n, True)
-        kept = torch.empty(size, device=dev, dtype=torch.uint8)
+        kept = x.new_empty(size, dtype=torch.uint8)
         base = kept.data_ptr()
         base_e = base + m * kp
         if wt is not None:
             tv, te = base + wt[0], base + wt[1]
-    ws = torch.empty(need.value, device=dev, dtype=torch.uint8) if need.value else None
-    y = torch.empty(x.shape[:-1] + (n,), device=dev, dtype=x.dtype)
+    ws = x.new_empty(need.value, dtype=torch.uint8) if need.value else None
+    y = x.new_empty(x.shape[:-1] + (n,))
     b = _lib.dense(bias)
     with _lib.on_device(dev):
         rc = lib.vmf_blocks8_linear_fwd(rows.data_ptr(), stride, _lib.address(w), w_stride, w_code, wv, we, tv, te,
@@ -341,13 +341,13 @@ class _Linear(torch.autograd.Function):
         code = _lib.FLOAT_CODES[gy.dtype]
         # the weight's gradient in the weight's type; a bias beside a laid-out weight has float32 sums
         out = w_dtype or torch.float32
-        gx = torch.empty(shape, device=dev, dtype=gy.dtype) if need_x else None
-        gw = torch.empty((n, k), device=dev, dtype=out) if need_w or need_b else None
-        gb = torch.empty(n, device=dev, dtype=out) if need_b else None
+        gx = gy.new_empty(shape) if need_x else None
+        gw = gy.new_empty((n, k), dtype=out) if need_w or need_b else None
+        gb = gy.new_empty(n, dtype=out) if need_b else None
         lib = _lib.lib()
         need = C.c_int64(0)
         _lib.check(lib.vmf_blocks8_linear_bwd_workspace(m, n, k, code, need), "vmf_blocks8_linear_bwd_workspace")
-        ws = torch.empty(need.value, device=dev, dtype=torch.uint8)
+        ws = gy.new_empty(need.value, dtype=torch.uint8)
         g, stride = _lib.as_rows(gy)
         base = kept.data_ptr()
         tv = te = None

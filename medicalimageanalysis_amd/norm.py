@@ -44,10 +44,10 @@ def _forward(x, w, b, eps, dev, code, wcode, keep):
     rows, stride = _lib.as_rows(x)
     n, width = rows.shape
     w, b = _lib.dense(w), _lib.dense(b)
-    y = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)  # (empty_like: half the host time of empty)
     stats = mean = rstd = None
     if keep:  # the rows' means, then their reciprocal deviations
-        stats = torch.empty(2 * n, device=dev, dtype=torch.float64 if code == _lib.VMF_F64 else torch.float32)
+        stats = rows.new_empty(2 * n, dtype=torch.float64 if code == _lib.VMF_F64 else torch.float32)
         mean = stats.data_ptr()
         rstd = mean + n * (8 if code == _lib.VMF_F64 else 4)
     with _lib.on_device(dev):
@@ -63,19 +63,19 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps, dev, code, wcode):
         y, rows, stride, w, stats = _forward(x, weight, bias, eps, dev, code, wcode, True)
         ctx.save_for_backward(rows, w, stats)
-        ctx.meta = (x.shape, rows.shape, stride, code, wcode, dev, None if bias is None else bias.dtype)
+        ctx.meta = (rows.shape, stride, code, wcode, dev, None if bias is None else bias.dtype)
         return y
 
     @staticmethod
     @_lib.first_order
     def backward(ctx, gy):
         rows, w, stats = ctx.saved_tensors
-        shape, (n, width), x_stride, code, wcode, dev, p_dtype = ctx.meta
+        (n, width), x_stride, code, wcode, dev, b_dtype = ctx.meta
         g, g_stride = _lib.as_rows(gy)
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        gx = torch.empty(shape, device=dev, dtype=gy.dtype) if need_x else None
-        gw = torch.empty(width, device=dev, dtype=w.dtype) if need_w else None
-        gb = torch.empty(width, device=dev, dtype=p_dtype) if need_b else None
+        gx = torch.empty_like(gy, memory_format=torch.contiguous_format) if need_x else None
+        gw = torch.empty_like(w) if need_w else None
+        gb = rows.new_empty(width, dtype=b_dtype) if need_b else None
         lib = _lib.lib()
         ws, need = None, C.c_int64(0)
         if need_w or need_b:
