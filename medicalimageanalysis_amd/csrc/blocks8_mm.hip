@@ -130,11 +130,19 @@ __device__ __forceinline__ int row_at(int at) {
   const int tile = at >> 4;
   return tile / F * (16 * F) + F * (at & 15) + tile % F;
 }
+// Where piece c of row q (of 16 side by side, 128 bytes each) lies in the row: c ^ swizzle(q).  A 16-byte LDS read is served
+// in groups of 16 lanes, which measured are lanes 0 - 3, 12 - 15 and 20 - 27 of each 32 and the others: the 16 rows, once
+// each, with piece c in rows 0 - 3 and 12 - 15 and c ^ 2 in rows 4 - 11.  Two rows fill the banks once, so the eight pairs of
+// rows have to read eight different places.
+__device__ __forceinline__ int swizzle(int q) {
+  const int h = q >> 1;
+  return h ^ (((h + 2) >> 1) & 2);
+}
 // a 16-row operand tile from LDS: lane l gets row l % 16, the 32 bytes of quarter l / 16
 __device__ __forceinline__ v8i operand(const uint8_t* tile, int lane) {
   const int q = lane & 15, c = (lane >> 4) * 2;
-  const v4i lo = *reinterpret_cast<const v4i*>(tile + q * B8 + ((c ^ (q >> 1)) << 4));
-  const v4i hi = *reinterpret_cast<const v4i*>(tile + q * B8 + (((c + 1) ^ (q >> 1)) << 4));
+  const v4i lo = *reinterpret_cast<const v4i*>(tile + q * B8 + ((c ^ swizzle(q)) << 4));
+  const v4i hi = *reinterpret_cast<const v4i*>(tile + q * B8 + (((c + 1) ^ swizzle(q)) << 4));
   return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 // What a wave holds of the result: lane l has the rows 4 FM * (l / 16) + t (t = FM * r + i: element r of row tile i) and
@@ -205,8 +213,7 @@ __device__ __forceinline__ void write_tile(const MmArgs& p, const v4f (&acc)[GM 
 //   one stage is multiplied the next is on its way, one barrier per block column.
 //   A 16-row operand tile takes the rows F * (lane & 15) + i (i = 0 .. F - 1 the tile's number): the exponents of a
 //   lane's F tiles are then one word, and a lane's results are F consecutive columns of a row.
-//   In LDS the 16 rows of an operand tile lie side by side, the 16-byte pieces of row q at piece ^ (q / 2): the 16 lanes
-//   that read the same piece of the 16 rows then read from all 64 banks (two rows fill the banks once).
+//   In LDS the 16 rows of an operand tile lie side by side, their pieces swizzled (see swizzle).
 template <int BM, int BN, int WM, int WN, bool WIDE, bool GATE, typename OUT>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p) {
   constexpr int WAVES_N = BN / WN, WAVES = (BM / WM) * WAVES_N;
@@ -232,7 +239,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p
     const bool is_b = r8 >= BM / 8;
     const int at = (is_b ? r8 - BM / 8 : r8) * 8 + (lane >> 3), q = at & 15;  // the row's place in LDS
     const int r = is_b ? row_at<FN>(at) : row_at<FM>(at);
-    const int piece = (lane & 7) ^ (q >> 1);
+    const int piece = (lane & 7) ^ swizzle(q);
     const Operand& o = is_b ? p.b : p.a;
     int64_t row = (is_b ? n0 : m0) + r;
     row = row < o.rows ? row : o.rows - 1;
@@ -355,7 +362,7 @@ __global__ __launch_bounds__(512, 2) void mm_large_kernel(MmArgs p) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int at = (wave & 3) * 64 + i * 8 + (lane >> 3), r = row_at<4>(at);
-    off[i] = (uint32_t)((r < last ? r : last) * mine.pitch) + (((lane & 7) ^ ((at & 15) >> 1)) << 4);
+    off[i] = (uint32_t)((r < last ? r : last) * mine.pitch) + (((lane & 7) ^ swizzle(at & 15)) << 4);
   }
   auto load = [&](int kb, int stage, int i) {
     __builtin_amdgcn_global_load_lds(GLOBAL_PTR(base + (int64_t)kb * B8 + off[i]),
