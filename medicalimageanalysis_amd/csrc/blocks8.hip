@@ -6,6 +6,8 @@ namespace {
 
 // A workgroup has 16 groups of 16 lanes: 1 << row_bits of them side by side in rows (so that the exponent bytes of
 // neighbouring rows, which lie side by side, leave together), the others in block columns.
+// Measured: 1048576x784 fp32 0.79 ms (5.2 TB/s), of softplus 0.81; bf16 0.47 ms (5.2), of softplus 0.80, bound by the vector
+// work (some 25 instructions to an element).
 struct RowArgs {
   const void* x;
   int64_t x_stride;
@@ -45,7 +47,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(RowArgs p) {
 }
 
 // One workgroup per 128 x 128 tile of a matrix (n rows, k columns): the tile's bytes in the matrix's order and, through
-// LDS, in the transpose's.
+// LDS, in the transpose's (4096x4096 fp32 18 us, 5.6 TB/s).
 struct TileArgs {
   const void* w;
   int64_t w_stride;
@@ -120,7 +122,8 @@ __global__ __launch_bounds__(256) void quantize_both_kernel(RowArgs r, TileArgs 
 }
 
 // out = value * 2^e (GRAD: out = g * slope of the softplus at the kept value).  A lane has as many elements as fill the 16
-// bytes of a store: 8 of 16 bits and, so that the lanes' stores lie side by side, 4 of 32.
+// bytes of a store: 8 of 16 bits and, so that the lanes' stores lie side by side, 4 of 32 (1048576x784 fp32 0.81 ms,
+// 5.0 TB/s, with 8 to a lane 1.30; bf16 0.56 ms; GRAD bf16 0.96 ms, 4.3 TB/s).
 template <typename T, bool GRAD>
 __global__ __launch_bounds__(256) void from_blocks_kernel(const T* __restrict__ g, int64_t g_stride,
                                                           const uint8_t* __restrict__ values, int64_t pitch,

@@ -155,8 +155,8 @@ static __device__ __noinline__ float softplus_scaled(float x, double beta, int e
 }
 
 // The block of softplus(h).  Which of two neighbouring 8-bit values is nearest to softplus(h) can hang on its last bits,
-// so a value is computed in 32 bits, and once more in 64 where its 32-bit error could change the result (a few of a
-// million): the bytes are those of the exactly computed softplus.
+// so a value is computed in 32 bits, and once more in 64 where its 32-bit error could change the result (some fifty of
+// a million): the bytes are those of the exactly computed softplus.
 __device__ __forceinline__ uint2 softplus8(const float (&h)[8], float beta, float inv_beta, double beta64, int& e_out) {
   constexpr float INF = __builtin_inff();
   // softplus grows with h: the block's largest comes from the largest h.  As integers the bits of floats order like them

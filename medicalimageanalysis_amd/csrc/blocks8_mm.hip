@@ -214,6 +214,8 @@ __device__ __forceinline__ void write_tile(const MmArgs& p, const v4f (&acc)[GM 
 //   A 16-row operand tile takes the rows F * (lane & 15) + i (i = 0 .. F - 1 the tile's number): the exponents of a
 //   lane's F tiles are then one word, and a lane's results are F consecutive columns of a row.
 //   In LDS the 16 rows of an operand tile lie side by side, their pieces swizzled (see swizzle).
+// Measured: WIDE (fp32) 16384x4096x4096 500 us (1.1 PFLOP/s of bf16 instructions, whose number bounds it), 16384x784x128
+// 17 us; 37x785x1000 7.4 us, a matter of latency.
 template <int BM, int BN, int WM, int WN, bool WIDE, bool GATE, typename OUT>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p) {
   constexpr int WAVES_N = BN / WN, WAVES = (BM / WM) * WAVES_N;
@@ -339,7 +341,9 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm_kernel(MmArgs p
 // also across block columns: the barrier that makes the next stage readable, and the stage read last writable, stands
 // before the last phase's products, whose operands are in registers by then.  The loads into LDS are spread over three
 // phases, so that they do not stand before the operand reads in the queue.
-// Bound: 2048 clocks of matrix instructions per block column and CU, against 1536 + 512 clocks of LDS reads and writes.
+// Bound: 2048 clocks of matrix instructions per block column and CU, against 768 + 512 clocks of LDS reads and writes; and the
+// clock itself, which falls to 1.8 - 2.0 GHz under them.  16384x4096x4096 bf16: 224 us by itself (2.45 PFLOP/s), 235 - 260 us
+// in a row of calls, GATE 260 - 275; 8192^3 2.5 PFLOP/s.
 // a by rows, b by tiles, as a layer has them.
 template <bool GATE, typename OUT>
 __global__ __launch_bounds__(512, 2) void mm_large_kernel(MmArgs p) {
@@ -488,7 +492,8 @@ __device__ __forceinline__ void few_result(const MmArgs& p, float (&sums)[8][16]
 }
 
 // Up to 16 rows: the weight's bytes are what there is to move.  A workgroup takes 16 columns, its eight waves share the
-// block columns and read both operands straight into registers; their sums are added through LDS.
+// block columns and read both operands straight into registers; their sums are added through LDS (1x4096x4096 4.5 us,
+// 3.7 TB/s of the weight).
 template <bool WIDE, typename OUT>
 __global__ __launch_bounds__(512) void mm_few_kernel(MmArgs p) {
   __shared__ float sums[8][16][17];
@@ -815,7 +820,8 @@ __device__ __forceinline__ void expand16(v4i a, uint32_t exp_byte, uint4* out) {
 //   written on the way too, the k tiles' workgroups taking turns.
 // Bound: per step and CU the 256 x 256 tile (bf16) takes 1024 clocks of matrix instructions against 640 + 256 of LDS reads
 // and writes; the 128 x 256 tile 1024 (fp16) and 1536 (fp32), where the vector work of taking gy apart comes next, which
-// is why this tile is wide in k.
+// is why this tile is wide in k.  16384x4096x4096: bf16 475 - 495 us (1.15 PFLOP/s; matrix instructions 55 % of the clocks, at
+// 1.9 GHz), fp16 920 us, fp32 1.29 ms; 16384x784x128 20, 25, 28 us.
 constexpr int WG_ROWS = 32;
 
 template <typename T, typename W, int BN, int BK, int WN, int WK, bool WHOLE>

