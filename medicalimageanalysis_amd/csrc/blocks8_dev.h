@@ -26,7 +26,8 @@ __device__ __forceinline__ int b8_exponent(float top) {
   return u == 0 ? 0 : e < B8_EMIN ? B8_EMIN : e > B8_EMAX ? B8_EMAX : e;
 }
 // Two values already divided by the block's 2^e -> two bytes (low half), rounded to nearest even.  Nothing finite is
-// above 448 then but a bound of softplus8, by a few 2^-20, which the conversion rounds to 448; infinities and NaN become NaN.  (e = 119, the largest,
+// above 448 then but a bound of softplus8, by a few 2^-20, which the conversion rounds to 448; infinities and NaN become
+// NaN.  (e = 119, the largest,
 // is the exception: b8_cut brings what is above 448 down to it first.)
 __device__ __forceinline__ uint32_t b8_pack2(float a, float b) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu;

@@ -382,8 +382,8 @@ __global__ __launch_bounds__(512, 2) void mm_large_kernel(MmArgs p) {
   const int64_t ct = (n0 + wn) >> 7;
   const uint8_t* eb = p.b.exps + (ct < p.b.exp_pitch ? ct : p.b.exp_pitch - 1);
   auto load_exps_of = [&](int kb) {
-    return Exps{*reinterpret_cast<const int*>(ea0 + kb * p.a.exp_pitch), *reinterpret_cast<const int*>(ea1 + kb * p.a.exp_pitch),
-                eb[kb * p.b.exp_pitch]};
+    return Exps{*reinterpret_cast<const int*>(ea0 + kb * p.a.exp_pitch),
+                *reinterpret_cast<const int*>(ea1 + kb * p.a.exp_pitch), eb[kb * p.b.exp_pitch]};
   };
 
   v4f acc[8][4];
@@ -732,7 +732,8 @@ __device__ __forceinline__ v8b transposed(int lane, F&& at) {
 }
 // a wave's part of the result: D of a product has column (k) lane % 32, rows (n) (e & 3) + 8 (e >> 2) + 4 (lane / 32)
 template <typename W, int FN, int FK>
-__device__ __forceinline__ void write_wgrad(const WgArgs& p, const v16f (&acc)[FN][FK], int split, int64_t n0, int64_t k0, int lane) {
+__device__ __forceinline__ void write_wgrad(const WgArgs& p, const v16f (&acc)[FN][FK], int split, int64_t n0, int64_t k0,
+                                            int lane) {
 #pragma unroll
   for (int i = 0; i < FN; ++i)
 #pragma unroll
@@ -818,8 +819,8 @@ __device__ __forceinline__ void expand16(v4i a, uint32_t exp_byte, uint4* out) {
 //   WHOLE: gy comes in whole aligned 16-byte pieces (n, the row stride and the address are multiples of them).
 //   The workgroups of the first k tile also add up gbias.  gy's 8-bit blocks (what the input gradient's product reads) are
 //   written on the way too, the k tiles' workgroups taking turns.
-// Bound: per step and CU the 256 x 256 tile (bf16) takes 1024 clocks of matrix instructions against 640 + 256 of LDS reads
-// and writes; the 128 x 256 tile 1024 (fp16) and 1536 (fp32), where the vector work of taking gy apart comes next, which
+// Bound: per step and CU the 256 x 256 tile (bf16) takes 1024 clocks of matrix instructions against 900 of LDS reads and
+// writes; the 128 x 256 tile 1024 (fp16) and 1536 (fp32), where the vector work of taking gy apart comes next, which
 // is why this tile is wide in k.  16384x4096x4096: bf16 475 - 495 us (1.15 PFLOP/s; matrix instructions 55 % of the clocks, at
 // 1.9 GHz), fp16 920 us, fp32 1.29 ms; 16384x784x128 20, 25, 28 us.
 constexpr int WG_ROWS = 32;
@@ -1220,9 +1221,9 @@ extern "C" int vmf_blocks8_matmul_workspace(int64_t m, int64_t n, int64_t k, int
 }
 
 // vmf_blocks8_matmul; few: not null, a are the rows there, quantised by the same launch (one that few_fits)
-static int matmul(const FewArgs* few, int activation, const uint8_t* a, const uint8_t* a_exponents, int64_t a_exp_pitch, int a_tiled,
-                  const uint8_t* b, const uint8_t* b_exponents, int64_t b_exp_pitch, int b_tiled, const void* bias,
-                  int bias_dtype, const uint8_t* gate, const uint8_t* gate_exponents, int64_t gate_exp_pitch,
+static int matmul(const FewArgs* few, int activation, const uint8_t* a, const uint8_t* a_exponents,
+                  int64_t a_exp_pitch, int a_tiled, const uint8_t* b, const uint8_t* b_exponents, int64_t b_exp_pitch,
+                  int b_tiled, const void* bias, int bias_dtype, const uint8_t* gate, const uint8_t* gate_exponents, int64_t gate_exp_pitch,
                   double beta, void* out, int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes,
                   int out_dtype, vmf_stream_t stream) {
   const char* what = "vmf_blocks8_matmul";

@@ -425,8 +425,8 @@ void run_fwd(const void* x, int64_t xs, const void* w, const void* b, void* y, v
   constexpr int V = LnVec<T>::value;
   // The fewest lanes that hold the row in 32 values each, and for them the shortest of these rows: 65536x128 bf16 with 16
   // lanes 8.1 us, with 32 13.5, with 64 22.6; 65536x784 bf16 in two vectors to a lane 45 us, in four 75; 16384x4096 bf16 in
-  // 256 lanes 47 us, in four vectors to a lane 83, in 1024 lanes 398 (without the rows ahead).  (64 values in one wave instead of 16 in four:
-  // 65536x4096 bf16 0.36 ms against 0.26.)
+  // 256 lanes 47 us, in four vectors to a lane 83, in 1024 lanes 398 (all without the rows ahead).  (64 values in one wave
+  // instead of 16 in four: 65536x4096 bf16 0.36 ms against 0.26.)
   constexpr int MAXC = 32 / V;
   const int64_t vectors = (width + V - 1) / V;
 #define LN_FWD(TPR, NCH) \
