@@ -6,7 +6,7 @@ namespace {
 
 // A workgroup has 16 groups of 16 lanes: 1 << row_bits of them side by side in rows (so that the exponent bytes of
 // neighbouring rows, which lie side by side, leave together), the others in block columns.
-// Measured: 1048576x784 fp32 0.79 ms (5.2 TB/s), of softplus 0.81; bf16 0.47 ms (5.2), of softplus 0.80, bound by the vector
+// Measured: 1048576x784 fp32 0.79 ms (5.2 TB/s), of softplus 0.79; bf16 0.47 ms (5.2), of softplus 0.64, bound by the vector
 // work (some 25 instructions to an element).
 struct RowArgs {
   const void* x;

@@ -57,8 +57,10 @@ __device__ __forceinline__ void b8_unpack4(uint32_t w, float scale, float* out) 
 // In 32 bits: log(1 + u), u = exp(-|t|) from the hardware's exponential (1 unit in the last place), as u times a polynomial
 // of degree 7 in u: the best one on [0, 1] by relative error (an exchange fit), 2e-7, with its roundings 3.4e-7.
 // beta, t = beta h and t log2(e) are rounded, 3 * 2^-24 |t| in the exponential's argument, which counts in full for
-// negative t only (for positive t its share is |t| exp(-t) <= 0.37 of that).  Together the result is off by less than
-// softplus_margin relative to its value.
+// negative t only (for positive t its share is |t| exp(-t) <= 0.37 of that).  With the exponential's 1.2e-7 and the
+// roundings of 1 / beta, its product and the bounds (2^-24 each) the result is off by less than softplus_margin relative to
+// its value: 8e-7 + 2e-7 |t|.  (Over all floats with |t| < 87 and five betas it is off by 4.0e-7 + 1.2e-7 |t|.)  Results of
+// exponentials below 2^-126 are 0.
 __device__ __forceinline__ float softplus32(float h, float beta, float inv_beta) {
   const float t = beta * h;
   const float u = __builtin_amdgcn_exp2f(-fabsf(t) * 1.44269504f);
@@ -72,9 +74,9 @@ __device__ __forceinline__ float softplus32(float h, float beta, float inv_beta)
   s = fmaf(s, u, 0.999999821f);
   return fmaf(u, s, __builtin_amdgcn_fmed3f(t, 0.0f, __builtin_inff())) * inv_beta;  // (a NaN is in u)
 }
-// (at most 0.48, also for -inf, the fill of short rows)
+// (below t = -88 there is nothing left to be off, down to -inf, the fill of short rows)
 __device__ __forceinline__ float softplus_margin(float h, float beta) {
-  return fmaf(__builtin_amdgcn_fmed3f(-beta * h, 0.0f, 1.6e6f), 3e-7f, 2e-6f);
+  return fmaf(__builtin_amdgcn_fmed3f(-beta * h, 0.0f, 88.0f), 2e-7f, 8e-7f);
 }
 
 // exp in 64 bits: t = n ln 2 + r, |r| <= 0.35, and the power series of exp(r) to r^13 (the next term is under 5e-18)
@@ -156,8 +158,8 @@ static __device__ __noinline__ float softplus_scaled(float x, double beta, int e
 }
 
 // The block of softplus(h).  Which of two neighbouring 8-bit values is nearest to softplus(h) can hang on its last bits,
-// so a value is computed in 32 bits, and once more in 64 where its 32-bit error could change the result (some fifty of
-// a million): the bytes are those of the exactly computed softplus.
+// so a value is computed in 32 bits, and once more in 64 where its 32-bit error could change the result (some twenty of
+// a million; of 16-bit inputs, which repeat, it can be more): the bytes are those of the exactly computed softplus.
 __device__ __forceinline__ uint2 softplus8(const float (&h)[8], float beta, float inv_beta, double beta64, int& e_out) {
   constexpr float INF = __builtin_inff();
   // softplus grows with h: the block's largest comes from the largest h.  As integers the bits of floats order like them
@@ -181,11 +183,13 @@ __device__ __forceinline__ uint2 softplus8(const float (&h)[8], float beta, floa
   if (top == -INF) e = 0;
   e_out = e;
   const float scale = inv_beta * b8_pow2(-e);
-  float lo[8], hi[8];
+  float lo[8], hi[8], least = h[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) least = fminf(least, h[i]);
+  const float m = softplus_margin(least, beta);  // (the largest of the eight)
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float a = softplus32(h[i], beta, scale);
-    const float m = softplus_margin(h[i], beta);
     lo[i] = fmaf(a, -m, a);
     hi[i] = fmaf(a, m, a);
   }

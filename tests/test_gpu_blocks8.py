@@ -106,6 +106,18 @@ def test_quantized_softplus_is_that_of_the_exact_softplus(dtype, beta):
     assert torch.equal(got, by_blocks(softplus(x, beta)))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("beta", [1.0, 0.3])
+def test_softplus_of_every_16_bit_value(dtype, beta):
+    """in order of size, and each beside a large one, which makes it one of the block's small elements"""
+    every = torch.arange(-2 ** 15, 2 ** 15, device=DEV).to(torch.int16).view(dtype)
+    x = torch.sort(every[every.isfinite()].float())[0].to(dtype)
+    x = torch.cat([x, x.new_zeros(-x.numel() % 127)]).view(-1, 127)
+    for top in (x[:, -1:], torch.full_like(x[:, :1], 6.0)):
+        h = torch.cat([x, top], 1)
+        assert torch.equal(blocks8.quantize(h, "softplus", beta).dequantize().double(), by_blocks(softplus(h, beta)))
+
+
 def test_softplus_over_many_values_and_at_ties():
     x = normal(4096, 2048, seed=5, scale=4.0)
     assert torch.equal(blocks8.quantize(x, "softplus").dequantize().double(), by_blocks(softplus(x, 1.0)))
