@@ -44,18 +44,28 @@ class Blocks8:
     __slots__ = ("storage", "shape", "rows", "width", "tiled", "exp_pitch", "exp_offset", "offset")
 
     def __init__(self, storage, shape, tiled=False, offset=0):
-        self.storage, self.shape, self.tiled, self.offset = storage, torch.Size(shape), bool(tiled), offset
-        if len(self.shape) < 1 or self.shape[-1] < 1 or (tiled and len(self.shape) != 2):
-            raise ValueError(f"Blocks8: shape {tuple(self.shape)}")
-        self.width = self.shape[-1]
-        self.rows = self.shape.numel() // self.width
-        self.exp_pitch = max(1, _up(self.rows, BLOCK) // BLOCK) if tiled else max(16, _up(self.rows, 16))
-        self.exp_offset = offset + self.rows * _up(self.width, BLOCK)
+        shape = torch.Size(shape)
+        if len(shape) < 1 or shape[-1] < 1 or (tiled and len(shape) != 2):
+            raise ValueError(f"Blocks8: shape {tuple(shape)}")
+        need = self.bytes_for(shape.numel() // shape[-1], shape[-1], tiled)
         if (storage.dtype != torch.uint8 or storage.dim() != 1 or not storage.is_contiguous() or offset < 0 or offset % 16
-                or storage.numel() < offset + self.bytes_for(self.rows, self.width, tiled)):
-            raise ValueError(f"Blocks8: {tuple(self.shape)} needs {self.bytes_for(self.rows, self.width, tiled)} bytes of a "
-                             f"dense uint8 tensor from a multiple of 16 on, got {storage.dtype} of {tuple(storage.shape)} "
-                             f"from {offset} on")
+                or storage.numel() < offset + need):
+            raise ValueError(f"Blocks8: {tuple(shape)} needs {need} bytes of a dense uint8 tensor from a multiple of 16 on, "
+                             f"got {storage.dtype} of {tuple(storage.shape)} from {offset} on")
+        self._set(storage, shape, shape.numel() // shape[-1], bool(tiled), offset)
+
+    def _set(self, storage, shape, rows, tiled, offset):
+        width = shape[-1]
+        self.storage, self.shape, self.rows, self.width, self.tiled, self.offset = storage, shape, rows, width, tiled, offset
+        self.exp_pitch = max(1, -(-rows // BLOCK)) if tiled else max(16, -(-rows // 16) * 16)
+        self.exp_offset = offset - (-width // BLOCK) * BLOCK * rows
+
+    @classmethod
+    def _empty(cls, like, shape, rows):
+        """blocks by rows, not yet written, on `like`'s device"""
+        q = cls.__new__(cls)
+        q._set(like.new_empty(cls.bytes_for(rows, shape[-1]), dtype=torch.uint8), shape, rows, False, 0)
+        return q
 
     @staticmethod
     def bytes_for(rows, width, tiled=False):
@@ -84,12 +94,13 @@ class Blocks8:
         """the elements as `dtype` (every one is exact in float32 and bfloat16)"""
         code = _code(dtype, "dequantize")
         dev = self.device
-        out = torch.empty(self.shape, device=dev, dtype=dtype)
+        out = self.storage.new_empty(self.shape, dtype=dtype)
         v, e = self._addresses()
         with _lib.on_device(dev):
             rc = _lib.lib().vmf_blocks8_dequantize(v, e, self.exp_pitch, self.tiled, out.data_ptr(), self.rows,
                                                    self.width, code, _lib.raw_stream(dev))
-        _lib.check(rc, "vmf_blocks8_dequantize")
+        if rc:
+            _lib.check(rc, "vmf_blocks8_dequantize")
         return out
 
     def __repr__(self):
@@ -140,12 +151,13 @@ def _width(x, what):
 def _quantize(x, act, beta, code, dev):
     rows, stride = _lib.as_rows(x.detach())
     n, width = rows.shape
-    q = Blocks8(torch.empty(Blocks8.bytes_for(n, width), device=dev, dtype=torch.uint8), x.shape)
+    q = Blocks8._empty(x, x.shape, n)
     v, e = q._addresses()
     with _lib.on_device(dev):
         rc = _lib.lib().vmf_blocks8_quantize(rows.data_ptr(), stride, v, e, q.exp_pitch, n, width, act, beta, code,
                                              _lib.raw_stream(dev))
-    _lib.check(rc, "vmf_blocks8_quantize")
+    if rc:
+        _lib.check(rc, "vmf_blocks8_quantize")
     return q
 
 
@@ -184,11 +196,11 @@ def quantize_weight(w, transpose=True):
 def _matmul(a, b, bias, gate, beta, dtype, dev):
     m, n, k = a.rows, b.rows, a.width
     code = _lib.FLOAT_CODES[dtype]
-    out = torch.empty(a.shape[:-1] + (n,), device=dev, dtype=dtype)
+    out = a.storage.new_empty(a.shape[:-1] + (n,), dtype=dtype)
     lib = _lib.lib()
     need = C.c_int64(0)
     _lib.check(lib.vmf_blocks8_matmul_workspace(m, n, k, code, need), "vmf_blocks8_matmul_workspace")
-    ws = torch.empty(need.value, device=dev, dtype=torch.uint8) if need.value else None
+    ws = a.storage.new_empty(need.value) if need.value else None
     av, ae = a._addresses()
     bv, be = b._addresses()
     gv, ge = gate._addresses() if gate is not None else (None, None)
@@ -197,7 +209,8 @@ def _matmul(a, b, bias, gate, beta, dtype, dev):
                                     _lib.FLOAT_CODES[bias.dtype] if bias is not None else 0, gv, ge,
                                     gate.exp_pitch if gate is not None else 0, beta, out.data_ptr(), m, n, k,
                                     _lib.address(ws), need.value, code, _lib.raw_stream(dev))
-    _lib.check(rc, "vmf_blocks8_matmul")
+    if rc:
+        _lib.check(rc, "vmf_blocks8_matmul")
     return out
 
 
@@ -228,12 +241,13 @@ def softplus_grad(g, q, beta=1.0):
         raise ValueError(f"softplus_grad: shapes {tuple(g.shape)} and {tuple(q.shape)}")
     dev = _lib.require_hip(g, q.storage)
     rows, stride = _lib.as_rows(g.detach())
-    out = torch.empty(g.shape, device=dev, dtype=g.dtype)
+    out = torch.empty_like(g, memory_format=torch.contiguous_format)
     v, e = q._addresses()
     with _lib.on_device(dev):
         rc = _lib.lib().vmf_blocks8_softplus_grad(rows.data_ptr(), stride, v, e, q.exp_pitch, out.data_ptr(), q.rows,
                                                   q.width, beta, code, _lib.raw_stream(dev))
-    _lib.check(rc, "vmf_blocks8_softplus_grad")
+    if rc:
+        _lib.check(rc, "vmf_blocks8_softplus_grad")
     return out
 
 
@@ -241,19 +255,20 @@ def _weight_grad(g, q, bias, dtype, dev):
     rows, stride = _lib.as_rows(g.detach())
     m, n = rows.shape
     k = q.width
-    gw = torch.empty((n, k), device=dev, dtype=dtype)
-    gb = torch.empty(n, device=dev, dtype=dtype) if bias else None
+    gw = g.new_empty((n, k), dtype=dtype)
+    gb = g.new_empty(n, dtype=dtype) if bias else None
     lib = _lib.lib()
     need = C.c_int64(0)
     code = _lib.FLOAT_CODES[g.dtype]
     _lib.check(lib.vmf_blocks8_weight_grad_workspace(m, n, k, code, need), "vmf_blocks8_weight_grad_workspace")
-    ws = torch.empty(need.value, device=dev, dtype=torch.uint8) if need.value else None
+    ws = q.storage.new_empty(need.value) if need.value else None
     v, e = q._addresses()
     with _lib.on_device(dev):
         rc = lib.vmf_blocks8_weight_grad(rows.data_ptr(), stride, v, e, q.exp_pitch, gw.data_ptr(), _lib.address(gb), None,
                                          None, 0, m, n, k, _lib.address(ws), need.value, code, _lib.FLOAT_CODES[dtype],
                                          _lib.raw_stream(dev))
-    _lib.check(rc, "vmf_blocks8_weight_grad")
+    if rc:
+        _lib.check(rc, "vmf_blocks8_weight_grad")
     return gw, gb
 
 
