@@ -67,9 +67,9 @@ __device__ __forceinline__ void store_some(T* p, int64_t left, const A* in) {
   }
 }
 
-// Reductions over groups of G consecutive lanes (G a power of two, 16 .. 64), the same bits in every lane: inside 16 lanes
-// by rotations in the vector unit (a rotation by half the distance left pairs every lane with one whose sum is over the
-// complementary lanes), across them through the LDS crossbar.
+// Reductions over groups of G consecutive lanes (G a power of two, 16 .. 64), the same bits in every lane, in the vector
+// unit: inside 16 lanes by rotations (a rotation by half the distance left pairs every lane with one whose sum is over the
+// complementary lanes), across them by swaps of 16 and of 32 lanes.
 template <int N, typename A>
 __device__ __forceinline__ A rotated16(A v) {
   if constexpr (sizeof(A) == 4) {
@@ -91,14 +91,44 @@ __device__ __forceinline__ A rotated16(A v) {
     return u.a;
   }
 }
+// The values of the lower and the upper N lanes (N: 16 or 32) of each 2 N: both of them in all 2 N lanes.
+template <int N>
+__device__ __forceinline__ void halves32(uint32_t v, uint32_t& lower, uint32_t& upper) {
+  typedef unsigned pair __attribute__((ext_vector_type(2)));
+  pair r;
+  if constexpr (N == 16) r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  else r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  lower = r[0];
+  upper = r[1];
+}
+template <int N, typename A>
+__device__ __forceinline__ void halves(A v, A& lower, A& upper) {
+  constexpr int W = (int)sizeof(A) / 4;
+  union {
+    A a;
+    uint32_t w[W];
+  } in, lo, hi;
+  in.a = v;
+#pragma unroll
+  for (int i = 0; i < W; ++i) halves32<N>(in.w[i], lo.w[i], hi.w[i]);
+  lower = lo.a;
+  upper = hi.a;
+}
 template <int G, typename A>
 __device__ __forceinline__ A lane_sum(A v) {
   v += rotated16<8>(v);
   v += rotated16<4>(v);
   v += rotated16<2>(v);
   v += rotated16<1>(v);
-#pragma unroll
-  for (int o = 16; o < G; o <<= 1) v += __shfl_xor(v, o, 64);
+  A lower, upper;
+  if constexpr (G > 16) {
+    halves<16>(v, lower, upper);
+    v = lower + upper;
+  }
+  if constexpr (G > 32) {
+    halves<32>(v, lower, upper);
+    v = lower + upper;
+  }
   return v;
 }
 template <typename A>
@@ -109,7 +139,14 @@ __device__ __forceinline__ A lane_max(A v) {
   v = larger(v, rotated16<4>(v));
   v = larger(v, rotated16<2>(v));
   v = larger(v, rotated16<1>(v));
-#pragma unroll
-  for (int o = 16; o < G; o <<= 1) v = larger(v, (A)__shfl_xor(v, o, 64));
+  A lower, upper;
+  if constexpr (G > 16) {
+    halves<16>(v, lower, upper);
+    v = larger(lower, upper);
+  }
+  if constexpr (G > 32) {
+    halves<32>(v, lower, upper);
+    v = larger(lower, upper);
+  }
   return v;
 }
