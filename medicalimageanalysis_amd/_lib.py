@@ -4,6 +4,7 @@ There is no CPU fallback: a missing library, a failed call or a tensor that is n
 raises.  PyTorch supplies device memory and the current stream; every kernel is in the .so.
 """
 import ctypes as C
+import functools
 import os
 import threading
 
@@ -225,6 +226,14 @@ def ptr(t):
 
 def stream_ptr(device):
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+@functools.lru_cache(maxsize=1024)
+def workspace_bytes(entry, *sizes):
+    """the answer of a `..._workspace` entry point, which hangs on the sizes alone"""
+    need = C.c_int64(0)
+    check(getattr(lib(), entry)(*sizes, need), entry)
+    return need.value
 
 
 def first_order(backward):

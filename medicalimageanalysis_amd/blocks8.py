@@ -19,8 +19,6 @@ bfloat16 ones from the faster 8-bit matrix instruction (1.3e-5 relative, a hundr
 infinities are NaN in blocks.  Only linear takes part in autograd: the other functions' results carry no gradient.  There
 is no CPU path.
 """
-import ctypes as C
-
 import torch
 
 from . import _lib
@@ -198,9 +196,8 @@ def _matmul(a, b, bias, gate, beta, dtype, dev):
     code = _lib.FLOAT_CODES[dtype]
     out = a.storage.new_empty(a.shape[:-1] + (n,), dtype=dtype)
     lib = _lib.lib()
-    need = C.c_int64(0)
-    _lib.check(lib.vmf_blocks8_matmul_workspace(m, n, k, code, need), "vmf_blocks8_matmul_workspace")
-    ws = a.storage.new_empty(need.value) if need.value else None
+    need = _lib.workspace_bytes("vmf_blocks8_matmul_workspace", m, n, k, code)
+    ws = a.storage.new_empty(need) if need else None
     av, ae = a._addresses()
     bv, be = b._addresses()
     gv, ge = gate._addresses() if gate is not None else (None, None)
@@ -208,7 +205,7 @@ def _matmul(a, b, bias, gate, beta, dtype, dev):
         rc = lib.vmf_blocks8_matmul(av, ae, a.exp_pitch, a.tiled, bv, be, b.exp_pitch, b.tiled, _lib.address(bias),
                                     _lib.FLOAT_CODES[bias.dtype] if bias is not None else 0, gv, ge,
                                     gate.exp_pitch if gate is not None else 0, beta, out.data_ptr(), m, n, k,
-                                    _lib.address(ws), need.value, code, _lib.raw_stream(dev))
+                                    _lib.address(ws), need, code, _lib.raw_stream(dev))
     if rc:
         _lib.check(rc, "vmf_blocks8_matmul")
     return out
@@ -258,14 +255,13 @@ def _weight_grad(g, q, bias, dtype, dev):
     gw = g.new_empty((n, k), dtype=dtype)
     gb = g.new_empty(n, dtype=dtype) if bias else None
     lib = _lib.lib()
-    need = C.c_int64(0)
     code = _lib.FLOAT_CODES[g.dtype]
-    _lib.check(lib.vmf_blocks8_weight_grad_workspace(m, n, k, code, need), "vmf_blocks8_weight_grad_workspace")
-    ws = q.storage.new_empty(need.value) if need.value else None
+    need = _lib.workspace_bytes("vmf_blocks8_weight_grad_workspace", m, n, k, code)
+    ws = q.storage.new_empty(need) if need else None
     v, e = q._addresses()
     with _lib.on_device(dev):
         rc = lib.vmf_blocks8_weight_grad(rows.data_ptr(), stride, v, e, q.exp_pitch, gw.data_ptr(), _lib.address(gb), None,
-                                         None, 0, m, n, k, _lib.address(ws), need.value, code, _lib.FLOAT_CODES[dtype],
+                                         None, 0, m, n, k, _lib.address(ws), need, code, _lib.FLOAT_CODES[dtype],
                                          _lib.raw_stream(dev))
     if rc:
         _lib.check(rc, "vmf_blocks8_weight_grad")
@@ -292,7 +288,6 @@ def _linear(x, weight, laid_out, bias, act, beta, dev, keep, columns):
     m, k = rows.shape
     code = _lib.FLOAT_CODES[x.dtype]
     lib = _lib.lib()
-    need = C.c_int64(0)
     w = wv = we = kept = wt = base = base_e = tv = te = None
     w_stride = w_code = pitch = 0
     if laid_out is None:
@@ -302,8 +297,7 @@ def _linear(x, weight, laid_out, bias, act, beta, dev, keep, columns):
     else:
         n = laid_out.rows.rows
         wv, we = laid_out.rows._addresses()
-    _lib.check(lib.vmf_blocks8_linear_fwd_workspace(m, n, k, laid_out is not None, keep, code, need),
-               "vmf_blocks8_linear_fwd_workspace")
+    need = _lib.workspace_bytes("vmf_blocks8_linear_fwd_workspace", m, n, k, laid_out is not None, keep, code)
     if keep:
         kp = _up(k, BLOCK)
         pitch = max(16, _up(m, 16))
@@ -316,13 +310,13 @@ def _linear(x, weight, laid_out, bias, act, beta, dev, keep, columns):
         base_e = base + m * kp
         if wt is not None:
             tv, te = base + wt[0], base + wt[1]
-    ws = x.new_empty(need.value, dtype=torch.uint8) if need.value else None
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
     y = x.new_empty(x.shape[:-1] + (n,))
     b = _lib.dense(bias)
     with _lib.on_device(dev):
         rc = lib.vmf_blocks8_linear_fwd(rows.data_ptr(), stride, _lib.address(w), w_stride, w_code, wv, we, tv, te,
                                         _lib.address(b), 0 if b is None else _lib.FLOAT_CODES[b.dtype], act, beta, base,
-                                        base_e, pitch, y.data_ptr(), m, n, k, _lib.address(ws), need.value, code,
+                                        base_e, pitch, y.data_ptr(), m, n, k, _lib.address(ws), need, code,
                                         _lib.raw_stream(dev))
     if rc:
         _lib.check(rc, "vmf_blocks8_linear_fwd")
@@ -331,7 +325,8 @@ def _linear(x, weight, laid_out, bias, act, beta, dev, keep, columns):
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, laid_out, bias, act, beta, dev):
+    def forward(ctx, x, weight, bias, how):
+        laid_out, act, beta, dev = how
         need_x = ctx.needs_input_grad[0]
         if need_x and laid_out is not None and laid_out.columns is None:
             raise ValueError("linear: the laid-out weight has no columns (quantize_weight(..., transpose=True)), which "
@@ -352,7 +347,7 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, gy):
         kept, other = ctx.saved_tensors
         shape, (m, n, k), wt, act, beta, w_dtype, bias_dtype, dev = ctx.meta
-        need_x, need_w, _, need_b = ctx.needs_input_grad[:4]
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
         code = _lib.FLOAT_CODES[gy.dtype]
         # the weight's gradient in the weight's type; a bias beside a laid-out weight has float32 sums
         out = w_dtype or torch.float32
@@ -360,9 +355,8 @@ class _Linear(torch.autograd.Function):
         gw = gy.new_empty((n, k), dtype=out) if need_w or need_b else None
         gb = gy.new_empty(n, dtype=out) if need_b else None
         lib = _lib.lib()
-        need = C.c_int64(0)
-        _lib.check(lib.vmf_blocks8_linear_bwd_workspace(m, n, k, code, need), "vmf_blocks8_linear_bwd_workspace")
-        ws = gy.new_empty(need.value, dtype=torch.uint8)
+        need = _lib.workspace_bytes("vmf_blocks8_linear_bwd_workspace", m, n, k, code)
+        ws = gy.new_empty(need, dtype=torch.uint8)
         g, stride = _lib.as_rows(gy)
         base = kept.data_ptr()
         tv = te = None
@@ -372,12 +366,12 @@ class _Linear(torch.autograd.Function):
         with _lib.on_device(dev):
             rc = lib.vmf_blocks8_linear_bwd(g.data_ptr(), stride, base, base + m * _up(k, BLOCK), max(16, _up(m, 16)), tv,
                                             te, act, beta, _lib.address(gx), _lib.address(gw), _lib.address(gb), m, n, k,
-                                            ws.data_ptr(), need.value, code, _lib.FLOAT_CODES[out], _lib.raw_stream(dev))
+                                            ws.data_ptr(), need, code, _lib.FLOAT_CODES[out], _lib.raw_stream(dev))
         if rc:
             _lib.check(rc, "vmf_blocks8_linear_bwd")
         if gb is not None and gb.dtype != bias_dtype:
             gb = gb.to(bias_dtype)
-        return gx, gw if need_w else None, None, gb, None, None, None
+        return gx, gw if need_w else None, gb, None
 
 
 def linear(x, weight, bias=None, activation=None, beta=1.0):
@@ -402,5 +396,5 @@ def linear(x, weight, bias=None, activation=None, beta=1.0):
     tensor = weight if laid_out is None else None
     if torch.is_grad_enabled() and (x.requires_grad or (tensor is not None and tensor.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
-        return _Linear.apply(x, tensor, laid_out, bias, act, beta, dev)
+        return _Linear.apply(x, tensor, bias, (laid_out, act, beta, dev))
     return _linear(x, tensor, laid_out, bias, act, beta, dev, False, False)[0]

@@ -7,8 +7,6 @@ float16 or bfloat16, the weight and the bias of the same type or, with 16-bit ro
 in 32 bits (64 for float64 rows).  x may be any view whose last dimension is dense and whose rows have one stride; other
 views are copied.  There is no CPU path.
 """
-import ctypes as C
-
 import torch
 
 from . import _lib
@@ -60,7 +58,8 @@ def _forward(x, w, b, eps, dev, code, wcode, keep):
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps, dev, code, wcode):
+    def forward(ctx, x, weight, bias, how):
+        eps, dev, code, wcode = how
         y, rows, stride, w, stats = _forward(x, weight, bias, eps, dev, code, wcode, True)
         ctx.save_for_backward(rows, w, stats)
         ctx.meta = (rows.shape, stride, code, wcode, dev, None if bias is None else bias.dtype)
@@ -76,21 +75,20 @@ class _LayerNorm(torch.autograd.Function):
         gx = torch.empty_like(gy, memory_format=torch.contiguous_format) if need_x else None
         gw = torch.empty_like(w) if need_w else None
         gb = rows.new_empty(width, dtype=b_dtype) if need_b else None
-        lib = _lib.lib()
-        ws, need = None, C.c_int64(0)
+        ws, need = None, 0
         if need_w or need_b:
-            _lib.check(lib.vmf_layer_norm_bwd_workspace(n, width, code, need), "vmf_layer_norm_bwd_workspace")
-            if need.value:
-                ws = torch.empty(need.value, device=dev, dtype=torch.uint8)
+            need = _lib.workspace_bytes("vmf_layer_norm_bwd_workspace", n, width, code)
+            if need:
+                ws = rows.new_empty(need, dtype=torch.uint8)
         mean = stats.data_ptr()
         with _lib.on_device(dev):
-            rc = lib.vmf_layer_norm_bwd(rows.data_ptr(), x_stride, g.data_ptr(), g_stride, _lib.address(w), mean,
-                                        mean + n * (8 if code == _lib.VMF_F64 else 4), _lib.address(gx),
-                                        _lib.address(gw), _lib.address(gb), n, width, _lib.address(ws), need.value, code,
-                                        wcode, _lib.raw_stream(dev))
+            rc = _lib.lib().vmf_layer_norm_bwd(rows.data_ptr(), x_stride, g.data_ptr(), g_stride, _lib.address(w), mean,
+                                               mean + n * (8 if code == _lib.VMF_F64 else 4), _lib.address(gx),
+                                               _lib.address(gw), _lib.address(gb), n, width, _lib.address(ws), need, code,
+                                               wcode, _lib.raw_stream(dev))
         if rc:
             _lib.check(rc, "vmf_layer_norm_bwd")
-        return gx, gw, gb, None, None, None, None
+        return gx, gw, gb, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -99,7 +97,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     eps = float(eps)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
-        return _LayerNorm.apply(x, weight, bias, eps, dev, code, wcode)
+        return _LayerNorm.apply(x, weight, bias, (eps, dev, code, wcode))
     return _forward(x, weight, bias, eps, dev, code, wcode, False)[0]
 
 
