@@ -453,7 +453,8 @@ struct BwdPlan {
   int threads;  // of a workgroup
   int parts;    // workgroups, each leaving a partial row of gw and gb; 0: none are left (few rows)
 };
-// Few rows (up to 512, rows of up to 256 lanes): one launch (512x784 fp32 4.1 us, with partials 7.5; 2048x784 17.2 and 10.0).
+// Few rows (up to 1024, rows of up to 256 lanes): one launch (128x128 fp32 3.1 us, with partials 8.9; 1024x784 7.8 and 8.6;
+// 1536x784 12.7 and 9.5).
 // Otherwise two workgroups for each of 256 compute units (1048576x784 fp32, a wave to a row, 1.88 ms, with four 2.00), four
 // where the other waves have more to fill: rows of 16 bits, whose loads are half as many (1048576x784 bf16 1.14 ms, with two
 // 1.88), and rows of four waves, which wait at barriers (65536x4096 bf16 0.33 ms, with two 0.50).  No more than have 32
@@ -465,7 +466,7 @@ BwdPlan bwd_plan(int64_t n, int64_t width) {
   BwdPlan p;
   p.tpr = lanes_for((width + V - 1) / V, bwd_chunks<T>());
   p.threads = p.tpr == 0 ? 256 : p.tpr > THREADS ? p.tpr : THREADS;
-  if (p.tpr != 0 && p.tpr <= THREADS && n <= 512) {
+  if (p.tpr != 0 && p.tpr <= THREADS && n <= 1024) {
     p.parts = 0;
     return p;
   }

@@ -88,7 +88,7 @@ def test_widths(width, dtype):
     check(*data(n, width, dtype, seed=width))
 
 
-@pytest.mark.parametrize("n", [1, 2, 3, 15, 16, 513, 20000])
+@pytest.mark.parametrize("n", [1, 2, 3, 15, 16, 513, 1025, 20000])
 @pytest.mark.parametrize("width,dtype", [(96, torch.float32), (300, torch.bfloat16), (5000, torch.float16)])
 def test_row_counts(n, width, dtype):
     check(*data(n, width, dtype, seed=n))

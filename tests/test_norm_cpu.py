@@ -43,7 +43,7 @@ def test_c_entry_refusals():
     assert fwd(4, 8, x=None) == -1 and fwd(4, 8, mean=p) == -1
     assert fwd(0, 8, x=None) == 0
     nb = C.c_int64(-1)
-    assert lib.vmf_layer_norm_bwd_workspace(1000, 128, 0, C.byref(nb)) == 0 and nb.value > 0
-    assert lib.vmf_layer_norm_bwd_workspace(1000, 128, 0, None) == -1
-    rc = lib.vmf_layer_norm_bwd(p, 128, p, 128, None, p, p, None, p, None, 1000, 128, p, nb.value - 1, 0, 0, None)
+    assert lib.vmf_layer_norm_bwd_workspace(10000, 128, 0, C.byref(nb)) == 0 and nb.value > 0
+    assert lib.vmf_layer_norm_bwd_workspace(10000, 128, 0, None) == -1
+    rc = lib.vmf_layer_norm_bwd(p, 128, p, 128, None, p, p, None, p, None, 10000, 128, p, nb.value - 1, 0, 0, None)
     assert rc == -1 and b"workspace" in lib.vmf_last_error_string()
