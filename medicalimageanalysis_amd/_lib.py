@@ -159,6 +159,16 @@ def as_rows(t):
     return r, (r.stride(0) if n > 1 else width)
 
 
+def unpacked(t, dtype, shape, device):
+    """A saved tensor as autograd hands it back.  Saved-tensor hooks (torch.autograd.graph.save_on_cpu among them) may give
+    it another layout, so strides are read from it and never remembered; one of another type, shape or device is refused
+    before a kernel gets its address."""
+    if t is not None and (t.dtype != dtype or t.shape != shape or t.device != device):
+        raise RuntimeError(f"a saved tensor came back as {t.dtype} of {tuple(t.shape)} on {t.device}, saved was {dtype} of "
+                           f"{tuple(shape)} on {device}")
+    return t
+
+
 def require_hip(*tensors):
     """Every tensor must live on one HIP device; returns that device."""
     dev = None

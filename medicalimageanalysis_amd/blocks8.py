@@ -339,14 +339,16 @@ class _Linear(torch.autograd.Function):
             other, wt = columns.storage, (columns.offset, columns.exp_offset)
         ctx.save_for_backward(kept, other)
         ctx.meta = (x.shape, sizes, wt, act, beta, None if weight is None else weight.dtype,
-                    None if bias is None else bias.dtype, dev)
+                    None if bias is None else bias.dtype, dev, kept.numel(), 0 if other is None else other.numel())
         return y
 
     @staticmethod
     @_lib.first_order
     def backward(ctx, gy):
         kept, other = ctx.saved_tensors
-        shape, (m, n, k), wt, act, beta, w_dtype, bias_dtype, dev = ctx.meta
+        shape, (m, n, k), wt, act, beta, w_dtype, bias_dtype, dev, kept_bytes, other_bytes = ctx.meta
+        kept = _lib.dense(_lib.unpacked(kept, torch.uint8, (kept_bytes,), dev))
+        other = _lib.dense(_lib.unpacked(other, torch.uint8, (other_bytes,), dev))
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         code = _lib.FLOAT_CODES[gy.dtype]
         # the weight's gradient in the weight's type; a bias beside a laid-out weight has float32 sums

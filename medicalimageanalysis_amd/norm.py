@@ -53,23 +53,28 @@ def _forward(x, w, b, eps, dev, code, wcode, keep):
                                            mean, rstd, n, width, eps, code, wcode, _lib.raw_stream(dev))
     if rc:
         _lib.check(rc, "vmf_layer_norm_fwd")
-    return y, rows, stride, w, stats
+    return y, rows, w, stats
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, how):
         eps, dev, code, wcode = how
-        y, rows, stride, w, stats = _forward(x, weight, bias, eps, dev, code, wcode, True)
+        y, rows, w, stats = _forward(x, weight, bias, eps, dev, code, wcode, True)
         ctx.save_for_backward(rows, w, stats)
-        ctx.meta = (rows.shape, stride, code, wcode, dev, None if bias is None else bias.dtype)
+        ctx.meta = (rows.shape, x.dtype, None if w is None else w.dtype, stats.dtype, code, wcode, dev,
+                    None if bias is None else bias.dtype)
         return y
 
     @staticmethod
     @_lib.first_order
     def backward(ctx, gy):
         rows, w, stats = ctx.saved_tensors
-        (n, width), x_stride, code, wcode, dev, b_dtype = ctx.meta
+        shape, x_dtype, w_dtype, stats_dtype, code, wcode, dev, b_dtype = ctx.meta
+        n, width = shape
+        rows, x_stride = _lib.as_rows(_lib.unpacked(rows, x_dtype, shape, dev))
+        w = _lib.dense(_lib.unpacked(w, w_dtype, (width,), dev))
+        stats = _lib.dense(_lib.unpacked(stats, stats_dtype, (2 * n,), dev))
         g, g_stride = _lib.as_rows(gy)
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         gx = torch.empty_like(gy, memory_format=torch.contiguous_format) if need_x else None

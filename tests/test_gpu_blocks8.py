@@ -475,3 +475,16 @@ def test_offsets_beyond_32_bits():
     gw, gb = blocks8.weight_grad(g, q)
     want = g[-9:].double().t() @ qt.dequantize().double()
     assert ((gw.double() - want).abs() <= 64 * 2.0 ** -24 * (g[-9:].abs().double().t() @ qt.dequantize().abs().double())).all()
+
+
+def test_linear_with_saved_tensors_moved_to_the_host_and_back():
+    x, w, b, gy = normal(70, 300, seed=1), normal(40, 300, seed=2), normal(40, seed=3), normal(70, 40, seed=4)
+    for weight in (w, blocks8.quantize_weight(w)):
+        leaves = [t.requires_grad_() for t in (x.clone(), w.clone(), b.clone())]
+        args = (leaves[0], leaves[1] if weight is w else weight, leaves[2], "softplus")
+        wanted = leaves if weight is w else leaves[::2]
+        want = torch.autograd.grad(blocks8.linear(*args), wanted, gy)
+        with torch.autograd.graph.save_on_cpu():
+            y = blocks8.linear(*args)
+        for p, q in zip(torch.autograd.grad(y, wanted, gy), want):
+            assert torch.equal(p, q)

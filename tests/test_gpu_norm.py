@@ -200,3 +200,17 @@ def test_offsets_beyond_32_bits():
     x[-8:] = tail
     y = norm.layer_norm(x)
     assert torch.equal(y[-8:], norm.layer_norm(tail)) and not y[:4].any()
+
+
+@pytest.mark.parametrize("n,width", [(40, 128), (2000, 300), (6, 40000)])
+def test_saved_tensors_moved_to_the_host_and_back(n, width):
+    """save_on_cpu returns the rows of a wider tensor as a dense one, with another row stride"""
+    x, w, b, gy = data(n, width, torch.float32, seed=n)
+    wide = torch.full((n, 2 * width), 3.0, device=DEV)
+    wide[:, :width] = x
+    leaves = [t.detach().requires_grad_() for t in (wide[:, :width], w, b)]
+    want = torch.autograd.grad(norm.layer_norm(*leaves), leaves, gy)
+    with torch.autograd.graph.save_on_cpu():
+        y = norm.layer_norm(*leaves)
+    for p, q in zip(torch.autograd.grad(y, leaves, gy), want):
+        assert torch.equal(p, q)

@@ -47,3 +47,66 @@ def test_c_entry_refusals():
     assert lib.vmf_layer_norm_bwd_workspace(10000, 128, 0, None) == -1
     rc = lib.vmf_layer_norm_bwd(p, 128, p, 128, None, p, p, None, p, None, 10000, 128, p, nb.value - 1, 0, 0, None)
     assert rc == -1 and b"workspace" in lib.vmf_last_error_string()
+
+
+class _Recorder:
+    """in the library's place: every call succeeds, the backward call's arguments are kept"""
+
+    def __init__(self):
+        self.bwd = None
+
+    def vmf_layer_norm_fwd(self, *args):
+        return 0
+
+    def vmf_layer_norm_bwd(self, *args):
+        self.bwd = args
+        return 0
+
+
+@pytest.fixture
+def recorder(monkeypatch):
+    r = _Recorder()
+    monkeypatch.setattr(_lib, "lib", lambda: r)
+    monkeypatch.setattr(_lib, "require_hip", lambda *tensors: torch.device("cpu"))
+    monkeypatch.setattr(_lib, "raw_stream", lambda dev: 0)
+    monkeypatch.setattr(_lib, "workspace_bytes", lambda *sizes: 64)
+    return r
+
+
+def _backward_under(unpack, x):
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        y = norm.layer_norm(x, torch.ones(x.shape[-1]), None)
+    return torch.autograd.grad(y, x, torch.ones_like(y))
+
+
+@pytest.mark.parametrize("rows,wide,width", [(40, 256, 128), (7, 5, 5), (1, 9, 4)])
+def test_backward_reads_the_row_stride_of_the_tensor_that_a_hook_returns(recorder, rows, wide, width):
+    """torch.autograd.graph.save_on_cpu gives a strided view back as a dense tensor; another hook may do the opposite"""
+    returned = {}
+
+    def dense(t):
+        if t.dim() == 2:
+            t = returned["x"] = t.clone(memory_format=torch.contiguous_format)
+        return t
+
+    def strided(t):
+        if t.dim() == 2:
+            out = torch.zeros(t.shape[0], t.shape[1] + 3, dtype=t.dtype)
+            out[:, 1:1 + t.shape[1]] = t
+            t = returned["x"] = out[:, 1:1 + t.shape[1]]
+        return t
+
+    for hook in (dense, strided):
+        x = torch.randn(rows, wide)[:, :width].requires_grad_()
+        _backward_under(hook, x)
+        assert recorder.bwd[0] == returned["x"].data_ptr()
+        if rows > 1:
+            assert recorder.bwd[1] == returned["x"].stride(0)
+
+
+@pytest.mark.parametrize("wrong", [lambda t: t.double(), lambda t: t[:-1], lambda t: t.to("meta")])
+def test_backward_refuses_a_hook_that_returns_another_tensor(recorder, wrong):
+    x = torch.randn(6, 8, requires_grad=True)
+    with pytest.raises(RuntimeError, match="saved tensor came back"):
+        _backward_under(wrong, x)
+    assert recorder.bwd is None
