@@ -79,8 +79,10 @@ __device__ __forceinline__ float softplus_margin(float h, float beta) {
   return fmaf(__builtin_amdgcn_fmed3f(-beta * h, 0.0f, 88.0f), 2e-7f, 8e-7f);
 }
 
-// exp in 64 bits: t = n ln 2 + r, |r| <= 0.35, and the power series of exp(r) to r^13 (the next term is under 5e-18)
+// exp in 64 bits, t <= 1: t = n ln 2 + r, |r| <= 0.35, and the power series of exp(r) to r^13 (the next term is under
+// 5e-18).  Below -1000, down to -inf, it is 0; n ln 2 would leave no digits of r there.
 __device__ __forceinline__ double exp64(double t) {
+  t = ::fmax(t, -1000.0);
   const double n = ::rint(t * 1.4426950408889634);
   const double r = ::fma(-n, 2.3190468138462996e-17, ::fma(-n, 0.69314718055994531, t));
   double s = 1.0 / 6227020800.0;
@@ -97,7 +99,7 @@ __device__ __forceinline__ double exp64(double t) {
   s = ::fma(s, r, 0.5);
   s = ::fma(s, r, 1.0);
   s = ::fma(s, r, 1.0);
-  return ::ldexp(s, n < -1100 ? -1100 : (int)n);
+  return ::ldexp(s, (int)n);
 }
 // softplus to 40 bits and more, for the few values that lie next to a rounding border (see softplus8).
 // l = log(1 + u), u = exp(-|t|): for small u its series; else from the 32-bit l0, with d = (1 + u) exp(-l0) - 1 under 1e-5,

@@ -488,3 +488,31 @@ def test_linear_with_saved_tensors_moved_to_the_host_and_back():
             y = blocks8.linear(*args)
         for p, q in zip(torch.autograd.grad(y, wanted, gy), want):
             assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width", [100, 128, 300])
+@pytest.mark.parametrize("beta", [1.0, 0.3])
+def test_softplus_blocks_of_the_largest_exponent(beta, width, dtype):
+    """in them every element takes the 64-bit path: minus infinity and large negative numbers are 0, so is the padding"""
+    x = normal(4, width, seed=3, scale=1e38).clamp(-3e38, 3e38)
+    x[:, 0] = 2.5e38
+    x[0, 1:4] = torch.tensor([-math.inf, -3e38, -1e3])
+    x = x.to(dtype)
+    q = blocks8.quantize(x, "softplus", beta)
+    want = by_blocks(softplus(x, beta))
+    assert int(q.exponents[0, 0]) == 119 + 127 and torch.equal(q.dequantize().double(), want)
+    assert not q.values[:, width:].any()
+    ones = blocks8.Blocks8(torch.full_like(q.storage, 0x38), q.shape)  # every value 1, behind the width too
+    ones.exponents.fill_(127 - 100)
+    near(blocks8.matmul(q, ones), want.sum(1, keepdim=True).expand(4, 4) * 2.0 ** -100,
+         want.sum(1, keepdim=True).expand(4, 4) * 2.0 ** -100, width)
+
+
+def test_linear_of_few_rows_through_blocks_of_the_largest_exponent():
+    """the one-launch form quantises for itself"""
+    x = normal(3, 200, seed=3)
+    x[1, 5], x[1, 6], x[1, 150] = 2.5e38, -math.inf, -2e38
+    w8 = blocks8.quantize_weight(normal(20, 200, seed=4, scale=1e-4))
+    a, w = by_blocks(softplus(x, 1.0)), w8.rows.dequantize().double()
+    near(blocks8.linear(x, w8, None, "softplus"), a @ w.t(), a.abs() @ w.abs().t(), 208)
