@@ -322,8 +322,8 @@ int vmf_layer_norm_bwd(const void* x, int64_t x_stride, const void* gy, int64_t 
 #define VMF_BLOCKS8_MAX_ROWS ((int64_t)1 << 26)
 #define VMF_BLOCKS8_MAX_WIDTH ((int64_t)1 << 22)
 enum vmf_activation { VMF_ACT_NONE = 0, VMF_ACT_SOFTPLUS = 1 };
-/* blocks of x, or of softplus(x) = log(1 + exp(beta x)) / beta: the bytes of its exact value, whatever x's type (values
- * below 2^-126 / beta may count as 0) */
+/* blocks of x, or of softplus(x) = log(1 + exp(beta x)) / beta: the bytes of its value in 64 bits, whatever x's type (where
+ * that is the middle of two 8-bit values to 2^-40, either of them; values below 2^-126 / beta may count as 0) */
 int vmf_blocks8_quantize(const void* x, int64_t x_stride, uint8_t* values, uint8_t* exponents, int64_t exp_pitch,
                          int64_t rows, int64_t width, int activation, double beta, int dtype, vmf_stream_t stream);
 /* tiles of w (rows, width), and the same tiles of its transpose (both or neither of values_t, exponents_t) */

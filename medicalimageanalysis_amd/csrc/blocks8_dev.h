@@ -161,7 +161,8 @@ static __device__ __noinline__ float softplus_scaled(float x, double beta, int e
 
 // The block of softplus(h).  Which of two neighbouring 8-bit values is nearest to softplus(h) can hang on its last bits,
 // so a value is computed in 32 bits, and once more in 64 where its 32-bit error could change the result (some twenty of
-// a million; of 16-bit inputs, which repeat, it can be more): the bytes are those of the exactly computed softplus.
+// a million; of 16-bit inputs, which repeat, it can be more): the bytes are those of the softplus computed in 64 bits.  (A large
+// h is its own softplus, and as the middle of two 8-bit values goes to either: beta h / beta is h but for its last bit.)
 __device__ __forceinline__ uint2 softplus8(const float (&h)[8], float beta, float inv_beta, double beta64, int& e_out) {
   constexpr float INF = __builtin_inff();
   // softplus grows with h: the block's largest comes from the largest h.  As integers the bits of floats order like them
@@ -177,7 +178,9 @@ __device__ __forceinline__ uint2 softplus8(const float (&h)[8], float beta, floa
     for (int i = 0; i < 8; ++i) top = h[i] < INF && h[i] > top ? h[i] : top;  // (neither infinity nor NaN)
     top = lane_max<16>(top);
   }
-  const float at = softplus32(top, beta, inv_beta), mt = softplus_margin(top, beta);
+  float at = softplus32(top, beta, inv_beta);
+  if (!(at < INF)) at = top;  // beta h is beyond 32 bits, softplus(h) is h to its last bit
+  const float mt = softplus_margin(top, beta);
   const float most32 = 3.4e38f;
   int e = b8_exponent(at < most32 ? at * (1.0f - mt) : most32);
   const int above = b8_exponent(at < most32 ? at * (1.0f + mt) : most32);
@@ -185,6 +188,8 @@ __device__ __forceinline__ uint2 softplus8(const float (&h)[8], float beta, floa
   if (top == -INF) e = 0;
   e_out = e;
   const float scale = inv_beta * b8_pow2(-e);
+  // (beta h or, with a small beta, 2^-e / beta may be beyond 32 bits where the elements are not)
+  const bool exact = e == B8_EMAX || !(larger(beta * top, scale) < INF);
   float lo[8], hi[8], least = h[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) least = fminf(least, h[i]);
@@ -197,11 +202,11 @@ __device__ __forceinline__ uint2 softplus8(const float (&h)[8], float beta, floa
   }
   uint32_t w[2] = {b8_pack4(lo), b8_pack4(lo + 4)};
   const uint32_t x[2] = {w[0] ^ b8_pack4(hi), w[1] ^ b8_pack4(hi + 4)};
-  if ((x[0] | x[1]) != 0 || e == B8_EMAX) {
+  if ((x[0] | x[1]) != 0 || exact) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int at = 8 * (i & 3);
-      if ((x[i >> 2] >> at & 0xff) != 0 || e == B8_EMAX) {
+      if ((x[i >> 2] >> at & 0xff) != 0 || exact) {
         const float v = softplus_scaled(h[i], beta64, e);
         w[i >> 2] = (w[i >> 2] & ~(0xffu << at)) | (b8_pack2(v, v) & 0xff) << at;
       }

@@ -516,3 +516,38 @@ def test_linear_of_few_rows_through_blocks_of_the_largest_exponent():
     w8 = blocks8.quantize_weight(normal(20, 200, seed=4, scale=1e-4))
     a, w = by_blocks(softplus(x, 1.0)), w8.rows.dequantize().double()
     near(blocks8.linear(x, w8, None, "softplus"), a @ w.t(), a.abs() @ w.abs().t(), 208)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("beta,top", [(7.5, 5e37), (7.5, 3.3e38), (3.0, 1.2e38), (1.5, 3.4e38), (1e6, 1e33), (1e6, 5e32),
+                                      (1e30, 1e9), (1e30, 4e8), (1e30, 3e38)])
+def test_softplus_where_beta_times_the_value_exceeds_float32(beta, top, dtype):
+    x = torch.linspace(-1, 1, 3 * 200, device=DEV).view(3, 200) * top
+    x[0, 3], x[1, 4], x[1, 5], x[2, :128] = top, -math.inf, top / 300, -top / beta
+    x[2, 7] = top / 1000
+    x = x.to(dtype)
+    q = blocks8.quantize(x, "softplus", beta)
+    exact = softplus(x, beta)
+    # Softplus of these large values is the value itself, and many are the middle of two 8-bit values: (x beta) / beta in
+    # 64 bits, a product by 1 / beta in torch, is up to 2^-51 off x to either side, so either neighbour is right there.
+    got, low, high = q.dequantize().double(), by_blocks(exact * (1 - 2.0 ** -50)), by_blocks(exact * (1 + 2.0 ** -50))
+    kept = torch.where(got == low, low, high)
+    assert same(got, kept) and same(low.isnan(), exact.isinf())  # (3.4e38 is infinite in bfloat16)
+    finite = torch.where(exact.isfinite(), exact, torch.zeros_like(exact))
+    tops = torch.stack([finite[:, :128].amax(1), finite[:, 128:].amax(1)])
+    assert torch.equal(q.exponents[:, :3].long() - 127, exponent(tops).long())
+    assert not q.values[:, 200:].any()
+    w8 = blocks8.quantize_weight(normal(20, 200, seed=4, scale=1.0 / top))
+    rows = exact.isfinite().all(1)
+    a, w = kept[rows], w8.rows.dequantize().double()
+    near(blocks8.linear(x.float(), w8, None, "softplus", beta)[rows], a @ w.t(), a.abs() @ w.abs().t(), 208)
+
+
+@pytest.mark.parametrize("beta", [1e-5, 3e-6, 1e-6, 1e-20, 1e-30])
+def test_softplus_of_very_small_results_with_a_small_beta(beta):
+    """2^-e / beta exceeds float32 in these blocks"""
+    x = torch.full((2, 150), -86.5, device=DEV)
+    x[0, 1], x[0, 2], x[0, 3], x[1, 130] = -84.0, -200.0, -math.inf, -87.0
+    x = (x.double() / beta).float()
+    q = blocks8.quantize(x, "softplus", beta)
+    assert torch.equal(q.dequantize().double(), by_blocks(softplus(x, beta))) and not q.values[:, 150:].any()
