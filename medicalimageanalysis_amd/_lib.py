@@ -9,6 +9,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -244,6 +245,19 @@ def workspace_bytes(entry, *sizes):
     need = C.c_int64(0)
     check(getattr(lib(), entry)(*sizes, need), entry)
     return need.value
+
+
+def differentiated(*tensors):
+    """Whether a call on these tensors goes through its autograd Function: a gradient is wanted of one of them, or
+    forward-mode derivatives are being taken (a dual tensor has no requires_grad; the Function refuses it, where the call
+    without one would drop its tangent)."""
+    if forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def first_order(backward):

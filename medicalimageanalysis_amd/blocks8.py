@@ -16,8 +16,8 @@ operand of the next layer's product and as the checkpoint that the backward pass
 linear's gradients: gx = (blocks(gy) tiles(weight)) * softplus slope, gw = gy^T blocks(activation(x)), gb = the sum of
 gy's rows; the roundings to 8 bits pass their gradient on as it is.  float32 results come from 32-bit sums, float16 and
 bfloat16 ones from the faster 8-bit matrix instruction (1.3e-5 relative, a hundredth of their own rounding).  NaN and
-infinities are NaN in blocks.  Only linear takes part in autograd: the other functions' results carry no gradient.  There
-is no CPU path.
+infinities are NaN in blocks.  Only linear takes part in autograd, backwards (forward-mode derivatives are refused): the
+other functions' results carry no gradient.  There is no CPU path.
 """
 import torch
 
@@ -396,7 +396,6 @@ def linear(x, weight, bias=None, activation=None, beta=1.0):
     _check_bias(bias, n, "linear")
     dev = _lib.require_hip(x, weight if laid_out is None else laid_out.rows.storage, bias)
     tensor = weight if laid_out is None else None
-    if torch.is_grad_enabled() and (x.requires_grad or (tensor is not None and tensor.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    if _lib.differentiated(x, tensor, bias):
         return _Linear.apply(x, tensor, bias, (laid_out, act, beta, dev))
     return _linear(x, tensor, laid_out, bias, act, beta, dev, False, False)[0]

@@ -2,10 +2,10 @@
 
     y = (x - mean) / sqrt(var + eps) * weight + bias
 
-layer_norm is differentiable once, in x, weight and bias; LayerNorm is the module.  The rows may be float32, float64,
-float16 or bfloat16, the weight and the bias of the same type or, with 16-bit rows, float32; sums and statistics are held
-in 32 bits (64 for float64 rows).  x may be any view whose last dimension is dense and whose rows have one stride; other
-views are copied.  There is no CPU path.
+layer_norm is differentiable once, in x, weight and bias, backwards only (forward-mode derivatives are refused); LayerNorm
+is the module.  The rows may be float32, float64, float16 or bfloat16, the weight and the bias of the same type or, with
+16-bit rows, float32; sums and statistics are held in 32 bits (64 for float64 rows).  x may be any view whose last dimension
+is dense and whose rows have one stride; other views are copied.  There is no CPU path.
 """
 import torch
 
@@ -100,8 +100,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x."""
     dev, code, wcode = _check(x, weight, bias)
     eps = float(eps)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    if _lib.differentiated(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, (eps, dev, code, wcode))
     return _forward(x, weight, bias, eps, dev, code, wcode, False)[0]
 

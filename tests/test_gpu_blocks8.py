@@ -551,3 +551,21 @@ def test_softplus_of_very_small_results_with_a_small_beta(beta):
     x = (x.double() / beta).float()
     q = blocks8.quantize(x, "softplus", beta)
     assert torch.equal(q.dequantize().double(), by_blocks(softplus(x, beta))) and not q.values[:, 150:].any()
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_forward_mode_derivatives_of_linear_are_refused(which):
+    from torch.autograd import forward_ad
+
+    plain = [normal(9, 40, seed=1), normal(30, 40, seed=2), normal(30, seed=3)]
+    want = blocks8.linear(*plain)
+    for grad in (False, True):
+        args = list(plain)
+        with torch.set_grad_enabled(grad), forward_ad.dual_level():
+            assert torch.equal(blocks8.linear(*args), want)
+            args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                blocks8.linear(*args)
+            if which != 1:
+                with pytest.raises(NotImplementedError, match="forward mode"):
+                    blocks8.linear(args[0], blocks8.quantize_weight(plain[1]), args[2])

@@ -110,3 +110,17 @@ def test_backward_refuses_a_hook_that_returns_another_tensor(recorder, wrong):
     with pytest.raises(RuntimeError, match="saved tensor came back"):
         _backward_under(wrong, x)
     assert recorder.bwd is None
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(recorder, which, grad):
+    """a dual tensor has no requires_grad; without an error its tangent would read as zero"""
+    from torch.autograd import forward_ad
+
+    args = [torch.randn(3, 4), torch.ones(4), torch.zeros(4)]
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        assert forward_ad.unpack_dual(norm.layer_norm(*args)).tangent is None
+        args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(NotImplementedError, match="forward mode"):
+            norm.layer_norm(*args)
