@@ -321,6 +321,7 @@ int vmf_layer_norm_bwd(const void* x, int64_t x_stride, const void* gy, int64_t 
  * x, g, out: VMF_F32, VMF_F16 or VMF_BF16, row strides in elements as in the layer norm; out is dense. */
 #define VMF_BLOCKS8_MAX_ROWS ((int64_t)1 << 26)
 #define VMF_BLOCKS8_MAX_WIDTH ((int64_t)1 << 22)
+#define VMF_GBIAS_F32 0x100 /* a flag beside a dtype */
 enum vmf_activation { VMF_ACT_NONE = 0, VMF_ACT_SOFTPLUS = 1 };
 /* blocks of x, or of softplus(x) = log(1 + exp(beta x)) / beta: the bytes of its value in 64 bits, whatever x's type (where
  * that is the middle of two 8-bit values to 2^-40, either of them; values below 2^-126 / beta may count as 0) */
@@ -348,7 +349,8 @@ int vmf_blocks8_matmul(const uint8_t* a, const uint8_t* a_exponents, int64_t a_e
                        int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes, int out_dtype,
                        vmf_stream_t stream);
 /* gweight[n][k] = sum_m gy[m][n] a[m][k], gbias[n] = sum_m gy[m][n] (may be null): gy (m, n) of dtype, a: m rows of width
- * k in blocks by rows, outputs of out_dtype (VMF_F32 or dtype).  Products are exact, sums 32-bit, in a fixed order.
+ * k in blocks by rows, outputs of out_dtype (VMF_F32 or dtype; with VMF_GBIAS_F32 added gbias is VMF_F32 in any case).
+ * Products are exact, sums 32-bit, in a fixed order.
  * m == 0 gives zeros.  gy_values / gy_exponents (may be null): receive gy's blocks by rows, the bytes that
  * vmf_blocks8_quantize gives (the operand of the input gradient's product) without another read of gy. */
 int vmf_blocks8_weight_grad_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes_out);
@@ -362,7 +364,7 @@ int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const uint8_t* a,
  * its tiles already.  a_values / a_exponents (may be null: not kept) receive x's blocks, which bwd takes; wt_values /
  * wt_exponents (may be null) the transposed weight's tiles, which bwd takes for gx.  y: dense, of dtype.
  * bwd: gx (may be null; of dtype) = (blocks(gy) tiles(weight)) * softplus slope, gweight (may be null) and gbias (may be
- * null, comes with gweight) as vmf_blocks8_weight_grad, of weight_dtype.
+ * null, comes with gweight) as vmf_blocks8_weight_grad, of weight_dtype (to which VMF_GBIAS_F32 may be added).
  * workspace: the _workspace call's bytes (laid_out: weight is null, kept: a_values is not), 16-byte aligned. */
 int vmf_blocks8_linear_fwd_workspace(int64_t m, int64_t n, int64_t k, int laid_out, int kept, int dtype,
                                      int64_t* bytes_out);

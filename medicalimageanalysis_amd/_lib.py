@@ -26,6 +26,7 @@ KL_STATIC_MAX_N = 1 << 30
 ELBO_WORKSPACE_DOUBLES = 2048
 LATENT_S1, LATENT_S2, LATENT_T2 = range(3)
 ACT_NONE, ACT_SOFTPLUS = range(2)
+GBIAS_F32 = 0x100
 
 # (the module object `C` is re-used by callers for byref / c_int64)
 _P, _I64, _U64, _I, _D = C.c_void_p, C.c_int64, C.c_uint64, C.c_int, C.c_double

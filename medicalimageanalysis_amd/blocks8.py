@@ -351,11 +351,13 @@ class _Linear(torch.autograd.Function):
         other = _lib.dense(_lib.unpacked(other, torch.uint8, (other_bytes,), dev))
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         code = _lib.FLOAT_CODES[gy.dtype]
-        # the weight's gradient in the weight's type; a bias beside a laid-out weight has float32 sums
+        # the weight's gradient in the weight's type, the bias's in its own where that is the weight's or float32, else
+        # from the 32-bit sums
         out = w_dtype or torch.float32
+        gb_dtype = bias_dtype if bias_dtype == out else torch.float32
         gx = gy.new_empty(shape) if need_x else None
         gw = gy.new_empty((n, k), dtype=out) if need_w or need_b else None
-        gb = gy.new_empty(n, dtype=out) if need_b else None
+        gb = gy.new_empty(n, dtype=gb_dtype) if need_b else None
         lib = _lib.lib()
         need = _lib.workspace_bytes("vmf_blocks8_linear_bwd_workspace", m, n, k, code)
         ws = gy.new_empty(need, dtype=torch.uint8)
@@ -368,7 +370,9 @@ class _Linear(torch.autograd.Function):
         with _lib.on_device(dev):
             rc = lib.vmf_blocks8_linear_bwd(g.data_ptr(), stride, base, base + m * _up(k, BLOCK), max(16, _up(m, 16)), tv,
                                             te, act, beta, _lib.address(gx), _lib.address(gw), _lib.address(gb), m, n, k,
-                                            ws.data_ptr(), need, code, _lib.FLOAT_CODES[out], _lib.raw_stream(dev))
+                                            ws.data_ptr(), need, code,
+                                            _lib.FLOAT_CODES[out] | (_lib.GBIAS_F32 if gb_dtype != out else 0),
+                                            _lib.raw_stream(dev))
         if rc:
             _lib.check(rc, "vmf_blocks8_linear_bwd")
         if gb is not None and gb.dtype != bias_dtype:

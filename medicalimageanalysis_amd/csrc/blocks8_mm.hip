@@ -714,6 +714,7 @@ struct WgArgs {
   int64_t m, n, k;
   int64_t rows_per_split;
   int nt, kt, splits;
+  bool gb32;  // gb is float whatever gw is
 };
 
 // 32 columns of the 16 rows that start at `rows`, as the operand of a 32 x 32 x 16 product: lane l gets column l % 32 of
@@ -765,6 +766,7 @@ __device__ __forceinline__ void write_gbias(const WgArgs& p, uint8_t* lds, const
     const int64_t n = n0 + threadIdx.x;
     if (n < p.n) {
       if (p.partial) p.partial[(int64_t)p.splits * p.n * p.k + (int64_t)split * p.n + n] = s;
+      else if (p.gb32) ((float*)p.gb)[n] = s;
       else ((W*)p.gb)[n] = (W)s;
     }
   }
@@ -1101,7 +1103,8 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void wgrad_kernel(Wg
 // One does where there are many fours and few splits (16384x1024x2048 fp32, 8 splits: 172.7 us, with eight threads 177).
 template <typename W, int PARTS>
 __global__ __launch_bounds__(256) void wgrad_join_kernel(const float* __restrict__ partial, W* __restrict__ gw,
-                                                         W* __restrict__ gb, int splits, int64_t nk, int64_t n) {
+                                                         void* __restrict__ gb, bool gb32, int splits, int64_t nk,
+                                                         int64_t n) {
   constexpr int FOURS = 256 / PARTS;
   __shared__ float red[PARTS > 1 ? PARTS : 1][FOURS][4];
   const int at = threadIdx.x % FOURS, part = threadIdx.x / FOURS;
@@ -1114,7 +1117,7 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(const float* __restrict
       i -= w_fours;
       src += splits * nk;
       size = n;
-      out = gb;
+      out = (W*)gb;
     }
     const int64_t left = first + at < total ? size - 4 * i : 0;
     float s[4] = {0, 0, 0, 0};
@@ -1139,7 +1142,10 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(const float* __restrict
           for (int j = 0; j < 4; ++j) s[j] += red[q][at][j];
       }
     }
-    if (part == 0) store_some<4>(out + 4 * i, left, s);
+    if (part == 0) {
+      if (gb32 && src != partial) store_some<4>((float*)gb + 4 * i, left, s);
+      else store_some<4>(out + 4 * i, left, s);
+    }
   }
 }
 
@@ -1312,6 +1318,8 @@ extern "C" int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const 
                                        vmf_stream_t stream) {
   VMF_RANGE("vmf_blocks8_weight_grad");
   const char* what = "vmf_blocks8_weight_grad";
+  const bool gb32 = out_dtype & VMF_GBIAS_F32;
+  out_dtype &= ~VMF_GBIAS_F32;
   int64_t need = 0;
   int rc = vmf_blocks8_weight_grad_workspace(m, n, k, dtype, &need);
   if (rc != VMF_OK) return rc;
@@ -1345,6 +1353,7 @@ extern "C" int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const 
   p.nt = pl.nt;
   p.kt = pl.kt;
   p.splits = pl.splits;
+  p.gb32 = gb32;
   hipStream_t st = (hipStream_t)stream;
   LOWP_DISPATCH(dtype, "vmf_blocks8_weight_grad", T, {
     if (out_dtype == VMF_F32) wgrad_launch<T, float>(pl, p, st);
@@ -1355,10 +1364,10 @@ extern "C" int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const 
   const int64_t fours = (n * k + 3) / 4 + (n + 3) / 4;
   LOWP_DISPATCH(out_dtype, "vmf_blocks8_weight_grad", W, {
     if (pl.splits > 8 || fours <= 1 << 16)
-      wgrad_join_kernel<W, 8><<<vmf_grid_for(fours, 32, 1 << 13), 256, 0, st>>>(p.partial, (W*)gweight, (W*)gbias,
+      wgrad_join_kernel<W, 8><<<vmf_grid_for(fours, 32, 1 << 13), 256, 0, st>>>(p.partial, (W*)gweight, gbias, gb32,
                                                                                pl.splits, n * k, n);
     else
-      wgrad_join_kernel<W, 1><<<vmf_grid_for(fours, 256, 1 << 13), 256, 0, st>>>(p.partial, (W*)gweight, (W*)gbias,
+      wgrad_join_kernel<W, 1><<<vmf_grid_for(fours, 256, 1 << 13), 256, 0, st>>>(p.partial, (W*)gweight, gbias, gb32,
                                                                                 pl.splits, n * k, n);
   });
   return vmf_check_launch(what);

@@ -24,6 +24,7 @@ TYPES = [torch.float32, torch.float16, torch.bfloat16]
 TABLE = torch.tensor([c * 2.0 ** -9 if c < 8 else (8 + c % 8) * 2.0 ** (c // 8 - 10) for c in range(127)],
                      dtype=torch.float64, device=DEV)
 POWERS = torch.tensor([2.0 ** i for i in range(-160, 161)], dtype=torch.float64, device=DEV)
+U32 = 2.0 ** -24
 
 
 def pow2(e):
@@ -569,3 +570,27 @@ def test_forward_mode_derivatives_of_linear_are_refused(which):
             if which != 1:
                 with pytest.raises(NotImplementedError, match="forward mode"):
                     blocks8.linear(args[0], blocks8.quantize_weight(plain[1]), args[2])
+
+
+@pytest.mark.parametrize("x_type,w_type,b_type", [
+    (torch.bfloat16, torch.bfloat16, torch.float32), (torch.float16, torch.float16, torch.float32),
+    (torch.bfloat16, torch.float32, torch.bfloat16), (torch.float16, torch.float16, torch.bfloat16),
+    (torch.bfloat16, torch.bfloat16, torch.float16), (torch.float32, torch.float32, torch.float16)])
+@pytest.mark.parametrize("m,n,k", [(5, 3, 20), (40, 130, 100), (5000, 130, 300), (16384, 300, 2100)])
+def test_bias_gradient_has_the_type_and_the_digits_of_the_bias(m, n, k, x_type, w_type, b_type):
+    """m sums of 32 bits each, rounded once to the bias's type; the weight's gradient is what it is without a bias"""
+    x, w = normal(m, k, seed=1).to(x_type), normal(n, k, seed=2, scale=k ** -0.5).to(w_type).requires_grad_()
+    b, gy = torch.zeros(n, device=DEV, dtype=b_type, requires_grad=True), normal(m, n, seed=3).to(x_type)
+    gw, gb = torch.autograd.grad(blocks8.linear(x, w, b), (w, b), gy)
+    assert gw.dtype == w_type and gb.dtype == b_type
+    want, size = gy.double().sum(0), gy.double().abs().sum(0)
+    bound = torch.finfo(b_type).eps / 2 * want.abs() + (m / 16 + 64) * U32 * size
+    assert ((gb.double() - want).abs() <= bound).all(), float(((gb.double() - want).abs() / bound).max())
+    assert torch.equal(gw, torch.autograd.grad(blocks8.linear(x, w), w, gy)[0])
+
+
+@pytest.mark.parametrize("m", [4000, 40])
+def test_float32_bias_gradient_beyond_the_weights_type(m):
+    x, w = normal(m, 64, seed=1).half(), normal(32, 64, seed=2).half().requires_grad_()
+    b, gy = torch.zeros(32, device=DEV, requires_grad=True), torch.full((m, 32), 2000.0, device=DEV).half()
+    assert (torch.autograd.grad(blocks8.linear(x, w, b), b, gy)[0] == 2000.0 * m).all()
