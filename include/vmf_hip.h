@@ -358,13 +358,18 @@ int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const uint8_t* a,
                             int64_t a_exp_pitch, void* gweight, void* gbias, uint8_t* gy_values, uint8_t* gy_exponents,
                             int64_t gy_exp_pitch, int64_t m, int64_t n, int64_t k, void* workspace,
                             int64_t workspace_bytes, int dtype, int out_dtype, vmf_stream_t stream);
+/* gbias alone, where the weight takes no gradient: a column sum of gy, of out_dtype (VMF_F32 or dtype), 32-bit sums in a
+ * fixed order.  m == 0 gives zeros. */
+int vmf_blocks8_bias_grad_workspace(int64_t m, int64_t n, int dtype, int64_t* bytes_out);
+int vmf_blocks8_bias_grad(const void* gy, int64_t gy_stride, void* gbias, int64_t m, int64_t n, void* workspace,
+                          int64_t workspace_bytes, int dtype, int out_dtype, vmf_stream_t stream);
 
 /* A layer's two directions in one call each: y = blocks(activation(x)) tiles(weight)^T + bias, and its gradients.
  * fwd: weight (n, k) of weight_dtype (dtype or VMF_F32) is quantised in the call, or (null) w_values / w_exponents hold
  * its tiles already.  a_values / a_exponents (may be null: not kept) receive x's blocks, which bwd takes; wt_values /
  * wt_exponents (may be null) the transposed weight's tiles, which bwd takes for gx.  y: dense, of dtype.
  * bwd: gx (may be null; of dtype) = (blocks(gy) tiles(weight)) * softplus slope, gweight (may be null) and gbias (may be
- * null, comes with gweight) as vmf_blocks8_weight_grad, of weight_dtype (to which VMF_GBIAS_F32 may be added).
+ * null, comes with gweight; alone: vmf_blocks8_bias_grad) as vmf_blocks8_weight_grad, of weight_dtype (to which VMF_GBIAS_F32 may be added).
  * workspace: the _workspace call's bytes (laid_out: weight is null, kept: a_values is not), 16-byte aligned. */
 int vmf_blocks8_linear_fwd_workspace(int64_t m, int64_t n, int64_t k, int laid_out, int kept, int dtype,
                                      int64_t* bytes_out);

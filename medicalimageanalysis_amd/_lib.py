@@ -82,6 +82,8 @@ _PROTOS = {
                            _I, _P],
     "vmf_blocks8_weight_grad_workspace": [_I64, _I64, _I64, _I, _I64P],
     "vmf_blocks8_weight_grad": [_P, _I64, _P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _I, _I, _P],
+    "vmf_blocks8_bias_grad_workspace": [_I64, _I64, _I, _I64P],
+    "vmf_blocks8_bias_grad": [_P, _I64, _P, _I64, _I64, _P, _I64, _I, _I, _P],
     "vmf_blocks8_linear_fwd_workspace": [_I64, _I64, _I64, _I, _I, _I, _I64P],
     "vmf_blocks8_linear_fwd": [_P, _I64, _P, _I64, _I, _P, _P, _P, _P, _P, _I, _I, _D, _P, _P, _I64, _P, _I64, _I64, _I64,
                                _P, _I64, _I, _P],

@@ -323,6 +323,17 @@ def _linear(x, weight, laid_out, bias, act, beta, dev, keep, columns):
     return y, kept, wt, (m, n, k)
 
 
+def _bias_grad(g, stride, gb, m, n, code, dev):
+    """the sum of g's rows into gb (float32 or g's type)"""
+    need = _lib.workspace_bytes("vmf_blocks8_bias_grad_workspace", m, n, code)
+    ws = g.new_empty(need, dtype=torch.uint8) if need else None
+    with _lib.on_device(dev):
+        rc = _lib.lib().vmf_blocks8_bias_grad(g.data_ptr(), stride, gb.data_ptr(), m, n, _lib.address(ws), need, code,
+                                              _lib.FLOAT_CODES[gb.dtype], _lib.raw_stream(dev))
+    if rc:
+        _lib.check(rc, "vmf_blocks8_bias_grad")
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, how):
@@ -331,7 +342,8 @@ class _Linear(torch.autograd.Function):
         if need_x and laid_out is not None and laid_out.columns is None:
             raise ValueError("linear: the laid-out weight has no columns (quantize_weight(..., transpose=True)), which "
                              "the gradient of x reads")
-        y, kept, wt, sizes = _linear(x, weight, laid_out, bias, act, beta, dev, True, need_x)
+        keep = need_x or ctx.needs_input_grad[1]  # (a bias's gradient reads neither)
+        y, kept, wt, sizes = _linear(x, weight, laid_out, bias, act, beta, dev, keep, need_x)
         # kept for the backward pass: x in 8 bits and, for its own gradient, the transposed weight in 8 bits
         other = None
         if need_x and laid_out is not None:
@@ -339,7 +351,8 @@ class _Linear(torch.autograd.Function):
             other, wt = columns.storage, (columns.offset, columns.exp_offset)
         ctx.save_for_backward(kept, other)
         ctx.meta = (x.shape, sizes, wt, act, beta, None if weight is None else weight.dtype,
-                    None if bias is None else bias.dtype, dev, kept.numel(), 0 if other is None else other.numel())
+                    None if bias is None else bias.dtype, dev, kept.numel() if keep else 0,
+                    0 if other is None else other.numel())
         return y
 
     @staticmethod
@@ -351,40 +364,50 @@ class _Linear(torch.autograd.Function):
         other = _lib.dense(_lib.unpacked(other, torch.uint8, (other_bytes,), dev))
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         code = _lib.FLOAT_CODES[gy.dtype]
-        # the weight's gradient in the weight's type, the bias's in its own where that is the weight's or float32, else
+        g, stride = _lib.as_rows(gy)
+        # the weight's gradient has the weight's type, the bias's its own: where the call that computes it does not give that,
         # from the 32-bit sums
         out = w_dtype or torch.float32
-        gb_dtype = bias_dtype if bias_dtype == out else torch.float32
-        gx = gy.new_empty(shape) if need_x else None
-        gw = gy.new_empty((n, k), dtype=out) if need_w or need_b else None
-        gb = gy.new_empty(n, dtype=gb_dtype) if need_b else None
-        lib = _lib.lib()
-        need = _lib.workspace_bytes("vmf_blocks8_linear_bwd_workspace", m, n, k, code)
-        ws = gy.new_empty(need, dtype=torch.uint8)
-        g, stride = _lib.as_rows(gy)
-        base = kept.data_ptr()
-        tv = te = None
-        if need_x:
-            at = base if other is None else other.data_ptr()
-            tv, te = at + wt[0], at + wt[1]
-        with _lib.on_device(dev):
-            rc = lib.vmf_blocks8_linear_bwd(g.data_ptr(), stride, base, base + m * _up(k, BLOCK), max(16, _up(m, 16)), tv,
-                                            te, act, beta, _lib.address(gx), _lib.address(gw), _lib.address(gb), m, n, k,
-                                            ws.data_ptr(), need, code,
-                                            _lib.FLOAT_CODES[out] | (_lib.GBIAS_F32 if gb_dtype != out else 0),
-                                            _lib.raw_stream(dev))
-        if rc:
-            _lib.check(rc, "vmf_blocks8_linear_bwd")
+        gx = gw = gb = gb_too = None
+        if need_b:
+            gb = gy.new_empty(n, dtype=bias_dtype if bias_dtype == (out if need_w else gy.dtype) else torch.float32)
+            if need_w:
+                gb_too = gb.data_ptr()
+            else:
+                _bias_grad(g, stride, gb, m, n, code, dev)
+        if need_x or need_w:
+            if need_x:
+                gx = gy.new_empty(shape)
+            if need_w:
+                gw = gy.new_empty((n, k), dtype=out)
+            need = _lib.workspace_bytes("vmf_blocks8_linear_bwd_workspace", m, n, k, code)
+            ws = gy.new_empty(need, dtype=torch.uint8)
+            base = kept.data_ptr()
+            tv = te = None
+            if need_x:
+                at = base if other is None else other.data_ptr()
+                tv, te = at + wt[0], at + wt[1]
+            out_code = _lib.FLOAT_CODES[out]
+            if gb_too is not None and gb.dtype != out:
+                out_code |= _lib.GBIAS_F32
+            with _lib.on_device(dev):
+                rc = _lib.lib().vmf_blocks8_linear_bwd(g.data_ptr(), stride, base, base + m * _up(k, BLOCK),
+                                                       max(16, _up(m, 16)), tv, te, act, beta, _lib.address(gx),
+                                                       _lib.address(gw), gb_too, m, n, k, ws.data_ptr(), need, code,
+                                                       out_code, _lib.raw_stream(dev))
+            if rc:
+                _lib.check(rc, "vmf_blocks8_linear_bwd")
         if gb is not None and gb.dtype != bias_dtype:
             gb = gb.to(bias_dtype)
-        return gx, gw if need_w else None, gb, None
+        return gx, gw, gb, None
 
 
 def linear(x, weight, bias=None, activation=None, beta=1.0):
     """blocks(activation(x)) tiles(weight)^T + bias for x (..., k): (..., n) of x's type.
 
     weight: a matrix (n, k) of x's type or float32, quantised in the call (training), or a Weight8 that was laid out once
-    (serving; no gradient of its own).  Keeps one byte per element of x for the backward pass."""
+    (serving; no gradient of its own).  Keeps one byte per element of x for the backward pass (none where only the bias takes
+    a gradient).  bias: float32, float16 or bfloat16, and so is its gradient."""
     _width(x, "linear")
     _code(x.dtype, "linear")
     act, beta = _activation(activation, beta, "linear")

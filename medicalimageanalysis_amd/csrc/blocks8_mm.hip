@@ -1113,7 +1113,8 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(const float* __restrict
     int64_t i = first + at, size = nk;
     const float* src = partial;
     W* out = gw;
-    if (i >= w_fours) {
+    const bool bias = i >= w_fours;
+    if (bias) {
       i -= w_fours;
       src += splits * nk;
       size = n;
@@ -1143,10 +1144,60 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(const float* __restrict
       }
     }
     if (part == 0) {
-      if (gb32 && src != partial) store_some<4>((float*)gb + 4 * i, left, s);
+      if (bias && gb32) store_some<4>((float*)gb + 4 * i, left, s);
       else store_some<4>(out + 4 * i, left, s);
     }
   }
+}
+
+// gbias by itself.  A workgroup takes 128 columns of its split's rows, in the lanes and the order that the weight gradient's
+// tiles have; the splits are joined as theirs are.
+template <typename T, typename W>
+__global__ __launch_bounds__(256) void bias_grad_kernel(const T* __restrict__ gy, int64_t gy_stride, W* __restrict__ gb,
+                                                        float* __restrict__ partial, int64_t m, int64_t n,
+                                                        int64_t rows_per_split) {
+  constexpr int E = 16 / (int)sizeof(T), GP = 128 / E, GROWS = 256 / GP;
+  __shared__ float red[GROWS][128];
+  const int gr = threadIdx.x / GP, gc = threadIdx.x % GP * E;
+  const int64_t n0 = (int64_t)blockIdx.x * 128, left = n - n0 - gc;
+  const int64_t m0 = (int64_t)blockIdx.y * rows_per_split, end = m0 + rows_per_split < m ? m0 + rows_per_split : m;
+  const T* p = gy + n0 + gc;
+  float s[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) s[i] = 0;
+  if (left > 0) {
+#pragma unroll 8
+    for (int64_t r = m0 + gr; r < end; r += GROWS) {
+      float v[E];
+      load_some<E>(p + r * gy_stride, left, 0.0f, v);
+#pragma unroll
+      for (int i = 0; i < E; ++i) s[i] += v[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < E; ++i) red[gr][gc + i] = s[i];
+  __syncthreads();
+  if (threadIdx.x >= 128 || n0 + threadIdx.x >= n) return;
+  float v = 0;
+#pragma unroll
+  for (int q = 0; q < GROWS; ++q) v += red[q][threadIdx.x];
+  if (partial) partial[(int64_t)blockIdx.y * n + n0 + threadIdx.x] = v;
+  else gb[n0 + threadIdx.x] = (W)v;
+}
+// four workgroups to a compute unit, at least 256 rows to a split
+struct BiasPlan {
+  int nt, splits;
+  int64_t per_split;
+};
+BiasPlan bias_plan(int64_t m, int64_t n) {
+  BiasPlan p;
+  p.nt = (int)((n + 127) / 128);
+  int64_t s = 1024 / p.nt;
+  if (s > m / 256) s = m / 256;
+  if (s < 1) s = 1;
+  p.per_split = ((m + s - 1) / s + WG_ROWS - 1) / WG_ROWS * WG_ROWS;
+  p.splits = p.per_split > 0 ? (int)((m + p.per_split - 1) / p.per_split) : 1;
+  return p;
 }
 
 struct WgPlan {
@@ -1369,6 +1420,46 @@ extern "C" int vmf_blocks8_weight_grad(const void* gy, int64_t gy_stride, const 
     else
       wgrad_join_kernel<W, 1><<<vmf_grid_for(fours, 256, 1 << 13), 256, 0, st>>>(p.partial, (W*)gweight, gbias, gb32,
                                                                                 pl.splits, n * k, n);
+  });
+  return vmf_check_launch(what);
+}
+
+extern "C" int vmf_blocks8_bias_grad_workspace(int64_t m, int64_t n, int dtype, int64_t* bytes_out) {
+  int rc = b8_check_shape("vmf_blocks8_bias_grad_workspace", m, n);
+  if (rc != VMF_OK) return rc;
+  VMF_REQUIRE(bytes_out, VMF_ERR_BAD_ARG, "vmf_blocks8_bias_grad_workspace: null pointer");
+  const BiasPlan pl = bias_plan(m, n);
+  *bytes_out = pl.splits > 1 ? (int64_t)pl.splits * n * 4 : 0;
+  return VMF_OK;
+}
+
+extern "C" int vmf_blocks8_bias_grad(const void* gy, int64_t gy_stride, void* gbias, int64_t m, int64_t n, void* workspace,
+                                     int64_t workspace_bytes, int dtype, int out_dtype, vmf_stream_t stream) {
+  VMF_RANGE("vmf_blocks8_bias_grad");
+  const char* what = "vmf_blocks8_bias_grad";
+  int64_t need = 0;
+  int rc = vmf_blocks8_bias_grad_workspace(m, n, dtype, &need);
+  if (rc != VMF_OK) return rc;
+  VMF_REQUIRE(out_dtype == VMF_F32 || out_dtype == dtype, VMF_ERR_DTYPE, "%s: out dtype %d", what, out_dtype);
+  VMF_REQUIRE(gy_stride >= 0, VMF_ERR_BAD_ARG, "%s: negative row stride", what);
+  VMF_REQUIRE(gbias && (m == 0 || gy), VMF_ERR_BAD_ARG, "%s: null pointer", what);
+  VMF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), VMF_ERR_BAD_ARG,
+              "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)need);
+  const BiasPlan pl = bias_plan(m, n);
+  float* partial = need ? (float*)workspace : nullptr;
+  const dim3 grid((unsigned)pl.nt, (unsigned)pl.splits);
+  hipStream_t st = (hipStream_t)stream;
+  LOWP_DISPATCH(dtype, "vmf_blocks8_bias_grad", T, {
+    if (out_dtype == VMF_F32)
+      bias_grad_kernel<T, float><<<grid, 256, 0, st>>>((const T*)gy, gy_stride, (float*)gbias, partial, m, n, pl.per_split);
+    else
+      bias_grad_kernel<T, T><<<grid, 256, 0, st>>>((const T*)gy, gy_stride, (T*)gbias, partial, m, n, pl.per_split);
+  });
+  rc = vmf_check_launch(what);
+  if (rc != VMF_OK || !need) return rc;
+  LOWP_DISPATCH(out_dtype, "vmf_blocks8_bias_grad", W, {
+    wgrad_join_kernel<W, 8><<<vmf_grid_for((n + 3) / 4, 32, 1 << 13), 256, 0, st>>>(partial, nullptr, gbias, false,
+                                                                                   pl.splits, 0, n);
   });
   return vmf_check_launch(what);
 }

@@ -128,3 +128,22 @@ def test_layer_entry_refusals():
 
     assert bwd(m=-1) == -1 and bwd(gw=None) == -1 and bwd(wt=None) == -1 and bwd(nbytes=need.value - 1) == -1
     assert bwd(w_dtype=2) == -2
+
+
+def test_bias_gradient_entry_refusals():
+    lib = _lib.lib()
+    p = C.c_void_p(256)
+    need = C.c_int64(-1)
+    assert lib.vmf_blocks8_bias_grad_workspace(100, 128, 0, need) == 0 and need.value == 0
+    assert lib.vmf_blocks8_bias_grad_workspace(1 << 16, 128, 0, need) == 0 and need.value > 0
+    assert lib.vmf_blocks8_bias_grad_workspace(-1, 128, 0, need) == -1
+    assert lib.vmf_blocks8_bias_grad_workspace(4, 0, 0, need) == -1
+    assert lib.vmf_blocks8_bias_grad_workspace(4, (1 << 22) + 1, 0, need) == -4
+    assert lib.vmf_blocks8_bias_grad_workspace(4, 4, 0, None) == -1
+
+    def grad(g=p, gb=p, stride=8, m=4, ws=None, nbytes=0, dtype=0, out_dtype=0):
+        return lib.vmf_blocks8_bias_grad(g, stride, gb, m, 128, ws, nbytes, dtype, out_dtype, None)
+
+    assert grad(g=None) == -1 and grad(gb=None) == -1 and grad(stride=-1) == -1 and grad(m=-1) == -1
+    assert grad(dtype=3, out_dtype=2) == -2 and grad(dtype=1, out_dtype=1) == -2
+    assert grad(m=1 << 16, ws=p, nbytes=need.value - 1) == -1

@@ -594,3 +594,54 @@ def test_float32_bias_gradient_beyond_the_weights_type(m):
     x, w = normal(m, 64, seed=1).half(), normal(32, 64, seed=2).half().requires_grad_()
     b, gy = torch.zeros(32, device=DEV, requires_grad=True), torch.full((m, 32), 2000.0, device=DEV).half()
     assert (torch.autograd.grad(blocks8.linear(x, w, b), b, gy)[0] == 2000.0 * m).all()
+
+
+@pytest.mark.parametrize("laid_out", [False, True])
+@pytest.mark.parametrize("x_type,b_type", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32),
+                                           (torch.bfloat16, torch.bfloat16), (torch.float16, torch.bfloat16),
+                                           (torch.float32, torch.float16)])
+@pytest.mark.parametrize("m,n", [(0, 5), (1, 1), (7, 3), (31, 129), (513, 130), (5000, 1001), (70000, 16), (300, 4097)])
+def test_bias_gradient_without_the_weights(m, n, x_type, b_type, laid_out):
+    w = normal(n, 40, seed=2)
+    weight = blocks8.quantize_weight(w) if laid_out else w
+    x, gy = normal(m, 40, seed=1).to(x_type), normal(m, n, seed=3).to(x_type)
+    b = torch.zeros(n, device=DEV, dtype=b_type, requires_grad=True)
+    y = blocks8.linear(x, weight, b, "softplus")
+    gb, = torch.autograd.grad(y, b, gy, retain_graph=True)
+    want, size = gy.double().sum(0), gy.double().abs().sum(0)
+    bound = torch.finfo(b_type).eps / 2 * want.abs() + (m / 16 + 64) * U32 * size
+    assert gb.dtype == b_type and ((gb.double() - want).abs() <= bound).all()
+    assert torch.equal(gb, torch.autograd.grad(y, b, gy, retain_graph=True)[0])  # the same bits on every run
+    wide = torch.full((m, n + 9), math.nan, device=DEV, dtype=x_type)
+    wide[:, 3:3 + n] = gy
+    assert torch.equal(gb, torch.autograd.grad(y, b, wide[:, 3:3 + n], retain_graph=True)[0])
+    gone = (gy[:1] / 64).expand(m, n) if m else gy
+    got = torch.autograd.grad(y, b, gone)[0].double()
+    assert ((got - gone.double().sum(0)).abs() <= torch.finfo(b_type).eps * gone.double().sum(0).abs()
+            + (m / 16 + 64) * U32 * gone.double().abs().sum(0)).all()
+    # x's gradient is what it is without the bias's
+    xs = x.clone().requires_grad_()
+    pair = torch.autograd.grad(blocks8.linear(xs, weight, b, "softplus"), (xs, b), gy)
+    alone = torch.autograd.grad(blocks8.linear(xs, weight, b.detach(), "softplus"), xs, gy)
+    assert torch.equal(pair[1], gb) and torch.equal(pair[0], alone[0])
+
+
+def test_bias_gradient_without_the_weights_computes_and_keeps_no_more_than_it_reads():
+    x, w8 = normal(64, 4096, seed=1), blocks8.quantize_weight(normal(4096, 4096, seed=2))
+    b, gy = torch.zeros(4096, device=DEV, requires_grad=True), normal(64, 4096, seed=3)
+    y = blocks8.linear(x, w8, b)
+    assert all(t is None for t in y.grad_fn.saved_tensors)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    torch.autograd.grad(y, b, gy)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before < 1 << 20  # the weight's gradient would have 64 MB
+
+
+def test_bias_gradient_of_non_finite_columns():
+    x, b = normal(300, 20, seed=1), torch.zeros(5, device=DEV, requires_grad=True)
+    gy = normal(300, 5, seed=3)
+    gy[4, 1], gy[200, 2] = math.inf, math.nan
+    gb, = torch.autograd.grad(blocks8.linear(x, normal(5, 20), b), b, gy)
+    assert gb[1] == math.inf and gb[2].isnan() and gb[[0, 3, 4]].isfinite().all()
