@@ -179,7 +179,7 @@ __device__ __forceinline__ uint2 softplus8(const float (&h)[8], float beta, floa
     top = lane_max<16>(top);
   }
   float at = softplus32(top, beta, inv_beta);
-  if (!(at < INF)) at = top;  // beta h is beyond 32 bits, softplus(h) is h to its last bit
+  if (beta > 1.0f && !(at < INF)) at = top;  // beta h is beyond 32 bits, softplus(h) is h to its last bit
   const float mt = softplus_margin(top, beta);
   const float most32 = 3.4e38f;
   int e = b8_exponent(at < most32 ? at * (1.0f - mt) : most32);
@@ -188,8 +188,10 @@ __device__ __forceinline__ uint2 softplus8(const float (&h)[8], float beta, floa
   if (top == -INF) e = 0;
   e_out = e;
   const float scale = inv_beta * b8_pow2(-e);
-  // (beta h or, with a small beta, 2^-e / beta may be beyond 32 bits where the elements are not)
-  const bool exact = e == B8_EMAX || !(larger(beta * top, scale) < INF);
+  // With a beta above 1 beta h, with one below 2^-17 2^-e / beta may be beyond 32 bits where the elements are not.  (beta is
+  // the launch's: the usual ones skip the test.)
+  bool exact = e == B8_EMAX;
+  if (beta > 1.0f || beta < 0x1p-17f) exact |= !(larger(beta * top, scale) < INF);
   float lo[8], hi[8], least = h[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) least = fminf(least, h[i]);
