@@ -454,7 +454,8 @@ struct BwdPlan {
   int parts;    // workgroups, each leaving a partial row of gw and gb; 0: none are left (few rows)
 };
 // Few rows (up to 1024, rows of up to 256 lanes): one launch (128x128 fp32 3.1 us, with partials 8.9; 1024x784 7.8 and 8.6;
-// 1536x784 12.7 and 9.5).
+// 1536x784 12.7 and 9.5; wide rows: 128x4096 3.5 and 9.8, 512x4096 10.1 and 15.8, 1024x4096 19.1 and 18.3, in bf16 14.3 and
+// 19.9).
 // Otherwise two workgroups for each of 256 compute units (1048576x784 fp32, a wave to a row, 1.88 ms, with four 2.00), four
 // where the other waves have more to fill: rows of 16 bits, whose loads are half as many (1048576x784 bf16 1.14 ms, with two
 // 1.88), and rows of four waves, which wait at barriers (65536x4096 bf16 0.33 ms, with two 0.50).  No more than have 32
@@ -466,14 +467,23 @@ BwdPlan bwd_plan(int64_t n, int64_t width) {
   BwdPlan p;
   p.tpr = lanes_for((width + V - 1) / V, bwd_chunks<T>());
   p.threads = p.tpr == 0 ? 256 : p.tpr > THREADS ? p.tpr : THREADS;
+  const int64_t most = sizeof(T) == 2 || p.tpr == THREADS ? 1024 : 512;
+  if (p.tpr == 0) {
+    // (its launch has a workgroup for each 256 columns of a part: more parts only where those do not fill the chip, since
+    // wide parts are large: 16 rows of 2^22 fp32 leave one of 34 MB, where one for each row takes 2.79 ms for 2.52)
+    const int64_t columns = (width + 255) / 256;
+    int64_t g = (n + 15) / 16;
+    if (g * columns < 1024) g = (1024 + columns - 1) / columns < n ? (1024 + columns - 1) / columns : n;
+    p.parts = (int)(g < 1 ? 1 : g > most ? most : g);
+    return p;
+  }
   if (p.tpr != 0 && p.tpr <= THREADS && n <= 1024) {
     p.parts = 0;
     return p;
   }
-  const int64_t most = sizeof(T) == 2 || p.tpr == THREADS ? 1024 : 512;
   // rows to a workgroup: those, or as many as it has side by side, or fewer where that leaves compute units without one
-  const int64_t at_once = p.tpr == 0 ? 1 : p.threads / p.tpr;
-  const int64_t few = p.tpr == 0 || p.tpr >= 64 ? 16 : 32, rows = at_once > few ? at_once : few;
+  const int64_t at_once = p.threads / p.tpr;
+  const int64_t few = p.tpr >= 64 ? 16 : 32, rows = at_once > few ? at_once : few;
   int64_t g = (n + rows - 1) / rows;
   if (g < 256) g = (n + at_once - 1) / at_once < 256 ? (n + at_once - 1) / at_once : 256;
   p.parts = (int)(g < 1 ? 1 : g > most ? most : g);

@@ -214,3 +214,9 @@ def test_saved_tensors_moved_to_the_host_and_back(n, width):
         y = norm.layer_norm(*leaves)
     for p, q in zip(torch.autograd.grad(y, leaves, gy), want):
         assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,width", [(1, 40001), (16, 300000), (40, 33000), (300, 40000)])
+def test_long_rows_and_their_parts(n, width, dtype):
+    check(*data(n, width, dtype, seed=n))

@@ -124,3 +124,12 @@ def test_forward_mode_derivatives_are_refused(recorder, which, grad):
         args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
         with pytest.raises(NotImplementedError, match="forward mode"):
             norm.layer_norm(*args)
+
+
+@pytest.mark.parametrize("dtype,size,wide", [(0, 4, 4), (1, 8, 8), (2, 2, 4), (3, 2, 4)])
+@pytest.mark.parametrize("n,width", [(1, 40000), (5, 40001), (16, 1 << 24), (300, 40000), (16384, 40000), (4000, 1 << 20)])
+def test_backward_workspace_of_long_rows_stays_below_the_input(n, width, dtype, size, wide):
+    """two parts of a row for each 16 rows, and 2 MB (double: 4) for few rows that have to fill the chip"""
+    need = C.c_int64(-1)
+    assert _lib.lib().vmf_layer_norm_bwd_workspace(n, width, dtype, need) == 0
+    assert 0 < need.value <= max(-(-n // 16) * 2 * width * wide, (1024 + -(-width // 256)) * 256 * 2 * wide)
