@@ -1565,6 +1565,11 @@ extern "C" int vmf_blocks8_linear_bwd(const void* gy, int64_t gy_stride, const u
               "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)need);
   VMF_REQUIRE(gweight || !gbias, VMF_ERR_BAD_ARG, "%s: gbias comes with gweight", what);
   VMF_REQUIRE(!gx || wt_values, VMF_ERR_BAD_ARG, "%s: gx needs the transposed weight", what);
+  VMF_REQUIRE(activation == VMF_ACT_NONE || activation == VMF_ACT_SOFTPLUS, VMF_ERR_BAD_ARG, "%s: activation %d", what,
+              activation);
+  const bool gate = gx && activation == VMF_ACT_SOFTPLUS;
+  VMF_REQUIRE(!gate || m == 0 || (a_values && a_exponents), VMF_ERR_BAD_ARG, "%s: the softplus gradient needs x's blocks",
+              what);
   // gy's blocks lie in front, what the products add up in parts behind them: one after the other, on one stream
   uint8_t* q = (uint8_t*)workspace;
   uint8_t* q_exps = q + m * b8_blocks(n) * B8;
@@ -1576,7 +1581,6 @@ extern "C" int vmf_blocks8_linear_bwd(const void* gy, int64_t gy_stride, const u
   else if (gx)
     rc = vmf_blocks8_quantize(gy, gy_stride, q, q_exps, exp_rows(m), m, n, VMF_ACT_NONE, 1.0, dtype, stream);
   if (rc != VMF_OK || !gx) return rc;
-  const bool gate = activation == VMF_ACT_SOFTPLUS;
   return vmf_blocks8_matmul(q, q_exps, exp_rows(m), 0, wt_values, wt_exponents, b8_blocks(k), 1, nullptr, 0,
                             gate ? a_values : nullptr, a_exponents, a_exp_pitch, beta, gx, m, k, n, parts, left, dtype,
                             stream);

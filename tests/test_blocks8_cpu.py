@@ -147,3 +147,24 @@ def test_bias_gradient_entry_refusals():
     assert grad(g=None) == -1 and grad(gb=None) == -1 and grad(stride=-1) == -1 and grad(m=-1) == -1
     assert grad(dtype=3, out_dtype=2) == -2 and grad(dtype=1, out_dtype=1) == -2
     assert grad(m=1 << 16, ws=p, nbytes=need.value - 1) == -1
+
+
+def test_layer_backward_needs_xs_blocks_for_the_softplus_gradient():
+    """without them gx would come out without its factor"""
+    lib = _lib.lib()
+    p = C.c_void_p(256)
+    need = C.c_int64(0)
+    assert lib.vmf_blocks8_linear_bwd_workspace(4, 4, 8, 0, need) == 0
+
+    def bwd(a=p, ae=p, act=1, gx=p, m=4):
+        return lib.vmf_blocks8_linear_bwd(None, 8, a, ae, 16, p, p, act, 1.0, gx, None, None, m, 4, 8, p, need.value, 0, 0,
+                                          None)
+
+    # (gy is null as well, so that no call gets past its checks)
+    for call in (dict(a=None), dict(ae=None)):
+        assert bwd(**call) == -1 and b"blocks" in lib.vmf_last_error_string()
+    for act in (-1, 2):
+        assert bwd(act=act) == -1 and b"activation" in lib.vmf_last_error_string()
+        assert bwd(act=act, gx=None) == -1
+    assert bwd() == -1 and b"null pointer" in lib.vmf_last_error_string()
+    assert bwd(a=None, m=0) == 0 and bwd(a=None, gx=None) == 0
