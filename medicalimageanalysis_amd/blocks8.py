@@ -91,7 +91,7 @@ class Blocks8:
     def dequantize(self, dtype=torch.float32):
         """the elements as `dtype` (every one is exact in float32 and bfloat16)"""
         code = _code(dtype, "dequantize")
-        dev = self.device
+        dev = _lib.require_hip(self.storage)
         out = self.storage.new_empty(self.shape, dtype=dtype)
         v, e = self._addresses()
         with _lib.on_device(dev):
@@ -112,6 +112,7 @@ class Weight8:
     __slots__ = ("rows", "columns", "dtype")
 
     def __init__(self, rows, columns, dtype):
+        _blocks("Weight8", rows, *(() if columns is None else (columns,)))
         if not rows.tiled or (columns is not None and (not columns.tiled or columns.shape != rows.shape[::-1]
                                                        or columns.device != rows.device)):
             raise ValueError(f"Weight8: {rows} and {columns} are not the tiles of a matrix and of its transpose")
@@ -130,6 +131,12 @@ def _code(dtype, what):
     if dtype not in _FLOATS:
         raise TypeError(f"{what} takes float32, float16 or bfloat16, got {dtype}")
     return _lib.FLOAT_CODES[dtype]
+
+
+def _blocks(what, *operands):
+    for q in operands:
+        if not isinstance(q, Blocks8):
+            raise TypeError(f"{what} takes Blocks8 (quantize, or the rows / columns of quantize_weight), got {type(q).__name__}")
 
 
 def _activation(activation, beta, what):
@@ -220,8 +227,7 @@ def _check_bias(bias, n, what):
 
 def matmul(a, b, bias=None, dtype=torch.float32):
     """a b^T + bias of two Blocks8 of the same width: (..., k), (n, k) -> (..., n)."""
-    if not isinstance(a, Blocks8) or not isinstance(b, Blocks8):
-        raise TypeError("matmul takes Blocks8 (quantize, or the rows / columns of quantize_weight)")
+    _blocks("matmul", a, b)
     if len(b.shape) != 2 or a.width != b.width:
         raise ValueError(f"matmul: shapes {tuple(a.shape)} and {tuple(b.shape)}")
     _code(dtype, "matmul")
@@ -232,6 +238,7 @@ def matmul(a, b, bias=None, dtype=torch.float32):
 
 def softplus_grad(g, q, beta=1.0):
     """g * (1 - exp(-beta q)), q = quantize(h, "softplus", beta): the gradient with respect to h."""
+    _blocks("softplus_grad", q)
     code = _code(g.dtype, "softplus_grad")
     _, beta = _activation("softplus", beta, "softplus_grad")
     if g.shape != q.shape or q.tiled:
@@ -271,6 +278,7 @@ def _weight_grad(g, q, bias, dtype, dev):
 def weight_grad(g, q, bias=True, dtype=torch.float32):
     """(g^T q, sum of g's rows) over all leading dimensions: the gradients of a layer's weight and bias from the
     gradient g (..., n) of its result and its kept input q (..., k); bias=False leaves the second out (None)."""
+    _blocks("weight_grad", q)
     _code(g.dtype, "weight_grad")
     _width(g, "weight_grad")
     if dtype not in (torch.float32, g.dtype):

@@ -168,3 +168,17 @@ def test_layer_backward_needs_xs_blocks_for_the_softplus_gradient():
         assert bwd(act=act, gx=None) == -1
     assert bwd() == -1 and b"null pointer" in lib.vmf_last_error_string()
     assert bwd(a=None, m=0) == 0 and bwd(a=None, gx=None) == 0
+
+
+@pytest.mark.parametrize("call,error,match", [
+    (lambda: blocks(3, 5).dequantize(), RuntimeError, "HIP device"),
+    (lambda: blocks(3, 5, True).dequantize(torch.bfloat16), RuntimeError, "HIP device"),
+    (lambda: blocks8.softplus_grad(torch.zeros(3, 5), torch.zeros(3, 5)), TypeError, "softplus_grad takes Blocks8"),
+    (lambda: blocks8.weight_grad(torch.zeros(3, 4), torch.zeros(3, 5)), TypeError, "weight_grad takes Blocks8"),
+    (lambda: blocks8.matmul(blocks(2, 3), torch.zeros(5, 3)), TypeError, "matmul takes Blocks8"),
+    (lambda: blocks8.Weight8(torch.zeros(3, 5), None, torch.float32), TypeError, "Weight8 takes Blocks8"),
+    (lambda: blocks8.Weight8(blocks(3, 5, True), torch.zeros(5, 3), torch.float32), TypeError, "Weight8 takes Blocks8"),
+])
+def test_refusals_of_other_operands_and_of_blocks_in_host_memory(call, error, match):
+    with pytest.raises(error, match=match):
+        call()
