@@ -340,7 +340,8 @@ int vmf_blocks8_softplus_grad(const void* g, int64_t g_stride, const uint8_t* va
 /* out[m][n] = (sum_k a[m][k] b[n][k] + bias[n]) * slope, a: m rows, b: n rows, both of width k, in blocks by rows or
  * (tiled = 1) by tiles.  slope (gate not null; blocks by rows, m x n): 1 - exp(-beta gate[m][n]), the softplus gradient.
  * out: dense, VMF_F32, VMF_F16 or VMF_BF16; bias (may be null): one of these types.  Sums are 32-bit for VMF_F32; for the
- * 16-bit types the 8-bit matrix instruction's, 1.3e-5 relative.  The same bits on every run.
+ * 16-bit types the 8-bit matrix instruction's, off by at most 7 * 2^-13 of the sum of the terms' magnitudes (1.3e-5 of the
+ * result for normal values).  The same bits on every run.
  * workspace: vmf_blocks8_matmul_workspace bytes (0 for most sizes), 16-byte aligned. */
 int vmf_blocks8_matmul_workspace(int64_t m, int64_t n, int64_t k, int out_dtype, int64_t* bytes_out);
 int vmf_blocks8_matmul(const uint8_t* a, const uint8_t* a_exponents, int64_t a_exp_pitch, int a_tiled, const uint8_t* b,
@@ -350,7 +351,7 @@ int vmf_blocks8_matmul(const uint8_t* a, const uint8_t* a_exponents, int64_t a_e
                        vmf_stream_t stream);
 /* gweight[n][k] = sum_m gy[m][n] a[m][k], gbias[n] = sum_m gy[m][n] (may be null): gy (m, n) of dtype, a: m rows of width
  * k in blocks by rows, outputs of out_dtype (VMF_F32 or dtype; with VMF_GBIAS_F32 added gbias is VMF_F32 in any case).
- * Products are exact, sums 32-bit, in a fixed order.
+ * Products are exact (but for digits of fp32 gy below 2^-133, which are cut off), sums 32-bit, in a fixed order.
  * m == 0 gives zeros.  gy_values / gy_exponents (may be null): receive gy's blocks by rows, the bytes that
  * vmf_blocks8_quantize gives (the operand of the input gradient's product) without another read of gy. */
 int vmf_blocks8_weight_grad_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes_out);

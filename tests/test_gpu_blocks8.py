@@ -645,3 +645,58 @@ def test_bias_gradient_of_non_finite_columns():
     gy[4, 1], gy[200, 2] = math.inf, math.nan
     gb, = torch.autograd.grad(blocks8.linear(x, normal(5, 20), b), b, gy)
     assert gb[1] == math.inf and gb[2].isnan() and gb[[0, 3, 4]].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("spread", [0.0, 1.0, 2.0])
+@pytest.mark.parametrize("m,n,k", [(9, 40, 1000), (48, 56, 1000), (48, 56, 128)])
+def test_sums_of_16_bit_results_element_by_element(m, n, k, spread, dtype):
+    """The 8-bit instruction adds eight products at a time and cuts seven of them off at 2^-13 of the largest one's power of
+    two, no more than the largest itself; the rest is the 32-bit sums' and the result's rounding."""
+    x = normal(m, k, seed=1) * torch.exp(spread * normal(m, k, seed=2))
+    y = normal(n, k, seed=3) * torch.exp(spread * normal(n, k, seed=4))
+    x, y = x.clamp(-40, 40), y.clamp(-40, 40)  # (results stay inside fp16)
+    a, b = blocks8.quantize(x), blocks8.quantize(y)
+    ad, bd = a.dequantize().double(), b.dequantize().double()
+    terms = ad[:, None, :] * bd[None, :, :]
+    want, size = terms.sum(-1), terms.abs().sum(-1)
+    eights = torch.nn.functional.pad(terms.abs(), (0, -k % 8)).view(m, n, -1, 8)
+    cut = 7 * 2.0 ** -13 * eights.amax(-1).sum(-1)
+    err = (blocks8.matmul(a, b, dtype=dtype).double() - want).abs()
+    bound = torch.finfo(dtype).eps / 2 * (want.abs() + cut) + cut + (k + 8) * U32 * size
+    assert (err <= bound).all(), float((err / bound).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", [(16, 4096, 4096), (256, 512, 128), (256, 512, 1024), (1000, 2000, 700), (4096, 4096, 256)])
+def test_sums_of_16_bit_results_of_normal_values(m, n, k, dtype):
+    """The stated 1.3e-5 of the norm, with a factor of 2.  A sum that is off by e_i rounds to the other neighbour, a step s_i
+    away, with a chance of |e_i| / s_i; the expected square of the difference from the rounded exact result is then
+    sum |e_i| s_i <= |e| |s| <= 2.6e-5 * eps * |want|^2 (a step is at most eps |want_i|).  A tenth more for chance: there are
+    hundreds of such elements (1 % of the results)."""
+    a = blocks8.quantize(normal(m, k, seed=1), "softplus")
+    b = blocks8.quantize_weight(normal(n, k, seed=2, scale=k ** -0.5)).rows
+    want = a.dequantize().double() @ b.dequantize().double().t()
+    off = (blocks8.matmul(a, b, dtype=dtype).double() - want.to(dtype).double()).norm() / want.norm()
+    assert off <= 1.1 * math.sqrt(2.6e-5 * torch.finfo(dtype).eps), float(off)
+
+
+def test_float32_products_have_32_bit_sums_whatever_the_sizes():
+    x = normal(40, 1000, seed=1) * torch.exp(2 * normal(40, 1000, seed=2))
+    y = normal(50, 1000, seed=3) * torch.exp(2 * normal(50, 1000, seed=4))
+    a, b = blocks8.quantize(x.bfloat16()), blocks8.quantize(y.bfloat16())
+    ad, bd = a.dequantize().double(), b.dequantize().double()
+    err = (blocks8.matmul(a, b).double() - ad @ bd.t()).abs()
+    assert (err <= 1008 * U32 * (ad.abs() @ bd.abs().t())).all()
+
+
+@pytest.mark.parametrize("size", [2.0 ** -100, 1.2e-36, 1.2e-38, 1e-40])
+def test_weight_grad_of_tiny_float32_gradients(size):
+    """three bf16 terms hold a value's digits down to 2^-133, the smallest bf16"""
+    g = normal(64, 5, seed=1, scale=size)
+    q = blocks8.quantize(normal(64, 30, seed=2).abs())
+    gd, qd = g.double(), q.dequantize().double()
+    want, terms = gd.t() @ qd, gd.abs().t() @ qd
+    lost = 2.0 ** -133 * qd.sum(0) + 64 * 2.0 ** -149  # and the sums' own smallest step
+    err = (blocks8.weight_grad(g, q)[0].double() - want).abs()
+    assert (err <= 72 * U32 * terms + lost).all(), float((err / (72 * U32 * terms + lost)).max())
