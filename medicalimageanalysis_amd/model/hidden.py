@@ -7,6 +7,8 @@ large batches.  Two optional config keys; without them the bodies are the stock 
   config["layer_norm"] = True    a layer norm in front of every softplus (norm.LayerNorm; modules encoder_norms and
                                  decoder_norms)
 """
+from collections.abc import Mapping
+
 import torch.nn as nn
 import torch.nn.functional as F
 
@@ -15,6 +17,8 @@ from ..norm import LayerNorm
 
 
 def _option(config, key, default):
+    if isinstance(config, Mapping) and key not in config:  # (a defaultdict would invent a value)
+        return default
     try:
         return config[key]
     except KeyError:

@@ -38,3 +38,14 @@ def test_unknown_kind_is_refused(model):
 def test_eight_bit_layers_need_a_hip_device():
     with pytest.raises(RuntimeError, match="HIP device"):
         HypersphericalVAE(dict(CONFIG, hidden="blocks8")).decode(torch.ones(5, 3))
+
+
+@pytest.mark.parametrize("model", MODELS)
+@pytest.mark.parametrize("default", [int, list, lambda: True])
+def test_a_configuration_with_defaults_of_its_own_is_a_stock_model(model, default):
+    from collections import defaultdict
+
+    config = defaultdict(default, CONFIG)
+    made = model(config)
+    assert made._hidden_kind is None and not any("norm" in k for k in made.state_dict())
+    assert "hidden" not in config and "layer_norm" not in config
