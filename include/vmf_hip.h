@@ -370,7 +370,8 @@ int vmf_blocks8_bias_grad(const void* gy, int64_t gy_stride, void* gbias, int64_
  * its tiles already.  a_values / a_exponents (may be null: not kept) receive x's blocks, which bwd takes; wt_values /
  * wt_exponents (may be null) the transposed weight's tiles, which bwd takes for gx.  y: dense, of dtype.
  * bwd: gx (may be null; of dtype) = (blocks(gy) tiles(weight)) * softplus slope, gweight (may be null) and gbias (may be
- * null, comes with gweight; alone: vmf_blocks8_bias_grad) as vmf_blocks8_weight_grad, of weight_dtype (to which VMF_GBIAS_F32 may be added).
+ * null, comes with gweight; alone: vmf_blocks8_bias_grad) as vmf_blocks8_weight_grad, of weight_dtype (to which
+ * VMF_GBIAS_F32 may be added).
  * workspace: the _workspace call's bytes (laid_out: weight is null, kept: a_values is not), 16-byte aligned. */
 int vmf_blocks8_linear_fwd_workspace(int64_t m, int64_t n, int64_t k, int laid_out, int kept, int dtype,
                                      int64_t* bytes_out);

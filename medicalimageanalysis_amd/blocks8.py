@@ -17,7 +17,8 @@ linear's gradients: gx = (blocks(gy) tiles(weight)) * softplus slope, gw = gy^T 
 gy's rows; the roundings to 8 bits pass their gradient on as it is.  float32 results come from 32-bit sums, float16 and
 bfloat16 ones from the 8-bit matrix instruction, which takes half the time: off by 1.3e-5 for normal values (a 37th and a
 300th of their own half step), by at most 8.5e-4 of the sum of the terms' magnitudes where sizes differ widely inside a
-block.  matmul(..., dtype=torch.float32) has 32-bit sums of any blocks.  The weight's gradient always has.  NaN and infinities are NaN in blocks.  Only linear takes part in autograd, backwards (forward-mode derivatives are refused): the
+block.  matmul(..., dtype=torch.float32) has 32-bit sums of any blocks, and so has the weight's gradient.  NaN and
+infinities are NaN in blocks.  Only linear takes part in autograd, backwards (forward-mode derivatives are refused): the
 other functions' results carry no gradient.  There is no CPU path.
 """
 import torch
@@ -137,7 +138,8 @@ def _code(dtype, what):
 def _blocks(what, *operands):
     for q in operands:
         if not isinstance(q, Blocks8):
-            raise TypeError(f"{what} takes Blocks8 (quantize, or the rows / columns of quantize_weight), got {type(q).__name__}")
+            raise TypeError(f"{what} takes Blocks8 (quantize, or the rows / columns of quantize_weight), got "
+                            f"{type(q).__name__}")
 
 
 def _activation(activation, beta, what):

@@ -25,10 +25,9 @@ __device__ __forceinline__ int b8_exponent(float top) {
   const int e = (int)((u + 0x1fffffu) >> 23) - 127 - 8;
   return u == 0 ? 0 : e < B8_EMIN ? B8_EMIN : e > B8_EMAX ? B8_EMAX : e;
 }
-// Two values already divided by the block's 2^e -> two bytes (low half), rounded to nearest even.  Nothing finite is
-// above 448 then but a bound of softplus8, by a few 2^-20, which the conversion rounds to 448; infinities and NaN become
-// NaN.  (e = 119, the largest,
-// is the exception: b8_cut brings what is above 448 down to it first.)
+// Two values already divided by the block's 2^e -> two bytes (low half), rounded to nearest even.  Nothing finite is above 448
+// then but a bound of softplus8, by a few 2^-20, which the conversion rounds to 448, and with e = 119, the largest, where
+// b8_cut brings it down first; infinities and NaN become NaN.
 __device__ __forceinline__ uint32_t b8_pack2(float a, float b) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu;
 }
@@ -161,8 +160,9 @@ static __device__ __noinline__ float softplus_scaled(float x, double beta, int e
 
 // The block of softplus(h).  Which of two neighbouring 8-bit values is nearest to softplus(h) can hang on its last bits,
 // so a value is computed in 32 bits, and once more in 64 where its 32-bit error could change the result (some twenty of
-// a million; of 16-bit inputs, which repeat, it can be more): the bytes are those of the softplus computed in 64 bits.  (A large
-// h is its own softplus, and as the middle of two 8-bit values goes to either: beta h / beta is h but for its last bit.)
+// a million; of 16-bit inputs, which repeat, it can be more): the bytes are those of the softplus computed in 64 bits.  (A
+// large h is its own softplus, and as the middle of two 8-bit values goes to either: beta h / beta is h but for its last
+// bit.)
 __device__ __forceinline__ uint2 softplus8(const float (&h)[8], float beta, float inv_beta, double beta64, int& e_out) {
   constexpr float INF = __builtin_inff();
   // softplus grows with h: the block's largest comes from the largest h.  As integers the bits of floats order like them

@@ -9,12 +9,12 @@
 // work.  Its sums are not 32-bit: it adds the products in eights (consecutive k), and of each cuts off what is below 2^-13 of
 // the largest one's power of two; the eights' sums are then added with the bits of fp32.  So a result is off by at most
 // 7 * 2^-13 = 8.5e-4 of the sum of its terms' magnitudes.  Measured: of normal values 1.3e-5, of the results' norm as of the
-// sum of magnitudes, for K = 128 as for K = 8192; of values whose sizes spread like exp(2 normal) inside a block up to 2.6e-4 of
-// the sum of magnitudes.  Half a step is 3.9e-3 in bf16, 4.9e-4 in fp16: the 1.3e-5 are a 300th and a 37th of that, and 1 % of
-// bf16 results, 7 % of fp16 ones, are rounded to the other neighbour.  It is used for 16-bit results, since it takes half the
-// time (16384x4096x4096 224 - 260 us against 500) and what the operands lost to their 3 bits of mantissa is far more.  A 32-bit
-// result is computed with the bf16 instruction instead: an element of a block is exact in bf16, so are the products, and the
-// sums are 32-bit (4e-8 at K = 1024).
+// sum of magnitudes, for K = 128 as for K = 8192; of values whose sizes spread like exp(2 normal) inside a block up to
+// 2.6e-4 of the sum of magnitudes.  Half a step is 3.9e-3 in bf16, 4.9e-4 in fp16: the 1.3e-5 are a 300th and a 37th of that,
+// and 1 % of bf16 results, 7 % of fp16 ones, are rounded to the other neighbour.  It is used for 16-bit results, since it
+// takes half the time (16384x4096x4096 224 - 260 us against 500) and what the operands lost to their 3 bits of mantissa is
+// far more.  A 32-bit result is computed with the bf16 instruction instead: an element of a block is exact in bf16, so are
+// the products, and the sums are 32-bit (4e-8 at K = 1024).
 #include <type_traits>
 
 #include "blocks8_dev.h"
@@ -1157,7 +1157,7 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(const float* __restrict
 }
 
 // gbias by itself.  A workgroup takes 128 columns of its split's rows, in the lanes and the order that the weight gradient's
-// tiles have; the splits are joined as theirs are.
+// tiles have; the splits are joined as theirs are.  A read of gy: 16384x4096 bf16 24 us (5.6 TB/s), 16384x784 fp32 17 us.
 template <typename T, typename W>
 __global__ __launch_bounds__(256) void bias_grad_kernel(const T* __restrict__ gy, int64_t gy_stride, W* __restrict__ gb,
                                                         float* __restrict__ partial, int64_t m, int64_t n,
@@ -1286,9 +1286,9 @@ extern "C" int vmf_blocks8_matmul_workspace(int64_t m, int64_t n, int64_t k, int
 // vmf_blocks8_matmul; few: not null, a are the rows there, quantised by the same launch (one that few_fits)
 static int matmul(const FewArgs* few, int activation, const uint8_t* a, const uint8_t* a_exponents,
                   int64_t a_exp_pitch, int a_tiled, const uint8_t* b, const uint8_t* b_exponents, int64_t b_exp_pitch,
-                  int b_tiled, const void* bias, int bias_dtype, const uint8_t* gate, const uint8_t* gate_exponents, int64_t gate_exp_pitch,
-                  double beta, void* out, int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes,
-                  int out_dtype, vmf_stream_t stream) {
+                  int b_tiled, const void* bias, int bias_dtype, const uint8_t* gate, const uint8_t* gate_exponents,
+                  int64_t gate_exp_pitch, double beta, void* out, int64_t m, int64_t n, int64_t k, void* workspace,
+                  int64_t workspace_bytes, int out_dtype, vmf_stream_t stream) {
   const char* what = "vmf_blocks8_matmul";
   int64_t need = 0;
   int rc = vmf_blocks8_matmul_workspace(m, n, k, out_dtype, &need);
