@@ -198,3 +198,37 @@ def test_two_captured_graphs_on_two_streams_do_not_share_scratch():
         for got, w in zip(results, want):
             for p, q in zip(got, w):
                 assert torch.equal(p, q)
+
+
+def test_captured_gradients_with_a_frozen_weight_and_a_bias_of_another_type():
+    """x's and the bias's gradients (column sums split over the rows) replayed on a stream of their own, beside eager calls"""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    r = lambda *s: torch.randn(*s, device=DEV, generator=g)  # noqa: E731
+    x, gy, w8 = r(3000, 300).bfloat16(), r(3000, 200).bfloat16(), blocks8.quantize_weight(r(200, 300))
+    w = r(200, 300).bfloat16()
+
+    def once():
+        xs, b = x.detach().requires_grad_(), torch.zeros(200, device=DEV, requires_grad=True)
+        ws = w.detach().requires_grad_()
+        first = torch.autograd.grad(blocks8.linear(xs, w8, b, "softplus"), (xs, b), gy)
+        return first + torch.autograd.grad(blocks8.linear(xs, ws, b, "softplus"), (ws, b), gy)
+
+    want = [t.clone() for t in once()]
+    s = torch.cuda.Stream(DEV)
+    s.wait_stream(torch.cuda.current_stream(DEV))
+    with torch.cuda.stream(s):
+        once()
+    torch.cuda.current_stream(DEV).wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = once()
+    keep = x.clone()
+    for i in range(4):
+        x.copy_(keep * (1 + i % 2))
+        with torch.cuda.stream(s):
+            s.wait_stream(torch.cuda.default_stream(DEV))
+            graph.replay()
+        eager = once()
+        torch.cuda.synchronize()
+        for p, q, first in zip(got, eager, want):
+            assert torch.equal(p, q) and (i % 2 == 1 or torch.equal(p, first))
